@@ -305,6 +305,68 @@ int tenmo_ce_fwd_bwd_f32(tenmo_ctx* ctx, const float* logits, int64_t ld_logits,
                          int reduction, float* softmax_out, float* loss_dev, int32_t* valid_count_dev,
                          const float* upstream_dev, float* dlogits);
 
+/* ---- transformer operators ----------------------------------------------------------------------
+ * Layer normalisation over the last axis (layernorm.mojo of the reference; no GPU-side counterpart on this path):
+ *   y = (x - mean) * rstd * gamma + bias,  rstd = 1 / sqrt(var + eps),  var the mean squared difference from the mean.
+ * x has leading dimension ldx, y / dy / dx are contiguous (M, C); gamma and bias are C floats.  mean and rstd (M floats each)
+ * are what the backward pass needs; either may be NULL when none follows.
+ * Backward: dx, dgamma = sum_m dy * xhat and dbias = sum_m dy (either may be NULL); beta == 1 adds to what all three hold.
+ * dx may be dy.  The column sums are added in a fixed order: results repeat bit for bit.  M == 0 writes zero sums. */
+int tenmo_layernorm_fwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const float* gamma, const float* bias, float eps,
+                            float* y, float* mean, float* rstd, int64_t M, int64_t C);
+int tenmo_layernorm_bwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const float* dy, const float* gamma,
+                            const float* mean, const float* rstd, float* dx, float* dgamma, float* dbias, float beta, int64_t M,
+                            int64_t C);
+
+/* Attention without a score matrix in memory (the fused form of the reference's matmul -> softmax -> matmul chain,
+ * tests/test_attn_matmul.mojo:194-259): o_i = sum_j softmax_j(scale * q_i . k_j) v_j over the visible keys of row i.
+ *   heads     q, o, go, dq: (batch, heads, q_len, dim); k, v, dk, dv: (batch, kv_heads, k_len, dim); heads is a multiple of
+ *             kv_heads and query head h reads key / value head h / (heads / kv_heads).  dim is 1 .. 128.
+ *   views     element (b, h, row, d) at ptr[b*batch_stride + h*head_stride + row*row_stride + d]: the dim axis is contiguous,
+ *             the others have any non-negative stride (0 broadcasts an input).  Outputs may not overlap: in themselves, with
+ *             one another or with an input.
+ *   mask      causal != 0: key j is visible to row i when j <= i + k_len - q_len (the last row sees every key).
+ *             k_lengths / q_lengths (batch int32 on the device, or NULL): keys / rows from the length on do not take part,
+ *             whatever they hold; a length outside [0, k_len] ([0, q_len]) counts as the nearest bound.
+ *             A row without a visible key gives o = 0 and dq = 0 and adds nothing to dk and dv; a key that no row sees gives
+ *             dk = dv = 0.
+ *   stats     (batch, heads, q_len, 2) floats: per row the largest score in units of log 2 and the sum of exponentials; written
+ *             by the forward pass (NULL when no backward pass follows) and read by the backward pass.
+ * Backward recomputes the probabilities; beta == 1 adds to what dq, dk, dv hold.  No atomics: results repeat bit for bit.
+ * A row whose scores hold a NaN or +inf gives NaN. */
+typedef struct {
+    int64_t batch, heads, kv_heads, q_len, k_len, dim;
+} tenmo_attn_shape;
+typedef struct {
+    float* ptr;
+    int64_t batch_stride, head_stride, row_stride;
+} tenmo_heads;
+int tenmo_attention_fwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const tenmo_heads* q, const tenmo_heads* k,
+                            const tenmo_heads* v, const tenmo_heads* o, float* stats, float scale, int causal,
+                            const int32_t* q_lengths, const int32_t* k_lengths);
+int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const tenmo_heads* q, const tenmo_heads* k,
+                            const tenmo_heads* v, const tenmo_heads* o, const float* stats, const tenmo_heads* go,
+                            const tenmo_heads* dq, const tenmo_heads* dk, const tenmo_heads* dv, float beta, float scale,
+                            int causal, const int32_t* q_lengths, const int32_t* k_lengths);
+
+/* Softmax cross-entropy of a linear layer's logits x . W + bias without keeping the logits: the head of a language model,
+ * Linear (net.mojo:179-216) followed by CrossEntropyLoss (crossentropy.mojo:1360-1391).
+ *   x       (N, D), any non-negative strides.  w: (D, V) as Linear keeps it, or the transposed view of a (V, D) embedding; one
+ *           of its axes has unit stride.  bias: V floats or NULL.
+ *   labels, ignore_index, label_smoothing, reduction, loss, valid_count: as tenmo_ce_fwd_f32 (with the mean over no rows 0).
+ *           Rows whose label is ignore_index take no part, whatever their x holds.
+ *   fwd_bwd loss and gradients in one call: dx (N, D) contiguous; dw contiguous in the order of w's storage, (D, V) or
+ *           (V, D); db V floats or NULL.  They are written, not added to.  upstream: 1 float (mean / sum) or N floats (none) on
+ *           the device, NULL for 1.
+ * The logits of a piece of the rows at a time live in the workspace. */
+int tenmo_linear_ce_fwd_f32(tenmo_ctx* ctx, const tenmo_mat* x, const tenmo_mat* w, const float* bias, const void* labels,
+                            int label_is_i64, int64_t N, int64_t D, int64_t V, int64_t ignore_index, float label_smoothing,
+                            int reduction, float* loss, int32_t* valid_count);
+int tenmo_linear_ce_fwd_bwd_f32(tenmo_ctx* ctx, const tenmo_mat* x, const tenmo_mat* w, const float* bias, const void* labels,
+                                int label_is_i64, int64_t N, int64_t D, int64_t V, int64_t ignore_index, float label_smoothing,
+                                int reduction, float* loss, int32_t* valid_count, const float* upstream, float* dx, float* dw,
+                                float* db);
+
 /* ---- optimiser ----------------------------------------------------------------------------------
  * SGD.step dense path for n_tensors parameters in ONE launch (optim.mojo:405-543,
  * kernels/sgd_kernel.mojo:7-128):  g' = g*grad_scale; if wd>0: g' += p*wd;

@@ -1,12 +1,12 @@
-"""CrossEntropyLoss for class-index targets (tenmo/crossentropy.mojo:1360-1391, 937-1083, 664-823)."""
+"""CrossEntropyLoss and LinearCrossEntropyLoss for class-index targets (tenmo/crossentropy.mojo:1360-1391, 937-1083, 664-823)."""
 from __future__ import annotations
 
 import numpy as np
 import torch
 
 from .lib import REDUCTION
-from .tensor import (BACKWARD_CE_CLASS_INDICES_INT32, BACKWARD_CE_CLASS_INDICES_INT64, Ancestry, NDBuffer, Tensor,
-                     handle, panic)
+from .tensor import (BACKWARD_CE_CLASS_INDICES_INT32, BACKWARD_CE_CLASS_INDICES_INT64, BACKWARD_LINEAR_CE, Ancestry,
+                     NDBuffer, Tensor, handle, panic)
 
 
 class CrossEntropyLoss:
@@ -68,6 +68,74 @@ def ce_class_indices_backward(output: Tensor, retain_graph: bool):
     if not retain_graph:
         output.gradbox.fill(0.0)
     return [logits]
+
+
+class LinearCrossEntropyLoss:
+    """``criterion(x, weight, target, bias)``: CrossEntropyLoss of the logits ``x @ weight + bias`` without keeping the logits,
+    for a head with many classes.  ``x`` is (N, D), ``weight`` (D, V) as Linear keeps it or the transposed view of a (V, D)
+    embedding; options and targets as CrossEntropyLoss.  The forward pass computes the loss alone; the backward pass computes
+    the logits again, a piece of the rows at a time, with all the gradients."""
+
+    def __init__(self, reduction="mean", ignore_index: int = -100, label_smoothing: float = 0.0):
+        options = CrossEntropyLoss(reduction, ignore_index, label_smoothing)
+        self.reduction, self.ignore_index, self.label_smoothing = options.reduction, ignore_index, options.label_smoothing
+        self.training = True
+
+    def __call__(self, x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None = None, validate: bool = True) -> Tensor:
+        if len(x.shape()) != 2 or len(weight.shape()) != 2 or x.shape()[1] != weight.shape()[0]:
+            panic("LinearCrossEntropyLoss: x", x.shape(), "and weight", weight.shape(), "do not multiply")
+        (N, D), V = x.shape(), weight.shape()[1]
+        if target.shape() != (N,):
+            panic("LinearCrossEntropyLoss: target shape", target.shape(), "does not match", x.shape())
+        if target.buffer.storage.dtype not in (torch.int64, torch.int32):
+            panic("LinearCrossEntropyLoss: class-index targets must be int64 or int32")
+        if bias is not None and bias.shape() != (V,):
+            panic("LinearCrossEntropyLoss: bias shape", bias.shape(), "does not match", weight.shape())
+        if 1 not in weight.strides():
+            panic("LinearCrossEntropyLoss: weight needs a unit stride on one axis, got", weight.strides())
+        red = REDUCTION[self.reduction]
+        loss = NDBuffer.empty((N,) if red == 2 else ())
+        arg = dict(x=x.buffer, w=weight.buffer, bias=bias.buffer.contiguous() if bias is not None else None,
+                   target=target.buffer.contiguous(), is_i64=target.buffer.storage.dtype == torch.int64, shape=(N, D, V),
+                   options=(self.ignore_index, self.label_smoothing, red), valid=torch.zeros(1, dtype=torch.int32, device="cuda"))
+        h = handle()
+        h.linear_ce_fwd(*_linear_ce_inputs(arg), loss.data_ptr(), arg["valid"].data_ptr())
+        if validate:
+            h.check_device_status()
+        out = Tensor(loss)
+        parents = [x, weight] + ([bias] if bias is not None else [])
+        if self.training and any(p.requires_grad for p in parents):
+            out.requires_grad = True
+            out.ancestry = Ancestry(BACKWARD_LINEAR_CE, parents, arg=arg)
+        return out
+
+
+def _linear_ce_inputs(a):
+    return (a["x"].mat(), a["w"].mat(), a["bias"].data_ptr() if a["bias"] is not None else 0, a["target"].data_ptr(), a["is_i64"],
+            *a["shape"], *a["options"])
+
+
+def linear_ce_backward(output: Tensor, retain_graph: bool):
+    a = output.ancestry.arg
+    N, D, V = a["shape"]
+    x, weight, *rest = output.ancestry.parents
+    # the weight gradient comes in the order of the weight's storage
+    stored_vd = a["w"].strides[0] == 1 and a["w"].strides[1] != 1
+    dx, dw = NDBuffer.empty((N, D)), NDBuffer.empty((V, D) if stored_vd else (D, V))
+    db = NDBuffer.empty((V,)) if rest else None
+    loss = NDBuffer.empty((N,) if a["options"][2] == 2 else ())
+    handle().linear_ce_fwd_bwd(*_linear_ce_inputs(a), loss.data_ptr(), a["valid"].data_ptr(), output.gradbox.data_ptr(),
+                               dx.data_ptr(), dw.data_ptr(), db.data_ptr() if rest else 0)
+    if stored_vd:
+        dw = dw.transpose()
+    touched = []
+    for parent, grad in zip([x, weight] + rest, (dx, dw, db)):
+        if parent.requires_grad:
+            parent.update_grad(grad)
+            touched.append(parent)
+    if not retain_graph:
+        output.gradbox.fill(0.0)
+    return touched
 
 
 class Accuracy:

@@ -1,0 +1,348 @@
+// Attention without a score matrix in memory, fp32: entry points and the kernels for small problems.
+//
+//   s_ij = scale * q_i . k_j  over the visible keys j of row i;  m_i = max_j s_ij;  l_i = sum_j exp(s_ij - m_i)
+//   o_i  = sum_j exp(s_ij - m_i) v_j / l_i
+//   p_ij = exp(s_ij - m_i) / l_i;  dv_j = sum_i p_ij go_i;  delta_i = go_i . o_i
+//   ds_ij = scale * p_ij (go_i . v_j - delta_i);  dq_i = sum_j ds_ij k_j;  dk_j = sum_i ds_ij q_i
+// A key / value head serves H / Hkv query heads; its gradients sum over them.  Key j is visible to row i when
+// j < k_lengths[b], i < q_lengths[b] and, if causal, j <= i + Sk - Sq.  A row that sees nothing gives o = 0 and no gradient.
+//
+// The backward pass recomputes the probabilities from q, k and the two saved numbers per row, m_i and l_i (kept apart: with
+// their sum, the log-sum-exp, a large m would cost p its last bits).
+//
+// Kernels here: one warp per row, scores 32 keys at a time (a lane is a key), the weighted sum with a lane per column.
+// No tile is filled and nothing waits on anything, so small problems finish in one launch latency per pass.
+#include "attention.cuh"
+
+#include <cfloat>
+
+namespace {
+
+constexpr int ROW_WARPS = 4;
+constexpr int DSLOTS = TENMO_ATTN_MAX_DIM / 32;
+
+// dot product of a row in shared memory (broadcast) and a row in global memory (this lane's)
+__device__ __forceinline__ float dot_row(const float* sh, const float* g, int D, bool vec) {
+    float a = 0.f, b = 0.f;
+    if (vec) {
+        for (int d = 0; d < D; d += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(sh + d);
+            const float4 y = __ldg(reinterpret_cast<const float4*>(g + d));
+            a = fmaf(x.x, y.x, a);
+            b = fmaf(x.y, y.y, b);
+            a = fmaf(x.z, y.z, a);
+            b = fmaf(x.w, y.w, b);
+        }
+    } else {
+        for (int d = 0; d < D; ++d) a = fmaf(sh[d], __ldg(g + d), a);
+    }
+    return a + b;
+}
+__device__ __forceinline__ bool row_vec(const TenmoHeadsView& v, int D) {
+    return D % 4 == 0 && v.sb % 4 == 0 && v.sh % 4 == 0 && v.sr % 4 == 0 && ((uintptr_t)v.ptr & 15u) == 0;
+}
+// keys that row i of batch entry b sees: the first n
+__device__ __forceinline__ int visible_keys(const TenmoAttnParams& p, int b, int i) {
+    if (i >= tenmo_attn_rows(p.q_lengths, b, p.Sq)) return 0;
+    int n = tenmo_attn_rows(p.k_lengths, b, p.Sk);
+    if (p.causal) n = min(n, max(0, i + p.Sk - p.Sq + 1));
+    return n;
+}
+
+// (b, h, i) of a warp's row; false past the end
+__device__ __forceinline__ bool warp_row(int64_t rows_per_head, int heads, int64_t total, int* b, int* h, int* i) {
+    const int64_t r = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    if (r >= total) return false;
+    *i = (int)(r % rows_per_head);
+    const int64_t bh = r / rows_per_head;
+    *h = (int)(bh % heads);
+    *b = (int)(bh / heads);
+    return true;
+}
+
+__global__ void __launch_bounds__(ROW_WARPS * 32) attn_fwd_row_kernel(const TenmoAttnParams p) {
+    __shared__ __align__(16) float sq[ROW_WARPS][TENMO_ATTN_MAX_DIM];
+    tenmo_grid_dependency_sync();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int b, h, i;
+    if (!warp_row(p.Sq, p.H, (int64_t)p.B * p.H * p.Sq, &b, &h, &i)) return;
+    const int kvh = h / (p.H / p.Hkv);
+    const float* q = p.q.ptr + b * p.q.sb + h * p.q.sh + i * p.q.sr;
+    const float* k = p.k.ptr + b * p.k.sb + kvh * p.k.sh;
+    const float* v = p.v.ptr + b * p.v.sb + kvh * p.v.sh;
+    const bool vec = row_vec(p.k, p.D);
+    for (int d = lane; d < p.D; d += 32) sq[warp][d] = __ldg(q + d);
+    __syncwarp();
+    const int n = visible_keys(p, b, i);
+    float m = -INFINITY, l = 0.f, acc[DSLOTS];
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) acc[t] = 0.f;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+        const int j = j0 + lane;
+        const float s = j < n ? dot_row(sq[warp], k + j * p.k.sr, p.D, vec) * p.scale_log2 : -INFINITY;
+        const float mn = fmaxf(m, tenmo_warp_max(s));
+        const float base = mn == -INFINITY ? 0.f : mn;  // every score so far is -inf
+        const float e = exp2f(s - base), shrink = exp2f(m - base);
+        m = mn;
+        l = l * shrink + tenmo_warp_sum(e);
+#pragma unroll
+        for (int t = 0; t < DSLOTS; ++t) acc[t] *= shrink;
+        const int cnt = min(32, n - j0);
+        for (int jj = 0; jj < cnt; ++jj) {
+            const float w = __shfl_sync(0xffffffffu, e, jj);
+            const float* row = v + (j0 + jj) * p.v.sr;
+#pragma unroll
+            for (int t = 0; t < DSLOTS; ++t) {
+                const int d = lane + 32 * t;
+                if (d < p.D) acc[t] = fmaf(w, __ldg(row + d), acc[t]);
+            }
+        }
+    }
+    // l is 0 for a row without visible keys (or with all scores -inf): its output is 0.  A NaN sum stays NaN.
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float* o = p.o.ptr + b * p.o.sb + h * p.o.sh + i * p.o.sr;
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) {
+        const int d = lane + 32 * t;
+        if (d < p.D) o[d] = acc[t] * inv;
+    }
+    if (p.stats && lane == 0) {
+        float* st = p.stats + (((int64_t)b * p.H + h) * p.Sq + i) * 2;
+        st[0] = m;
+        st[1] = l;
+    }
+}
+
+// probability from the recomputed score and the saved (maximum, sum)
+__device__ __forceinline__ float prob(float s_log2, float m, float inv_l) { return exp2f(s_log2 - m) * inv_l; }
+
+__global__ void __launch_bounds__(ROW_WARPS * 32) attn_bwd_dq_row_kernel(const TenmoAttnParams p) {
+    __shared__ __align__(16) float sq[ROW_WARPS][TENMO_ATTN_MAX_DIM], sg[ROW_WARPS][TENMO_ATTN_MAX_DIM];
+    tenmo_grid_dependency_sync();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int b, h, i;
+    if (!warp_row(p.Sq, p.H, (int64_t)p.B * p.H * p.Sq, &b, &h, &i)) return;
+    const int kvh = h / (p.H / p.Hkv);
+    const float* q = p.q.ptr + b * p.q.sb + h * p.q.sh + i * p.q.sr;
+    const float* go = p.go.ptr + b * p.go.sb + h * p.go.sh + i * p.go.sr;
+    const float* o = p.o.ptr + b * p.o.sb + h * p.o.sh + i * p.o.sr;
+    const float* k = p.k.ptr + b * p.k.sb + kvh * p.k.sh;
+    const float* v = p.v.ptr + b * p.v.sb + kvh * p.v.sh;
+    const bool vk = row_vec(p.k, p.D), vv = row_vec(p.v, p.D);
+    float delta = 0.f;
+    for (int d = lane; d < p.D; d += 32) {
+        sq[warp][d] = __ldg(q + d);
+        const float g = __ldg(go + d);
+        sg[warp][d] = g;
+        delta = fmaf(g, __ldg(o + d), delta);
+    }
+    delta = tenmo_warp_sum(delta);
+    __syncwarp();
+    const int64_t r = ((int64_t)b * p.H + h) * p.Sq + i;
+    const float m = __ldg(p.stats + 2 * r), l = __ldg(p.stats + 2 * r + 1);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int n = l == 0.f ? 0 : visible_keys(p, b, i);
+    if (lane == 0) p.delta[r] = delta;
+    float acc[DSLOTS];
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) acc[t] = 0.f;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+        const int j = j0 + lane;
+        float ds = 0.f;
+        if (j < n) {
+            const float pr = prob(dot_row(sq[warp], k + j * p.k.sr, p.D, vk) * p.scale_log2, m, inv);
+            ds = pr * (dot_row(sg[warp], v + j * p.v.sr, p.D, vv) - delta) * p.scale;
+        }
+        const int cnt = min(32, n - j0);
+        for (int jj = 0; jj < cnt; ++jj) {
+            const float w = __shfl_sync(0xffffffffu, ds, jj);
+            const float* row = k + (j0 + jj) * p.k.sr;
+#pragma unroll
+            for (int t = 0; t < DSLOTS; ++t) {
+                const int d = lane + 32 * t;
+                if (d < p.D) acc[t] = fmaf(w, __ldg(row + d), acc[t]);
+            }
+        }
+    }
+    float* dq = p.dq.ptr + b * p.dq.sb + h * p.dq.sh + i * p.dq.sr;
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) {
+        const int d = lane + 32 * t;
+        if (d < p.D) dq[d] = p.beta != 0.f ? dq[d] + acc[t] : acc[t];
+    }
+}
+
+__global__ void __launch_bounds__(ROW_WARPS * 32) attn_bwd_dkv_row_kernel(const TenmoAttnParams p) {
+    __shared__ __align__(16) float sk[ROW_WARPS][TENMO_ATTN_MAX_DIM], sv[ROW_WARPS][TENMO_ATTN_MAX_DIM];
+    tenmo_grid_dependency_sync();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int b, kvh, j;
+    if (!warp_row(p.Sk, p.Hkv, (int64_t)p.B * p.Hkv * p.Sk, &b, &kvh, &j)) return;
+    const int group = p.H / p.Hkv;
+    const float* k = p.k.ptr + b * p.k.sb + kvh * p.k.sh + j * p.k.sr;
+    const float* v = p.v.ptr + b * p.v.sb + kvh * p.v.sh + j * p.v.sr;
+    for (int d = lane; d < p.D; d += 32) {
+        sk[warp][d] = __ldg(k + d);
+        sv[warp][d] = __ldg(v + d);
+    }
+    __syncwarp();
+    float ak[DSLOTS], av[DSLOTS];
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) ak[t] = av[t] = 0.f;
+    const bool vq = row_vec(p.q, p.D), vg = row_vec(p.go, p.D);
+    const int rows = tenmo_attn_rows(p.q_lengths, b, p.Sq);
+    const bool seen = j < tenmo_attn_rows(p.k_lengths, b, p.Sk);
+    const int first = p.causal ? max(0, j - (p.Sk - p.Sq)) : 0;
+    for (int h = kvh * group; seen && h < (kvh + 1) * group; ++h) {
+        const float* q = p.q.ptr + b * p.q.sb + h * p.q.sh;
+        const float* go = p.go.ptr + b * p.go.sb + h * p.go.sh;
+        const int64_t r0 = ((int64_t)b * p.H + h) * p.Sq;
+        for (int i0 = first; i0 < rows; i0 += 32) {
+            const int i = i0 + lane;
+            float pr = 0.f, ds = 0.f;
+            if (i < rows) {
+                const float m = __ldg(p.stats + 2 * (r0 + i)), l = __ldg(p.stats + 2 * (r0 + i) + 1);
+                if (l != 0.f) {
+                    pr = prob(dot_row(sk[warp], q + i * p.q.sr, p.D, vq) * p.scale_log2, m, 1.f / l);
+                    ds = pr * (dot_row(sv[warp], go + i * p.go.sr, p.D, vg) - __ldg(p.delta + r0 + i)) * p.scale;
+                }
+            }
+            const int cnt = min(32, rows - i0);
+            for (int ii = 0; ii < cnt; ++ii) {
+                const float wp = __shfl_sync(0xffffffffu, pr, ii), wd = __shfl_sync(0xffffffffu, ds, ii);
+                const float* rq = q + (i0 + ii) * p.q.sr;
+                const float* rg = go + (i0 + ii) * p.go.sr;
+#pragma unroll
+                for (int t = 0; t < DSLOTS; ++t) {
+                    const int d = lane + 32 * t;
+                    if (d < p.D) {
+                        ak[t] = fmaf(wd, __ldg(rq + d), ak[t]);
+                        av[t] = fmaf(wp, __ldg(rg + d), av[t]);
+                    }
+                }
+            }
+        }
+    }
+    float* dk = p.dk.ptr + b * p.dk.sb + kvh * p.dk.sh + j * p.dk.sr;
+    float* dv = p.dv.ptr + b * p.dv.sb + kvh * p.dv.sh + j * p.dv.sr;
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) {
+        const int d = lane + 32 * t;
+        if (d < p.D) {
+            dk[d] = p.beta != 0.f ? dk[d] + ak[t] : ak[t];
+            dv[d] = p.beta != 0.f ? dv[d] + av[t] : av[t];
+        }
+    }
+}
+
+int check_shape(tenmo_ctx* ctx, const char* who, const tenmo_attn_shape* s, float scale, TenmoAttnParams* p) {
+    if (!s) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: shape is NULL", who);
+    if (s->batch < 0 || s->heads < 1 || s->kv_heads < 1 || s->q_len < 0 || s->k_len < 0 || s->dim < 1)
+        return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: batch %lld, heads %lld / %lld, lengths %lld / %lld, dim %lld", who,
+                               (long long)s->batch, (long long)s->heads, (long long)s->kv_heads, (long long)s->q_len,
+                               (long long)s->k_len, (long long)s->dim);
+    if (s->heads % s->kv_heads)
+        return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: %lld query heads are not a multiple of %lld key/value heads", who,
+                               (long long)s->heads, (long long)s->kv_heads);
+    if (s->dim > TENMO_ATTN_MAX_DIM)
+        return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "%s: head dimension %lld is above %d", who, (long long)s->dim,
+                               TENMO_ATTN_MAX_DIM);
+    const int64_t lim = (int64_t)1 << 30;
+    if (s->batch > lim || s->heads > 65535 || s->q_len > lim || s->k_len > lim || s->batch * s->heads > lim)
+        return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "%s: sizes beyond 2^30 rows", who);
+    const int64_t longest = s->q_len > s->k_len ? s->q_len : s->k_len;
+    if (s->batch * s->heads * longest >= ((int64_t)1 << 32))
+        return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "%s: more than 2^32 rows in one call", who);
+    if (!(fabsf(scale) <= FLT_MAX)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: scale is not finite", who);
+    p->B = (int)s->batch; p->H = (int)s->heads; p->Hkv = (int)s->kv_heads;
+    p->Sq = (int)s->q_len; p->Sk = (int)s->k_len; p->D = (int)s->dim;
+    p->scale = scale;
+    p->scale_log2 = (float)((double)scale * 1.4426950408889634074);
+    return TENMO_OK;
+}
+
+int take_view(tenmo_ctx* ctx, const char* who, const char* name, const tenmo_heads* t, bool needed, bool output, int64_t rows, int64_t dim,
+              TenmoHeadsView* v) {
+    if (!t || (!t->ptr && needed)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: %s is NULL", who, name);
+    if (t->batch_stride < 0 || t->head_stride < 0 || t->row_stride < 0)
+        return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: %s has a negative stride", who, name);
+    // rows of an output that overlap would be written by several warps at once
+    if (output && rows > 1 && t->row_stride < dim)
+        return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: rows of %s overlap (row stride %lld, dim %lld)", who, name,
+                               (long long)t->row_stride, (long long)dim);
+    *v = TenmoHeadsView{t->ptr, t->batch_stride, t->head_stride, t->row_stride};
+    return TENMO_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tenmo_attention_fwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const tenmo_heads* q, const tenmo_heads* k,
+                            const tenmo_heads* v, const tenmo_heads* o, float* stats, float scale, int causal,
+                            const int32_t* q_lengths, const int32_t* k_lengths) {
+    TENMO_CHECK_CTX(ctx);
+    const char* who = "attention_fwd";
+    TenmoAttnParams p = {};
+    int st = check_shape(ctx, who, shape, scale, &p);
+    if (st != TENMO_OK) return st;
+    const bool any_q = p.B && p.Sq, any_k = p.B && p.Sk && p.Sq;
+    if ((st = take_view(ctx, who, "q", q, any_k, false, p.Sq, p.D, &p.q)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "k", k, any_k, false, p.Sk, p.D, &p.k)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "v", v, any_k, false, p.Sk, p.D, &p.v)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "o", o, any_q, true, p.Sq, p.D, &p.o)) != TENMO_OK) return st;
+    if (!any_q) return TENMO_OK;
+    p.stats = stats;
+    p.causal = causal != 0;
+    p.q_lengths = q_lengths;
+    p.k_lengths = k_lengths;
+    TenmoDeviceGuard guard(ctx);
+    const int64_t grid = ((int64_t)p.B * p.H * p.Sq + ROW_WARPS - 1) / ROW_WARPS;
+    TENMO_CUDA_TRY(ctx, tenmo_launch(attn_fwd_row_kernel, (unsigned)grid, ROW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, grid), p));
+    TENMO_LAUNCH_CHECK(ctx, "attn_fwd_row_kernel");
+    return TENMO_OK;
+}
+
+int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const tenmo_heads* q, const tenmo_heads* k,
+                            const tenmo_heads* v, const tenmo_heads* o, const float* stats, const tenmo_heads* go,
+                            const tenmo_heads* dq, const tenmo_heads* dk, const tenmo_heads* dv, float beta, float scale,
+                            int causal, const int32_t* q_lengths, const int32_t* k_lengths) {
+    TENMO_CHECK_CTX(ctx);
+    const char* who = "attention_bwd";
+    TenmoAttnParams p = {};
+    int st = check_shape(ctx, who, shape, scale, &p);
+    if (st != TENMO_OK) return st;
+    if (beta != 0.f && beta != 1.f) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "attention_bwd: beta must be 0 or 1");
+    const bool any_q = p.B && p.Sq, any_k = p.B && p.Sk;
+    if ((st = take_view(ctx, who, "q", q, any_q, false, p.Sq, p.D, &p.q)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "k", k, any_k, false, p.Sk, p.D, &p.k)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "v", v, any_k, false, p.Sk, p.D, &p.v)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "o", o, any_q, false, p.Sq, p.D, &p.o)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "go", go, any_q, false, p.Sq, p.D, &p.go)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "dq", dq, any_q, true, p.Sq, p.D, &p.dq)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "dk", dk, any_k, true, p.Sk, p.D, &p.dk)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "dv", dv, any_k, true, p.Sk, p.D, &p.dv)) != TENMO_OK) return st;
+    if (any_q && !stats) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "attention_bwd: stats is NULL");
+    p.stats = const_cast<float*>(stats);
+    p.causal = causal != 0;
+    p.q_lengths = q_lengths;
+    p.k_lengths = k_lengths;
+    p.beta = beta;
+    TenmoDeviceGuard guard(ctx);
+    void* ws = nullptr;
+    if ((st = tenmo_op_workspace(ctx, (size_t)p.B * p.H * p.Sq * sizeof(float) + 16, &ws)) != TENMO_OK) return st;
+    p.delta = (float*)ws;
+    if (any_q) {
+        const int64_t grid = ((int64_t)p.B * p.H * p.Sq + ROW_WARPS - 1) / ROW_WARPS;
+        TENMO_CUDA_TRY(ctx, tenmo_launch(attn_bwd_dq_row_kernel, (unsigned)grid, ROW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, grid), p));
+        TENMO_LAUNCH_CHECK(ctx, "attn_bwd_dq_row_kernel");
+    }
+    if (any_k) {
+        const int64_t grid = ((int64_t)p.B * p.Hkv * p.Sk + ROW_WARPS - 1) / ROW_WARPS;
+        TENMO_CUDA_TRY(ctx, tenmo_launch(attn_bwd_dkv_row_kernel, (unsigned)grid, ROW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, grid), p));
+        TENMO_LAUNCH_CHECK(ctx, "attn_bwd_dkv_row_kernel");
+    }
+    return TENMO_OK;
+}
+
+}  // extern "C"

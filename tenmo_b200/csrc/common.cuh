@@ -41,6 +41,13 @@ struct tenmo_ctx {
     // workspace (grown on demand, never shrunk): lo planes for the 3xTF32 kernel, reduction partials
     void* ws = nullptr;
     size_t ws_bytes = 0;
+    // workspace of the transformer operators (tenmo_op_workspace).  A block that a captured CUDA graph uses is never freed
+    // before the context: growing puts it on the retired list.
+    void* op_ws = nullptr;
+    size_t op_ws_bytes = 0;
+    bool op_ws_captured = false;
+    void* op_retired[16] = {nullptr};
+    int n_op_retired = 0;
     // small fixed device scratch: [0] status word, [8..15] cross-entropy tickets/accumulators
     uint32_t* dev_status = nullptr;
     // ticket counters of the split column-sum kernel: zero between calls (the last CTA resets its own)

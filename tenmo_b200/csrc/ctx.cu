@@ -1,5 +1,6 @@
 // Context lifetime, error strings, stream binding, workspace.
 #include "common.cuh"
+#include "op_util.cuh"
 
 // errors of calls that have no context (tenmo_cuda_init, tenmo_colsum_f32_static): one buffer per host thread
 static thread_local char g_init_error[512] = {0};
@@ -47,6 +48,40 @@ int tenmo_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
         ctx->ws_bytes = want;
     }
     *out = ctx->ws;
+    return TENMO_OK;
+}
+
+int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    const bool capturing = cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
+    if (bytes > ctx->op_ws_bytes) {
+        if (capturing)
+            return tenmo_set_error(ctx, TENMO_ERR_STATE,
+                                   "the workspace must grow to %zu bytes but the stream is capturing: run the call once outside the capture first",
+                                   bytes);
+        if (ctx->op_ws) {
+            const int slots = (int)(sizeof(ctx->op_retired) / sizeof(ctx->op_retired[0]));
+            if (ctx->op_ws_captured && ctx->n_op_retired == slots)
+                return tenmo_set_error(ctx, TENMO_ERR_STATE, "the workspace has grown %d times between graph captures: make the largest call first", slots);
+            cudaError_t e = sync_bound_streams(ctx);  // the old block may be in use on any stream the context was bound to
+            if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace sync: %s", cudaGetErrorString(e));
+            if (ctx->op_ws_captured) ctx->op_retired[ctx->n_op_retired++] = ctx->op_ws;
+            else cudaFree(ctx->op_ws);
+            ctx->op_ws = nullptr;
+            ctx->op_ws_bytes = 0;
+            ctx->op_ws_captured = false;
+        }
+        const size_t want = (bytes + ((size_t)1 << 20) - 1) & ~(((size_t)1 << 20) - 1);
+        cudaError_t e = cudaMalloc(&ctx->op_ws, want);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            ctx->op_ws = nullptr;
+            return tenmo_set_error(ctx, TENMO_ERR_NOMEM, "workspace of %zu bytes: %s", want, cudaGetErrorString(e));
+        }
+        ctx->op_ws_bytes = want;
+    }
+    if (capturing) ctx->op_ws_captured = true;
+    *out = ctx->op_ws;
     return TENMO_OK;
 }
 
@@ -146,6 +181,8 @@ void tenmo_cuda_destroy(tenmo_ctx* ctx) {
     if (ctx->p2p_buf) tenmo_dp_p2p_close(ctx);
     if (ctx->stream) cudaStreamSynchronize(ctx->stream);
     if (ctx->ws) cudaFree(ctx->ws);
+    if (ctx->op_ws) cudaFree(ctx->op_ws);
+    for (int i = 0; i < ctx->n_op_retired; ++i) cudaFree(ctx->op_retired[i]);
     if (ctx->dev_status) cudaFree(ctx->dev_status);
     if (ctx->tickets) cudaFree(ctx->tickets);
     if (ctx->sgd_desc_dev) cudaFree(ctx->sgd_desc_dev);

@@ -1,0 +1,21 @@
+// Shared by the transformer operators (layer norm, attention, linear cross-entropy).
+#pragma once
+#include "common.cuh"
+
+// Makes the context's device current for the length of an entry point and puts the caller's back.
+struct TenmoDeviceGuard {
+    int before = -1;
+    explicit TenmoDeviceGuard(const tenmo_ctx* ctx) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = now;
+    }
+    ~TenmoDeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+    TenmoDeviceGuard(const TenmoDeviceGuard&) = delete;
+    TenmoDeviceGuard& operator=(const TenmoDeviceGuard&) = delete;
+};
+
+// A second workspace block, apart from the one of tenmo_workspace: these operators call the library's GEMMs while they
+// hold intermediate results.  Same rules: grown on demand, refused while the stream is being captured.
+int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out);

@@ -30,6 +30,8 @@ EXPORTS = [
     "tenmo_conv_out_size", "tenmo_conv2d_fwd_f32", "tenmo_conv2d_bwd_input_f32", "tenmo_conv2d_bwd_weight_f32", "tenmo_im2col_f32", "tenmo_col2im_f32", "tenmo_channel_sum_f32", "tenmo_maxpool2d_fwd_f32",
     "tenmo_maxpool2d_bwd_f32",
     "tenmo_colsum_f32_static", "tenmo_softmax_fwd_f32", "tenmo_softmax_bwd_f32", "tenmo_ce_fwd_f32", "tenmo_ce_bwd_f32", "tenmo_ce_fwd_bwd_f32", "tenmo_sgd_step_f32", "tenmo_sgd_step_lo_f32", "tenmo_accuracy_f32", "tenmo_dp_get_unique_id",
+    "tenmo_layernorm_fwd_f32", "tenmo_layernorm_bwd_f32", "tenmo_attention_fwd_f32", "tenmo_attention_bwd_f32",
+    "tenmo_linear_ce_fwd_f32", "tenmo_linear_ce_fwd_bwd_f32",
     "tenmo_dp_init", "tenmo_dp_allreduce_sum_f32", "tenmo_dp_finalize",
     "tenmo_dp_p2p_alloc", "tenmo_dp_p2p_connect", "tenmo_dp_p2p_allreduce_sum_f32", "tenmo_dp_p2p_sgd_step_f32", "tenmo_dp_p2p_set_coresident", "tenmo_dp_p2p_close",
 ]
@@ -70,6 +72,27 @@ class GemmOpts(C.Structure):
         ("mul_mask", C.c_void_p),
         ("bias_m", C.c_void_p),
     ]
+
+
+class AttnShape(C.Structure):
+    """``tenmo_attn_shape``."""
+
+    _fields_ = [(n, C.c_int64) for n in ("batch", "heads", "kv_heads", "q_len", "k_len", "dim")]
+
+
+class Heads(C.Structure):
+    """``tenmo_heads``: a (batch, heads, rows, dim) view whose last axis is contiguous."""
+
+    _fields_ = [("ptr", C.c_void_p), ("batch_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+
+def make_heads(ptr: int, strides) -> Heads:
+    """``strides`` in elements of the (batch, heads, rows) axes; a fourth one, of the dim axis, has to be 1."""
+    if len(strides) not in (3, 4):
+        raise ValueError("make_heads needs the strides of the batch, head and row axes")
+    if len(strides) == 4 and strides[3] != 1:
+        raise ValueError("make_heads: the dim axis has to be contiguous")
+    return Heads(ptr, strides[0], strides[1], strides[2])
 
 
 def make_mat(ptr: int, shape, strides, offset: int = 0) -> Mat:
@@ -136,6 +159,12 @@ def _bind(lib):
         "tenmo_ce_fwd_f32": (I, [P, P, I64, P, I, I64, I64, I64, F, I, P, P, P]),
         "tenmo_ce_bwd_f32": (I, [P, P, P, I, I64, I64, I64, F, I, P, P, P, F]),
         "tenmo_ce_fwd_bwd_f32": (I, [P, P, I64, P, I, I64, I64, I64, F, I, P, P, P, P, P]),
+        "tenmo_layernorm_fwd_f32": (I, [P, P, I64, P, P, F, P, P, P, I64, I64]),
+        "tenmo_layernorm_bwd_f32": (I, [P, P, I64, P, P, P, P, P, P, P, F, I64, I64]),
+        "tenmo_attention_fwd_f32": (I, [P, C.POINTER(AttnShape)] + [C.POINTER(Heads)] * 4 + [P, F, I, P, P]),
+        "tenmo_attention_bwd_f32": (I, [P, C.POINTER(AttnShape)] + [C.POINTER(Heads)] * 4 + [P] + [C.POINTER(Heads)] * 4 + [F, F, I, P, P]),
+        "tenmo_linear_ce_fwd_f32": (I, [P, C.POINTER(Mat), C.POINTER(Mat), P, P, I, I64, I64, I64, I64, F, I, P, P]),
+        "tenmo_linear_ce_fwd_bwd_f32": (I, [P, C.POINTER(Mat), C.POINTER(Mat), P, P, I, I64, I64, I64, I64, F, I, P, P, P, P, P, P]),
         "tenmo_sgd_step_f32": (I, [P, I, P, P, P, P, F, F, F, F]),
         "tenmo_sgd_step_lo_f32": (I, [P, I, P, P, P, P, P, P, F, F, F, F]),
         "tenmo_accuracy_f32": (I, [P, P, I64, P, I, I64, I64, P, P]),
@@ -361,6 +390,38 @@ class TenmoCuda:
                valid_count, dlogits, beta=0.0):
         self._call("tenmo_ce_bwd_f32", softmax, labels, 1 if label_is_i64 else 0, M, Cn, ignore_index,
                    label_smoothing, reduction, upstream or None, valid_count or None, dlogits, beta)
+
+    def layernorm_fwd(self, x, ldx, gamma, bias, eps, y, mean, rstd, M, Cn):
+        """Layer norm over the last axis; mean / rstd (0: not wanted) are what the backward pass needs."""
+        self._call("tenmo_layernorm_fwd_f32", x, ldx, gamma, bias, eps, y, mean or None, rstd or None, M, Cn)
+
+    def layernorm_bwd(self, x, ldx, dy, gamma, mean, rstd, dx, dgamma, dbias, M, Cn, beta=0.0):
+        self._call("tenmo_layernorm_bwd_f32", x, ldx, dy, gamma, mean, rstd, dx, dgamma or None, dbias or None, beta, M, Cn)
+
+    def attention_fwd(self, shape, q: Heads, k: Heads, v: Heads, o: Heads, stats, scale, *, causal=False, q_lengths=0, k_lengths=0):
+        """softmax(scale * q k^T + mask) v per head; ``shape`` is (batch, heads, kv_heads, q_len, k_len, dim).  ``stats`` (0: no
+        backward pass follows) receives two floats per row."""
+        self._call("tenmo_attention_fwd_f32", C.byref(AttnShape(*shape)), C.byref(q), C.byref(k), C.byref(v), C.byref(o),
+                   stats or None, scale, 1 if causal else 0, q_lengths or None, k_lengths or None)
+
+    def attention_bwd(self, shape, q: Heads, k: Heads, v: Heads, o: Heads, stats, go: Heads, dq: Heads, dk: Heads, dv: Heads, scale,
+                      *, causal=False, q_lengths=0, k_lengths=0, beta=0.0):
+        """Gradients of attention_fwd from the gradient ``go`` of its output; the probabilities are recomputed."""
+        self._call("tenmo_attention_bwd_f32", C.byref(AttnShape(*shape)), C.byref(q), C.byref(k), C.byref(v), C.byref(o),
+                   stats, C.byref(go), C.byref(dq), C.byref(dk), C.byref(dv), beta, scale, 1 if causal else 0, q_lengths or None,
+                   k_lengths or None)
+
+    def linear_ce_fwd(self, x: Mat, w: Mat, bias, labels, label_is_i64, N, D, V, ignore_index, label_smoothing, reduction, loss,
+                      valid_count):
+        """Cross-entropy of the logits x . w (+ bias) without keeping the logits: the loss alone."""
+        self._call("tenmo_linear_ce_fwd_f32", C.byref(x), C.byref(w), bias or None, labels, 1 if label_is_i64 else 0, N, D, V,
+                   ignore_index, label_smoothing, reduction, loss, valid_count)
+
+    def linear_ce_fwd_bwd(self, x: Mat, w: Mat, bias, labels, label_is_i64, N, D, V, ignore_index, label_smoothing, reduction,
+                          loss, valid_count, upstream, dx, dw, db=0):
+        """Loss and gradients in one call; dw has the order of w's storage."""
+        self._call("tenmo_linear_ce_fwd_bwd_f32", C.byref(x), C.byref(w), bias or None, labels, 1 if label_is_i64 else 0, N, D, V,
+                   ignore_index, label_smoothing, reduction, loss, valid_count, upstream or None, dx, dw, db or None)
 
     def sgd_step(self, p_ptrs, g_ptrs, v_ptrs, numels, lr, momentum=0.0, weight_decay=0.0, grad_scale=1.0, lo_ptrs=None,
                  lo_numels=None):

@@ -1,11 +1,11 @@
-"""Linear / ReLU / Sigmoid / Sequential (tenmo/net.mojo:49-216, 692-698, 1069-1181)."""
+"""Linear / ReLU / Sigmoid / LayerNorm / Sequential (tenmo/net.mojo:49-216, 692-698, 1069-1181)."""
 from __future__ import annotations
 
 import math
 
 import numpy as np
 
-from .tensor import Tensor, panic
+from .tensor import BACKWARD_LAYER_NORM, Ancestry, NDBuffer, Tensor, handle, panic
 
 
 class Linear:
@@ -68,6 +68,57 @@ class Sigmoid:
         return []
 
 
+class LayerNorm:
+    """Layer normalisation over the last axis with a learned gain and bias (tenmo/layernorm.mojo); weight starts at one,
+    bias at zero."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-5):
+        if int(normalized_shape) < 1:
+            panic("LayerNorm: normalized_shape must be positive, got", normalized_shape)
+        self.normalized_shape, self.eps = int(normalized_shape), float(eps)
+        self.training = True
+        self.weight = Tensor.ones(self.normalized_shape, requires_grad=True)
+        self.bias = Tensor.zeros(self.normalized_shape, requires_grad=True)
+
+    def __call__(self, xs: Tensor) -> Tensor:
+        if not xs.shape() or xs.shape()[-1] != self.normalized_shape:
+            panic("LayerNorm forward: last dim of", xs.shape(), "is not", self.normalized_shape)
+        x = xs.buffer.contiguous()
+        C = self.normalized_shape
+        M = x.numels() // C
+        out, mean, rstd = NDBuffer.empty(x.shape), NDBuffer.empty((M,)), NDBuffer.empty((M,))
+        handle().layernorm_fwd(x.data_ptr(), C, self.weight.buffer.data_ptr(), self.bias.buffer.data_ptr(), self.eps,
+                               out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), M, C)
+        t = Tensor(out)
+        if self.training and (xs.requires_grad or self.weight.requires_grad or self.bias.requires_grad):
+            t.requires_grad = True
+            t.ancestry = Ancestry(BACKWARD_LAYER_NORM, [xs, self.weight, self.bias], arg=dict(x=x, mean=mean, rstd=rstd))
+        return t
+
+    def parameters(self):
+        return [self.weight, self.bias]
+
+
+def layer_norm_backward(output: Tensor, retain_graph: bool):
+    """dx, and the gain's and bias's gradients as column sums, from one pass over x and the upstream gradient."""
+    xs, weight, bias = output.ancestry.parents
+    a, g = output.ancestry.arg, output.gradbox
+    x = a["x"]
+    C = x.shape[-1]
+    M = x.numels() // C
+    dx, dw, db = NDBuffer.empty(x.shape), NDBuffer.empty((C,)), NDBuffer.empty((C,))
+    handle().layernorm_bwd(x.data_ptr(), C, g.data_ptr(), weight.buffer.data_ptr(), a["mean"].data_ptr(), a["rstd"].data_ptr(),
+                           dx.data_ptr(), dw.data_ptr(), db.data_ptr(), M, C)
+    touched = []
+    for parent, grad in ((xs, dx), (weight, dw), (bias, db)):
+        if parent.requires_grad:
+            parent.update_grad(grad)
+            touched.append(parent)
+    if not retain_graph:
+        g.fill(0.0)
+    return touched
+
+
 class Sequential:
     def __init__(self, *modules):
         self.modules = list(modules)
@@ -92,7 +143,7 @@ class Sequential:
         """Names as the reference's checkpoints use them: "<idx>.weight", "<idx>.bias" (net.mojo:235-244,1102-1109)."""
         out = {}
         for i, m in enumerate(self.modules):
-            if isinstance(m, Linear):
+            if isinstance(m, (Linear, LayerNorm)):
                 out[f"{prefix}{i}.weight"] = m.weight
                 if m.bias is not None:
                     out[f"{prefix}{i}.bias"] = m.bias

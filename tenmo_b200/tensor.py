@@ -32,6 +32,10 @@ BACKWARD_VECTOR_MATMUL = 21
 BACKWARD_ADD_BROADCAST = 23
 BACKWARD_DOT = 30
 BACKWARD_CE_CLASS_INDICES_INT64 = 66
+# operators that the reference has as chains of others (or, layer norm, under a tag of its own table): values above its table
+BACKWARD_LAYER_NORM = 201
+BACKWARD_ATTENTION = 202
+BACKWARD_LINEAR_CE = 203
 
 _handles: dict[int, TenmoCuda] = {}
 _gemm_algo = _lib.ALGO_AUTO
@@ -515,6 +519,18 @@ class Backward:
             from .crossentropy import ce_class_indices_backward
 
             return ce_class_indices_backward(output, retain_graph)
+        elif code == BACKWARD_LAYER_NORM:
+            from .net import layer_norm_backward
+
+            return layer_norm_backward(output, retain_graph)
+        elif code == BACKWARD_ATTENTION:
+            from .attention import attention_backward
+
+            return attention_backward(output, retain_graph)
+        elif code == BACKWARD_LINEAR_CE:
+            from .crossentropy import linear_ce_backward
+
+            return linear_ce_backward(output, retain_graph)
         panic("Backward.invoke: unknown op code", code)
 
     @staticmethod
