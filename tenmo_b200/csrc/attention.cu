@@ -12,7 +12,7 @@
 //
 // Kernels here: one warp per row, scores 32 keys at a time (a lane is a key), the weighted sum with a lane per column.
 // No tile is filled and nothing waits on anything, so small problems finish in one launch latency per pass.
-#include "attention.cuh"
+#include "attention_tc.cuh"
 
 #include <cfloat>
 
@@ -297,6 +297,7 @@ int tenmo_attention_fwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
     p.q_lengths = q_lengths;
     p.k_lengths = k_lengths;
     TenmoDeviceGuard guard(ctx);
+    if (tenmo_attn_tc_profitable(p, false)) return tenmo_attn_tc_fwd(ctx, p);
     const int64_t grid = ((int64_t)p.B * p.H * p.Sq + ROW_WARPS - 1) / ROW_WARPS;
     TENMO_CUDA_TRY(ctx, tenmo_launch(attn_fwd_row_kernel, (unsigned)grid, ROW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, grid), p));
     TENMO_LAUNCH_CHECK(ctx, "attn_fwd_row_kernel");

@@ -1,0 +1,454 @@
+// Tensor-core attention, forward: tile images and the fused kernel.
+//
+// Kernel.  A CTA owns 128 rows of one head.  Its q rows are split into fp16 pairs (scaled per row) and kept in tensor memory as
+// the left operand; k and v come as 64-row tile images through a ring of three stages.  Per tile j:
+//   S_j = q k_j^T          left operand and accumulator in tensor memory
+//   P_j = exp2(S_j c - m)  by a warpgroup, a row per thread, written over S_j as fp16 pairs: the next left operand
+//   O_j = P_j v_j          a fresh accumulator, added to the row's registers (and rescaled) with rounding
+// Two warpgroups take the tiles alternately, each with its own running maximum, sum and output; the two are joined once at
+// the end.  So while one works on P_j the tensor core computes S_{j+1}, and no warpgroup waits for the other.  The running
+// reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.
+// One thread issues all copies and MMAs.  Up to dim 64 everything fits twice into an SM (96 KB, 256 columns): two CTAs fill each
+// other's gaps.  Up to dim 128 one CTA has the SM, with a third S buffer so that S_{j+1} need not wait for P_{j-1} v_{j-1}.
+// Bound: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
+#include "attention_tc.cuh"
+
+#include "tcgen05.cuh"
+
+namespace {
+
+constexpr int ROWS = 128;
+constexpr int T = ATTN_TILE;
+constexpr int THREADS = 288;  // two warpgroups and the issuing warp
+constexpr int STAGES = 3;
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Tile images.  A block makes one tile: 8 columns (a 16-byte chunk of each plane) per thread and step.
+// ---------------------------------------------------------------------------------------------------------------------
+template <int DP>
+__global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs jobs) {
+    constexpr int CHUNKS = DP / 8, STEPS = T * CHUNKS / 256;
+    __shared__ float largest[8];
+    const TenmoTileJob& j = jobs.job[blockIdx.y];
+    const int64_t t = blockIdx.x;
+    if (t >= (int64_t)jobs.B * j.heads * j.tiles) return;
+    const int tile = (int)(t % j.tiles);
+    const int64_t bh = t / j.tiles;
+    const int h = (int)(bh % j.heads), b = (int)(bh / j.heads);
+    const int rows = tenmo_attn_rows(j.lengths, b, j.rows) - tile * T;
+    if (rows <= 0) return;  // no kernel reads a tile behind the length
+    const float* src = j.src.ptr + b * j.src.sb + h * j.src.sh + (int64_t)tile * T * j.src.sr;
+    float x[STEPS][8];
+    float mx = 0.f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int q = threadIdx.x + s * 256, r = q / CHUNKS, d = (q % CHUNKS) * 8;
+        const float* p = src + r * j.src.sr + d;
+        if (r < rows && j.vec && d + 8 <= jobs.D) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), c = __ldg(reinterpret_cast<const float4*>(p) + 1);
+            x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
+            x[s][4] = c.x; x[s][5] = c.y; x[s][6] = c.z; x[s][7] = c.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[s][e] = r < rows && d + e < jobs.D ? __ldg(p + e) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, tc::finite_abs(x[s][e]));
+    }
+    mx = tenmo_warp_max(mx);
+    if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, largest[w]);
+    float inverse;
+    const float scale = tc::block_scale(mx, &inverse);
+    if (threadIdx.x == 0) j.inverse[t] = inverse;
+    uint8_t* img = j.img + t * (T * DP * 4);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int q = threadIdx.x + s * 256, r = q / CHUNKS, c = q % CHUNKS;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tc::split_pair(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);
+        const int at = (c >> 3) * (T * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(img + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(img + T * DP * 2 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------------------------------------------------
+struct FwdParams {
+    TenmoAttnParams a;
+    const uint8_t* k_img; const uint8_t* v_img;
+    const float* k_inv; const float* v_inv;
+    int tiles;    // tiles of a head of k
+    int q_tiles;  // 128-row tiles of a head of q
+    int q_vec, o_vec;
+    uint32_t* status;
+};
+
+template <int DP>
+struct FwdCfg {
+    static constexpr int NB = DP == 64 ? 2 : 3;     // S / P buffers
+    static constexpr int PLANE = T * DP * 2;        // bytes of one plane of a tile
+    static constexpr int STAGE = 4 * PLANE;         // k hi, k lo, v hi, v lo
+    static constexpr int Q_COLS = DP;               // hi DP/2, lo DP/2
+    static constexpr int S_COL = Q_COLS, O_COL = Q_COLS + NB * T;
+    static constexpr int TMEM = DP == 64 ? 256 : 512;
+    static constexpr int SMEM = STAGES * STAGE + 2048;
+    static_assert(O_COL + DP <= TMEM, "tensor memory");
+};
+
+template <int DP>
+__global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams p) {
+    using C = FwdCfg<DP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    float* const shared_f = reinterpret_cast<float*>(smem + STAGES * C::STAGE);  // [2][128] row statistics
+    const uint32_t bars = smem_u32(smem + STAGES * C::STAGE + 1024);
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto s_full = [&](int w) { return bars + 8u * (3 + w); };
+    auto p_full = [&](int w) { return bars + 8u * (5 + w); };
+    auto o_full = [&](int w) { return bars + 8u * (7 + w); };
+    const uint32_t o_free = bars + 8u * 9;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * C::STAGE + 1024 + 128);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const TenmoAttnParams& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the longest rows of a causal head first: the last tiles have the most keys
+    const int q_tile = p.q_tiles - 1 - (int)(blockIdx.x / ((unsigned)a.B * a.H));
+    const int bh = (int)(blockIdx.x % ((unsigned)a.B * a.H));
+    const int h = bh % a.H, b = bh / a.H, kvh = h / (a.H / a.Hkv);
+    const int q_rows = tenmo_attn_rows(a.q_lengths, b, a.Sq), keys = tenmo_attn_rows(a.k_lengths, b, a.Sk);
+    // keys that the last row of the tile that takes part sees
+    const int last = min(q_rows, (q_tile + 1) * ROWS) - 1;
+    int seen = last >= q_tile * ROWS ? keys : 0;
+    if (a.causal) seen = min(seen, max(0, last + a.Sk - a.Sq + 1));
+    const int n_tiles = (seen + T - 1) / T;
+    const int64_t tile0 = ((int64_t)b * a.Hkv + kvh) * p.tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1);
+        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
+        mbar_init(o_free, 4);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) tc::alloc(tmem_slot, C::TMEM);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    auto load = [&](int j) {  // one thread
+        const uint32_t dst = smem_u32(smem) + (j % STAGES) * C::STAGE, bar = full(j % STAGES);
+        mbar_expect_tx(bar, C::STAGE);
+        tc::bulk_load(dst, p.k_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
+        tc::bulk_load(dst + 2 * C::PLANE, p.v_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
+    };
+    int loaded = 0;
+    if (threadIdx.x == 256)
+        for (; loaded < min(n_tiles, STAGES); ++loaded) load(loaded);
+
+    // ---- q into tensor memory: warpgroup w splits columns [w DP/2, (w + 1) DP/2) of its thread's row ----
+    const int wg = warp >> 2, row = threadIdx.x & 127;
+    const int64_t i = (int64_t)q_tile * ROWS + row;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    float q_inv = 1.f;
+    if (warp < 8) {
+        constexpr int W = DP / 2;
+        float x[W];
+        const float* src = a.q.ptr + b * a.q.sb + h * a.q.sh + i * a.q.sr;
+        const bool in = i < q_rows;
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < W; e += 4) {
+            const int d = wg * W + e;
+            if (in && p.q_vec && d + 4 <= a.D) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(src + d));
+                x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[e + u] = in && d + u < a.D ? __ldg(src + d + u) : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx = fmaxf(mx, tc::finite_abs(x[e + u]));
+        }
+        shared_f[wg * 128 + row] = mx;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        mx = fmaxf(mx, shared_f[(wg ^ 1) * 128 + row]);
+        float scale = tc::block_scale(mx, &q_inv);
+        if (a.scale < 0.f) scale = -scale;  // the sign goes with q: the factor of the scores is then never negative
+#pragma unroll
+        for (int g = 0; g < W / 32; ++g) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) tc::split_pair(x[32 * g + 2 * e] * scale, x[32 * g + 2 * e + 1] * scale, hi[e], lo[e]);
+            const uint32_t col = (uint32_t)(wg * (W / 2) + 16 * g);
+            tc::st16(lane_base + col, hi);
+            tc::st16(lane_base + DP / 2 + col, lo);
+        }
+        tc::st_wait();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+
+    float m = -INFINITY, l = 0.f, o[DP];
+#pragma unroll
+    for (int d = 0; d < DP; ++d) o[d] = 0.f;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_O = tc::idesc_f16(DP, true);
+            bool ok = true;
+            auto wait = [&](uint32_t bar, int phase) { ok = ok && mbar_wait(bar, (uint32_t)phase & 1u, abort_flag); };
+            auto scores = [&](int j) {
+                wait(full(j % STAGES), j / STAGES);
+                if (!ok) return;
+                tc::fence_after();
+                const uint32_t hi = smem_u32(smem) + (j % STAGES) * C::STAGE, lo = hi + C::PLANE;
+                const uint32_t d = tmem + C::S_COL + (uint32_t)(j % C::NB) * T;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + DP / 2 + 8 * k, tc::desc_k(hi, T, k), ID_S, k > 0);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(lo, T, k), ID_S, true);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(hi, T, k), ID_S, true);
+                tc::commit(s_full(j & 1));
+            };
+            if (n_tiles > 0) scores(0);
+            for (int j = 0; ok && j < n_tiles; ++j) {
+                if (j + 1 < n_tiles) {
+                    // the buffer of S_{j+1} held P_{j+1-NB}: with three buffers its product is known to be done (its output was read)
+                    if (C::NB == 2 && j >= 1) wait(o_full((j - 1) & 1), (j - 1) >> 1);
+                    if (ok) scores(j + 1);
+                }
+                wait(p_full(j & 1), j >> 1);
+                if (j >= 1) wait(o_free, j - 1);
+                if (!ok) break;
+                tc::fence_after();
+                const uint32_t hi = smem_u32(smem) + (j % STAGES) * C::STAGE + 2 * C::PLANE, lo = hi + C::PLANE;
+                const uint32_t pr = tmem + C::S_COL + (uint32_t)(j % C::NB) * T, d = tmem + C::O_COL;
+                // keys 16 k ..: columns 32 (k / 2) + 8 (k & 1) of the pair chunk, lo 16 columns further
+#pragma unroll
+                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, pr + 32 * (k >> 1) + 16 + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_O, k > 0);
+#pragma unroll
+                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, pr + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(lo, T, k), ID_O, true);
+#pragma unroll
+                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, pr + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_O, true);
+                tc::commit(o_full(j & 1));
+                // tile j - 1 has been read by both of its products (o_free above): its stage takes tile j + 2
+                if (j >= 1 && j + 2 < n_tiles) load(loaded++);
+            }
+            // Every copy has landed before shared memory is given back, and every MMA is done before tensor memory is: in
+            // order, the readers of O have seen to both; after a wait that ran out, wait again (bounded) here.
+            if (!ok) {
+                const uint32_t drain = bars + 8u * 10;
+                mbar_init(drain, 1);
+                tc::commit(drain);
+                int never = 0;
+                mbar_wait(drain, 0, &never);
+                for (int t = max(0, loaded - STAGES); t < loaded; ++t) mbar_wait(full(t % STAGES), (uint32_t)(t / STAGES) & 1u, &never);
+            }
+        }
+    } else {
+        const float c_row = fabsf(a.scale_log2) * q_inv;
+        int n_row = i < q_rows ? keys : 0;
+        if (a.causal) n_row = min(n_row, (int)max((int64_t)0, i + a.Sk - a.Sq + 1));
+        bool ok = true;
+        for (int j = wg; j < n_tiles; j += 2) {
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full(wg), (uint32_t)(j >> 1) & 1u, abort_flag));
+            if (!ok) break;
+            tc::fence_after();
+            const float c = c_row * __ldg(p.k_inv + tile0 + j), v_inv = __ldg(p.v_inv + tile0 + j);
+            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T;
+            const int lim = n_row - j * T;
+            const bool whole = __all_sync(0xffffffffu, lim >= T);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < T / 32; ++g) {
+                float s[32];
+                tc::ld32(s_addr + 32 * g, s);
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e] = 32 * g + e < lim ? s[e] : -INFINITY;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
+            }
+            const float m_new = mx == -INFINITY ? m : fmaxf(m, ceilf(mx * c));
+            const float shrink = m == -INFINITY ? 0.f : tc::ex2(m - m_new);
+            m = m_new;
+            // p = 2^15 exp2(s c - m): the factor 2^15 brings p into fp16's range and divides out with l
+            const float base = m == -INFINITY ? 0.f : 15.f - m;
+            const uint64_t c2 = tc::pack2(c, c), b2 = tc::pack2(base, base);
+            uint64_t sum2 = 0;
+#pragma unroll
+            for (int g = 0; g < T / 32; ++g) {
+                float s[32];
+                tc::ld32(s_addr + 32 * g, s);
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float x, y;
+                    tc::unpack2(tc::fma2(tc::pack2(s[2 * e], s[2 * e + 1]), c2, b2), x, y);
+                    x = tc::ex2(x);
+                    y = tc::ex2(y);
+                    if (!whole) {
+                        x = 32 * g + 2 * e < lim ? x : 0.f;
+                        y = 32 * g + 2 * e + 1 < lim ? y : 0.f;
+                    }
+                    sum2 = tc::add2(sum2, tc::pack2(x, y));
+                    tc::split_pair(x, y, hi[e], lo[e]);
+                }
+                tc::st16(s_addr + 32 * g, hi);
+                tc::st16(s_addr + 32 * g + 16, lo);
+            }
+            tc::st_wait();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(wg));
+            float x, y;
+            tc::unpack2(sum2, x, y);
+            l = fmaf(l, shrink, x + y);
+            ok = __all_sync(0xffffffffu, mbar_wait(o_full(wg), (uint32_t)(j >> 1) & 1u, abort_flag));
+            if (!ok) break;
+            tc::fence_after();
+            const uint64_t sh2 = tc::pack2(shrink, shrink), vi2 = tc::pack2(v_inv, v_inv);
+#pragma unroll
+            for (int g = 0; g < DP / 32; ++g) {
+                float t[32];
+                tc::ld32(lane_base + C::O_COL + 32 * g, t);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const uint64_t add = tc::mul2(tc::pack2(t[e], t[e + 1]), vi2);
+                    tc::unpack2(tc::fma2(tc::pack2(o[32 * g + e], o[32 * g + e + 1]), sh2, add), o[32 * g + e], o[32 * g + e + 1]);
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+        }
+    }
+    __syncthreads();
+
+    // ---- join the two warpgroups: 16-byte chunk q of row r lies at chunk q ^ (r & 7) of the buffer (the stages are free) ----
+    float* const buf = reinterpret_cast<float*>(smem);
+    float* const ms = shared_f;  // m and l of the second warpgroup
+    if (warp >= 4 && warp < 8) {
+        ms[row] = m;
+        ms[128 + row] = l;
+#pragma unroll
+        for (int d = 0; d < DP; d += 4)
+            *reinterpret_cast<float4*>(buf + row * DP + (((d >> 2) ^ (row & 7)) << 2)) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+    }
+    __syncthreads();
+    if (warp < 4) {
+        const float m1 = ms[row], l1 = ms[128 + row], top = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.f : tc::ex2(m - top), f1 = m1 == -INFINITY ? 0.f : tc::ex2(m1 - top);
+        const float sum = l * f0 + l1 * f1;
+        // rows without keys: sum 0, output 0 (0 * 0); a NaN in the sum reaches the output
+        const float inv = sum == 0.f ? 0.f : 1.f / sum, g0 = f0 * inv, g1 = f1 * inv;
+#pragma unroll
+        for (int d = 0; d < DP; d += 4) {
+            float4* at = reinterpret_cast<float4*>(buf + row * DP + (((d >> 2) ^ (row & 7)) << 2));
+            const float4 x = *at;
+            *at = make_float4(o[d] * g0 + x.x * g1, o[d + 1] * g0 + x.y * g1, o[d + 2] * g0 + x.z * g1, o[d + 3] * g0 + x.w * g1);
+        }
+        if (a.stats && i < a.Sq) {
+            float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + i) * 2;
+            st[0] = top;
+            st[1] = sum * 3.0517578125e-5f;  // 2^-15
+        }
+    }
+    __syncthreads();
+    const int rows_here = min(ROWS, a.Sq - q_tile * ROWS);
+    float* out = a.o.ptr + b * a.o.sb + h * a.o.sh + (int64_t)q_tile * ROWS * a.o.sr;
+    for (int e = threadIdx.x; e < rows_here * (DP / 4); e += THREADS) {
+        const int r = e / (DP / 4), q = e % (DP / 4), d = 4 * q;
+        if (d >= a.D) continue;
+        const float4 x = *reinterpret_cast<const float4*>(buf + r * DP + ((q ^ (r & 7)) << 2));
+        float* dst = out + r * a.o.sr + d;
+        if (p.o_vec) {
+            *reinterpret_cast<float4*>(dst) = x;
+        } else {
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            for (int u = 0; u < 4 && d + u < a.D; ++u) dst[u] = v[u];
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, TENMO_DEV_TIMEOUT);
+    if (warp == 8) {
+        tc::fence_after();
+        tc::dealloc(tmem, C::TMEM);
+    }
+}
+
+size_t align_up(size_t n) { return (n + 1023) & ~(size_t)1023; }
+
+}  // namespace
+
+bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D) {
+    return D % 4 == 0 && v.sb % 4 == 0 && v.sh % 4 == 0 && v.sr % 4 == 0 && ((uintptr_t)v.ptr & 15u) == 0;
+}
+
+int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp) {
+    int64_t most = 0;
+    for (int c = 0; c < count; ++c) {
+        const int64_t n = (int64_t)jobs.B * jobs.job[c].heads * jobs.job[c].tiles;
+        if (n > most) most = n;
+    }
+    const dim3 grid((unsigned)most, (unsigned)count);
+    if (dp == 64) attn_tiles_kernel<64><<<grid, 256, 0, ctx->stream>>>(jobs);
+    else attn_tiles_kernel<128><<<grid, 256, 0, ctx->stream>>>(jobs);
+    TENMO_LAUNCH_CHECK(ctx, "attn_tiles_kernel");
+    return TENMO_OK;
+}
+
+// The tensor-core kernels work on tiles of 128 rows x 64 keys whatever the sizes; below a good part of a tile, and where the
+// whole call is a few launches' latency, the row kernels are faster.
+bool tenmo_attn_tc_profitable(const TenmoAttnParams& p, bool backward) {
+    (void)backward;
+    return p.Sq >= 64 && p.Sk >= 64 && (int64_t)p.Sq * p.Sk >= 128 * 128;
+}
+
+int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
+    const int dp = tenmo_attn_padded(a.D);
+    FwdParams p = {};
+    p.a = a;
+    p.tiles = (a.Sk + T - 1) / T;
+    p.q_tiles = (a.Sq + ROWS - 1) / ROWS;
+    p.q_vec = tenmo_attn_row_vec(a.q, a.D);
+    p.o_vec = tenmo_attn_row_vec(a.o, a.D);
+    p.status = ctx->dev_status;
+    const int64_t n = (int64_t)a.B * a.Hkv * p.tiles;
+    const size_t img = align_up((size_t)n * T * dp * 4), inv = align_up((size_t)n * sizeof(float));
+    void* ws = nullptr;
+    int st = tenmo_op_workspace(ctx, 2 * (img + inv), &ws);
+    if (st != TENMO_OK) return st;
+    uint8_t* w = (uint8_t*)ws;
+    p.k_img = w;
+    p.v_img = w + img;
+    p.k_inv = (float*)(w + 2 * img);
+    p.v_inv = (float*)(w + 2 * img + inv);
+    TenmoTileJobs jobs = {};
+    jobs.B = a.B;
+    jobs.D = a.D;
+    jobs.job[0] = TenmoTileJob{a.k, a.k_lengths, w, (float*)p.k_inv, a.Hkv, a.Sk, p.tiles, tenmo_attn_row_vec(a.k, a.D)};
+    jobs.job[1] = TenmoTileJob{a.v, a.k_lengths, w + img, (float*)p.v_inv, a.Hkv, a.Sk, p.tiles, tenmo_attn_row_vec(a.v, a.D)};
+    if ((st = tenmo_attn_make_tiles(ctx, jobs, 2, dp)) != TENMO_OK) return st;
+    const unsigned grid = (unsigned)((int64_t)a.B * a.H * p.q_tiles);
+    if (dp == 64) {
+        TENMO_CUDA_TRY(ctx, cudaFuncSetAttribute(attn_fwd_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdCfg<64>::SMEM));
+        attn_fwd_tc_kernel<64><<<grid, THREADS, FwdCfg<64>::SMEM, ctx->stream>>>(p);
+    } else {
+        TENMO_CUDA_TRY(ctx, cudaFuncSetAttribute(attn_fwd_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdCfg<128>::SMEM));
+        attn_fwd_tc_kernel<128><<<grid, THREADS, FwdCfg<128>::SMEM, ctx->stream>>>(p);
+    }
+    TENMO_LAUNCH_CHECK(ctx, "attn_fwd_tc_kernel");
+    return TENMO_OK;
+}

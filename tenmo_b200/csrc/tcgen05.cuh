@@ -1,0 +1,165 @@
+// Fifth-generation tensor core pieces shared by the fp16-pair kernels: fp32 products on fp16 tensor cores.
+//
+// Arithmetic.  A block of an fp32 operand is scaled by a power of two 2^e (its largest finite entry comes to lie in
+// [2^14, 2^15)) and written as hi + lo, two fp16 numbers: hi = fp16(x 2^e), lo = fp16(x 2^e - hi).  That keeps 22 bits of an
+// entry down to 2^-18 of the block's largest one and an absolute 2^-40 of it below.  A product of two such operands is
+// lo.hi + hi.lo + hi.hi, three tcgen05.mma of kind::f16 into one fp32 accumulator (the dropped lo.lo is below 2^-22 of the
+// term); the powers of two come off in fp32, exactly.  fp16 runs at twice the rate of TF32 and its planes are half as
+// large, which is why these kernels do not use the three TF32 products of the dense GEMM.
+// The tensor core adds into its accumulator with truncation, so a chain is kept short (one tile) and tiles are added in
+// registers with rounding; within a chain the two small products go first, while the accumulator is small.
+//
+// Tile image.  A tile of R rows x DP columns (DP a multiple of 64) is stored as the hi plane and then the lo plane, each as
+// DP / 64 panels of R rows x 128 bytes, 16-byte chunk c of row r at chunk c ^ (r & 7): the 128-byte swizzle the tensor core
+// reads.  The image is made once in global memory, so one plain bulk copy brings a tile in and no tensor map is needed.
+// The same image serves a product over the columns (rows are M or N, "K-major") and one over the rows ("MN-major").
+#pragma once
+#include <cuda_fp16.h>
+
+#include "op_util.cuh"
+#include "tma_util.cuh"
+
+namespace tc {
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// generic-proxy writes to shared memory become visible to the tensor core and the copy engine
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void alloc(uint32_t* slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void dealloc(uint32_t base, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+// arrives on `bar` when all MMAs issued so far by this thread are done
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[tmem] (+)= A[smem] . B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] . B[smem]: A holds row r in lane r, two fp16 per 32-bit column
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// instruction descriptor: fp32 accumulator, fp16 operands, 128 rows
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+// shared-memory operand: 128-byte swizzle, descriptor version 1; offsets in bytes
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// 16 columns from `16 * step` on of a K-major panel set of `rows` rows (8-row groups 1024 bytes apart)
+__device__ __forceinline__ uint64_t desc_k(uint32_t plane, int rows, int step) {
+    return desc(plane + (uint32_t)(step >> 2) * (uint32_t)(rows * 128) + (uint32_t)(step & 3) * 32u, 16u, 1024u);
+}
+// 16 rows from `16 * step` on, all columns: panels (64 columns) `rows * 128` bytes apart, 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_mn(uint32_t plane, int rows, int step) {
+    return desc(plane + (uint32_t)step * 2048u, (uint32_t)(rows * 128), 1024u);
+}
+
+// 32 / 16 consecutive columns of this warp's 32 lanes; the wait is part of the instruction, so nothing reads too early
+__device__ __forceinline__ void ld32(uint32_t addr, float (&f)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a contiguous copy from global memory that completes on an mbarrier (16-byte aligned, size a multiple of 16)
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// packed pairs: two round-to-nearest operations per instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// fp16 pairs (first value in the low half)
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+// hi / lo of two values.  hi is the value cut to 11 significant bits (a logical AND instead of a conversion back), which fp16
+// holds exactly down to 2^-14; below that hi is rounded to the fp16 grid and the pair is good to 2^-25 absolute, the same floor
+// that lo has.  The cut leaves lo at most 13 bits, of which fp16 keeps 11: 22 bits together.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+    hi = half_pair(ah, bh);
+    lo = half_pair(a - ah, b - bh);
+}
+
+// 2^e that brings `largest` (finite, >= 0) into [2^14, 2^15), and its inverse.  0 and what is too small to be brought there
+// without leaving fp32's range take the nearest factor that has an inverse.
+__device__ __forceinline__ float block_scale(float largest, float* inverse) {
+    const int ex = (int)((__float_as_uint(largest) >> 23) & 255u) - 127;
+    const int e = largest > 0.f ? min(14 - ex, 120) : 0;
+    *inverse = __uint_as_float((uint32_t)(127 - e) << 23);
+    return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+// |x| for the search of the largest entry: infinities and NaN do not count
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a <= 3.402823466e38f ? a : 0.f;
+}
+
+}  // namespace tc
