@@ -13,8 +13,6 @@
 // Bound: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
 #include "attention_tc.cuh"
 
-#include "tcgen05.cuh"
-
 namespace {
 
 constexpr int ROWS = 128;
@@ -25,6 +23,58 @@ constexpr int STAGES = 3;
 // ---------------------------------------------------------------------------------------------------------------------
 // Tile images.  A block makes one tile: 8 columns (a 16-byte chunk of each plane) per thread and step.
 // ---------------------------------------------------------------------------------------------------------------------
+// delta_i = sum_d go o and the saved statistics of a tile's rows (x: this thread's columns of go)
+template <int DP>
+__device__ __forceinline__ void attn_row_numbers(const TenmoTileJobs& jobs, const TenmoTileJob& j, int64_t t, int b, int h, int tile, int rows,
+                                                 const float (&x)[T * (DP / 8) / 256][8]) {
+    constexpr int CHUNKS = DP / 8, STEPS = T * CHUNKS / 256;
+    __shared__ float delta[T], most[2][2];
+    const float* src = j.o.ptr + b * j.o.sb + h * j.o.sh + (int64_t)tile * T * j.o.sr;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int q = threadIdx.x + s * 256, r = q / CHUNKS, d = (q % CHUNKS) * 8;
+        const float* p = src + r * j.o.sr + d;
+        float sum = 0.f;
+        if (r < rows && j.o_vec && d + 8 <= jobs.D) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), c = __ldg(reinterpret_cast<const float4*>(p) + 1);
+            sum = (x[s][0] * a.x + x[s][1] * a.y) + (x[s][2] * a.z + x[s][3] * a.w) + (x[s][4] * c.x + x[s][5] * c.y) + (x[s][6] * c.z + x[s][7] * c.w);
+        } else if (r < rows) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (d + e < jobs.D) sum = fmaf(x[s][e], __ldg(p + e), sum);
+        }
+#pragma unroll
+        for (int w = CHUNKS / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (q % CHUNKS == 0) delta[r] = sum;
+    }
+    __syncthreads();
+    const int r = threadIdx.x;
+    float m = INFINITY, il = 0.f, dl = 0.f;
+    if (r < T) {
+        if (r < rows) {
+            const float* st = j.stats + (((int64_t)b * j.heads + h) * j.rows + (int64_t)tile * T + r) * 2;
+            if (st[1] != 0.f) {
+                m = st[0];
+                il = 1.f / st[1];
+                dl = delta[r];
+            }
+        }
+        const float a = tenmo_warp_max(tc::finite_abs(il)), c = tenmo_warp_max(tc::finite_abs(dl));
+        if ((r & 31) == 0) { most[0][r >> 5] = a; most[1][r >> 5] = c; }
+    }
+    __syncthreads();
+    if (r < T) {
+        const float il_max = fmaxf(most[0][0], most[0][1]);
+        const float ps = il_max > 0.f ? 32768.f * tc::pow2_below_inverse(il_max) : 1.f;
+        float* info = j.info + t * ATTN_INFO;
+        info[r] = m;
+        info[T + r] = il * ps;
+        info[2 * T + r] = dl;
+        if (r == 0) { info[3 * T] = ps; info[3 * T + 1] = fmaxf(most[1][0], most[1][1]); }
+    }
+    __syncthreads();
+}
+
 template <int DP>
 __global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs jobs) {
     constexpr int CHUNKS = DP / 8, STEPS = T * CHUNKS / 256;
@@ -55,6 +105,7 @@ __global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs job
 #pragma unroll
         for (int e = 0; e < 8; ++e) mx = fmaxf(mx, tc::finite_abs(x[s][e]));
     }
+    if (j.o.ptr) attn_row_numbers<DP>(jobs, j, t, b, h, tile, rows, x);
     mx = tenmo_warp_max(mx);
     if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = mx;
     __syncthreads();
@@ -157,41 +208,9 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(
     const int64_t i = (int64_t)q_tile * ROWS + row;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float q_inv = 1.f;
-    if (warp < 8) {
-        constexpr int W = DP / 2;
-        float x[W];
-        const float* src = a.q.ptr + b * a.q.sb + h * a.q.sh + i * a.q.sr;
-        const bool in = i < q_rows;
-        float mx = 0.f;
-#pragma unroll
-        for (int e = 0; e < W; e += 4) {
-            const int d = wg * W + e;
-            if (in && p.q_vec && d + 4 <= a.D) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(src + d));
-                x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) x[e + u] = in && d + u < a.D ? __ldg(src + d + u) : 0.f;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) mx = fmaxf(mx, tc::finite_abs(x[e + u]));
-        }
-        shared_f[wg * 128 + row] = mx;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        mx = fmaxf(mx, shared_f[(wg ^ 1) * 128 + row]);
-        float scale = tc::block_scale(mx, &q_inv);
-        if (a.scale < 0.f) scale = -scale;  // the sign goes with q: the factor of the scores is then never negative
-#pragma unroll
-        for (int g = 0; g < W / 32; ++g) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) tc::split_pair(x[32 * g + 2 * e] * scale, x[32 * g + 2 * e + 1] * scale, hi[e], lo[e]);
-            const uint32_t col = (uint32_t)(wg * (W / 2) + 16 * g);
-            tc::st16(lane_base + col, hi);
-            tc::st16(lane_base + DP / 2 + col, lo);
-        }
-        tc::st_wait();
-    }
+    if (warp < 8)  // the sign of the scale goes with q: the factor of the scores is then never negative
+        q_inv = tenmo_attn_stationary<DP, false>(a.q.ptr + b * a.q.sb + h * a.q.sh + i * a.q.sr, i < q_rows, p.q_vec, a.D, a.scale < 0.f,
+                                                 wg, row, lane_base, nullptr, shared_f);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();

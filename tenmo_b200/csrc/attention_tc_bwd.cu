@@ -1,0 +1,561 @@
+// Tensor-core attention, backward: one kernel template for dq and for dk / dv.
+//
+// Two passes recompute the scores, one with the rows of q stationary and one with the keys: seven products instead of the five of
+// a single pass, but no gradient is added by atomics (results repeat bit for bit) and no score tile crosses shared memory.
+//   dq pass    X1 = q, X2 = go (128 rows, tensor memory), tiles of Y1 = k, Y2 = v:   S = X1 Y1^T, dP = X2 Y2^T,
+//              dS = exp2(S c - m) (dP - delta),  dq += dS Y1
+//   dkv pass   X1 = k, X2 = v (128 keys), tiles of Y1 = q, Y2 = go:  the same transposed, and  dv += P^T Y2,  dk += dS^T Y1
+// P and dS are written as fp16 pairs over S and dP in tensor memory, where they are the next products' left operand; the tile
+// images serve both as the right operand over the columns (S, dP) and over the rows (gradients).  The gradients of a tile are
+// fresh accumulators that the warpgroups add to their registers with rounding.
+// fp16 range of dS: |dP - delta| is bounded by the operands' scales (dim * 2^30 times the two inverse scales) and by the largest
+// |delta|; a power of two from that bound brings dS to at most 2^15, exactly taken back when the tile is added.
+// Two warpgroups share every tile (32 columns of S and half of the gradient's columns each); one thread issues copies and MMAs.
+// Up to dim 64 S and dP have two buffers: the scores of tile j + 1 are computed while tile j is worked on.  Up to dim 128 there
+// is one of each, and v of the dkv pass moves to shared memory; the products still follow each other without a gap because
+// each has one product of another kind between itself and what it waits for.
+// Shared key / value heads: the dkv pass works per query head into the workspace and a last kernel adds the heads of a group
+// in order (per group it would leave most SMs idle behind the longest).
+// Bound: tensor pipe, 3 * 14 * rows * keys * dim flop.
+#include "attention_tc.cuh"
+
+namespace {
+
+constexpr int ROWS = 128;
+constexpr int T = ATTN_TILE;
+constexpr int THREADS = 384;  // two warpgroups and the issuing warp's (whose registers go to the other two)
+
+struct BwdParams {
+    TenmoAttnParams a;
+    const uint8_t* y1_img; const uint8_t* y2_img;
+    const float* y1_inv; const float* y2_inv;
+    const float* info;   // row numbers per 64-row tile of q
+    int tiles;           // tiles of a head of Y
+    int q_info_tiles;    // 64-row tiles of a head of q
+    int x_tiles;         // 128-row tiles of a head of X
+    TenmoHeadsView x1, x2, out1, out2;  // out1: dq or dk, out2: dv
+    int x1_vec, x2_vec, out1_vec, out2_vec;
+    float beta;
+    uint32_t* status;
+};
+
+template <int DP, bool DKV>
+struct BwdCfg {
+    static constexpr int NB = DP == 64 ? 2 : 1;
+    static constexpr bool X2S = DKV && DP == 128;  // X2 in shared memory
+    static constexpr int STAGES = X2S ? 2 : 3;
+    static constexpr int PLANE = T * DP * 2;
+    static constexpr int STAGE = 4 * PLANE + (DKV ? 1024 : 0);  // Y1 hi, lo, Y2 hi, lo, row numbers
+    static constexpr int X2_BYTES = X2S ? ROWS * DP * 4 : 0;
+    static constexpr int X2_COL = DP;
+    static constexpr int S_COL = X2S ? DP : 2 * DP, P_COL = S_COL + NB * T, A1_COL = P_COL + NB * T, A2_COL = A1_COL + DP;
+    static constexpr int TMEM = 512;
+    static_assert(A1_COL + (DKV ? 2 : 1) * DP <= TMEM, "tensor memory");
+    static constexpr int TILES = STAGES * STAGE + X2_BYTES;
+    static constexpr int SMEM = TILES + 2048;
+    static_assert(STAGES * STAGE >= ROWS * DP * 4, "the output goes through the stages");
+};
+
+template <int DP, bool DKV>
+__global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_constant__ BwdParams p) {
+    using C = BwdCfg<DP, DKV>;
+    constexpr int NB = C::NB, W = DP / 2;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* const x2_plane = smem + C::STAGES * C::STAGE;
+    float* const exchange = reinterpret_cast<float*>(smem + C::TILES);
+    const uint32_t bars = smem_u32(smem + C::TILES + 1024);
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto s_full = [&](int j) { return bars + 8u * (3 + (j & 1)); };
+    auto d_full = [&](int j) { return bars + 8u * (5 + (j & 1)); };
+    // a warp may be a tile ahead of another one: what the eight warps arrive on has a barrier for even and one for odd tiles
+    auto p_full = [&](int j) { return bars + 8u * (7 + (j & 1)); };
+    auto ds_full = [&](int j) { return bars + 8u * (9 + (j & 1)); };
+    const uint32_t s_read = bars + 8u * 11, pv_done = bars + 8u * 12;
+    const uint32_t acc_full = bars + 8u * 13, acc_free = bars + 8u * 14, drain = bars + 8u * 15;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 1024 + 128);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const TenmoAttnParams& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2, row = threadIdx.x & 127;
+    const unsigned heads = (unsigned)a.B * a.H;
+    // causal: the last rows of q see the most keys, the first keys are seen by the most rows; those blocks start first
+    const int x_tile = DKV ? (int)(blockIdx.x / heads) : p.x_tiles - 1 - (int)(blockIdx.x / heads);
+    const int bh = (int)(blockIdx.x % heads);
+    const int h = bh % a.H, b = bh / a.H, kvh = h / (a.H / a.Hkv);
+    const int q_rows = tenmo_attn_rows(a.q_lengths, b, a.Sq), keys = tenmo_attn_rows(a.k_lengths, b, a.Sk);
+    const int off = a.Sk - a.Sq;  // causal: key j is visible to row i when j <= i + off
+    const int x_rows = DKV ? keys : q_rows;
+    const int64_t i = (int64_t)x_tile * ROWS + row;  // this thread's row of X
+    // tiles of Y that this block needs: [first, first + n)
+    int first = 0, n = 0;
+    const int top = min(x_rows, (x_tile + 1) * ROWS) - 1;  // last row of X that takes part
+    if (top >= x_tile * ROWS) {
+        if (DKV) {
+            if (a.causal) first = max(0, x_tile * ROWS - off) / T;
+            n = max(0, (q_rows + T - 1) / T - first);
+        } else {
+            int seen = keys;
+            if (a.causal) seen = min(seen, max(0, top + off + 1));
+            n = (seen + T - 1) / T;
+        }
+    }
+    const int yh = DKV ? h : kvh, y_heads = DKV ? a.H : a.Hkv;
+    const int64_t tile0 = ((int64_t)b * y_heads + yh) * p.tiles + first;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 3; ++s) mbar_init(full(s), 1);
+        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(d_full(w), 1); mbar_init(p_full(w), 8); mbar_init(ds_full(w), 8); }
+        mbar_init(s_read, 8);
+        mbar_init(pv_done, 1);
+        mbar_init(acc_full, 1);
+        mbar_init(acc_free, 8);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) tc::alloc(tmem_slot, C::TMEM);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+
+    auto load = [&](int j) {  // one thread
+        const uint32_t dst = smem_u32(smem) + (j % C::STAGES) * C::STAGE, bar = full(j % C::STAGES);
+        mbar_expect_tx(bar, 4 * C::PLANE + (DKV ? 1024u : 0u));
+        tc::bulk_load(dst, p.y1_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
+        tc::bulk_load(dst + 2 * C::PLANE, p.y2_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
+        if (DKV) tc::bulk_load(dst + 4 * C::PLANE, p.info + (tile0 + j) * ATTN_INFO, 1024, bar);
+    };
+    int loaded = 0;
+    if (threadIdx.x == 256)
+        for (; loaded < min(n, C::STAGES); ++loaded) load(loaded);
+
+    float x1_inv = 1.f, x2_inv = 1.f;
+    if (warp < 8) {
+        const int xh = DKV ? kvh : h;
+        x1_inv = tenmo_attn_stationary<DP, false>(p.x1.ptr + b * p.x1.sb + xh * p.x1.sh + i * p.x1.sr, i < x_rows, p.x1_vec, a.D,
+                                                  a.scale < 0.f, wg, row, lane_base, nullptr, exchange);
+        x2_inv = tenmo_attn_stationary<DP, C::X2S>(p.x2.ptr + b * p.x2.sb + xh * p.x2.sh + i * p.x2.sr, i < x_rows, p.x2_vec, a.D, false,
+                                                   wg, row, lane_base + C::X2_COL, x2_plane, exchange);
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+
+    if (warp >= 8) {
+        tc::regs_down<40>();
+        if (threadIdx.x == 256) {
+            constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_G = tc::idesc_f16(DP, true);
+            bool ok = true;
+            auto wait = [&](uint32_t bar, int phase) { ok = ok && mbar_wait(bar, (uint32_t)phase & 1u, abort_flag); };
+            auto y1 = [&](int j) { return smem_u32(smem) + (j % C::STAGES) * C::STAGE; };
+            auto scores = [&](int j) {  // S_j
+                wait(full(j % C::STAGES), j / C::STAGES);
+                if (!ok) return;
+                tc::fence_after();
+                const uint32_t hi = y1(j), lo = hi + C::PLANE, d = tmem + C::S_COL + (uint32_t)(j % NB) * T;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + DP / 2 + 8 * k, tc::desc_k(hi, T, k), ID_S, k > 0);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(lo, T, k), ID_S, true);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(hi, T, k), ID_S, true);
+                tc::commit(s_full(j));
+            };
+            auto grads = [&](int j) {  // dP_j (its tile has arrived: S_j was issued before)
+                if (!ok) return;
+                const uint32_t hi = y1(j) + 2 * C::PLANE, lo = hi + C::PLANE, d = tmem + C::P_COL + (uint32_t)(j % NB) * T;
+                if (C::X2S) {
+                    const uint32_t xh = smem_u32(x2_plane), xl = xh + ROWS * DP * 2;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) tc::mma_ss(d, tc::desc_k(xl, ROWS, k), tc::desc_k(hi, T, k), ID_S, k > 0);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) tc::mma_ss(d, tc::desc_k(xh, ROWS, k), tc::desc_k(lo, T, k), ID_S, true);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) tc::mma_ss(d, tc::desc_k(xh, ROWS, k), tc::desc_k(hi, T, k), ID_S, true);
+                } else {
+                    const uint32_t x = tmem + C::X2_COL;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, x + DP / 2 + 8 * k, tc::desc_k(hi, T, k), ID_S, k > 0);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, x + 8 * k, tc::desc_k(lo, T, k), ID_S, true);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, x + 8 * k, tc::desc_k(hi, T, k), ID_S, true);
+                }
+                tc::commit(d_full(j));
+            };
+            // D += A Y over the rows of the tile; A: fp16 pairs over a 64-column buffer, keys 16 k .. in columns 32 (k / 2) + 8 (k & 1)
+            auto times_y = [&](uint32_t d, uint32_t x, uint32_t hi) {
+                const uint32_t lo = hi + C::PLANE;
+#pragma unroll
+                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, x + 32 * (k >> 1) + 16 + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_G, k > 0);
+#pragma unroll
+                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, x + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(lo, T, k), ID_G, true);
+#pragma unroll
+                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, x + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_G, true);
+            };
+            if (n > 0) {
+                scores(0);
+                grads(0);
+            }
+            for (int j = 0; ok && j < n; ++j) {
+                const uint32_t s = tmem + C::S_COL + (uint32_t)(j % NB) * T, ds = tmem + C::P_COL + (uint32_t)(j % NB) * T;
+                const bool more = j + 1 < n;
+                if (NB == 2) {
+                    // the buffers of tile j + 1 were last read by the products of tile j - 1
+                    if (j >= 1) wait(acc_full, j - 1);
+                    if (more) { scores(j + 1); grads(j + 1); }
+                } else if (!DKV && more) {
+                    wait(s_read, j);  // S_j is in registers, nothing is written back
+                    scores(j + 1);
+                }
+                if (DKV) {
+                    wait(p_full(j), j >> 1);
+                    if (j >= 1) wait(acc_free, j - 1);
+                    if (!ok) break;
+                    tc::fence_after();
+                    times_y(tmem + C::A2_COL, s, y1(j) + 2 * C::PLANE);
+                    if (NB == 1) tc::commit(pv_done);
+                }
+                wait(ds_full(j), j >> 1);
+                if (!DKV && j >= 1) wait(acc_free, j - 1);
+                if (!ok) break;
+                tc::fence_after();
+                times_y(tmem + C::A1_COL, ds, y1(j));
+                tc::commit(acc_full);
+                if (NB == 1 && more) {
+                    if (DKV) {
+                        wait(pv_done, j);  // P_j has been read
+                        scores(j + 1);
+                    }
+                    wait(acc_full, j);  // dS_j has been read
+                    tc::fence_after();
+                    grads(j + 1);
+                }
+                // refill: with NB == 2 tile j - 1 is over (acc_full above), with NB == 1 tile j is (acc_full)
+                if (NB == 2) {
+                    if (j >= 1 && loaded < n) { load(loaded); ++loaded; }
+                } else if (more && loaded < n) {
+                    load(loaded);
+                    ++loaded;
+                }
+            }
+            if (!ok) {  // a wait ran out: see the copies and MMAs in flight to their end (bounded) before memory is given back
+                tc::commit(drain);
+                int never = 0;
+                mbar_wait(drain, 0, &never);
+                for (int t = max(0, loaded - C::STAGES); t < loaded; ++t) mbar_wait(full(t % C::STAGES), (uint32_t)(t / C::STAGES) & 1u, &never);
+            }
+        }
+        __syncthreads();
+        __syncthreads();
+        if (DKV) { __syncthreads(); __syncthreads(); }
+    } else {
+        tc::regs_up<232>();
+        float acc1[W], acc2[DKV ? W : 1];
+#pragma unroll
+        for (int d = 0; d < W; ++d) acc1[d] = 0.f;
+#pragma unroll
+        for (int d = 0; d < (DKV ? W : 1); ++d) acc2[d] = 0.f;
+        const float c_row = fabsf(a.scale_log2) * x1_inv;
+        // dq pass: the row's numbers
+        float m_row = INFINITY, il_row = 0.f, delta_row = 0.f;
+        int n_row = 0;
+        if (!DKV && i < q_rows) {
+            const float* info = p.info + (((int64_t)b * a.H + h) * p.q_info_tiles + (i >> 6)) * ATTN_INFO;
+            m_row = info[i & 63];
+            il_row = info[T + (i & 63)] / info[3 * T];
+            delta_row = info[2 * T + (i & 63)];
+            n_row = keys;
+            if (a.causal) n_row = min(n_row, (int)max((int64_t)0, i + off + 1));
+        }
+        // factors that the tile in flight in the accumulators is added with
+        float f1 = 0.f, f2 = 0.f;
+        bool ok = true;
+        auto await = [&](uint32_t bar, int phase) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, abort_flag)); };
+        auto add_tile = [&](int j) {  // registers += accumulators of tile j
+            await(acc_full, j);
+            if (!ok) return;
+            tc::fence_after();
+            const uint64_t g1 = tc::pack2(f1, f1), g2 = tc::pack2(f2, f2);
+#pragma unroll
+            for (int g = 0; g < W / 32; ++g) {
+                float t[32];
+                tc::ld32(lane_base + C::A1_COL + wg * W + 32 * g, t);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2)
+                    tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), g1, tc::pack2(acc1[32 * g + e], acc1[32 * g + e + 1])), acc1[32 * g + e],
+                                acc1[32 * g + e + 1]);
+                if (DKV) {
+                    tc::ld32(lane_base + C::A2_COL + wg * W + 32 * g, t);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+                        tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), g2, tc::pack2(acc2[(32 * g + e) % (DKV ? W : 1)], acc2[(32 * g + e + 1) % (DKV ? W : 1)])),
+                                    acc2[(32 * g + e) % (DKV ? W : 1)], acc2[(32 * g + e + 1) % (DKV ? W : 1)]);
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_free);
+        };
+        for (int j = 0; j < n; ++j) {
+            // one buffer, dkv pass: the sums of tile j - 1 are taken first, while S_j is being computed
+            if (NB == 1 && DKV && j >= 1) add_tile(j - 1);
+            await(s_full(j), j >> 1);
+            if (!ok) break;
+            tc::fence_after();
+            const float y1_inv = __ldg(p.y1_inv + tile0 + j), y2_inv = __ldg(p.y2_inv + tile0 + j);
+            const float c = c_row * y1_inv;
+            const float f = x2_inv * y2_inv;  // dP = f * accumulator
+            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % NB) * T + 32 * wg, d_addr = lane_base + C::P_COL + (uint32_t)(j % NB) * T + 32 * wg;
+            const uint64_t c2 = tc::pack2(c, c);
+            float e[32];
+            tc::ld32(s_addr, e);
+            float G;  // power of two: dS at most 2^15
+            uint64_t nd2, fg2;
+            const float* info = nullptr;
+            if (DKV) {
+                await(full(j % C::STAGES), j / C::STAGES);  // the row numbers that came with the tile
+                if (!ok) break;
+                info = reinterpret_cast<const float*>(smem + (j % C::STAGES) * C::STAGE + 4 * C::PLANE);
+                G = tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, info[3 * T + 1]));
+                fg2 = tc::pack2(f * G, f * G);
+                nd2 = tc::pack2(-G, -G);
+                // visible columns start at lim (causal)
+                const int lim = a.causal ? (int)max((int64_t)-1, min((int64_t)T, i - off - (int64_t)(first + j) * T)) - 32 * wg : 0;
+                const bool whole = __all_sync(0xffffffffu, lim <= 0);
+                uint32_t hi[16], lo[16];
+                const float2* mi = reinterpret_cast<const float2*>(info + 32 * wg);
+                const float2* il = reinterpret_cast<const float2*>(info + T + 32 * wg);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    const float2 mm = mi[u], ii = il[u];
+                    float x, y;
+                    tc::unpack2(tc::fma2(tc::pack2(e[2 * u], e[2 * u + 1]), c2, tc::pack2(-mm.x, -mm.y)), x, y);
+                    tc::unpack2(tc::mul2(tc::pack2(tc::ex2(x), tc::ex2(y)), tc::pack2(ii.x, ii.y)), x, y);
+                    if (!whole) {
+                        x = 2 * u >= lim ? x : 0.f;
+                        y = 2 * u + 1 >= lim ? y : 0.f;
+                    }
+                    e[2 * u] = x;
+                    e[2 * u + 1] = y;
+                    tc::split_pair(x, y, hi[u], lo[u]);
+                }
+                tc::st16(s_addr, hi);
+                tc::st16(s_addr + 16, lo);
+                tc::st_wait();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(j));
+            } else {
+                tc::fence_before();
+                __syncwarp();
+                if (NB == 1 && lane == 0) mbar_arrive(s_read);
+                G = 32768.f * tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, fabsf(delta_row)));
+                fg2 = tc::pack2(f * G, f * G);
+                nd2 = tc::pack2(-delta_row * G, -delta_row * G);
+                const int lim = n_row - j * T - 32 * wg;
+                const bool whole = __all_sync(0xffffffffu, lim >= 32);
+                const uint64_t m2 = tc::pack2(-m_row, -m_row);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    float x, y;
+                    tc::unpack2(tc::fma2(tc::pack2(e[2 * u], e[2 * u + 1]), c2, m2), x, y);
+                    x = tc::ex2(x);
+                    y = tc::ex2(y);
+                    if (!whole) {
+                        x = 2 * u < lim ? x : 0.f;
+                        y = 2 * u + 1 < lim ? y : 0.f;
+                    }
+                    e[2 * u] = x;
+                    e[2 * u + 1] = y;
+                }
+                if (NB == 1 && j >= 1) add_tile(j - 1);  // while dP_j is being computed
+            }
+            await(d_full(j), j >> 1);
+            if (!ok) break;
+            tc::fence_after();
+            {
+                float t[32];
+                tc::ld32(d_addr, t);
+                uint32_t hi[16], lo[16];
+                const float2* dl = reinterpret_cast<const float2*>(info + 2 * T + 32 * wg);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    uint64_t shift = nd2;
+                    if (DKV) {
+                        const float2 d = dl[u];
+                        shift = tc::mul2(tc::pack2(d.x, d.y), nd2);
+                    }
+                    const uint64_t v = tc::mul2(tc::pack2(e[2 * u], e[2 * u + 1]), tc::fma2(tc::pack2(t[2 * u], t[2 * u + 1]), fg2, shift));
+                    float x, y;
+                    tc::unpack2(v, x, y);
+                    tc::split_pair(x, y, hi[u], lo[u]);
+                }
+                tc::st16(d_addr, hi);
+                tc::st16(d_addr + 16, lo);
+            }
+            tc::st_wait();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_full(j));
+            if (NB == 2 && j >= 1) add_tile(j - 1);
+            // now the factors of tile j
+            if (DKV) {
+                const float ps_inv = 1.f / info[3 * T];
+                f1 = a.scale * y1_inv * ps_inv / G;
+                f2 = y2_inv * ps_inv;
+            } else {
+                f1 = a.scale * il_row * y1_inv / G;
+            }
+        }
+        if (ok && n > 0) add_tile(n - 1);
+
+        // ---- through the stages to memory: 16-byte chunk q of row r at chunk q ^ (r & 7) ----
+        float* const buf = reinterpret_cast<float*>(smem);
+        const bool valid = i < x_rows;
+        auto write = [&](const float* acc, const TenmoHeadsView& out, int vec) {
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < W; d += 4) {
+                const int q = (wg * W + d) >> 2;
+                *reinterpret_cast<float4*>(buf + row * DP + ((q ^ (row & 7)) << 2)) =
+                    valid ? make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            __syncthreads();
+            const int total = DKV ? a.Sk : a.Sq, here = min(ROWS, total - x_tile * ROWS);
+            float* base = out.ptr + b * out.sb + h * out.sh + (int64_t)x_tile * ROWS * out.sr;
+            for (int q = threadIdx.x; q < here * (DP / 4); q += 256) {
+                const int r = q / (DP / 4), ch = q % (DP / 4), d = 4 * ch;
+                if (d >= a.D) continue;
+                float4 x = *reinterpret_cast<const float4*>(buf + r * DP + ((ch ^ (r & 7)) << 2));
+                float* dst = base + r * out.sr + d;
+                if (vec) {
+                    if (p.beta != 0.f) {
+                        const float4 o = *reinterpret_cast<const float4*>(dst);
+                        x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
+                    }
+                    *reinterpret_cast<float4*>(dst) = x;
+                } else {
+                    const float v[4] = {x.x, x.y, x.z, x.w};
+                    for (int u = 0; u < 4 && d + u < a.D; ++u) dst[u] = p.beta != 0.f ? dst[u] + v[u] : v[u];
+                }
+            }
+        };
+        write(acc1, p.out1, p.out1_vec);
+        if (DKV) write(acc2, p.out2, p.out2_vec);
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, TENMO_DEV_TIMEOUT);
+    if (warp == 8) {
+        tc::fence_after();
+        tc::dealloc(tmem, C::TMEM);
+    }
+}
+
+// dk, dv (+)= the sums of the partial gradients of a group's heads, in order
+__global__ void __launch_bounds__(256) attn_fold_kernel(const float* dk_part, const float* dv_part, const TenmoAttnParams a) {
+    const int group = a.H / a.Hkv;
+    const int64_t total = (int64_t)a.B * a.Hkv * a.Sk * a.D, per_head = (int64_t)a.Sk * a.D;
+    const float* part = blockIdx.y ? dv_part : dk_part;
+    const TenmoHeadsView& out = blockIdx.y ? a.dv : a.dk;
+    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t bh = e / per_head, at = e % per_head;
+        const int b = (int)(bh / a.Hkv), kvh = (int)(bh % a.Hkv);
+        const float* src = part + ((int64_t)b * a.H + (int64_t)kvh * group) * per_head + at;
+        float s = 0.f;
+        for (int g = 0; g < group; ++g) s += __ldg(src + g * per_head);
+        float* dst = out.ptr + b * out.sb + kvh * out.sh + (at / a.D) * out.sr + at % a.D;
+        *dst = a.beta != 0.f ? *dst + s : s;
+    }
+}
+
+size_t align_up(size_t n) { return (n + 1023) & ~(size_t)1023; }
+
+template <int DP, bool DKV>
+int launch(tenmo_ctx* ctx, const BwdParams& p) {
+    const int smem = BwdCfg<DP, DKV>::SMEM;
+    TENMO_CUDA_TRY(ctx, cudaFuncSetAttribute(attn_bwd_tc_kernel<DP, DKV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const unsigned grid = (unsigned)((int64_t)p.a.B * p.a.H * p.x_tiles);
+    attn_bwd_tc_kernel<DP, DKV><<<grid, THREADS, smem, ctx->stream>>>(p);
+    TENMO_LAUNCH_CHECK(ctx, "attn_bwd_tc_kernel");
+    return TENMO_OK;
+}
+
+}  // namespace
+
+int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
+    const int dp = tenmo_attn_padded(a.D);
+    const int k_tiles = (a.Sk + T - 1) / T, q_tiles = (a.Sq + T - 1) / T;
+    const int64_t nk = (int64_t)a.B * a.Hkv * k_tiles, nq = (int64_t)a.B * a.H * q_tiles;
+    const size_t k_img = align_up((size_t)nk * T * dp * 4), q_img = align_up((size_t)nq * T * dp * 4);
+    const size_t k_inv = align_up((size_t)nk * sizeof(float)), q_inv = align_up((size_t)nq * sizeof(float));
+    const size_t info = align_up((size_t)nq * ATTN_INFO * sizeof(float));
+    const bool grouped = a.H != a.Hkv;
+    const size_t part = grouped ? align_up((size_t)a.B * a.H * a.Sk * a.D * sizeof(float)) : 0;
+    void* ws = nullptr;
+    int st = tenmo_op_workspace(ctx, 2 * (k_img + q_img + k_inv + q_inv + part) + info, &ws);
+    if (st != TENMO_OK) return st;
+    uint8_t* w = (uint8_t*)ws;
+    uint8_t *ik = w, *iv = ik + k_img, *iq = iv + k_img, *ig = iq + q_img;
+    float* vk = (float*)(ig + q_img);
+    float* vv = (float*)((uint8_t*)vk + k_inv);
+    float* vq = (float*)((uint8_t*)vv + k_inv);
+    float* vg = (float*)((uint8_t*)vq + q_inv);
+    float* in = (float*)((uint8_t*)vg + q_inv);
+    float* pk = (float*)((uint8_t*)in + info);
+    float* pv = (float*)((uint8_t*)pk + part);
+    TenmoTileJobs jobs = {};
+    jobs.B = a.B;
+    jobs.D = a.D;
+    jobs.job[0] = TenmoTileJob{a.k, a.k_lengths, ik, vk, a.Hkv, a.Sk, k_tiles, tenmo_attn_row_vec(a.k, a.D)};
+    jobs.job[1] = TenmoTileJob{a.v, a.k_lengths, iv, vv, a.Hkv, a.Sk, k_tiles, tenmo_attn_row_vec(a.v, a.D)};
+    jobs.job[2] = TenmoTileJob{a.q, a.q_lengths, iq, vq, a.H, a.Sq, q_tiles, tenmo_attn_row_vec(a.q, a.D)};
+    jobs.job[3] = TenmoTileJob{a.go, a.q_lengths, ig, vg, a.H, a.Sq, q_tiles, tenmo_attn_row_vec(a.go, a.D)};
+    jobs.job[3].o = a.o;
+    jobs.job[3].o_vec = tenmo_attn_row_vec(a.o, a.D);
+    jobs.job[3].stats = a.stats;
+    jobs.job[3].info = in;
+    if ((st = tenmo_attn_make_tiles(ctx, jobs, 4, dp)) != TENMO_OK) return st;
+
+    BwdParams p = {};
+    p.a = a;
+    p.info = in;
+    p.q_info_tiles = q_tiles;
+    p.status = ctx->dev_status;
+    // dq
+    p.y1_img = ik; p.y2_img = iv; p.y1_inv = vk; p.y2_inv = vv;
+    p.tiles = k_tiles;
+    p.x_tiles = (a.Sq + ROWS - 1) / ROWS;
+    p.x1 = a.q; p.x2 = a.go; p.out1 = a.dq; p.out2 = a.dq;
+    p.x1_vec = tenmo_attn_row_vec(a.q, a.D); p.x2_vec = tenmo_attn_row_vec(a.go, a.D);
+    p.out1_vec = p.out2_vec = tenmo_attn_row_vec(a.dq, a.D);
+    p.beta = a.beta;
+    if ((st = dp == 64 ? launch<64, false>(ctx, p) : launch<128, false>(ctx, p)) != TENMO_OK) return st;
+    // dk, dv
+    p.y1_img = iq; p.y2_img = ig; p.y1_inv = vq; p.y2_inv = vg;
+    p.tiles = q_tiles;
+    p.x_tiles = (a.Sk + ROWS - 1) / ROWS;
+    p.x1 = a.k; p.x2 = a.v;
+    p.x1_vec = tenmo_attn_row_vec(a.k, a.D); p.x2_vec = tenmo_attn_row_vec(a.v, a.D);
+    if (grouped) {
+        const int64_t per = (int64_t)a.Sk * a.D;
+        p.out1 = TenmoHeadsView{pk, per * a.H, per, a.D};
+        p.out2 = TenmoHeadsView{pv, per * a.H, per, a.D};
+        p.beta = 0.f;
+    } else {
+        p.out1 = a.dk;
+        p.out2 = a.dv;
+    }
+    p.out1_vec = tenmo_attn_row_vec(p.out1, a.D);
+    p.out2_vec = tenmo_attn_row_vec(p.out2, a.D);
+    if ((st = dp == 64 ? launch<64, true>(ctx, p) : launch<128, true>(ctx, p)) != TENMO_OK) return st;
+    if (grouped) {
+        const dim3 grid((unsigned)tenmo_stream_grid(ctx, (int64_t)a.B * a.Hkv * a.Sk * a.D, 1024, 8), 2);
+        attn_fold_kernel<<<grid, 256, 0, ctx->stream>>>(pk, pv, a);
+        TENMO_LAUNCH_CHECK(ctx, "attn_fold_kernel");
+    }
+    return TENMO_OK;
+}

@@ -98,6 +98,10 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A warpgroup's share of the registers that the block was launched with.
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // a contiguous copy from global memory that completes on an mbarrier (16-byte aligned, size a multiple of 16)
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
@@ -154,6 +158,12 @@ __device__ __forceinline__ float block_scale(float largest, float* inverse) {
     const int ex = (int)((__float_as_uint(largest) >> 23) & 255u) - 127;
     const int e = largest > 0.f ? min(14 - ex, 120) : 0;
     *inverse = __uint_as_float((uint32_t)(127 - e) << 23);
+    return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+// the largest power of two (2^-121 .. 2^100) that is at most 1 / x, for x > 0
+__device__ __forceinline__ float pow2_below_inverse(float x) {
+    const int ex = (int)((__float_as_uint(x) >> 23) & 255u) - 127;
+    const int e = max(-121, min(100, -(ex + 1)));
     return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 // |x| for the search of the largest entry: infinities and NaN do not count
