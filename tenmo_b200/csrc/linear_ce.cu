@@ -10,7 +10,7 @@
 // Ignored rows: their x is replaced by zeros, so that whatever padding holds (NaN included) reaches no gradient.
 #include <cfloat>
 
-#include "op_util.cuh"
+#include "gemm_h3.cuh"
 
 namespace {
 
@@ -116,6 +116,115 @@ __global__ void __launch_bounds__(LCE_THREADS) lce_row_kernel(const LceRow p) {
     }
 }
 
+// ---- tensor-core path: the softmax statistics come out of the product's epilogue ----
+struct LceStats {
+    const float2* stats; const float* sums; const float* at_label;  // per 64-column group and row, see gemm_h3.cuh
+    int64_t groups, rows, row0, V, ignore;
+    const void* labels;
+    const float* upstream; const float* factor;
+    float* row_loss;
+    float4* numbers;  // per row of the piece: maximum, 1 / sum of exponentials, u_n, unused
+    uint32_t* status;
+    float ls;
+    int is_i64, reduction;
+};
+// 32 rows per block; 8 warps take the column groups in turn, joined in order
+__global__ void __launch_bounds__(256) lce_stats_kernel(const LceStats p) {
+    __shared__ float sm[8][32], sl[8][32], sa[8][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t r = (int64_t)blockIdx.x * 32 + lane;
+    float m = -INFINITY, l = 0.f, all = 0.f;
+    if (r < p.rows) {
+        for (int64_t g = w; g < p.groups; g += 8) {
+            const float2 v = __ldg(p.stats + g * p.rows + r);
+            const float top = fmaxf(m, v.x);
+            if (top == -INFINITY) {  // nothing but -inf or NaN so far: 0, or the NaN of the sum
+                l += v.y;
+                continue;
+            }
+            l = l * expf(m - top) + v.y * expf(v.x - top);
+            m = top;
+            if (p.sums) all += __ldg(p.sums + g * p.rows + r);
+        }
+    }
+    sm[w][lane] = m;
+    sl[w][lane] = l;
+    sa[w][lane] = all;
+    __syncthreads();
+    if (w || r >= p.rows) return;
+    for (int k = 1; k < 8; ++k) m = fmaxf(m, sm[k][lane]);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    all = 0.f;
+    for (int k = 0; k < 8; ++k) {
+        l += sl[k][lane] * expf(sm[k][lane] - base);
+        all += sa[k][lane];
+    }
+    const int64_t n = p.row0 + r, y = lce_label(p.labels, p.is_i64, n);
+    const bool counted = y != p.ignore, good = counted && y >= 0 && y < p.V;
+    if (counted && !good) atomicOr(p.status, TENMO_DEV_BAD_LABEL);
+    float loss = 0.f, u = 0.f;
+    if (good) {
+        const float lse = logf(l);
+        loss = (1.f - p.ls) * (lse - (p.at_label[r] - base));
+        if (p.ls > 0.f) loss += p.ls * (lse - (all / (float)p.V - base));
+        u = *p.factor;
+        if (p.upstream) u *= p.upstream[p.reduction == 2 ? n : 0];
+    }
+    p.row_loss[n] = loss;
+    if (p.numbers) p.numbers[r] = make_float4(base, 1.f / l, u, good ? 1.f : 0.f);
+}
+
+// The logits of a 128 x 128 block become the gradient, as an operand image in their place, and its column sums per block row.
+__global__ void __launch_bounds__(256) lce_grad_kernel(uint8_t* z, float* inverse, const float4* numbers, const void* labels, int is_i64,
+                                                       int64_t row0, int64_t rows, int64_t V, int block_cols, float ls, float* db_part) {
+    __shared__ float sums[16][H3_BLOCK];
+    const int64_t block = blockIdx.x;
+    const int64_t r0 = block / block_cols * H3_BLOCK, c0 = block % block_cols * H3_BLOCK;
+    const int c = 8 * (threadIdx.x & 15);
+    const float* src = reinterpret_cast<const float*>(z + block * H3_BLOCK_BYTES);
+    const float smooth = ls / (float)V;
+    float x[8][8], col[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) col[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        const int lr = (threadIdx.x >> 4) + 16 * s;
+        const int64_t r = r0 + lr;
+        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+        int64_t y = -1;
+        if (r < rows) {
+            num = __ldg(numbers + r);
+            y = lce_label(labels, is_i64, row0 + r) - c0 - c;
+        }
+        const bool in = num.w != 0.f;
+        if (in) {
+            const float4 a = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c), b = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c + 4);
+            x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
+            x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float p = tc::ex2((x[s][e] - num.x) * 1.44269504088896341f) * num.y;
+            x[s][e] = in && c0 + c + e < V ? (p - smooth - (e == y ? 1.f - ls : 0.f)) * num.z : 0.f;
+            col[e] += x[s][e];
+        }
+    }
+    if (db_part) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 4][c + e] = col[e];
+        __syncthreads();
+        if (threadIdx.x < H3_BLOCK && c0 + threadIdx.x < V) {
+            float t = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) t += sums[k][threadIdx.x];
+            db_part[block / block_cols * V + c0 + threadIdx.x] = t;
+        }
+    }
+    // every thread's logits are in registers (the barrier inside) before the image is written over them
+    tenmo_h3_write_block(x, z + block * H3_BLOCK_BYTES, inverse + block);
+}
+
 // loss from the row losses, added in a fixed order (double: the mean of many rows keeps the bits of each)
 __global__ void __launch_bounds__(1024) lce_loss_kernel(const float* row_loss, int64_t N, int reduction, const int32_t* valid, float* loss) {
     __shared__ double slots[32];
@@ -176,10 +285,98 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     return TENMO_OK;
 }
 
+// Large problems: the products on tensor cores (gemm_h3.cu).  Without a gradient no logit is ever stored: the product's epilogue
+// reduces them to two numbers per row and 64 columns.
+bool tc_profitable(const LceCall& c) { return c.N >= 64 && c.D >= 32 && c.V >= 128 && 2.0 * c.N * c.D * c.V >= 2e9; }
+
+int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
+    const int64_t vb = (c.V + H3_BLOCK - 1) / H3_BLOCK;
+    const bool tied = c.w->row_stride == 1 && c.w->col_stride != 1;  // storage is (V, D)
+    // a piece's rows: logits (with a gradient) or statistics within the budget, whole tiles of 256 rows
+    const size_t per_row = c.grad ? (size_t)vb * H3_BLOCK * sizeof(float) : (size_t)vb * 2 * sizeof(float2);
+    int64_t piece = (int64_t)(LCE_PIECE_BYTES / per_row) / 256 * 256;
+    if (piece < 256) piece = 256;
+    if (piece > c.N) piece = c.N;
+    TenmoH3Operand W = {nullptr, nullptr, tied ? c.V : c.D, tied ? c.D : c.V}, X = {nullptr, nullptr, piece, c.D}, Z = {nullptr, nullptr, piece, c.V};
+    const int64_t groups = (c.V + 63) / 64;
+    size_t need = 0;
+    auto take = [&](size_t bytes) { const size_t at = need; need += (bytes + 1023) & ~(size_t)1023; return at; };
+    const size_t w_img = take(W.img_bytes()), w_inv = take(W.inverse_bytes()), x_img = take(X.img_bytes()), x_inv = take(X.inverse_bytes());
+    const size_t z_img = c.grad ? take(Z.img_bytes()) : 0, z_inv = c.grad ? take(Z.inverse_bytes()) : 0;
+    const size_t stats = take((size_t)groups * piece * sizeof(float2)), sums = c.ls > 0.f ? take((size_t)groups * piece * sizeof(float)) : 0;
+    const size_t at_label = take(piece * sizeof(float)), numbers = c.grad ? take(piece * sizeof(float4)) : 0;
+    const size_t row_loss = take(c.N * sizeof(float)), factor = take(sizeof(float));
+    const size_t db_part = c.db ? take((size_t)((piece + H3_BLOCK - 1) / H3_BLOCK) * c.V * sizeof(float)) : 0;
+    size_t part = 0;
+    if (c.grad) {
+        part = tenmo_h3_partial_bytes(ctx, piece, c.D, c.V, true);
+        const size_t last = c.N % piece ? tenmo_h3_partial_bytes(ctx, c.N % piece, c.D, c.V, true) : 0;
+        const size_t dw = tied ? tenmo_h3_partial_bytes(ctx, c.V, c.D, piece, true) : tenmo_h3_partial_bytes(ctx, c.D, c.V, piece, true);
+        if (last > part) part = last;
+        if (dw > part) part = dw;
+    }
+    const size_t partial = take(part);
+    void* ws = nullptr;
+    int st = tenmo_op_workspace(ctx, need, &ws);
+    if (st != TENMO_OK) return st;
+    uint8_t* at = (uint8_t*)ws;
+    W.img = at + w_img; W.inverse = (float*)(at + w_inv);
+    X.img = at + x_img; X.inverse = (float*)(at + x_inv);
+    Z.img = at + z_img; Z.inverse = (float*)(at + z_inv);
+    TENMO_CUDA_TRY(ctx, tenmo_launch(lce_count_kernel, 1, 1024, 0, ctx->stream, ctx->pdl, c.labels, c.is_i64, c.N, c.ignore, c.reduction,
+                                     c.valid, (float*)(at + factor)));
+    TENMO_LAUNCH_CHECK(ctx, "lce_count_kernel");
+    const float* wp = c.w->ptr + c.w->offset;
+    if ((st = tenmo_h3_make(ctx, wp, tied ? c.w->col_stride : c.w->row_stride, 1, W, nullptr, 0, 0)) != TENMO_OK) return st;
+    const size_t label_bytes = c.is_i64 ? 8 : 4;
+    for (int64_t r0 = 0; r0 < c.N; r0 += piece) {
+        const int64_t rows = r0 + piece < c.N ? piece : c.N - r0;
+        X.rows = Z.rows = rows;
+        const void* labels = (const char*)c.labels + r0 * label_bytes;
+        if ((st = tenmo_h3_make(ctx, c.x->ptr + c.x->offset + r0 * c.x->row_stride, c.x->row_stride, c.x->col_stride, X, labels, c.is_i64, c.ignore)) != TENMO_OK)
+            return st;
+        TenmoH3Epilogue e = {};
+        e.C = c.grad ? (float*)Z.img : nullptr;
+        e.blocked = 1;
+        e.bias = c.bias;
+        e.stats = (float2*)(at + stats);
+        e.sums = c.ls > 0.f ? (float*)(at + sums) : nullptr;
+        e.at_label = (float*)(at + at_label);
+        e.labels = labels;
+        e.label_is_i64 = c.is_i64;
+        if ((st = tenmo_h3_gemm(ctx, rows, c.V, c.D, X, false, W, !tied, e, nullptr)) != TENMO_OK) return st;
+        const LceStats ps{e.stats, e.sums, e.at_label, groups, rows, r0, c.V, c.ignore, c.labels, c.upstream, (const float*)(at + factor),
+                          (float*)(at + row_loss), c.grad ? (float4*)(at + numbers) : nullptr, ctx->dev_status, c.ls, c.is_i64, c.reduction};
+        lce_stats_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, ctx->stream>>>(ps);
+        TENMO_LAUNCH_CHECK(ctx, "lce_stats_kernel");
+        if (!c.grad) continue;
+        lce_grad_kernel<<<(unsigned)Z.blocks(), 256, 0, ctx->stream>>>(Z.img, Z.inverse, ps.numbers, c.labels, c.is_i64, r0, rows, c.V, (int)vb, c.ls,
+                                                                       c.db ? (float*)(at + db_part) : nullptr);
+        TENMO_LAUNCH_CHECK(ctx, "lce_grad_kernel");
+        TenmoH3Epilogue ex = {};
+        ex.C = c.dx + r0 * c.D;
+        ex.ldc = c.D;
+        if ((st = tenmo_h3_gemm(ctx, rows, c.D, c.V, Z, false, W, tied, ex, at + partial)) != TENMO_OK) return st;
+        TenmoH3Epilogue ew = {};
+        ew.C = c.dw;
+        ew.ldc = tied ? c.D : c.V;
+        ew.add = r0 > 0;
+        st = tied ? tenmo_h3_gemm(ctx, c.V, c.D, rows, Z, true, X, true, ew, at + partial) : tenmo_h3_gemm(ctx, c.D, c.V, rows, X, true, Z, true, ew, at + partial);
+        if (st != TENMO_OK) return st;
+        if (c.db && (st = tenmo_colsum_f32(ctx, (const float*)(at + db_part), Z.block_rows(), c.V, c.V, c.db, r0 ? 1.f : 0.f)) != TENMO_OK) return st;
+    }
+    const int grid = c.reduction == 2 ? tenmo_stream_grid(ctx, c.N, 1024, 1) : 1;
+    TENMO_CUDA_TRY(ctx, tenmo_launch(lce_loss_kernel, grid, 1024, 0, ctx->stream, ctx->pdl, (const float*)(at + row_loss), c.N, c.reduction,
+                                     (const int32_t*)c.valid, c.loss));
+    TENMO_LAUNCH_CHECK(ctx, "lce_loss_kernel");
+    return TENMO_OK;
+}
+
 int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     int st = check(ctx, who, c);
     if (st != TENMO_OK) return st;
     TenmoDeviceGuard guard(ctx);
+    if (tc_profitable(c)) return lce_run_tc(ctx, c);
     int64_t piece = (int64_t)(LCE_PIECE_BYTES / ((size_t)c.V * sizeof(float))) / 128 * 128;
     if (piece < 128) piece = 128;
     if (piece > c.N) piece = c.N;
