@@ -10,8 +10,9 @@
 // The backward pass recomputes the probabilities from q, k and the two saved numbers per row, m_i and l_i (kept apart: with
 // their sum, the log-sum-exp, a large m would cost p its last bits).
 //
-// Kernels here: one warp per row, scores 32 keys at a time (a lane is a key), the weighted sum with a lane per column.
-// No tile is filled and nothing waits on anything, so small problems finish in one launch latency per pass.
+// Kernels here, without tensor cores: the forward pass for few rows (one new token against a long cache, small problems), and
+// the backward pass of small problems with one warp per row, scores 32 keys at a time (a lane is a key) and the weighted sum
+// with a lane per column.  No large tile is filled, so small problems finish in one launch latency per pass.
 #include "attention_tc.cuh"
 
 #include <cfloat>
@@ -60,57 +61,230 @@ __device__ __forceinline__ bool warp_row(int64_t rows_per_head, int heads, int64
     return true;
 }
 
-__global__ void __launch_bounds__(ROW_WARPS * 32) attn_fwd_row_kernel(const TenmoAttnParams p) {
-    __shared__ __align__(16) float sq[ROW_WARPS][TENMO_ATTN_MAX_DIM];
+// ---------------------------------------------------------------------------------------------------------------------
+// Forward with few rows: R rows of a key/value head (its query heads' rows, flattened) against a slice of the keys.
+// A lane holds four columns; LPK lanes are a row of k or v, so a warp's load covers 32 / LPK whole rows.  Scores: partial dot products of
+// eight loads, summed over the lanes by halving (a lane passes on the half it does not keep: V shuffles for V sums instead of
+// log2(LPK) V).  The exponentials of 32 keys are taken with a lane per key, and go through shared memory to be multiplied with v.
+// Four warps take 32 keys in turn and are joined at the end; with few rows and many keys the keys are cut into slices, one block
+// each, which attn_join_kernel adds in order.
+// Bound: HBM for one token (k and v are read once, 16 bytes a lane), launch latency for the smallest calls.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int FEW_WARPS = 4;
+struct FewParams {
+    TenmoAttnParams a;
+    int groups, slices;   // row groups of a key/value head, slices of the keys
+    int k_vec, v_vec;
+    float* partial;       // slices > 1: per (b, h, i, slice): D sums, then m, l
+    int ldp;
+};
+
+// row rr of a key/value head: query head and position
+__device__ __forceinline__ void few_row(const TenmoAttnParams& p, int kvh, int rr, int* h, int* i) {
+    *h = kvh * (p.H / p.Hkv) + rr / p.Sq;
+    *i = rr % p.Sq;
+}
+
+template <int LPK, int R>
+__global__ void __launch_bounds__(FEW_WARPS * 32) attn_fwd_few_kernel(const FewParams f) {
+    constexpr int KPL = 32 / LPK, V = 8 * R;  // rows per load; partial sums of eight loads
+    __shared__ __align__(16) float pk[FEW_WARPS][32 * R];
+    __shared__ __align__(16) float so[FEW_WARPS][R][4 * LPK];
+    __shared__ float sm[FEW_WARPS][R], sl[FEW_WARPS][R];
+    const TenmoAttnParams& p = f.a;
     tenmo_grid_dependency_sync();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int b, h, i;
-    if (!warp_row(p.Sq, p.H, (int64_t)p.B * p.H * p.Sq, &b, &h, &i)) return;
-    const int kvh = h / (p.H / p.Hkv);
-    const float* q = p.q.ptr + b * p.q.sb + h * p.q.sh + i * p.q.sr;
-    const float* k = p.k.ptr + b * p.k.sb + kvh * p.k.sh;
-    const float* v = p.v.ptr + b * p.v.sb + kvh * p.v.sh;
-    const bool vec = row_vec(p.k, p.D);
-    for (int d = lane; d < p.D; d += 32) sq[warp][d] = __ldg(q + d);
-    __syncwarp();
-    const int n = visible_keys(p, b, i);
-    float m = -INFINITY, l = 0.f, acc[DSLOTS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l4 = 4 * (lane % LPK), sub = lane / LPK;
+    const int slice = blockIdx.x % f.slices, gi = blockIdx.x / f.slices;
+    const int group = gi % f.groups, kvh = gi / f.groups % p.Hkv, b = gi / f.groups / p.Hkv;
+    const int total = p.H / p.Hkv * p.Sq, row0 = group * R;
+    float4 q[R];
+    int seen[R], most = 0;
 #pragma unroll
-    for (int t = 0; t < DSLOTS; ++t) acc[t] = 0.f;
-    for (int j0 = 0; j0 < n; j0 += 32) {
-        const int j = j0 + lane;
-        const float s = j < n ? dot_row(sq[warp], k + j * p.k.sr, p.D, vec) * p.scale_log2 : -INFINITY;
-        const float mn = fmaxf(m, tenmo_warp_max(s));
-        const float base = mn == -INFINITY ? 0.f : mn;  // every score so far is -inf
-        const float e = exp2f(s - base), shrink = exp2f(m - base);
-        m = mn;
-        l = l * shrink + tenmo_warp_sum(e);
-#pragma unroll
-        for (int t = 0; t < DSLOTS; ++t) acc[t] *= shrink;
-        const int cnt = min(32, n - j0);
-        for (int jj = 0; jj < cnt; ++jj) {
-            const float w = __shfl_sync(0xffffffffu, e, jj);
-            const float* row = v + (j0 + jj) * p.v.sr;
-#pragma unroll
-            for (int t = 0; t < DSLOTS; ++t) {
-                const int d = lane + 32 * t;
-                if (d < p.D) acc[t] = fmaf(w, __ldg(row + d), acc[t]);
+    for (int r = 0; r < R; ++r) {
+        seen[r] = 0;
+        q[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row0 + r < total) {
+            int h, i;
+            few_row(p, kvh, row0 + r, &h, &i);
+            seen[r] = visible_keys(p, b, i);
+            most = max(most, seen[r]);
+            const float* src = p.q.ptr + b * p.q.sb + h * p.q.sh + i * p.q.sr;
+            if (seen[r]) {
+                if (l4 < p.D) q[r].x = __ldg(src + l4);
+                if (l4 + 1 < p.D) q[r].y = __ldg(src + l4 + 1);
+                if (l4 + 2 < p.D) q[r].z = __ldg(src + l4 + 2);
+                if (l4 + 3 < p.D) q[r].w = __ldg(src + l4 + 3);
             }
         }
     }
-    // l is 0 for a row without visible keys (or with all scores -inf): its output is 0.  A NaN sum stays NaN.
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // this block's keys: whole groups of 128
+    const int per = ((most + f.slices - 1) / f.slices + 127) / 128 * 128;
+    const int begin = min(most, slice * per), end = min(most, begin + per);
+    const float* k = p.k.ptr + b * p.k.sb + kvh * p.k.sh;
+    const float* v = p.v.ptr + b * p.v.sb + kvh * p.v.sh;
+    auto load = [&](const float* base, int64_t stride, int j, bool vec) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < end) {
+            const float* src = base + j * stride + l4;
+            if (vec) {
+                if (l4 < p.D) x = __ldg(reinterpret_cast<const float4*>(src));
+            } else {
+                if (l4 < p.D) x.x = __ldg(src);
+                if (l4 + 1 < p.D) x.y = __ldg(src + 1);
+                if (l4 + 2 < p.D) x.z = __ldg(src + 2);
+                if (l4 + 3 < p.D) x.w = __ldg(src + 3);
+            }
+        }
+        return x;
+    };
+    float m[R], l[R];
+    float4 o[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float* const mine = pk[warp];
+    for (int j0 = begin + 32 * warp; j0 < end; j0 += 32 * FEW_WARPS) {
+#pragma unroll
+        for (int t0 = 0; t0 < LPK; t0 += 8) {
+            float4 x[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) x[t] = load(k, p.k.sr, j0 + (t0 + t) * KPL + sub, f.k_vec);
+            float s[V];
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    s[t * R + r] = fmaf(x[t].x, q[r].x, x[t].y * q[r].y) + fmaf(x[t].z, q[r].z, x[t].w * q[r].w);
+            int n = V, at = 0;
+#pragma unroll
+            for (int w = LPK / 2; w > 0; w >>= 1) {
+                if (n > 1) {
+                    n >>= 1;
+                    const bool up = (lane & w) != 0;
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e)
+                        if (e < n) {
+                            const float give = up ? s[e] : s[e + n], keep = up ? s[e + n] : s[e];
+                            s[e] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+                        }
+                    at += up ? n : 0;
+                } else {
+                    s[0] += __shfl_xor_sync(0xffffffffu, s[0], w);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < n) {
+                    const int t = (at + e) / R, r = (at + e) % R;
+                    mine[((t0 + t) * KPL + sub) * R + r] = s[e];
+                }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float s = j0 + lane < min(end, seen[r]) ? mine[lane * R + r] * p.scale_log2 : -INFINITY;
+            const float top = fmaxf(m[r], tenmo_warp_max(s));
+            const float base = top == -INFINITY ? 0.f : top;  // every score so far is -inf
+            const float e = exp2f(s - base), shrink = exp2f(m[r] - base);
+            m[r] = top;
+            l[r] = l[r] * shrink + e;
+            o[r].x *= shrink; o[r].y *= shrink; o[r].z *= shrink; o[r].w *= shrink;
+            mine[lane * R + r] = e;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int t0 = 0; t0 < LPK; t0 += 8) {
+            float4 x[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) x[t] = load(v, p.v.sr, j0 + (t0 + t) * KPL + sub, f.v_vec);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float* w = mine + ((t0 + t) * KPL + sub) * R;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    o[r].x = fmaf(w[r], x[t].x, o[r].x);
+                    o[r].y = fmaf(w[r], x[t].y, o[r].y);
+                    o[r].z = fmaf(w[r], x[t].z, o[r].z);
+                    o[r].w = fmaf(w[r], x[t].w, o[r].w);
+                }
+            }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l[r] = tenmo_warp_sum(l[r]);
+#pragma unroll
+        for (int w = LPK; w < 32; w <<= 1) {
+            o[r].x += __shfl_xor_sync(0xffffffffu, o[r].x, w);
+            o[r].y += __shfl_xor_sync(0xffffffffu, o[r].y, w);
+            o[r].z += __shfl_xor_sync(0xffffffffu, o[r].z, w);
+            o[r].w += __shfl_xor_sync(0xffffffffu, o[r].w, w);
+        }
+        if (sub == 0) *reinterpret_cast<float4*>(&so[warp][r][l4]) = o[r];
+        if (lane == 0) { sm[warp][r] = m[r]; sl[warp][r] = l[r]; }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * 4 * LPK; e += FEW_WARPS * 32) {
+        const int r = e / (4 * LPK), d = e % (4 * LPK);
+        if (row0 + r >= total) continue;
+        float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, sm[w][r]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) {
+            const float s = exp2f(sm[w][r] - base);
+            sum = fmaf(sl[w][r], s, sum);
+            x = fmaf(so[w][r][d], s, x);
+        }
+        int h, i;
+        few_row(p, kvh, row0 + r, &h, &i);
+        const int64_t row = ((int64_t)b * p.H + h) * p.Sq + i;
+        if (f.slices > 1) {
+            float* dst = f.partial + (row * f.slices + slice) * f.ldp;
+            if (d < p.D) dst[d] = x;
+            if (d == 0) { dst[p.D] = top; dst[p.D + 1] = sum; }
+        } else {
+            // the sum is 0 for a row without visible keys (or with all scores -inf): its output is 0.  A NaN sum stays NaN.
+            if (d < p.D) p.o.ptr[b * p.o.sb + h * p.o.sh + i * p.o.sr + d] = sum == 0.f ? 0.f : x / sum;
+            if (d == 0 && p.stats) { p.stats[2 * row] = top; p.stats[2 * row + 1] = sum; }
+        }
+    }
+}
+
+// A warp joins the slices of a row, in order.
+__global__ void __launch_bounds__(128) attn_join_kernel(const FewParams f) {
+    tenmo_grid_dependency_sync();
+    const TenmoAttnParams& p = f.a;
+    int b, h, i;
+    if (!warp_row(p.Sq, p.H, (int64_t)p.B * p.H * p.Sq, &b, &h, &i)) return;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = ((int64_t)b * p.H + h) * p.Sq + i;
+    const float* src = f.partial + row * f.slices * f.ldp;
+    float top = -INFINITY;
+    for (int s = lane; s < f.slices; s += 32) top = fmaxf(top, src[s * f.ldp + p.D]);
+    top = tenmo_warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x[DSLOTS];
+#pragma unroll
+    for (int t = 0; t < DSLOTS; ++t) x[t] = 0.f;
+    for (int s = 0; s < f.slices; ++s) {
+        const float* part = src + s * f.ldp;
+        const float w = exp2f(part[p.D] - base);
+        sum = fmaf(part[p.D + 1], w, sum);
+#pragma unroll
+        for (int t = 0; t < DSLOTS; ++t)
+            if (lane + 32 * t < p.D) x[t] = fmaf(part[lane + 32 * t], w, x[t]);
+    }
     float* o = p.o.ptr + b * p.o.sb + h * p.o.sh + i * p.o.sr;
 #pragma unroll
-    for (int t = 0; t < DSLOTS; ++t) {
-        const int d = lane + 32 * t;
-        if (d < p.D) o[d] = acc[t] * inv;
-    }
-    if (p.stats && lane == 0) {
-        float* st = p.stats + (((int64_t)b * p.H + h) * p.Sq + i) * 2;
-        st[0] = m;
-        st[1] = l;
-    }
+    for (int t = 0; t < DSLOTS; ++t)
+        if (lane + 32 * t < p.D) o[lane + 32 * t] = sum == 0.f ? 0.f : x[t] / sum;
+    if (p.stats && lane == 0) { p.stats[2 * row] = top; p.stats[2 * row + 1] = sum; }
 }
 
 // probability from the recomputed score and the saved (maximum, sum)
@@ -235,6 +409,48 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) attn_bwd_dkv_row_kernel(const 
     }
 }
 
+template <int R>
+int few_launch(tenmo_ctx* ctx, const FewParams& f, int64_t grid) {
+    auto go = [&](auto kernel) -> int {
+        TENMO_CUDA_TRY(ctx, tenmo_launch(kernel, (unsigned)grid, FEW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, grid), f));
+        TENMO_LAUNCH_CHECK(ctx, "attn_fwd_few_kernel");
+        return TENMO_OK;
+    };
+    return f.a.D <= 32 ? go(attn_fwd_few_kernel<8, R>) : f.a.D <= 64 ? go(attn_fwd_few_kernel<16, R>) : go(attn_fwd_few_kernel<32, R>);
+}
+
+int few_fwd(tenmo_ctx* ctx, const TenmoAttnParams& p) {
+    FewParams f = {};
+    f.a = p;
+    const int64_t total = (int64_t)(p.H / p.Hkv) * p.Sq;
+    const int R = total >= 8 ? 8 : total >= 3 ? 4 : total == 2 ? 2 : 1;
+    const int64_t groups = (total + R - 1) / R, blocks = groups * p.Hkv * p.B;
+    if (groups > INT32_MAX || blocks > INT32_MAX / 64) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "attention_fwd: too many rows in one call");
+    f.groups = (int)groups;
+    // slices of at least 256 keys, as many as it takes to give every SM about four blocks
+    int64_t slices = (4 * (int64_t)ctx->sm_count + blocks - 1) / blocks;
+    if (slices > p.Sk / 256) slices = p.Sk / 256;
+    if (slices > 64) slices = 64;
+    if (slices < 1) slices = 1;
+    f.slices = (int)slices;
+    f.k_vec = tenmo_attn_row_vec(p.k, p.D);
+    f.v_vec = tenmo_attn_row_vec(p.v, p.D);
+    f.ldp = p.D + 2;
+    int st;
+    if (slices > 1) {
+        void* ws = nullptr;
+        if ((st = tenmo_op_workspace(ctx, (size_t)p.B * p.H * p.Sq * slices * f.ldp * sizeof(float), &ws)) != TENMO_OK) return st;
+        f.partial = (float*)ws;
+    }
+    const int64_t grid = blocks * slices;
+    st = R == 8 ? few_launch<8>(ctx, f, grid) : R == 4 ? few_launch<4>(ctx, f, grid) : R == 2 ? few_launch<2>(ctx, f, grid) : few_launch<1>(ctx, f, grid);
+    if (st != TENMO_OK || slices == 1) return st;
+    const int64_t join = ((int64_t)p.B * p.H * p.Sq + ROW_WARPS - 1) / ROW_WARPS;
+    TENMO_CUDA_TRY(ctx, tenmo_launch(attn_join_kernel, (unsigned)join, ROW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, join), f));
+    TENMO_LAUNCH_CHECK(ctx, "attn_join_kernel");
+    return TENMO_OK;
+}
+
 int check_shape(tenmo_ctx* ctx, const char* who, const tenmo_attn_shape* s, float scale, TenmoAttnParams* p) {
     if (!s) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: shape is NULL", who);
     if (s->batch < 0 || s->heads < 1 || s->kv_heads < 1 || s->q_len < 0 || s->k_len < 0 || s->dim < 1)
@@ -298,10 +514,7 @@ int tenmo_attention_fwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
     p.k_lengths = k_lengths;
     TenmoDeviceGuard guard(ctx);
     if (tenmo_attn_tc_profitable(p, false)) return tenmo_attn_tc_fwd(ctx, p);
-    const int64_t grid = ((int64_t)p.B * p.H * p.Sq + ROW_WARPS - 1) / ROW_WARPS;
-    TENMO_CUDA_TRY(ctx, tenmo_launch(attn_fwd_row_kernel, (unsigned)grid, ROW_WARPS * 32, 0, ctx->stream, tenmo_pdl_ok(ctx, grid), p));
-    TENMO_LAUNCH_CHECK(ctx, "attn_fwd_row_kernel");
-    return TENMO_OK;
+    return few_fwd(ctx, p);
 }
 
 int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const tenmo_heads* q, const tenmo_heads* k,
