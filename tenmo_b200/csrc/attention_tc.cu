@@ -5,11 +5,14 @@
 //   S_j = q k_j^T          left operand and accumulator in tensor memory
 //   P_j = exp2(S_j c - m)  by a warpgroup, a row per thread, written over S_j as fp16 pairs: the next left operand
 //   O_j = P_j v_j          a fresh accumulator, added to the row's registers (and rescaled) with rounding
-// Two warpgroups take the tiles alternately, each with its own running maximum, sum and output; the two are joined once at
-// the end.  So while one works on P_j the tensor core computes S_{j+1}, and no warpgroup waits for the other.  The running
-// reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.
-// One thread issues all copies and MMAs.  Up to dim 64 everything fits twice into an SM (96 KB, 256 columns): two CTAs fill each
-// other's gaps.  Up to dim 128 one CTA has the SM, with a third S buffer so that S_{j+1} need not wait for P_{j-1} v_{j-1}.
+// The running reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.
+// A warp of its own issues all copies and MMAs (one thread).
+// Up to dim 64 everything fits twice into an SM (96 KB, 256 columns), with one warpgroup a CTA: it works on P_{j+1} while P_j v_j
+// runs, the two CTAs fill each other's gaps, and at ten warps an SM a thread has the 168 registers that a row of S and a row of O
+// take (with two warpgroups in each CTA it had 96, and the spills, which miss the small L1 that is left, cost more than all
+// the arithmetic: 184 us instead of ___ at 384 heads of 512 x 64).
+// Up to dim 128 one CTA has the SM: two warpgroups take the tiles alternately, each with its own m, l and O, joined once at the
+// end, and a third S buffer lets S_{j+1} start before P_{j-1} v_{j-1} is done.
 // Bound: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
 #include "attention_tc.cuh"
 
@@ -17,7 +20,6 @@ namespace {
 
 constexpr int ROWS = 128;
 constexpr int T = ATTN_TILE;
-constexpr int THREADS = 288;  // two warpgroups and the issuing warp
 constexpr int STAGES = 3;
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -70,7 +72,7 @@ __device__ __forceinline__ void attn_row_numbers(const TenmoTileJobs& jobs, cons
         info[r] = m;
         info[T + r] = il * ps;
         info[2 * T + r] = dl;
-        if (r == 0) { info[3 * T] = ps; info[3 * T + 1] = fmaxf(most[1][0], most[1][1]); }
+        if (r == 0) { info[3 * T] = ps; info[3 * T + 1] = fmaxf(most[1][0], most[1][1]); info[3 * T + 2] = 1.f / ps; }
     }
     __syncthreads();
 }
@@ -142,9 +144,13 @@ struct FwdParams {
 
 template <int DP>
 struct FwdCfg {
+    static constexpr int WGS = DP == 64 ? 1 : 2;    // warpgroups
+    static constexpr int THREADS = DP == 64 ? 192 : 384;  // and two more warps (or a warpgroup, whose registers move)
+    static constexpr int ISSUER = 4 * WGS, LOADER = ISSUER + 1;
     static constexpr int NB = DP == 64 ? 2 : 3;     // S / P buffers
     static constexpr int PLANE = T * DP * 2;        // bytes of one plane of a tile
-    static constexpr int STAGE = 4 * PLANE;         // k hi, k lo, v hi, v lo
+    static constexpr int IMG = 2 * PLANE;           // a tile's hi and lo plane
+    static constexpr int STAGE = 2 * IMG;           // a slot for k, one for v
     static constexpr int Q_COLS = DP;               // hi DP/2, lo DP/2
     static constexpr int S_COL = Q_COLS, O_COL = Q_COLS + NB * T;
     static constexpr int TMEM = DP == 64 ? 256 : 512;
@@ -153,17 +159,18 @@ struct FwdCfg {
 };
 
 template <int DP>
-__global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams p) {
+__global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams p) {
     using C = FwdCfg<DP>;
     extern __shared__ __align__(1024) uint8_t smem[];
     float* const shared_f = reinterpret_cast<float*>(smem + STAGES * C::STAGE);  // [2][128] row statistics
     const uint32_t bars = smem_u32(smem + STAGES * C::STAGE + 1024);
-    auto full = [&](int s) { return bars + 8u * s; };
-    auto s_full = [&](int w) { return bars + 8u * (3 + w); };
-    auto p_full = [&](int w) { return bars + 8u * (5 + w); };
-    auto o_full = [&](int w) { return bars + 8u * (7 + w); };
-    const uint32_t o_free = bars + 8u * 9;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * C::STAGE + 1024 + 128);
+    auto full = [&](int which, int slot) { return bars + 8u * (3 * which + slot); };         // which: 0 k, 1 v
+    auto empty = [&](int which, int slot) { return bars + 8u * (16 + 3 * which + slot); };
+    auto s_full = [&](int j) { return bars + 8u * (6 + (j & 1)); };
+    auto p_full = [&](int j) { return bars + 8u * (8 + (j & 1)); };
+    auto o_full = [&](int j) { return bars + 8u * (10 + (j & 1)); };
+    const uint32_t o_free = bars + 8u * 12, drain = bars + 8u * 13;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * C::STAGE + 1024 + 256);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const TenmoAttnParams& a = p.a;
@@ -181,160 +188,125 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(
     const int64_t tile0 = ((int64_t)b * a.Hkv + kvh) * p.tiles;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1);
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full(0, s), 1); mbar_init(full(1, s), 1); mbar_init(empty(0, s), 1); mbar_init(empty(1, s), 1); }
         for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
         mbar_init(o_free, 4);
+        mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tc::alloc(tmem_slot, C::TMEM);
+    if (warp == C::ISSUER) tc::alloc(tmem_slot, C::TMEM);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    auto load = [&](int j) {  // one thread
-        const uint32_t dst = smem_u32(smem) + (j % STAGES) * C::STAGE, bar = full(j % STAGES);
-        mbar_expect_tx(bar, C::STAGE);
-        tc::bulk_load(dst, p.k_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
-        tc::bulk_load(dst + 2 * C::PLANE, p.v_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
+    // The ring of tiles: slot s holds k and v of a tile j = s mod STAGES, each refilled as soon as its product is done (one thread).
+    int fetched = 0, fetch_slot = 0, fetch_round = 0;
+    auto fetch = [&](int until) {
+        for (; fetched < until; ++fetched) {
+            for (int which = 0; which < 2; ++which) {
+                if (fetch_round && !mbar_wait(empty(which, fetch_slot), (uint32_t)(fetch_round - 1) & 1u, abort_flag)) return;
+                const uint32_t bar = full(which, fetch_slot);
+                mbar_expect_tx(bar, C::IMG);
+                tc::bulk_load(smem_u32(smem) + (fetch_slot * 2 + which) * C::IMG, (which ? p.v_img : p.k_img) + (tile0 + fetched) * C::IMG, C::IMG, bar);
+            }
+            if (++fetch_slot == STAGES) { fetch_slot = 0; ++fetch_round; }
+        }
     };
-    int loaded = 0;
-    if (threadIdx.x == 256)
-        for (; loaded < min(n_tiles, STAGES); ++loaded) load(loaded);
+    if (threadIdx.x == 32 * C::LOADER) fetch(min(n_tiles, STAGES));
 
-    // ---- q into tensor memory: warpgroup w splits columns [w DP/2, (w + 1) DP/2) of its thread's row ----
+    // ---- q into tensor memory ----
     const int wg = warp >> 2, row = threadIdx.x & 127;
     const int64_t i = (int64_t)q_tile * ROWS + row;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float q_inv = 1.f;
-    if (warp < 8)  // the sign of the scale goes with q: the factor of the scores is then never negative
-        q_inv = tenmo_attn_stationary<DP, false>(a.q.ptr + b * a.q.sb + h * a.q.sh + i * a.q.sr, i < q_rows, p.q_vec, a.D, a.scale < 0.f,
+    if (warp < C::ISSUER)  // the sign of the scale goes with q: the factor of the scores is then never negative
+        q_inv = tenmo_attn_stationary<DP, false, C::WGS>(a.q.ptr + b * a.q.sb + h * a.q.sh + i * a.q.sr, i < q_rows, p.q_vec, a.D, a.scale < 0.f,
                                                  wg, row, lane_base, nullptr, shared_f);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
 
-    float m = -INFINITY, l = 0.f, o[DP];
-#pragma unroll
-    for (int d = 0; d < DP; ++d) o[d] = 0.f;
-
-    if (warp == 8) {
-        if (lane == 0) {
+    // rows of the second warpgroup join the first's through these
+    float m = -INFINITY, l = 0.f;
+    float* const buf = reinterpret_cast<float*>(smem);  // the stages, when all products are done
+    if (warp >= C::ISSUER) {
+        if (C::WGS == 2) tc::regs_down<88>();
+        if (warp == C::LOADER) {
+            if (lane == 0) {
+                fetch(n_tiles);
+                // every copy has landed before shared memory is given back (bounded): by now they are the last STAGES tiles'
+                int never = 0;
+                for (int t = max(0, fetched - STAGES); t < fetched; ++t)
+                    for (int which = 0; which < 2; ++which) mbar_wait(full(which, t % STAGES), (uint32_t)(t / STAGES) & 1u, &never);
+            }
+        } else if (warp == C::ISSUER) {
+            const uint32_t tm = tc::uniform(tmem), stages = tc::uniform(smem_u32(smem));
+            const int n = tc::uniform(n_tiles);
             constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_O = tc::idesc_f16(DP, true);
-            bool ok = true;
-            auto wait = [&](uint32_t bar, int phase) { ok = ok && mbar_wait(bar, (uint32_t)phase & 1u, abort_flag); };
+            auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
+            int s_slot = 0, s_phase = 0, s_buf = 0;  // of the next S
             auto scores = [&](int j) {
-                wait(full(j % STAGES), j / STAGES);
-                if (!ok) return;
+                if (!wait(full(0, s_slot), s_phase)) return false;
                 tc::fence_after();
-                const uint32_t hi = smem_u32(smem) + (j % STAGES) * C::STAGE, lo = hi + C::PLANE;
-                const uint32_t d = tmem + C::S_COL + (uint32_t)(j % C::NB) * T;
+                const uint32_t hi = stages + s_slot * C::STAGE, d = tm + C::S_COL + (uint32_t)s_buf * T;
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + DP / 2 + 8 * k, tc::desc_k(hi, T, k), ID_S, k > 0);
+                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + DP / 2 + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, c == 0);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(lo, T, k), ID_S, true);
+                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + C::PLANE + c * T * 128), ID_S, false);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(hi, T, k), ID_S, true);
-                tc::commit(s_full(j & 1));
+                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, false);
+                tc::commit(s_full(j));
+                tc::commit(empty(0, s_slot));
+                if (++s_slot == STAGES) { s_slot = 0; s_phase ^= 1; }
+                if (++s_buf == C::NB) s_buf = 0;
+                return true;
             };
-            if (n_tiles > 0) scores(0);
-            for (int j = 0; ok && j < n_tiles; ++j) {
-                if (j + 1 < n_tiles) {
-                    // the buffer of S_{j+1} held P_{j+1-NB}: with three buffers its product is known to be done (its output was read)
-                    if (C::NB == 2 && j >= 1) wait(o_full((j - 1) & 1), (j - 1) >> 1);
-                    if (ok) scores(j + 1);
-                }
-                wait(p_full(j & 1), j >> 1);
-                if (j >= 1) wait(o_free, j - 1);
+            bool ok = n == 0 || scores(0);
+            int v_slot = 0, v_phase = 0, p_buf = 0;
+            for (int j = 0; ok && j < n; ++j) {
+                // Two buffers: S_{j+1} replaces P_{j-1}, whose product must be done.  Three: P_{j-2}, whose output has been read (o_free below).
+                if (C::NB == 2 && j >= 1) ok = wait(o_full(j - 1), (uint32_t)((j - 1) >> 1) & 1u);
+                if (ok && j + 1 < n) ok = scores(j + 1);
+                ok = ok && wait(full(1, v_slot), v_phase) && wait(p_full(j), (uint32_t)(j >> 1) & 1u) && (j == 0 || wait(o_free, (uint32_t)(j - 1) & 1u));
                 if (!ok) break;
                 tc::fence_after();
-                const uint32_t hi = smem_u32(smem) + (j % STAGES) * C::STAGE + 2 * C::PLANE, lo = hi + C::PLANE;
-                const uint32_t pr = tmem + C::S_COL + (uint32_t)(j % C::NB) * T, d = tmem + C::O_COL;
-                // keys 16 k ..: columns 32 (k / 2) + 8 (k & 1) of the pair chunk, lo 16 columns further
-#pragma unroll
-                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, pr + 32 * (k >> 1) + 16 + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_O, k > 0);
-#pragma unroll
-                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, pr + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(lo, T, k), ID_O, true);
-#pragma unroll
-                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, pr + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_O, true);
-                tc::commit(o_full(j & 1));
-                // tile j - 1 has been read by both of its products (o_free above): its stage takes tile j + 2
-                if (j >= 1 && j + 2 < n_tiles) load(loaded++);
+                const uint32_t hi = stages + v_slot * C::STAGE + C::IMG;
+                const uint32_t pr = tm + C::S_COL + (uint32_t)p_buf * T, d = tm + C::O_COL;
+                // keys 16 k ..: eight columns of hi pairs from 16 k on, then eight of lo pairs
+                tc::mma4_ts<16, tc::STEP_MN>(d, pr + 8, tc::desc_mn(hi, T), ID_O, true);
+                tc::mma4_ts<16, tc::STEP_MN>(d, pr, tc::desc_mn(hi + C::PLANE, T), ID_O, false);
+                tc::mma4_ts<16, tc::STEP_MN>(d, pr, tc::desc_mn(hi, T), ID_O, false);
+                tc::commit(o_full(j));
+                tc::commit(empty(1, v_slot));
+                if (++v_slot == STAGES) { v_slot = 0; v_phase ^= 1; }
+                if (++p_buf == C::NB) p_buf = 0;
             }
-            // Every copy has landed before shared memory is given back, and every MMA is done before tensor memory is: in
-            // order, the readers of O have seen to both; after a wait that ran out, wait again (bounded) here.
+            // Every MMA is done before tensor memory is given back: the readers of O have seen to it; after a wait that ran out, wait
+            // again (bounded) here.
             if (!ok) {
-                const uint32_t drain = bars + 8u * 10;
-                mbar_init(drain, 1);
-                tc::commit(drain);
                 int never = 0;
+                tc::commit(drain);
                 mbar_wait(drain, 0, &never);
-                for (int t = max(0, loaded - STAGES); t < loaded; ++t) mbar_wait(full(t % STAGES), (uint32_t)(t / STAGES) & 1u, &never);
             }
         }
+        __syncthreads();
+        if (C::WGS == 2) __syncthreads();
     } else {
+        if (C::WGS == 2) tc::regs_up<208>();
+        float o[DP];
+#pragma unroll
+        for (int d = 0; d < DP; ++d) o[d] = 0.f;
         const float c_row = fabsf(a.scale_log2) * q_inv;
         int n_row = i < q_rows ? keys : 0;
         if (a.causal) n_row = min(n_row, (int)max((int64_t)0, i + a.Sk - a.Sq + 1));
         bool ok = true;
-        for (int j = wg; j < n_tiles; j += 2) {
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full(wg), (uint32_t)(j >> 1) & 1u, abort_flag));
-            if (!ok) break;
-            tc::fence_after();
-            const float c = c_row * __ldg(p.k_inv + tile0 + j), v_inv = __ldg(p.v_inv + tile0 + j);
-            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T;
-            const int lim = n_row - j * T;
-            const bool whole = __all_sync(0xffffffffu, lim >= T);
-            float mx = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < T / 32; ++g) {
-                float s[32];
-                tc::ld32(s_addr + 32 * g, s);
-                if (!whole) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e] = 32 * g + e < lim ? s[e] : -INFINITY;
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
-            }
-            const float m_new = mx == -INFINITY ? m : fmaxf(m, ceilf(mx * c));
-            const float shrink = m == -INFINITY ? 0.f : tc::ex2(m - m_new);
-            m = m_new;
-            // p = 2^15 exp2(s c - m): the factor 2^15 brings p into fp16's range and divides out with l
-            const float base = m == -INFINITY ? 0.f : 15.f - m;
-            const uint64_t c2 = tc::pack2(c, c), b2 = tc::pack2(base, base);
-            uint64_t sum2 = 0;
-#pragma unroll
-            for (int g = 0; g < T / 32; ++g) {
-                float s[32];
-                tc::ld32(s_addr + 32 * g, s);
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float x, y;
-                    tc::unpack2(tc::fma2(tc::pack2(s[2 * e], s[2 * e + 1]), c2, b2), x, y);
-                    x = tc::ex2(x);
-                    y = tc::ex2(y);
-                    if (!whole) {
-                        x = 32 * g + 2 * e < lim ? x : 0.f;
-                        y = 32 * g + 2 * e + 1 < lim ? y : 0.f;
-                    }
-                    sum2 = tc::add2(sum2, tc::pack2(x, y));
-                    tc::split_pair(x, y, hi[e], lo[e]);
-                }
-                tc::st16(s_addr + 32 * g, hi);
-                tc::st16(s_addr + 32 * g + 16, lo);
-            }
-            tc::st_wait();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(wg));
-            float x, y;
-            tc::unpack2(sum2, x, y);
-            l = fmaf(l, shrink, x + y);
-            ok = __all_sync(0xffffffffu, mbar_wait(o_full(wg), (uint32_t)(j >> 1) & 1u, abort_flag));
-            if (!ok) break;
+        auto await = [&](uint32_t bar, int phase) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, abort_flag)); };
+        float shrink = 0.f, v_inv = 0.f;  // of the tile whose output is next
+        auto add_output = [&](int j) {    // o = o * shrink + O_j
+            await(o_full(j), j >> 1);
+            if (!ok) return;
             tc::fence_after();
             const uint64_t sh2 = tc::pack2(shrink, shrink), vi2 = tc::pack2(v_inv, v_inv);
 #pragma unroll
@@ -350,43 +322,126 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(
             tc::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
+        };
+        for (int j = wg; j < n_tiles; j += C::WGS) {
+            const float c = c_row * __ldg(p.k_inv + tile0 + j), v_next = __ldg(p.v_inv + tile0 + j);
+            await(s_full(j), j >> 1);
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T;
+            const int lim = n_row - j * T;
+            const bool whole = __all_sync(0xffffffffu, lim >= T);
+            float s[T];  // dim 128: only for the maximum, and loaded again in parts for the exponentials
+            tc::ld64(s_addr, s);
+            float mx = -INFINITY;
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < T; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
+            } else {
+#pragma unroll
+                for (int e = 0; e < T; ++e) mx = fmaxf(mx, e < lim ? s[e] : -INFINITY);
+            }
+            const float m_new = mx == -INFINITY ? m : fmaxf(m, ceilf(mx * c));
+            const float shrink_next = m == -INFINITY ? 0.f : tc::ex2(m - m_new);
+            m = m_new;
+            // p = 2^15 exp2(s c - m): the factor 2^15 brings p into fp16's range and divides out with l
+            const float base = m == -INFINITY ? 0.f : 15.f - m;
+            const uint64_t c2 = tc::pack2(c, c), b2 = tc::pack2(base, base);
+            uint64_t sum2 = 0;
+#pragma unroll
+            for (int g = 0; g < T / 16; ++g) {
+                float r[16];
+                if (DP == 128) {
+                    tc::ld16(s_addr + 16 * g, r);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) r[e] = s[16 * g + e];
+                }
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x, y;
+                    tc::unpack2(tc::fma2(tc::pack2(r[2 * e], r[2 * e + 1]), c2, b2), x, y);
+                    x = tc::ex2(x);
+                    y = tc::ex2(y);
+                    if (!whole) {
+                        x = 16 * g + 2 * e < lim ? x : 0.f;
+                        y = 16 * g + 2 * e + 1 < lim ? y : 0.f;
+                    }
+                    sum2 = tc::add2(sum2, tc::pack2(x, y));
+                    tc::split_pair(x, y, hi[e], lo[e]);
+                }
+                // 16 keys: columns 16 g .. + 7 the hi pairs, + 8 .. + 15 the lo pairs (the scores that they replace have been read)
+                tc::st8(s_addr + 16 * g, hi);
+                tc::st8(s_addr + 16 * g + 8, lo);
+            }
+            tc::st_wait();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(j));
+            float x, y;
+            tc::unpack2(sum2, x, y);
+            l = fmaf(l, shrink_next, x + y);
+            // one warpgroup: the output of the tile before, whose product ran meanwhile; two: this tile's (the other one works on)
+            if (C::WGS == 1) {
+                if (j > 0) add_output(j - 1);
+                shrink = shrink_next;
+                v_inv = v_next;
+            } else {
+                shrink = shrink_next;
+                v_inv = v_next;
+                add_output(j);
+            }
+            if (!ok) break;
         }
-    }
-    __syncthreads();
+        if (C::WGS == 1 && ok && n_tiles > 0) add_output(n_tiles - 1);
 
-    // ---- join the two warpgroups: 16-byte chunk q of row r lies at chunk q ^ (r & 7) of the buffer (the stages are free) ----
-    float* const buf = reinterpret_cast<float*>(smem);
-    float* const ms = shared_f;  // m and l of the second warpgroup
-    if (warp >= 4 && warp < 8) {
-        ms[row] = m;
-        ms[128 + row] = l;
+        // ---- to the output: 16-byte chunk q of row r lies at chunk q ^ (r & 7) of the buffer ----
+        __syncthreads();
+        auto at = [&](int d) { return reinterpret_cast<float4*>(buf + row * DP + (((d >> 2) ^ (row & 7)) << 2)); };
+        float f = 1.f;
+        if (C::WGS == 2) {
+            if (wg == 1) {
+                shared_f[row] = m;
+                shared_f[128 + row] = l;
 #pragma unroll
-        for (int d = 0; d < DP; d += 4)
-            *reinterpret_cast<float4*>(buf + row * DP + (((d >> 2) ^ (row & 7)) << 2)) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-    }
-    __syncthreads();
-    if (warp < 4) {
-        const float m1 = ms[row], l1 = ms[128 + row], top = fmaxf(m, m1);
-        const float f0 = m == -INFINITY ? 0.f : tc::ex2(m - top), f1 = m1 == -INFINITY ? 0.f : tc::ex2(m1 - top);
-        const float sum = l * f0 + l1 * f1;
-        // rows without keys: sum 0, output 0 (0 * 0); a NaN in the sum reaches the output
-        const float inv = sum == 0.f ? 0.f : 1.f / sum, g0 = f0 * inv, g1 = f1 * inv;
-#pragma unroll
-        for (int d = 0; d < DP; d += 4) {
-            float4* at = reinterpret_cast<float4*>(buf + row * DP + (((d >> 2) ^ (row & 7)) << 2));
-            const float4 x = *at;
-            *at = make_float4(o[d] * g0 + x.x * g1, o[d + 1] * g0 + x.y * g1, o[d + 2] * g0 + x.z * g1, o[d + 3] * g0 + x.w * g1);
+                for (int d = 0; d < DP; d += 4) *at(d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+            }
+            __syncthreads();
         }
-        if (a.stats && i < a.Sq) {
-            float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + i) * 2;
-            st[0] = top;
-            st[1] = sum * 3.0517578125e-5f;  // 2^-15
+        if (wg == 0) {
+            float f1 = 0.f;
+            if (C::WGS == 2) {
+                const float m1 = shared_f[row], top = fmaxf(m, m1);
+                f = m == -INFINITY ? 0.f : tc::ex2(m - top);
+                f1 = m1 == -INFINITY ? 0.f : tc::ex2(m1 - top);
+                l = l * f + shared_f[128 + row] * f1;
+                m = top;
+            }
+            // rows without keys: sum 0, output 0 (0 * 0); a NaN in the sum reaches the output
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            f *= inv;
+            f1 *= inv;
+#pragma unroll
+            for (int d = 0; d < DP; d += 4) {
+                float4 x = make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
+                if (C::WGS == 2) {
+                    const float4 u = *at(d);
+                    x.x = fmaf(u.x, f1, x.x); x.y = fmaf(u.y, f1, x.y); x.z = fmaf(u.z, f1, x.z); x.w = fmaf(u.w, f1, x.w);
+                }
+                *at(d) = x;
+            }
+            if (a.stats && i < a.Sq) {
+                float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + i) * 2;
+                st[0] = m;
+                st[1] = l * 3.0517578125e-5f;  // 2^-15
+            }
         }
     }
     __syncthreads();
     const int rows_here = min(ROWS, a.Sq - q_tile * ROWS);
     float* out = a.o.ptr + b * a.o.sb + h * a.o.sh + (int64_t)q_tile * ROWS * a.o.sr;
-    for (int e = threadIdx.x; e < rows_here * (DP / 4); e += THREADS) {
+    for (int e = threadIdx.x; e < rows_here * (DP / 4); e += C::THREADS) {
         const int r = e / (DP / 4), q = e % (DP / 4), d = 4 * q;
         if (d >= a.D) continue;
         const float4 x = *reinterpret_cast<const float4*>(buf + r * DP + ((q ^ (r & 7)) << 2));
@@ -401,7 +456,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(
     tc::fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, TENMO_DEV_TIMEOUT);
-    if (warp == 8) {
+    if (warp == C::ISSUER) {
         tc::fence_after();
         tc::dealloc(tmem, C::TMEM);
     }
@@ -462,9 +517,11 @@ int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     if ((st = tenmo_attn_make_tiles(ctx, jobs, 2, dp)) != TENMO_OK) return st;
     const unsigned grid = (unsigned)((int64_t)a.B * a.H * p.q_tiles);
     if (dp == 64) {
+        constexpr int THREADS = FwdCfg<64>::THREADS;
         TENMO_CUDA_TRY(ctx, cudaFuncSetAttribute(attn_fwd_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdCfg<64>::SMEM));
         attn_fwd_tc_kernel<64><<<grid, THREADS, FwdCfg<64>::SMEM, ctx->stream>>>(p);
     } else {
+        constexpr int THREADS = FwdCfg<128>::THREADS;
         TENMO_CUDA_TRY(ctx, cudaFuncSetAttribute(attn_fwd_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdCfg<128>::SMEM));
         attn_fwd_tc_kernel<128><<<grid, THREADS, FwdCfg<128>::SMEM, ctx->stream>>>(p);
     }

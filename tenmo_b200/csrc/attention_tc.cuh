@@ -18,7 +18,7 @@ struct TenmoTileJob {
     int heads, rows, tiles, vec;
     // With o.ptr set (src is the gradient of o): the per-row numbers of the backward pass as well.  Per tile 256 floats:
     // [0, 64) m_i (+inf for rows that take no part), [64, 128) 1 / l_i times the tile's power of two PS that brings the largest
-    // to at most 2^15 (0 for those rows), [128, 192) delta_i, 192: PS, 193: the largest |delta|; [194 ..) unused.
+    // to at most 2^15 (0 for those rows), [128, 192) delta_i, 192: PS, 193: the largest |delta|, 194: 1 / PS; the rest is unused.
     TenmoHeadsView o;
     const float* stats;
     float* info;
@@ -33,13 +33,13 @@ int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, 
 bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D);
 static inline int tenmo_attn_padded(int D) { return D <= 64 ? 64 : 128; }
 
-// This warpgroup's columns [wg * DP / 2, (wg + 1) * DP / 2) of a row of an operand, split into fp16 pairs scaled by the row's
-// power of two, into tensor memory (hi from `addr` on, lo DP / 2 columns further) or, with `plane` set, into a 128-row tile image
-// in shared memory.  Called by the 256 threads of two warpgroups; `exchange` holds 256 floats.  Returns the inverse scale.
-template <int DP, bool SMEM>
+// A row of an operand, split into fp16 pairs scaled by the row's power of two, into tensor memory (hi from `addr` on, lo DP / 2
+// columns further) or, with `plane` set, into a 128-row tile image in shared memory.  Called by the threads of WGS warpgroups, which
+// share the columns of a row; `exchange` holds 256 floats.  Returns the inverse scale.
+template <int DP, bool SMEM, int WGS>
 __device__ __forceinline__ float tenmo_attn_stationary(const float* src, bool in, bool vec, int D, bool negate, int wg, int row,
                                                        uint32_t addr, uint8_t* plane, float* exchange) {
-    constexpr int W = DP / 2;
+    constexpr int W = DP / WGS;
     float x[W];
     float mx = 0.f;
 #pragma unroll
@@ -55,10 +55,12 @@ __device__ __forceinline__ float tenmo_attn_stationary(const float* src, bool in
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx = fmaxf(mx, tc::finite_abs(x[e + u]));
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");  // an earlier use of `exchange` is over
-    exchange[wg * 128 + row] = mx;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    mx = fmaxf(mx, exchange[(wg ^ 1) * 128 + row]);
+    if (WGS == 2) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // an earlier use of `exchange` is over
+        exchange[wg * 128 + row] = mx;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        mx = fmaxf(mx, exchange[(wg ^ 1) * 128 + row]);
+    }
     float inverse;
     float scale = tc::block_scale(mx, &inverse);
     if (negate) scale = -scale;

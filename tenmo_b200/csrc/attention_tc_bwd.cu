@@ -43,7 +43,7 @@ template <int DP, bool DKV>
 struct BwdCfg {
     static constexpr int NB = DP == 64 ? 2 : 1;
     static constexpr bool X2S = DKV && DP == 128;  // X2 in shared memory
-    static constexpr int STAGES = X2S ? 2 : 3;
+    static constexpr int STAGES = DP == 64 ? 5 : X2S ? 2 : 3;
     static constexpr int PLANE = T * DP * 2;
     static constexpr int STAGE = 4 * PLANE + (DKV ? 1024 : 0);  // Y1 hi, lo, Y2 hi, lo, row numbers
     static constexpr int X2_BYTES = X2S ? ROWS * DP * 4 : 0;
@@ -64,15 +64,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
     uint8_t* const x2_plane = smem + C::STAGES * C::STAGE;
     float* const exchange = reinterpret_cast<float*>(smem + C::TILES);
     const uint32_t bars = smem_u32(smem + C::TILES + 1024);
-    auto full = [&](int s) { return bars + 8u * s; };
-    auto s_full = [&](int j) { return bars + 8u * (3 + (j & 1)); };
-    auto d_full = [&](int j) { return bars + 8u * (5 + (j & 1)); };
+    auto full = [&](int slot) { return bars + 8u * (16 + slot); };
+    auto empty = [&](int slot) { return bars + 8u * (24 + slot); };
+    auto s_full = [&](int j) { return bars + 8u * (j & 1); };
+    auto d_full = [&](int j) { return bars + 8u * (2 + (j & 1)); };
     // a warp may be a tile ahead of another one: what the eight warps arrive on has a barrier for even and one for odd tiles
     auto p_full = [&](int j) { return bars + 8u * (7 + (j & 1)); };
     auto ds_full = [&](int j) { return bars + 8u * (9 + (j & 1)); };
-    const uint32_t s_read = bars + 8u * 11, pv_done = bars + 8u * 12;
-    const uint32_t acc_full = bars + 8u * 13, acc_free = bars + 8u * 14, drain = bars + 8u * 15;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 1024 + 128);
+    auto s_read = [&](int j) { return bars + 8u * (4 + (j & 1)); };
+    const uint32_t pv_done = bars + 8u * 11, acc_full = bars + 8u * 12, acc_free = bars + 8u * 13, drain = bars + 8u * 14;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 1024 + 256);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const TenmoAttnParams& a = p.a;
@@ -103,9 +104,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
     const int64_t tile0 = ((int64_t)b * y_heads + yh) * p.tiles + first;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 3; ++s) mbar_init(full(s), 1);
-        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(d_full(w), 1); mbar_init(p_full(w), 8); mbar_init(ds_full(w), 8); }
-        mbar_init(s_read, 8);
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(d_full(w), 1); mbar_init(p_full(w), 8); mbar_init(ds_full(w), 8); mbar_init(s_read(w), 8); }
         mbar_init(pv_done, 1);
         mbar_init(acc_full, 1);
         mbar_init(acc_free, 8);
@@ -120,23 +120,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
     const uint32_t tmem = *tmem_slot;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 
-    auto load = [&](int j) {  // one thread
-        const uint32_t dst = smem_u32(smem) + (j % C::STAGES) * C::STAGE, bar = full(j % C::STAGES);
-        mbar_expect_tx(bar, 4 * C::PLANE + (DKV ? 1024u : 0u));
-        tc::bulk_load(dst, p.y1_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
-        tc::bulk_load(dst + 2 * C::PLANE, p.y2_img + (tile0 + j) * (2 * C::PLANE), 2 * C::PLANE, bar);
-        if (DKV) tc::bulk_load(dst + 4 * C::PLANE, p.info + (tile0 + j) * ATTN_INFO, 1024, bar);
+    // the ring of tiles (one thread): a slot is refilled when all products of its tile are done
+    int fetched = 0, fetch_slot = 0, fetch_round = 0;
+    auto fetch = [&](int until) {
+        for (; fetched < until; ++fetched) {
+            if (fetch_round && !mbar_wait(empty(fetch_slot), (uint32_t)(fetch_round - 1) & 1u, abort_flag)) return;
+            const uint32_t dst = smem_u32(smem) + fetch_slot * C::STAGE, bar = full(fetch_slot);
+            mbar_expect_tx(bar, 4 * C::PLANE + (DKV ? 1024u : 0u));
+            tc::bulk_load(dst, p.y1_img + (tile0 + fetched) * (2 * C::PLANE), 2 * C::PLANE, bar);
+            tc::bulk_load(dst + 2 * C::PLANE, p.y2_img + (tile0 + fetched) * (2 * C::PLANE), 2 * C::PLANE, bar);
+            if (DKV) tc::bulk_load(dst + 4 * C::PLANE, p.info + (tile0 + fetched) * ATTN_INFO, 1024, bar);
+            if (++fetch_slot == C::STAGES) { fetch_slot = 0; ++fetch_round; }
+        }
     };
-    int loaded = 0;
-    if (threadIdx.x == 256)
-        for (; loaded < min(n, C::STAGES); ++loaded) load(loaded);
+    if (threadIdx.x == 32 * 9) fetch(min(n, C::STAGES));
 
     float x1_inv = 1.f, x2_inv = 1.f;
     if (warp < 8) {
         const int xh = DKV ? kvh : h;
-        x1_inv = tenmo_attn_stationary<DP, false>(p.x1.ptr + b * p.x1.sb + xh * p.x1.sh + i * p.x1.sr, i < x_rows, p.x1_vec, a.D,
+        x1_inv = tenmo_attn_stationary<DP, false, 2>(p.x1.ptr + b * p.x1.sb + xh * p.x1.sh + i * p.x1.sr, i < x_rows, p.x1_vec, a.D,
                                                   a.scale < 0.f, wg, row, lane_base, nullptr, exchange);
-        x2_inv = tenmo_attn_stationary<DP, C::X2S>(p.x2.ptr + b * p.x2.sb + xh * p.x2.sh + i * p.x2.sr, i < x_rows, p.x2_vec, a.D, false,
+        x2_inv = tenmo_attn_stationary<DP, C::X2S, 2>(p.x2.ptr + b * p.x2.sb + xh * p.x2.sh + i * p.x2.sr, i < x_rows, p.x2_vec, a.D, false,
                                                    wg, row, lane_base + C::X2_COL, x2_plane, exchange);
     }
     tc::fence_before();
@@ -144,115 +148,110 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
     tc::fence_after();
 
     if (warp >= 8) {
-        tc::regs_down<40>();
-        if (threadIdx.x == 256) {
+        tc::regs_down<88>();
+        if (warp == 9) {
+            if (lane == 0) {
+                fetch(n);
+                // every copy has landed before shared memory is given back (bounded)
+                int never = 0;
+                for (int t = max(0, fetched - C::STAGES); t < fetched; ++t) mbar_wait(full(t % C::STAGES), (uint32_t)(t / C::STAGES) & 1u, &never);
+            }
+        } else if (warp == 8) {
+            const uint32_t tm = tc::uniform(tmem), stages = tc::uniform(smem_u32(smem));
+            const int tiles = tc::uniform(n);
             constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_G = tc::idesc_f16(DP, true);
-            bool ok = true;
-            auto wait = [&](uint32_t bar, int phase) { ok = ok && mbar_wait(bar, (uint32_t)phase & 1u, abort_flag); };
-            auto y1 = [&](int j) { return smem_u32(smem) + (j % C::STAGES) * C::STAGE; };
-            auto scores = [&](int j) {  // S_j
-                wait(full(j % C::STAGES), j / C::STAGES);
-                if (!ok) return;
-                tc::fence_after();
-                const uint32_t hi = y1(j), lo = hi + C::PLANE, d = tmem + C::S_COL + (uint32_t)(j % NB) * T;
+            auto wait = [&](uint32_t bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, abort_flag)) != 0; };
+            // S or dP: D = X Y^T over the columns; x: tensor memory (hi, then lo DP / 2 columns further)
+            auto over_columns = [&](uint32_t d, uint32_t x, uint32_t hi) {
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + DP / 2 + 8 * k, tc::desc_k(hi, T, k), ID_S, k > 0);
+                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, x + DP / 2 + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, c == 0);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(lo, T, k), ID_S, true);
+                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, x + 32 * c, tc::desc_k(hi + C::PLANE + c * T * 128), ID_S, false);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, tmem + 8 * k, tc::desc_k(hi, T, k), ID_S, true);
-                tc::commit(s_full(j));
+                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, x + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, false);
             };
-            auto grads = [&](int j) {  // dP_j (its tile has arrived: S_j was issued before)
-                if (!ok) return;
-                const uint32_t hi = y1(j) + 2 * C::PLANE, lo = hi + C::PLANE, d = tmem + C::P_COL + (uint32_t)(j % NB) * T;
+            int s_slot = 0, s_phase = 0;  // of the next S
+            auto scores = [&](int j) {
+                if (!wait(full(s_slot), s_phase)) return false;
+                tc::fence_after();
+                over_columns(tm + C::S_COL + (uint32_t)(j % NB) * T, tm, stages + s_slot * C::STAGE);
+                tc::commit(s_full(j));
+                return true;
+            };
+            auto grads = [&](int j) {  // dP_j; its tile has arrived: S_j was issued before
+                const uint32_t hi = stages + s_slot * C::STAGE + 2 * C::PLANE, d = tm + C::P_COL + (uint32_t)(j % NB) * T;
                 if (C::X2S) {
-                    const uint32_t xh = smem_u32(x2_plane), xl = xh + ROWS * DP * 2;
+                    const uint32_t xh = stages + C::STAGES * C::STAGE, xl = xh + ROWS * DP * 2;
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) tc::mma_ss(d, tc::desc_k(xl, ROWS, k), tc::desc_k(hi, T, k), ID_S, k > 0);
+                    for (int c = 0; c < DP / 64; ++c)
+                        tc::mma4_ss<tc::STEP_K, tc::STEP_K>(d, tc::desc_k(xl + c * ROWS * 128), tc::desc_k(hi + c * T * 128), ID_S, c == 0);
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) tc::mma_ss(d, tc::desc_k(xh, ROWS, k), tc::desc_k(lo, T, k), ID_S, true);
+                    for (int c = 0; c < DP / 64; ++c)
+                        tc::mma4_ss<tc::STEP_K, tc::STEP_K>(d, tc::desc_k(xh + c * ROWS * 128), tc::desc_k(hi + C::PLANE + c * T * 128), ID_S, false);
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) tc::mma_ss(d, tc::desc_k(xh, ROWS, k), tc::desc_k(hi, T, k), ID_S, true);
+                    for (int c = 0; c < DP / 64; ++c)
+                        tc::mma4_ss<tc::STEP_K, tc::STEP_K>(d, tc::desc_k(xh + c * ROWS * 128), tc::desc_k(hi + c * T * 128), ID_S, false);
                 } else {
-                    const uint32_t x = tmem + C::X2_COL;
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, x + DP / 2 + 8 * k, tc::desc_k(hi, T, k), ID_S, k > 0);
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, x + 8 * k, tc::desc_k(lo, T, k), ID_S, true);
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) tc::mma_ts(d, x + 8 * k, tc::desc_k(hi, T, k), ID_S, true);
+                    over_columns(d, tm + C::X2_COL, hi);
                 }
                 tc::commit(d_full(j));
+                if (++s_slot == C::STAGES) { s_slot = 0; s_phase ^= 1; }
             };
-            // D += A Y over the rows of the tile; A: fp16 pairs over a 64-column buffer, keys 16 k .. in columns 32 (k / 2) + 8 (k & 1)
-            auto times_y = [&](uint32_t d, uint32_t x, uint32_t hi) {
-                const uint32_t lo = hi + C::PLANE;
-#pragma unroll
-                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, x + 32 * (k >> 1) + 16 + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_G, k > 0);
-#pragma unroll
-                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, x + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(lo, T, k), ID_G, true);
-#pragma unroll
-                for (int k = 0; k < T / 16; ++k) tc::mma_ts(d, x + 32 * (k >> 1) + 8 * (k & 1), tc::desc_mn(hi, T, k), ID_G, true);
+            // D = A Y over the rows of the tile; A: rows 16 k .. in eight columns of hi pairs from 16 k on, then eight of lo pairs
+            auto over_rows = [&](uint32_t d, uint32_t x, uint32_t hi) {
+                tc::mma4_ts<16, tc::STEP_MN>(d, x + 8, tc::desc_mn(hi, T), ID_G, true);
+                tc::mma4_ts<16, tc::STEP_MN>(d, x, tc::desc_mn(hi + C::PLANE, T), ID_G, false);
+                tc::mma4_ts<16, tc::STEP_MN>(d, x, tc::desc_mn(hi, T), ID_G, false);
             };
-            if (n > 0) {
-                scores(0);
-                grads(0);
+            // Order: the products of tile j that use P_j and dS_j, then S and dP of tile j + NB, which replace them.  Each waits for
+            // something that is done while another product runs: S for P_j v (dkv) or for S_j's readers (dq), dP for the products of dS_j.
+            bool ok = true;
+            for (int j = 0; ok && j < min(tiles, NB); ++j) {
+                ok = scores(j);
+                if (ok) grads(j);
             }
-            for (int j = 0; ok && j < n; ++j) {
-                const uint32_t s = tmem + C::S_COL + (uint32_t)(j % NB) * T, ds = tmem + C::P_COL + (uint32_t)(j % NB) * T;
-                const bool more = j + 1 < n;
-                if (NB == 2) {
-                    // the buffers of tile j + 1 were last read by the products of tile j - 1
-                    if (j >= 1) wait(acc_full, j - 1);
-                    if (more) { scores(j + 1); grads(j + 1); }
-                } else if (!DKV && more) {
-                    wait(s_read, j);  // S_j is in registers, nothing is written back
-                    scores(j + 1);
+            int slot = 0;  // of tile j
+            for (int j = 0; ok && j < tiles; ++j) {
+                const uint32_t s = tm + C::S_COL + (uint32_t)(j % NB) * T, ds = tm + C::P_COL + (uint32_t)(j % NB) * T, y1 = stages + slot * C::STAGE;
+                const bool more = j + NB < tiles;
+                if (!DKV && NB == 1 && more) {  // one buffer: S_{j+1} runs while the warpgroups make dS_j
+                    ok = wait(s_read(j), j >> 1) && scores(j + 1);
+                    if (!ok) break;
                 }
                 if (DKV) {
-                    wait(p_full(j), j >> 1);
-                    if (j >= 1) wait(acc_free, j - 1);
+                    ok = wait(p_full(j), j >> 1) && (j == 0 || wait(acc_free, j - 1));
                     if (!ok) break;
                     tc::fence_after();
-                    times_y(tmem + C::A2_COL, s, y1(j) + 2 * C::PLANE);
-                    if (NB == 1) tc::commit(pv_done);
+                    over_rows(tm + C::A2_COL, s, y1 + 2 * C::PLANE);
+                    tc::commit(pv_done);
                 }
-                wait(ds_full(j), j >> 1);
-                if (!DKV && j >= 1) wait(acc_free, j - 1);
+                ok = wait(ds_full(j), j >> 1) && (DKV || j == 0 || wait(acc_free, j - 1));
                 if (!ok) break;
                 tc::fence_after();
-                times_y(tmem + C::A1_COL, ds, y1(j));
+                over_rows(tm + C::A1_COL, ds, y1);
                 tc::commit(acc_full);
-                if (NB == 1 && more) {
-                    if (DKV) {
-                        wait(pv_done, j);  // P_j has been read
-                        scores(j + 1);
-                    }
-                    wait(acc_full, j);  // dS_j has been read
+                tc::commit(empty(slot));  // the tile is over
+                if (++slot == C::STAGES) slot = 0;
+                if (more) {
+                    if (DKV) ok = wait(pv_done, j) && scores(j + NB);                        // P_j has been read
+                    else if (NB == 2) ok = wait(s_read(j), j >> 1) && scores(j + NB);       // S_j has (long ago)
+                    ok = ok && wait(acc_full, j);                                           // dS_j has been read
+                    if (!ok) break;
                     tc::fence_after();
-                    grads(j + 1);
-                }
-                // refill: with NB == 2 tile j - 1 is over (acc_full above), with NB == 1 tile j is (acc_full)
-                if (NB == 2) {
-                    if (j >= 1 && loaded < n) { load(loaded); ++loaded; }
-                } else if (more && loaded < n) {
-                    load(loaded);
-                    ++loaded;
+                    grads(j + NB);
                 }
             }
-            if (!ok) {  // a wait ran out: see the copies and MMAs in flight to their end (bounded) before memory is given back
+            if (!ok) {  // a wait ran out: see the MMAs in flight to their end (bounded) before tensor memory is given back
                 tc::commit(drain);
                 int never = 0;
                 mbar_wait(drain, 0, &never);
-                for (int t = max(0, loaded - C::STAGES); t < loaded; ++t) mbar_wait(full(t % C::STAGES), (uint32_t)(t / C::STAGES) & 1u, &never);
             }
         }
         __syncthreads();
         __syncthreads();
         if (DKV) { __syncthreads(); __syncthreads(); }
     } else {
-        tc::regs_up<232>();
+        tc::regs_up<208>();
         float acc1[W], acc2[DKV ? W : 1];
 #pragma unroll
         for (int d = 0; d < W; ++d) acc1[d] = 0.f;
@@ -299,13 +298,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_free);
         };
+        float y1_next = n > 0 ? __ldg(p.y1_inv + tile0) : 1.f, y2_next = n > 0 ? __ldg(p.y2_inv + tile0) : 1.f;
         for (int j = 0; j < n; ++j) {
             // one buffer, dkv pass: the sums of tile j - 1 are taken first, while S_j is being computed
             if (NB == 1 && DKV && j >= 1) add_tile(j - 1);
+            const float y1_inv = y1_next, y2_inv = y2_next;  // loaded a tile ahead: they come from L2
+            if (j + 1 < n) {
+                y1_next = __ldg(p.y1_inv + tile0 + j + 1);
+                y2_next = __ldg(p.y2_inv + tile0 + j + 1);
+            }
             await(s_full(j), j >> 1);
             if (!ok) break;
             tc::fence_after();
-            const float y1_inv = __ldg(p.y1_inv + tile0 + j), y2_inv = __ldg(p.y2_inv + tile0 + j);
             const float c = c_row * y1_inv;
             const float f = x2_inv * y2_inv;  // dP = f * accumulator
             const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % NB) * T + 32 * wg, d_addr = lane_base + C::P_COL + (uint32_t)(j % NB) * T + 32 * wg;
@@ -315,10 +319,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
             float G;  // power of two: dS at most 2^15
             uint64_t nd2, fg2;
             const float* info = nullptr;
+            float ps_inv = 1.f;  // read before dS is handed over: the stage may be refilled from then on
             if (DKV) {
                 await(full(j % C::STAGES), j / C::STAGES);  // the row numbers that came with the tile
                 if (!ok) break;
                 info = reinterpret_cast<const float*>(smem + (j % C::STAGES) * C::STAGE + 4 * C::PLANE);
+                ps_inv = info[3 * T + 2];
                 G = tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, info[3 * T + 1]));
                 fg2 = tc::pack2(f * G, f * G);
                 nd2 = tc::pack2(-G, -G);
@@ -342,8 +348,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
                     e[2 * u + 1] = y;
                     tc::split_pair(x, y, hi[u], lo[u]);
                 }
-                tc::st16(s_addr, hi);
-                tc::st16(s_addr + 16, lo);
+                tc::st_pairs(s_addr, hi, lo);
                 tc::st_wait();
                 tc::fence_before();
                 __syncwarp();
@@ -351,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
             } else {
                 tc::fence_before();
                 __syncwarp();
-                if (NB == 1 && lane == 0) mbar_arrive(s_read);
+                if (lane == 0) mbar_arrive(s_read(j));
                 G = 32768.f * tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, fabsf(delta_row)));
                 fg2 = tc::pack2(f * G, f * G);
                 nd2 = tc::pack2(-delta_row * G, -delta_row * G);
@@ -393,8 +398,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
                     tc::unpack2(v, x, y);
                     tc::split_pair(x, y, hi[u], lo[u]);
                 }
-                tc::st16(d_addr, hi);
-                tc::st16(d_addr + 16, lo);
+                tc::st_pairs(d_addr, hi, lo);
             }
             tc::st_wait();
             tc::fence_before();
@@ -403,11 +407,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
             if (NB == 2 && j >= 1) add_tile(j - 1);
             // now the factors of tile j
             if (DKV) {
-                const float ps_inv = 1.f / info[3 * T];
-                f1 = a.scale * y1_inv * ps_inv / G;
+                f1 = a.scale * y1_inv * ps_inv * tc::pow2_inverse(G);
                 f2 = y2_inv * ps_inv;
             } else {
-                f1 = a.scale * il_row * y1_inv / G;
+                f1 = a.scale * il_row * y1_inv * tc::pow2_inverse(G);
             }
         }
         if (ok && n > 0) add_tile(n - 1);

@@ -33,26 +33,56 @@ __device__ __forceinline__ void alloc(uint32_t* slot, uint32_t cols) {
 __device__ __forceinline__ void dealloc(uint32_t base, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
 }
-// arrives on `bar` when all MMAs issued so far by this thread are done
+// MMAs and commits are written for a whole converged warp, and one elected lane (always the same) executes them: what they are
+// computed from then is uniform over the warp and the compiler keeps it in uniform registers, where the tensor core wants it.  Issued
+// from a branch that a single thread takes, every MMA cost about 85 cycles of register moves, more than most take to run.
+// arrives on `bar` when all MMAs issued so far are done
 __device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// D[tmem] (+)= A[smem] . B[smem]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
-// D[tmem] (+)= A[tmem] . B[smem]: A holds row r in lane r, two fp16 per 32-bit column
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// Four steps of a product (64 of the contraction): D[tmem] (+)= A . B, B in shared memory.  A tensor-memory operand (TS) holds row r
+// in lane r, two fp16 per 32-bit column, and a step is AS columns further; of a shared-memory operand (SS), as of B, a step is
+// AS / BS units of 16 bytes, an addition to the descriptor's low word (the address; a tile ends below 256 KB).  `first`: the first
+// step overwrites D.  One election serves the four; the high words are constants.
+struct Desc { uint32_t lo, hi; };
+template <int AS, int BS>
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, Desc b, uint32_t idesc, bool first) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 b0, b1, b2, b3;\n\t.reg .b32 l1, l2, l3, a1, a2, a3;\n\t"
+        "add.u32 l1, %2, %6;\n\tadd.u32 l2, %2, %7;\n\tadd.u32 l3, %2, %8;\n\t"
+        "add.u32 a1, %1, %9;\n\tadd.u32 a2, %1, %10;\n\tadd.u32 a3, %1, %11;\n\t"
+        "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {l1, %3};\n\tmov.b64 b2, {l2, %3};\n\tmov.b64 b3, {l3, %3};\n\t"
+        "setp.eq.b32 p, %5, 0;\n\tsetp.eq.b32 q, 0, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b0, %4, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %4, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %4, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %4, q;\n\t}"
+        ::"r"(d), "r"(a), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"((uint32_t)first), "n"(BS), "n"(2 * BS), "n"(3 * BS), "n"(AS), "n"(2 * AS), "n"(3 * AS)
         : "memory");
 }
+template <int AS, int BS>
+__device__ __forceinline__ void mma4_ss(uint32_t d, Desc a, Desc b, uint32_t idesc, bool first) {
+    asm volatile(
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t.reg .b32 l1, l2, l3, m1, m2, m3;\n\t"
+        "add.u32 l1, %3, %7;\n\tadd.u32 l2, %3, %8;\n\tadd.u32 l3, %3, %9;\n\t"
+        "add.u32 m1, %1, %10;\n\tadd.u32 m2, %1, %11;\n\tadd.u32 m3, %1, %12;\n\t"
+        "mov.b64 b0, {%3, %4};\n\tmov.b64 b1, {l1, %4};\n\tmov.b64 b2, {l2, %4};\n\tmov.b64 b3, {l3, %4};\n\t"
+        "mov.b64 a0, {%1, %2};\n\tmov.b64 a1, {m1, %2};\n\tmov.b64 a2, {m2, %2};\n\tmov.b64 a3, {m3, %2};\n\t"
+        "setp.eq.b32 p, %6, 0;\n\tsetp.eq.b32 q, 0, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %5, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %5, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %5, q;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %5, q;\n\t}"
+        ::"r"(d), "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"((uint32_t)first), "n"(BS), "n"(2 * BS), "n"(3 * BS), "n"(AS),
+        "n"(2 * AS), "n"(3 * AS)
+        : "memory");
+}
+// a value that is the same in all lanes, known as such to the compiler
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 // instruction descriptor: fp32 accumulator, fp16 operands, 128 rows
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
     return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
@@ -62,16 +92,17 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t s
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// 16 columns from `16 * step` on of a K-major panel set of `rows` rows (8-row groups 1024 bytes apart)
-__device__ __forceinline__ uint64_t desc_k(uint32_t plane, int rows, int step) {
-    return desc(plane + (uint32_t)(step >> 2) * (uint32_t)(rows * 128) + (uint32_t)(step & 3) * 32u, 16u, 1024u);
+__device__ __forceinline__ Desc desc2(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return Desc{((addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16), ((sbo >> 4) & 0x3FFF) | (1u << 14) | (2u << 29)};
 }
-// 16 rows from `16 * step` on, all columns: panels (64 columns) `rows * 128` bytes apart, 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t desc_mn(uint32_t plane, int rows, int step) {
-    return desc(plane + (uint32_t)step * 2048u, (uint32_t)(rows * 128), 1024u);
-}
+// a panel (64 columns, rows 128 bytes apart) as an operand over its columns; a step of 16 columns is 2 units
+constexpr int STEP_K = 2;
+__device__ __forceinline__ Desc desc_k(uint32_t panel) { return desc2(panel, 16u, 1024u); }
+// `rows`-row panels side by side as an operand over their rows, from a row on; a step of 16 rows is 128 units
+constexpr int STEP_MN = 128;
+__device__ __forceinline__ Desc desc_mn(uint32_t plane, int rows) { return desc2(plane, (uint32_t)(rows * 128), 1024u); }
 
-// 32 / 16 consecutive columns of this warp's 32 lanes; the wait is part of the instruction, so nothing reads too early
+// 64 / 32 / 16 consecutive columns of this warp's 32 lanes; the wait is part of the instruction, so nothing reads too early
 __device__ __forceinline__ void ld32(uint32_t addr, float (&f)[32]) {
     uint32_t r[32];
     asm volatile(
@@ -87,6 +118,27 @@ __device__ __forceinline__ void ld32(uint32_t addr, float (&f)[32]) {
         : "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void ld64(uint32_t addr, float (&f)[64]) {
+    uint32_t r[64];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]),
+          "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]),
+          "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]),
+          "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void ld16(uint32_t addr, float (&f)[16]) {
     uint32_t r[16];
@@ -108,6 +160,24 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// 32 values as fp16 pairs over the 32 columns that they came from: of every 16 columns eight of hi pairs, then eight of lo pairs
+__device__ __forceinline__ void st_pairs(uint32_t addr, const uint32_t (&hi)[16], const uint32_t (&lo)[16]) {
+    uint32_t a[16], b[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a[i] = hi[i];
+        a[8 + i] = lo[i];
+        b[i] = hi[8 + i];
+        b[8 + i] = lo[8 + i];
+    }
+    st16(addr, a);
+    st16(addr + 16, b);
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -162,7 +232,9 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
     const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
     hi = half_pair(ah, bh);
-    lo = half_pair(a - ah, b - bh);
+    float al, bl;
+    unpack2(fma2(pack2(ah, bh), pack2(-1.f, -1.f), pack2(a, b)), al, bl);  // both differences, exact, in one instruction
+    lo = half_pair(al, bl);
 }
 
 // 2^e that brings `largest` (finite, >= 0) into [2^14, 2^15), and its inverse.  0 and what is too small to be brought there
@@ -179,6 +251,8 @@ __device__ __forceinline__ float pow2_below_inverse(float x) {
     const int e = max(-121, min(100, -(ex + 1)));
     return __uint_as_float((uint32_t)(127 + e) << 23);
 }
+// 1 / x of a power of two in 2^-126 .. 2^126
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 // |x| for the search of the largest entry: infinities and NaN do not count
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
