@@ -3,16 +3,14 @@
 // Kernel.  A CTA owns 128 rows of one head.  Its q rows are split into fp16 pairs (scaled per row) and kept in tensor memory as
 // the left operand; k and v come as 64-row tile images through a ring of three stages.  Per tile j:
 //   S_j = q k_j^T          left operand and accumulator in tensor memory
-//   P_j = exp2(S_j c - m)  by a warpgroup, a row per thread, written over S_j as fp16 pairs: the next left operand
+//   P_j = exp2(S_j c - m)  by warpgroups, a row per thread, written over S_j as fp16 pairs: the next left operand
 //   O_j = P_j v_j          a fresh accumulator, added to the row's registers (and rescaled) with rounding
 // The running reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.
-// A warp of its own issues all copies and MMAs (one thread).
-// Up to dim 64 everything fits twice into an SM (96 KB, 256 columns), with one warpgroup a CTA: it works on P_{j+1} while P_j v_j
-// runs, the two CTAs fill each other's gaps, and at ten warps an SM a thread has the 168 registers that a row of S and a row of O
-// take (with two warpgroups in each CTA it had 96, and the spills, which miss the small L1 that is left, cost more than all
-// the arithmetic: 184 us instead of ___ at 384 heads of 512 x 64).
-// Up to dim 128 one CTA has the SM: two warpgroups take the tiles alternately, each with its own m, l and O, joined once at the
-// end, and a third S buffer lets S_{j+1} start before P_{j-1} v_{j-1} is done.
+// What bounds the kernel is not a pipe but the chain S -> maximum -> exponentials -> P -> O of a tile, a few thousand cycles of
+// latencies.  So the columns of a tile are shared by two warpgroups (dim up to 64; 32 columns of S and of O a thread) or four (up
+// to 128), which exchange their maxima through shared memory; the output of tile j - 1 is added after P_j; two or three S buffers
+// let S_{j+1} run meanwhile; and up to dim 64, where everything fits twice into an SM (96 KB, 256 columns), two CTAs fill each
+// other's gaps.  One warp issues the MMAs, one the copies.
 // Bound: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
 #include "attention_tc.cuh"
 
@@ -69,8 +67,8 @@ __device__ __forceinline__ void attn_row_numbers(const TenmoTileJobs& jobs, cons
         const float il_max = fmaxf(most[0][0], most[0][1]);
         const float ps = il_max > 0.f ? 32768.f * tc::pow2_below_inverse(il_max) : 1.f;
         float* info = j.info + t * ATTN_INFO;
-        info[r] = m;
-        info[T + r] = il * ps;
+        info[4 * (r >> 1) + (r & 1)] = -m;
+        info[4 * (r >> 1) + 2 + (r & 1)] = il * ps;
         info[2 * T + r] = dl;
         if (r == 0) { info[3 * T] = ps; info[3 * T + 1] = fmaxf(most[1][0], most[1][1]); info[3 * T + 2] = 1.f / ps; }
     }
@@ -144,9 +142,10 @@ struct FwdParams {
 
 template <int DP>
 struct FwdCfg {
-    static constexpr int WGS = DP == 64 ? 1 : 2;    // warpgroups
-    static constexpr int THREADS = DP == 64 ? 192 : 384;  // and two more warps (or a warpgroup, whose registers move)
+    static constexpr int WGS = DP / 32;             // warpgroups that share a tile
+    static constexpr int THREADS = 128 * WGS + 64;
     static constexpr int ISSUER = 4 * WGS, LOADER = ISSUER + 1;
+    static constexpr int NC = T / WGS, W = DP / WGS;  // columns of S and of O of a thread
     static constexpr int NB = DP == 64 ? 2 : 3;     // S / P buffers
     static constexpr int PLANE = T * DP * 2;        // bytes of one plane of a tile
     static constexpr int IMG = 2 * PLANE;           // a tile's hi and lo plane
@@ -154,7 +153,7 @@ struct FwdCfg {
     static constexpr int Q_COLS = DP;               // hi DP/2, lo DP/2
     static constexpr int S_COL = Q_COLS, O_COL = Q_COLS + NB * T;
     static constexpr int TMEM = DP == 64 ? 256 : 512;
-    static constexpr int SMEM = STAGES * STAGE + 2048;
+    static constexpr int SMEM = STAGES * STAGE + 2 * WGS * 128 * 4 + 512;
     static_assert(O_COL + DP <= TMEM, "tensor memory");
 };
 
@@ -162,15 +161,15 @@ template <int DP>
 __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams p) {
     using C = FwdCfg<DP>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    float* const shared_f = reinterpret_cast<float*>(smem + STAGES * C::STAGE);  // [2][128] row statistics
-    const uint32_t bars = smem_u32(smem + STAGES * C::STAGE + 1024);
+    float* const shared_f = reinterpret_cast<float*>(smem + STAGES * C::STAGE);  // [2][WGS][128] row maxima
+    const uint32_t bars = smem_u32(smem + STAGES * C::STAGE + 2 * C::WGS * 128 * 4);
     auto full = [&](int which, int slot) { return bars + 8u * (3 * which + slot); };         // which: 0 k, 1 v
     auto empty = [&](int which, int slot) { return bars + 8u * (16 + 3 * which + slot); };
     auto s_full = [&](int j) { return bars + 8u * (6 + (j & 1)); };
     auto p_full = [&](int j) { return bars + 8u * (8 + (j & 1)); };
     auto o_full = [&](int j) { return bars + 8u * (10 + (j & 1)); };
     const uint32_t o_free = bars + 8u * 12, drain = bars + 8u * 13;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * C::STAGE + 1024 + 256);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * C::STAGE + 2 * C::WGS * 128 * 4 + 256);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const TenmoAttnParams& a = p.a;
@@ -189,8 +188,8 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(0, s), 1); mbar_init(full(1, s), 1); mbar_init(empty(0, s), 1); mbar_init(empty(1, s), 1); }
-        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
-        mbar_init(o_free, 4);
+        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4 * C::WGS); mbar_init(o_full(w), 1); }
+        mbar_init(o_free, 4 * C::WGS);
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             if (++fetch_slot == STAGES) { fetch_slot = 0; ++fetch_round; }
         }
     };
-    if (threadIdx.x == 32 * C::LOADER) fetch(min(n_tiles, STAGES));
+    if (threadIdx.x == 32 * C::LOADER) fetch(min(n_tiles, STAGES - 1));  // the last slot is scratch for now
 
     // ---- q into tensor memory ----
     const int wg = warp >> 2, row = threadIdx.x & 127;
@@ -222,17 +221,14 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float q_inv = 1.f;
     if (warp < C::ISSUER)  // the sign of the scale goes with q: the factor of the scores is then never negative
-        q_inv = tenmo_attn_stationary<DP, false, C::WGS>(a.q.ptr + b * a.q.sb + h * a.q.sh + i * a.q.sr, i < q_rows, p.q_vec, a.D, a.scale < 0.f,
-                                                 wg, row, lane_base, nullptr, shared_f);
+        q_inv = tenmo_attn_stationary<DP, false, C::WGS>(a.q.ptr + b * a.q.sb + h * a.q.sh + (int64_t)q_tile * ROWS * a.q.sr, a.q.sr,
+                                                         q_rows - q_tile * ROWS, p.q_vec, a.D, a.scale < 0.f, lane_base, nullptr, shared_f,
+                                                         reinterpret_cast<float*>(smem + (STAGES - 1) * C::STAGE));
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
 
-    // rows of the second warpgroup join the first's through these
-    float m = -INFINITY, l = 0.f;
-    float* const buf = reinterpret_cast<float*>(smem);  // the stages, when all products are done
     if (warp >= C::ISSUER) {
-        if (C::WGS == 2) tc::regs_down<88>();
         if (warp == C::LOADER) {
             if (lane == 0) {
                 fetch(n_tiles);
@@ -291,56 +287,68 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
                 mbar_wait(drain, 0, &never);
             }
         }
-        __syncthreads();
-        if (C::WGS == 2) __syncthreads();
     } else {
-        if (C::WGS == 2) tc::regs_up<208>();
-        float o[DP];
+        constexpr int NC = C::NC, W = C::W;
+        float m = -INFINITY, l = 0.f, o[W];  // l: of this thread's columns
 #pragma unroll
-        for (int d = 0; d < DP; ++d) o[d] = 0.f;
+        for (int d = 0; d < W; ++d) o[d] = 0.f;
         const float c_row = fabsf(a.scale_log2) * q_inv;
         int n_row = i < q_rows ? keys : 0;
         if (a.causal) n_row = min(n_row, (int)max((int64_t)0, i + a.Sk - a.Sq + 1));
         bool ok = true;
         auto await = [&](uint32_t bar, int phase) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, abort_flag)); };
+        auto sync_rows = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(128 * C::WGS) : "memory"); };
         float shrink = 0.f, v_inv = 0.f;  // of the tile whose output is next
         auto add_output = [&](int j) {    // o = o * shrink + O_j
             await(o_full(j), j >> 1);
             if (!ok) return;
             tc::fence_after();
-            const uint64_t sh2 = tc::pack2(shrink, shrink), vi2 = tc::pack2(v_inv, v_inv);
-#pragma unroll
-            for (int g = 0; g < DP / 32; ++g) {
-                float t[32];
-                tc::ld32(lane_base + C::O_COL + 32 * g, t);
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const uint64_t add = tc::mul2(tc::pack2(t[e], t[e + 1]), vi2);
-                    tc::unpack2(tc::fma2(tc::pack2(o[32 * g + e], o[32 * g + e + 1]), sh2, add), o[32 * g + e], o[32 * g + e + 1]);
-                }
-            }
+            float t[W];
+            tc::ldn(lane_base + C::O_COL + wg * W, t);
             tc::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
+            const uint64_t sh2 = tc::pack2(shrink, shrink), vi2 = tc::pack2(v_inv, v_inv);
+            if (__all_sync(0xffffffffu, shrink == 1.f)) {
+#pragma unroll
+                for (int e = 0; e < W; e += 2) tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), vi2, tc::pack2(o[e], o[e + 1])), o[e], o[e + 1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; e += 2) {
+                    const uint64_t add = tc::mul2(tc::pack2(t[e], t[e + 1]), vi2);
+                    tc::unpack2(tc::fma2(tc::pack2(o[e], o[e + 1]), sh2, add), o[e], o[e + 1]);
+                }
+            }
         };
-        for (int j = wg; j < n_tiles; j += C::WGS) {
-            const float c = c_row * __ldg(p.k_inv + tile0 + j), v_next = __ldg(p.v_inv + tile0 + j);
+        // the tiles' scales come from L2: loaded a tile ahead
+        float k_ahead = n_tiles ? __ldg(p.k_inv + tile0) : 1.f, v_ahead = n_tiles ? __ldg(p.v_inv + tile0) : 1.f;
+        for (int j = 0; j < n_tiles; ++j) {
+            const float c = c_row * k_ahead, v_next = v_ahead;
+            if (j + 1 < n_tiles) {
+                k_ahead = __ldg(p.k_inv + tile0 + j + 1);
+                v_ahead = __ldg(p.v_inv + tile0 + j + 1);
+            }
             await(s_full(j), j >> 1);
-            if (!ok) break;
             tc::fence_after();
-            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T;
-            const int lim = n_row - j * T;
-            const bool whole = __all_sync(0xffffffffu, lim >= T);
-            float s[T];  // dim 128: only for the maximum, and loaded again in parts for the exponentials
-            tc::ld64(s_addr, s);
+            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T + wg * NC;
+            const int lim = n_row - j * T - wg * NC;  // visible columns of this thread
+            const bool whole = __all_sync(0xffffffffu, lim >= NC);
+            float s[NC];
+            tc::ldn(s_addr, s);
             float mx = -INFINITY;
             if (whole) {
 #pragma unroll
-                for (int e = 0; e < T; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
+                for (int e = 0; e < NC; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
             } else {
 #pragma unroll
-                for (int e = 0; e < T; ++e) mx = fmaxf(mx, e < lim ? s[e] : -INFINITY);
+                for (int e = 0; e < NC; ++e) mx = fmaxf(mx, e < lim ? s[e] : -INFINITY);
             }
+            float* const row_max = shared_f + (j & 1) * (C::WGS * 128) + row;
+            row_max[wg * 128] = mx;
+            sync_rows();  // reached by all in every tile, also when a wait has run out
+#pragma unroll
+            for (int w = 0; w < C::WGS; ++w) mx = fmaxf(mx, row_max[w * 128]);
+            if (!ok) continue;
             const float m_new = mx == -INFINITY ? m : fmaxf(m, ceilf(mx * c));
             const float shrink_next = m == -INFINITY ? 0.f : tc::ex2(m - m_new);
             m = m_new;
@@ -349,32 +357,20 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             const uint64_t c2 = tc::pack2(c, c), b2 = tc::pack2(base, base);
             uint64_t sum2 = 0;
 #pragma unroll
-            for (int g = 0; g < T / 16; ++g) {
-                float r[16];
-                if (DP == 128) {
-                    tc::ld16(s_addr + 16 * g, r);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) r[e] = s[16 * g + e];
+            for (int e = 0; e < NC; e += 2) {
+                float x, y;
+                tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
+                x = tc::ex2(x);
+                y = tc::ex2(y);
+                if (!whole) {
+                    x = e < lim ? x : 0.f;
+                    y = e + 1 < lim ? y : 0.f;
                 }
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float x, y;
-                    tc::unpack2(tc::fma2(tc::pack2(r[2 * e], r[2 * e + 1]), c2, b2), x, y);
-                    x = tc::ex2(x);
-                    y = tc::ex2(y);
-                    if (!whole) {
-                        x = 16 * g + 2 * e < lim ? x : 0.f;
-                        y = 16 * g + 2 * e + 1 < lim ? y : 0.f;
-                    }
-                    sum2 = tc::add2(sum2, tc::pack2(x, y));
-                    tc::split_pair(x, y, hi[e], lo[e]);
-                }
-                // 16 keys: columns 16 g .. + 7 the hi pairs, + 8 .. + 15 the lo pairs (the scores that they replace have been read)
-                tc::st8(s_addr + 16 * g, hi);
-                tc::st8(s_addr + 16 * g + 8, lo);
+                sum2 = tc::add2(sum2, tc::pack2(x, y));
+                s[e] = x;
+                s[e + 1] = y;
             }
+            tc::st_split(s_addr, s);  // over the scores that they come from
             tc::st_wait();
             tc::fence_before();
             __syncwarp();
@@ -382,76 +378,31 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             float x, y;
             tc::unpack2(sum2, x, y);
             l = fmaf(l, shrink_next, x + y);
-            // one warpgroup: the output of the tile before, whose product ran meanwhile; two: this tile's (the other one works on)
-            if (C::WGS == 1) {
-                if (j > 0) add_output(j - 1);
-                shrink = shrink_next;
-                v_inv = v_next;
-            } else {
-                shrink = shrink_next;
-                v_inv = v_next;
-                add_output(j);
-            }
-            if (!ok) break;
+            if (j > 0) add_output(j - 1);  // the tile before: its product ran meanwhile
+            shrink = shrink_next;
+            v_inv = v_next;
         }
-        if (C::WGS == 1 && ok && n_tiles > 0) add_output(n_tiles - 1);
+        if (ok && n_tiles > 0) add_output(n_tiles - 1);
 
-        // ---- to the output: 16-byte chunk q of row r lies at chunk q ^ (r & 7) of the buffer ----
-        __syncthreads();
-        auto at = [&](int d) { return reinterpret_cast<float4*>(buf + row * DP + (((d >> 2) ^ (row & 7)) << 2)); };
-        float f = 1.f;
-        if (C::WGS == 2) {
-            if (wg == 1) {
-                shared_f[row] = m;
-                shared_f[128 + row] = l;
+        // ---- the sum over the warpgroups' columns, and the output through the stages: all products are done ----
+        sync_rows();
+        shared_f[wg * 128 + row] = l;
+        sync_rows();
+        l = 0.f;
 #pragma unroll
-                for (int d = 0; d < DP; d += 4) *at(d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-            }
-            __syncthreads();
-        }
-        if (wg == 0) {
-            float f1 = 0.f;
-            if (C::WGS == 2) {
-                const float m1 = shared_f[row], top = fmaxf(m, m1);
-                f = m == -INFINITY ? 0.f : tc::ex2(m - top);
-                f1 = m1 == -INFINITY ? 0.f : tc::ex2(m1 - top);
-                l = l * f + shared_f[128 + row] * f1;
-                m = top;
-            }
-            // rows without keys: sum 0, output 0 (0 * 0); a NaN in the sum reaches the output
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            f *= inv;
-            f1 *= inv;
+        for (int w = 0; w < C::WGS; ++w) l += shared_f[w * 128 + row];
+        // rows without keys: sum 0, output 0 (0 * 0); a NaN in the sum reaches the output
+        const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-            for (int d = 0; d < DP; d += 4) {
-                float4 x = make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
-                if (C::WGS == 2) {
-                    const float4 u = *at(d);
-                    x.x = fmaf(u.x, f1, x.x); x.y = fmaf(u.y, f1, x.y); x.z = fmaf(u.z, f1, x.z); x.w = fmaf(u.w, f1, x.w);
-                }
-                *at(d) = x;
-            }
-            if (a.stats && i < a.Sq) {
-                float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + i) * 2;
-                st[0] = m;
-                st[1] = l * 3.0517578125e-5f;  // 2^-15
-            }
+        for (int d = 0; d < W; ++d) o[d] *= inv;
+        if (wg == 0 && a.stats && i < a.Sq) {
+            float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + i) * 2;
+            st[0] = m;
+            st[1] = l * 3.0517578125e-5f;  // 2^-15
         }
-    }
-    __syncthreads();
-    const int rows_here = min(ROWS, a.Sq - q_tile * ROWS);
-    float* out = a.o.ptr + b * a.o.sb + h * a.o.sh + (int64_t)q_tile * ROWS * a.o.sr;
-    for (int e = threadIdx.x; e < rows_here * (DP / 4); e += C::THREADS) {
-        const int r = e / (DP / 4), q = e % (DP / 4), d = 4 * q;
-        if (d >= a.D) continue;
-        const float4 x = *reinterpret_cast<const float4*>(buf + r * DP + ((q ^ (r & 7)) << 2));
-        float* dst = out + r * a.o.sr + d;
-        if (p.o_vec) {
-            *reinterpret_cast<float4*>(dst) = x;
-        } else {
-            const float v[4] = {x.x, x.y, x.z, x.w};
-            for (int u = 0; u < 4 && d + u < a.D; ++u) dst[u] = v[u];
-        }
+        const int row0 = q_tile * ROWS + 32 * (warp & 3);
+        tenmo_attn_write_rows<W>(o, a.o.ptr + b * a.o.sb + h * a.o.sh + (int64_t)row0 * a.o.sr + wg * W, a.o.sr, a.Sq - row0, a.D - wg * W, p.o_vec,
+                                 false, reinterpret_cast<float*>(smem) + warp * (32 * W));
     }
     tc::fence_before();
     __syncthreads();

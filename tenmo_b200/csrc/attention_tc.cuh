@@ -17,8 +17,8 @@ struct TenmoTileJob {
     float* inverse;          // 2^-e of every tile
     int heads, rows, tiles, vec;
     // With o.ptr set (src is the gradient of o): the per-row numbers of the backward pass as well.  Per tile 256 floats:
-    // [0, 64) m_i (+inf for rows that take no part), [64, 128) 1 / l_i times the tile's power of two PS that brings the largest
-    // to at most 2^15 (0 for those rows), [128, 192) delta_i, 192: PS, 193: the largest |delta|, 194: 1 / PS; the rest is unused.
+    // for rows 2 r, 2 r + 1 the four at 4 r: their -m (-inf for rows that take no part) and their 1 / l times the tile's power of two
+    // PS that brings the largest to at most 2^15 (0 for those rows); [128, 192) delta; 192: PS, 193: the largest |delta|, 194: 1 / PS.
     TenmoHeadsView o;
     const float* stats;
     float* info;
@@ -33,57 +33,115 @@ int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, 
 bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D);
 static inline int tenmo_attn_padded(int D) { return D <= 64 ? 64 : 128; }
 
-// A row of an operand, split into fp16 pairs scaled by the row's power of two, into tensor memory (hi from `addr` on, lo DP / 2
-// columns further) or, with `plane` set, into a 128-row tile image in shared memory.  Called by the threads of WGS warpgroups, which
-// share the columns of a row; `exchange` holds 256 floats.  Returns the inverse scale.
+// A warp's 32 rows x W columns between memory and one row per thread, through `scratch` (32 * W floats of the warp's own): the 16-byte
+// chunks of a row are permuted so that neither the row-wise nor the thread-wise accesses conflict, and memory sees whole
+// rows (a thread that walks its own row touches 32 rows per instruction).
+template <int W>
+__device__ __forceinline__ float4* tenmo_attn_chunk(float* scratch, int r, int q) {
+    return reinterpret_cast<float4*>(scratch + r * W + ((q ^ (W >= 32 ? r & 7 : (r >> 1) & 3)) << 2));
+}
+// x: columns [0, cols) of this lane's row; rows from `rows` on and columns from `cols` on are zeros
+template <int W>
+__device__ __forceinline__ void tenmo_attn_read_rows(float (&x)[W], const float* src, int64_t stride, int rows, int cols, bool vec, float* scratch) {
+    constexpr int LPR = W / 4, RPI = 32 / LPR;
+    const int lane = threadIdx.x & 31, q = lane % LPR;
+    const float* p = src + (lane / LPR) * stride + 4 * q;
+    float4 v[LPR];  // all loads are in flight before the first is used
+    if (vec) {
+#pragma unroll
+        for (int it = 0; it < LPR; ++it)
+            v[it] = it * RPI + lane / LPR < rows && 4 * q < cols ? __ldg(reinterpret_cast<const float4*>(p + it * RPI * stride)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+#pragma unroll
+        for (int it = 0; it < LPR; ++it) {
+            const bool in = it * RPI + lane / LPR < rows;
+            const float* r = p + it * RPI * stride;
+            v[it].x = in && 4 * q < cols ? __ldg(r) : 0.f;
+            v[it].y = in && 4 * q + 1 < cols ? __ldg(r + 1) : 0.f;
+            v[it].z = in && 4 * q + 2 < cols ? __ldg(r + 2) : 0.f;
+            v[it].w = in && 4 * q + 3 < cols ? __ldg(r + 3) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int it = 0; it < LPR; ++it) *tenmo_attn_chunk<W>(scratch, it * RPI + lane / LPR, q) = v[it];
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < LPR; ++c) {
+        const float4 v = *tenmo_attn_chunk<W>(scratch, lane, c);
+        x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
+    }
+    __syncwarp();
+}
+template <int W>
+__device__ __forceinline__ void tenmo_attn_write_rows(const float (&x)[W], float* dst, int64_t stride, int rows, int cols, bool vec, bool add, float* scratch) {
+    constexpr int LPR = W / 4, RPI = 32 / LPR;
+    const int lane = threadIdx.x & 31, q = lane % LPR;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < LPR; ++c) *tenmo_attn_chunk<W>(scratch, lane, c) = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+    __syncwarp();
+#pragma unroll 8
+    for (int it = 0; it < LPR; ++it) {
+        const int r = it * RPI + lane / LPR;
+        float4 v = *tenmo_attn_chunk<W>(scratch, r, q);
+        if (r >= rows || 4 * q >= cols) continue;
+        float* p = dst + r * stride + 4 * q;
+        if (vec) {
+            if (add) {
+                const float4 o = *reinterpret_cast<const float4*>(p);
+                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+            }
+            *reinterpret_cast<float4*>(p) = v;
+        } else {
+            const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (4 * q + u < cols) p[u] = add ? p[u] + f[u] : f[u];
+        }
+    }
+}
+
+// The rows of an operand (128 of them), split into fp16 pairs scaled by a power of two per row, into tensor memory (hi from `addr` on,
+// lo DP / 2 columns further) or, with SMEM, into a 128-row tile image in shared memory.  Called by the threads of WGS warpgroups, which
+// share the columns of a row; `exchange` holds WGS * 128 floats, `scratch` 128 * DP.  Returns the row's inverse scale.
 template <int DP, bool SMEM, int WGS>
-__device__ __forceinline__ float tenmo_attn_stationary(const float* src, bool in, bool vec, int D, bool negate, int wg, int row,
-                                                       uint32_t addr, uint8_t* plane, float* exchange) {
+__device__ __forceinline__ float tenmo_attn_stationary(const float* src, int64_t stride, int rows, bool vec, int D, bool negate, uint32_t addr,
+                                                       uint8_t* plane, float* exchange, float* scratch) {
     constexpr int W = DP / WGS;
+    const int warp = threadIdx.x >> 5, wg = warp >> 2, row = threadIdx.x & 127, row0 = 32 * (warp & 3);
     float x[W];
+    tenmo_attn_read_rows<W>(x, src + row0 * stride + wg * W, stride, rows - row0, D - wg * W, vec, scratch + warp * (32 * W));
     float mx = 0.f;
 #pragma unroll
-    for (int e = 0; e < W; e += 4) {
-        const int d = wg * W + e;
-        if (in && vec && d + 4 <= D) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(src + d));
-            x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
-        } else {
+    for (int e = 0; e < W; ++e) mx = fmaxf(mx, tc::finite_abs(x[e]));
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * WGS) : "memory");  // an earlier use of `exchange` is over
+    exchange[wg * 128 + row] = mx;
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * WGS) : "memory");
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[e + u] = in && d + u < D ? __ldg(src + d + u) : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mx = fmaxf(mx, tc::finite_abs(x[e + u]));
-    }
-    if (WGS == 2) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // an earlier use of `exchange` is over
-        exchange[wg * 128 + row] = mx;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        mx = fmaxf(mx, exchange[(wg ^ 1) * 128 + row]);
-    }
+    for (int w = 0; w < WGS; ++w) mx = fmaxf(mx, exchange[w * 128 + row]);
     float inverse;
     float scale = tc::block_scale(mx, &inverse);
     if (negate) scale = -scale;
 #pragma unroll
-    for (int g = 0; g < W / 32; ++g) {
-        uint32_t hi[16], lo[16];
+    for (int g = 0; g < W / 16; ++g) {
+        uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) tc::split_pair(x[32 * g + 2 * e] * scale, x[32 * g + 2 * e + 1] * scale, hi[e], lo[e]);
+        for (int e = 0; e < 8; ++e) tc::split_pair(x[16 * g + 2 * e] * scale, x[16 * g + 2 * e + 1] * scale, hi[e], lo[e]);
         if (SMEM) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int c = (wg * W + 32 * g) / 8 + q;
+            for (int q = 0; q < 2; ++q) {
+                const int c = (wg * W + 16 * g) / 8 + q;
                 const int at = (c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
                 *reinterpret_cast<uint4*>(plane + at) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
                 *reinterpret_cast<uint4*>(plane + 128 * DP * 2 + at) = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
             }
         } else {
-            const uint32_t col = (uint32_t)(wg * (W / 2) + 16 * g);
-            tc::st16(addr + col, hi);
-            tc::st16(addr + DP / 2 + col, lo);
+            const uint32_t col = (uint32_t)((wg * W + 16 * g) / 2);
+            tc::st8(addr + col, hi);
+            tc::st8(addr + DP / 2 + col, lo);
         }
     }
-    if (SMEM) tc::fence_proxy_async();
-    else tc::st_wait();
+    tc::fence_proxy_async();  // the scratch is a stage that a copy fills next (and with SMEM the tensor core reads the image)
+    if (!SMEM) tc::st_wait();
     return inverse;
 }

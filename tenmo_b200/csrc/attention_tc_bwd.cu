@@ -10,10 +10,11 @@
 // fresh accumulators that the warpgroups add to their registers with rounding.
 // fp16 range of dS: |dP - delta| is bounded by the operands' scales (dim * 2^30 times the two inverse scales) and by the largest
 // |delta|; a power of two from that bound brings dS to at most 2^15, exactly taken back when the tile is added.
-// Two warpgroups share every tile (32 columns of S and half of the gradient's columns each); one thread issues copies and MMAs.
-// Up to dim 64 S and dP have two buffers: the scores of tile j + 1 are computed while tile j is worked on.  Up to dim 128 there
-// is one of each, and v of the dkv pass moves to shared memory; the products still follow each other without a gap because
-// each has one product of another kind between itself and what it waits for.
+// One warp issues the MMAs, one the copies.  As in the forward pass the chain of a tile (S -> P -> dP -> dS -> sums) decides, so its
+// columns are shared by four warpgroups (16 of the 64 columns of S a thread, a quarter of the gradient's; the dkv pass of dim 128, whose
+// sums take 256 registers a row, has two).  Up to dim 64 S and dP have two buffers: the scores of tiles j + 1 and j + 2 are computed
+// while tile j is worked on.  Up to dim 128 there is one of each and v of the dkv pass moves to shared memory; the products still
+// follow each other without large gaps because each has one of another kind between itself and what it waits for.
 // Shared key / value heads: the dkv pass works per query head into the workspace and a last kernel adds the heads of a group
 // in order (per group it would leave most SMs idle behind the longest).
 // Bound: tensor pipe, 3 * 14 * rows * keys * dim flop.
@@ -23,7 +24,6 @@ namespace {
 
 constexpr int ROWS = 128;
 constexpr int T = ATTN_TILE;
-constexpr int THREADS = 384;  // two warpgroups and the issuing warp's (whose registers go to the other two)
 
 struct BwdParams {
     TenmoAttnParams a;
@@ -41,7 +41,11 @@ struct BwdParams {
 
 template <int DP, bool DKV>
 struct BwdCfg {
-    static constexpr int NB = DP == 64 ? 2 : 1;
+    static constexpr int WGS = DKV && DP == 128 ? 2 : 4;              // warpgroups that share a tile
+    static constexpr int THREADS = WGS == 2 ? 384 : 128 * WGS + 64;  // two: the issuing warpgroup's registers go to them
+    static constexpr int ISSUER = 4 * WGS, LOADER = ISSUER + 1;
+    static constexpr int NC = T / WGS, W = DP / WGS;                 // columns of S and of the gradient of a thread
+    static constexpr int NB = DP == 64 ? 2 : 1;                      // buffers of S and dP
     static constexpr bool X2S = DKV && DP == 128;  // X2 in shared memory
     static constexpr int STAGES = DP == 64 ? 5 : X2S ? 2 : 3;
     static constexpr int PLANE = T * DP * 2;
@@ -52,28 +56,30 @@ struct BwdCfg {
     static constexpr int TMEM = 512;
     static_assert(A1_COL + (DKV ? 2 : 1) * DP <= TMEM, "tensor memory");
     static constexpr int TILES = STAGES * STAGE + X2_BYTES;
-    static constexpr int SMEM = TILES + 2048;
+    static constexpr int SMEM = TILES + 2048 + 512;
     static_assert(STAGES * STAGE >= ROWS * DP * 4, "the output goes through the stages");
 };
 
 template <int DP, bool DKV>
-__global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_constant__ BwdParams p) {
+__global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kernel(const __grid_constant__ BwdParams p) {
     using C = BwdCfg<DP, DKV>;
-    constexpr int NB = C::NB, W = DP / 2;
+    constexpr int NB = C::NB, NC = C::NC, W = C::W;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const x2_plane = smem + C::STAGES * C::STAGE;
     float* const exchange = reinterpret_cast<float*>(smem + C::TILES);
-    const uint32_t bars = smem_u32(smem + C::TILES + 1024);
+    const uint32_t bars = smem_u32(smem + C::TILES + 2048);
     auto full = [&](int slot) { return bars + 8u * (16 + slot); };
     auto empty = [&](int slot) { return bars + 8u * (24 + slot); };
     auto s_full = [&](int j) { return bars + 8u * (j & 1); };
     auto d_full = [&](int j) { return bars + 8u * (2 + (j & 1)); };
-    // a warp may be a tile ahead of another one: what the eight warps arrive on has a barrier for even and one for odd tiles
+    // a warp may be a tile ahead of another one: what warps arrive on has a barrier for even and one for odd tiles
     auto p_full = [&](int j) { return bars + 8u * (7 + (j & 1)); };
     auto ds_full = [&](int j) { return bars + 8u * (9 + (j & 1)); };
     auto s_read = [&](int j) { return bars + 8u * (4 + (j & 1)); };
-    const uint32_t pv_done = bars + 8u * 11, acc_full = bars + 8u * 12, acc_free = bars + 8u * 13, drain = bars + 8u * 14;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 1024 + 256);
+    auto acc_full = [&](int j) { return bars + 8u * (11 + (j & 1)); };
+    auto acc_free = [&](int j) { return bars + 8u * (13 + (j & 1)); };
+    const uint32_t pv_done = bars + 8u * 15, drain = bars + 8u * 6;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 2048 + 256);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const TenmoAttnParams& a = p.a;
@@ -105,15 +111,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(d_full(w), 1); mbar_init(p_full(w), 8); mbar_init(ds_full(w), 8); mbar_init(s_read(w), 8); }
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(s_full(w), 1);
+            mbar_init(d_full(w), 1);
+            mbar_init(acc_full(w), 1);
+            mbar_init(s_read(w), 4 * C::WGS);
+            mbar_init(p_full(w), 4 * C::WGS);
+            mbar_init(ds_full(w), 4 * C::WGS);
+            mbar_init(acc_free(w), 4 * C::WGS);
+        }
         mbar_init(pv_done, 1);
-        mbar_init(acc_full, 1);
-        mbar_init(acc_free, 8);
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tc::alloc(tmem_slot, C::TMEM);
+    if (warp == C::ISSUER) tc::alloc(tmem_slot, C::TMEM);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -133,30 +145,32 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
             if (++fetch_slot == C::STAGES) { fetch_slot = 0; ++fetch_round; }
         }
     };
-    if (threadIdx.x == 32 * 9) fetch(min(n, C::STAGES));
+    if (threadIdx.x == 32 * C::LOADER) fetch(min(n, C::STAGES - 1));  // the last slot is scratch for now
 
     float x1_inv = 1.f, x2_inv = 1.f;
-    if (warp < 8) {
-        const int xh = DKV ? kvh : h;
-        x1_inv = tenmo_attn_stationary<DP, false, 2>(p.x1.ptr + b * p.x1.sb + xh * p.x1.sh + i * p.x1.sr, i < x_rows, p.x1_vec, a.D,
-                                                  a.scale < 0.f, wg, row, lane_base, nullptr, exchange);
-        x2_inv = tenmo_attn_stationary<DP, C::X2S, 2>(p.x2.ptr + b * p.x2.sb + xh * p.x2.sh + i * p.x2.sr, i < x_rows, p.x2_vec, a.D, false,
-                                                   wg, row, lane_base + C::X2_COL, x2_plane, exchange);
+    if (warp < C::ISSUER) {
+        const int xh = DKV ? kvh : h, rows = x_rows - x_tile * ROWS;
+        const int64_t x0 = (int64_t)x_tile * ROWS;
+        float* const scratch = reinterpret_cast<float*>(smem + (C::STAGES - 1) * C::STAGE);
+        x1_inv = tenmo_attn_stationary<DP, false, C::WGS>(p.x1.ptr + b * p.x1.sb + xh * p.x1.sh + x0 * p.x1.sr, p.x1.sr, rows, p.x1_vec, a.D, a.scale < 0.f,
+                                                     lane_base, nullptr, exchange, scratch);
+        x2_inv = tenmo_attn_stationary<DP, C::X2S, C::WGS>(p.x2.ptr + b * p.x2.sb + xh * p.x2.sh + x0 * p.x2.sr, p.x2.sr, rows, p.x2_vec, a.D, false,
+                                                      lane_base + C::X2_COL, x2_plane, exchange, scratch);
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
 
-    if (warp >= 8) {
-        tc::regs_down<88>();
-        if (warp == 9) {
+    if (warp >= C::ISSUER) {
+        if (C::WGS == 2) tc::regs_down<88>();
+        if (warp == C::LOADER) {
             if (lane == 0) {
                 fetch(n);
                 // every copy has landed before shared memory is given back (bounded)
                 int never = 0;
                 for (int t = max(0, fetched - C::STAGES); t < fetched; ++t) mbar_wait(full(t % C::STAGES), (uint32_t)(t / C::STAGES) & 1u, &never);
             }
-        } else if (warp == 8) {
+        } else if (warp == C::ISSUER) {
             const uint32_t tm = tc::uniform(tmem), stages = tc::uniform(smem_u32(smem));
             const int tiles = tc::uniform(n);
             constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_G = tc::idesc_f16(DP, true);
@@ -214,28 +228,29 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
             for (int j = 0; ok && j < tiles; ++j) {
                 const uint32_t s = tm + C::S_COL + (uint32_t)(j % NB) * T, ds = tm + C::P_COL + (uint32_t)(j % NB) * T, y1 = stages + slot * C::STAGE;
                 const bool more = j + NB < tiles;
-                if (!DKV && NB == 1 && more) {  // one buffer: S_{j+1} runs while the warpgroups make dS_j
+                auto sums_taken = [&]() { return j == 0 || wait(acc_free(j - 1), (j - 1) >> 1); };
+                if (NB == 1 && !DKV && more) {  // one buffer: S_{j+1} runs while the warpgroups make dS_j
                     ok = wait(s_read(j), j >> 1) && scores(j + 1);
                     if (!ok) break;
                 }
                 if (DKV) {
-                    ok = wait(p_full(j), j >> 1) && (j == 0 || wait(acc_free, j - 1));
+                    ok = wait(p_full(j), j >> 1) && sums_taken();
                     if (!ok) break;
                     tc::fence_after();
                     over_rows(tm + C::A2_COL, s, y1 + 2 * C::PLANE);
                     tc::commit(pv_done);
                 }
-                ok = wait(ds_full(j), j >> 1) && (DKV || j == 0 || wait(acc_free, j - 1));
+                ok = wait(ds_full(j), j >> 1) && (DKV || sums_taken());
                 if (!ok) break;
                 tc::fence_after();
                 over_rows(tm + C::A1_COL, ds, y1);
-                tc::commit(acc_full);
+                tc::commit(acc_full(j));
                 tc::commit(empty(slot));  // the tile is over
                 if (++slot == C::STAGES) slot = 0;
                 if (more) {
-                    if (DKV) ok = wait(pv_done, j) && scores(j + NB);                        // P_j has been read
-                    else if (NB == 2) ok = wait(s_read(j), j >> 1) && scores(j + NB);       // S_j has (long ago)
-                    ok = ok && wait(acc_full, j);                                           // dS_j has been read
+                    if (DKV) ok = wait(pv_done, j) && scores(j + NB);  // P_j has been read
+                    else if (NB == 2) ok = scores(j + NB);             // S_j has, before dS_j was there
+                    ok = ok && wait(acc_full(j), j >> 1);              // dS_j has been read
                     if (!ok) break;
                     tc::fence_after();
                     grads(j + NB);
@@ -247,212 +262,195 @@ __global__ void __launch_bounds__(THREADS, 1) attn_bwd_tc_kernel(const __grid_co
                 mbar_wait(drain, 0, &never);
             }
         }
-        __syncthreads();
-        __syncthreads();
-        if (DKV) { __syncthreads(); __syncthreads(); }
     } else {
-        tc::regs_up<208>();
-        float acc1[W], acc2[DKV ? W : 1];
+        if (C::WGS == 2) tc::regs_up<208>();
+        constexpr int W2 = DKV ? W : 2;   // the dq pass has no second gradient
+        constexpr int LD = W < 32 ? W : 32;  // columns at a time
+        float acc1[W], acc2[W2];
 #pragma unroll
         for (int d = 0; d < W; ++d) acc1[d] = 0.f;
 #pragma unroll
-        for (int d = 0; d < (DKV ? W : 1); ++d) acc2[d] = 0.f;
+        for (int d = 0; d < W2; ++d) acc2[d] = 0.f;
         const float c_row = fabsf(a.scale_log2) * x1_inv;
         // dq pass: the row's numbers
-        float m_row = INFINITY, il_row = 0.f, delta_row = 0.f;
+        float negm_row = -INFINITY, il_row = 0.f, delta_row = 0.f;
         int n_row = 0;
         if (!DKV && i < q_rows) {
             const float* info = p.info + (((int64_t)b * a.H + h) * p.q_info_tiles + (i >> 6)) * ATTN_INFO;
-            m_row = info[i & 63];
-            il_row = info[T + (i & 63)] / info[3 * T];
-            delta_row = info[2 * T + (i & 63)];
+            const int r = (int)(i & 63);
+            negm_row = info[4 * (r >> 1) + (r & 1)];
+            il_row = info[4 * (r >> 1) + 2 + (r & 1)] * info[3 * T + 2];
+            delta_row = info[2 * T + r];
             n_row = keys;
             if (a.causal) n_row = min(n_row, (int)max((int64_t)0, i + off + 1));
         }
-        // factors that the tile in flight in the accumulators is added with
-        float f1 = 0.f, f2 = 0.f;
         bool ok = true;
         auto await = [&](uint32_t bar, int phase) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, abort_flag)); };
+        // factors that the tile in flight in the accumulators is added with
+        float f1 = 0.f, f2 = 0.f;
         auto add_tile = [&](int j) {  // registers += accumulators of tile j
-            await(acc_full, j);
+            await(acc_full(j), j >> 1);
             if (!ok) return;
             tc::fence_after();
             const uint64_t g1 = tc::pack2(f1, f1), g2 = tc::pack2(f2, f2);
 #pragma unroll
-            for (int g = 0; g < W / 32; ++g) {
-                float t[32];
-                tc::ld32(lane_base + C::A1_COL + wg * W + 32 * g, t);
+            for (int g = 0; g < W / LD; ++g) {
+                float t[LD];
+                tc::ldn(lane_base + C::A1_COL + wg * W + LD * g, t);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2)
-                    tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), g1, tc::pack2(acc1[32 * g + e], acc1[32 * g + e + 1])), acc1[32 * g + e],
-                                acc1[32 * g + e + 1]);
+                for (int e = 0; e < LD; e += 2)
+                    tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), g1, tc::pack2(acc1[LD * g + e], acc1[LD * g + e + 1])), acc1[LD * g + e],
+                                acc1[LD * g + e + 1]);
                 if (DKV) {
-                    tc::ld32(lane_base + C::A2_COL + wg * W + 32 * g, t);
+                    tc::ldn(lane_base + C::A2_COL + wg * W + LD * g, t);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), g2, tc::pack2(acc2[(32 * g + e) % (DKV ? W : 1)], acc2[(32 * g + e + 1) % (DKV ? W : 1)])),
-                                    acc2[(32 * g + e) % (DKV ? W : 1)], acc2[(32 * g + e + 1) % (DKV ? W : 1)]);
+                    for (int e = 0; e < LD; e += 2)
+                        tc::unpack2(tc::fma2(tc::pack2(t[e], t[e + 1]), g2, tc::pack2(acc2[(LD * g + e) % W2], acc2[(LD * g + e + 1) % W2])),
+                                    acc2[(LD * g + e) % W2], acc2[(LD * g + e + 1) % W2]);
                 }
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_free);
+            if (lane == 0) mbar_arrive(acc_free(j));
         };
-        float y1_next = n > 0 ? __ldg(p.y1_inv + tile0) : 1.f, y2_next = n > 0 ? __ldg(p.y2_inv + tile0) : 1.f;
+        // What a tile's elements need besides S and dP: P = exp2(S c + (-m)) (il), dS = P (dP f G - delta G).  G, a power of two, brings dS
+        // to at most 2^15; PS is the power of two in il (dkv pass).
+        struct Tile {
+            uint64_t c2, fg2, ng2;  // c, f * G, -G (dkv) or -delta * G (dq)
+            float G, ps_inv;
+            const float* info;
+            int lim;                // first visible column (dkv) or their number (dq), of this thread's columns
+            bool whole;
+        };
+        auto set_up = [&](int j, float y1_inv, float y2_inv) {
+            Tile t;
+            const float c = c_row * y1_inv, f = x2_inv * y2_inv;  // dP = f * accumulator
+            const int col0 = NC * wg;
+            t.c2 = tc::pack2(c, c);
+            if (DKV) {
+                t.info = reinterpret_cast<const float*>(smem + (j % C::STAGES) * C::STAGE + 4 * C::PLANE);
+                t.ps_inv = t.info[3 * T + 2];  // read before dS is handed over: the stage may be refilled from then on
+                t.G = tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, t.info[3 * T + 1]));
+                t.ng2 = tc::pack2(-t.G, -t.G);
+                t.lim = a.causal ? (int)max((int64_t)-1, min((int64_t)T, i - off - (int64_t)(first + j) * T)) - col0 : 0;
+                t.whole = __all_sync(0xffffffffu, t.lim <= 0);
+            } else {
+                t.info = nullptr;
+                t.ps_inv = 1.f;
+                t.G = 32768.f * tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, fabsf(delta_row)));
+                t.ng2 = tc::pack2(-delta_row * t.G, -delta_row * t.G);
+                t.lim = n_row - j * T - col0;
+                t.whole = __all_sync(0xffffffffu, t.lim >= NC);
+            }
+            t.fg2 = tc::pack2(f * t.G, f * t.G);
+            return t;
+        };
+        const uint64_t negm2 = tc::pack2(negm_row, negm_row);
+        // columns u, u + 1 (of this thread's; info0: their rows' place in the tile): P, and its masking
+        auto prob2 = [&](const Tile& t, float x, float y, int u, int info0) {
+            uint64_t v;
+            if (DKV) {
+                const float4 mi = *reinterpret_cast<const float4*>(t.info + 2 * info0);
+                v = tc::fma2(tc::pack2(x, y), t.c2, tc::pack2(mi.x, mi.y));
+                tc::unpack2(v, x, y);
+                v = tc::mul2(tc::pack2(tc::ex2(x), tc::ex2(y)), tc::pack2(mi.z, mi.w));
+            } else {
+                v = tc::fma2(tc::pack2(x, y), t.c2, negm2);
+                tc::unpack2(v, x, y);
+                v = tc::pack2(tc::ex2(x), tc::ex2(y));
+            }
+            if (!t.whole) {
+                tc::unpack2(v, x, y);
+                x = (DKV ? u >= t.lim : u < t.lim) ? x : 0.f;
+                y = (DKV ? u + 1 >= t.lim : u + 1 < t.lim) ? y : 0.f;
+                v = tc::pack2(x, y);
+            }
+            return v;
+        };
+        auto dscore2 = [&](const Tile& t, uint64_t prob, float x, float y, int info0) {
+            uint64_t shift = t.ng2;
+            if (DKV) {
+                const float2 d = *reinterpret_cast<const float2*>(t.info + 2 * T + info0);
+                shift = tc::mul2(tc::pack2(d.x, d.y), t.ng2);
+            }
+            return tc::mul2(prob, tc::fma2(tc::pack2(x, y), t.fg2, shift));
+        };
+        auto factors = [&](const Tile& t, float y1_inv, float y2_inv) {
+            f1 = a.scale * y1_inv * tc::pow2_inverse(t.G) * (DKV ? t.ps_inv : il_row);
+            f2 = y2_inv * t.ps_inv;
+        };
+        // the tiles' scales come from L2: loaded a tile ahead
+        float y1_next = n ? __ldg(p.y1_inv + tile0) : 1.f, y2_next = n ? __ldg(p.y2_inv + tile0) : 1.f;
         for (int j = 0; j < n; ++j) {
-            // one buffer, dkv pass: the sums of tile j - 1 are taken first, while S_j is being computed
-            if (NB == 1 && DKV && j >= 1) add_tile(j - 1);
-            const float y1_inv = y1_next, y2_inv = y2_next;  // loaded a tile ahead: they come from L2
+            const float y1_inv = y1_next, y2_inv = y2_next;
             if (j + 1 < n) {
                 y1_next = __ldg(p.y1_inv + tile0 + j + 1);
                 y2_next = __ldg(p.y2_inv + tile0 + j + 1);
             }
+            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % NB) * T + NC * wg, d_addr = s_addr + (C::P_COL - C::S_COL);
+            // one buffer, dkv pass: the sums of tile j - 1 are taken first, while S_j is being computed
+            if (NB == 1 && DKV && j >= 1) add_tile(j - 1);
+            if (DKV) await(full(j % C::STAGES), j / C::STAGES);  // the row numbers that came with the tile
             await(s_full(j), j >> 1);
             if (!ok) break;
             tc::fence_after();
-            const float c = c_row * y1_inv;
-            const float f = x2_inv * y2_inv;  // dP = f * accumulator
-            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % NB) * T + 32 * wg, d_addr = lane_base + C::P_COL + (uint32_t)(j % NB) * T + 32 * wg;
-            const uint64_t c2 = tc::pack2(c, c);
-            float e[32];
-            tc::ld32(s_addr, e);
-            float G;  // power of two: dS at most 2^15
-            uint64_t nd2, fg2;
-            const float* info = nullptr;
-            float ps_inv = 1.f;  // read before dS is handed over: the stage may be refilled from then on
-            if (DKV) {
-                await(full(j % C::STAGES), j / C::STAGES);  // the row numbers that came with the tile
-                if (!ok) break;
-                info = reinterpret_cast<const float*>(smem + (j % C::STAGES) * C::STAGE + 4 * C::PLANE);
-                ps_inv = info[3 * T + 2];
-                G = tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, info[3 * T + 1]));
-                fg2 = tc::pack2(f * G, f * G);
-                nd2 = tc::pack2(-G, -G);
-                // visible columns start at lim (causal)
-                const int lim = a.causal ? (int)max((int64_t)-1, min((int64_t)T, i - off - (int64_t)(first + j) * T)) - 32 * wg : 0;
-                const bool whole = __all_sync(0xffffffffu, lim <= 0);
-                uint32_t hi[16], lo[16];
-                const float2* mi = reinterpret_cast<const float2*>(info + 32 * wg);
-                const float2* il = reinterpret_cast<const float2*>(info + T + 32 * wg);
+            const Tile t = set_up(j, y1_inv, y2_inv);
+            float e[NC];
+            tc::ldn(s_addr, e);
+            if (!DKV) {  // nothing is written over S
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_read(j));
+            }
 #pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    const float2 mm = mi[u], ii = il[u];
-                    float x, y;
-                    tc::unpack2(tc::fma2(tc::pack2(e[2 * u], e[2 * u + 1]), c2, tc::pack2(-mm.x, -mm.y)), x, y);
-                    tc::unpack2(tc::mul2(tc::pack2(tc::ex2(x), tc::ex2(y)), tc::pack2(ii.x, ii.y)), x, y);
-                    if (!whole) {
-                        x = 2 * u >= lim ? x : 0.f;
-                        y = 2 * u + 1 >= lim ? y : 0.f;
-                    }
-                    e[2 * u] = x;
-                    e[2 * u + 1] = y;
-                    tc::split_pair(x, y, hi[u], lo[u]);
-                }
-                tc::st_pairs(s_addr, hi, lo);
+            for (int u = 0; u < NC; u += 2) tc::unpack2(prob2(t, e[u], e[u + 1], u, NC * wg + u), e[u], e[u + 1]);
+            if (DKV) {
+                tc::st_split(s_addr, e);
                 tc::st_wait();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(j));
-            } else {
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_read(j));
-                G = 32768.f * tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, fabsf(delta_row)));
-                fg2 = tc::pack2(f * G, f * G);
-                nd2 = tc::pack2(-delta_row * G, -delta_row * G);
-                const int lim = n_row - j * T - 32 * wg;
-                const bool whole = __all_sync(0xffffffffu, lim >= 32);
-                const uint64_t m2 = tc::pack2(-m_row, -m_row);
-#pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    float x, y;
-                    tc::unpack2(tc::fma2(tc::pack2(e[2 * u], e[2 * u + 1]), c2, m2), x, y);
-                    x = tc::ex2(x);
-                    y = tc::ex2(y);
-                    if (!whole) {
-                        x = 2 * u < lim ? x : 0.f;
-                        y = 2 * u + 1 < lim ? y : 0.f;
-                    }
-                    e[2 * u] = x;
-                    e[2 * u + 1] = y;
-                }
-                if (NB == 1 && j >= 1) add_tile(j - 1);  // while dP_j is being computed
+            } else if (NB == 1 && j >= 1) {
+                add_tile(j - 1);  // while dP_j is being computed
             }
             await(d_full(j), j >> 1);
             if (!ok) break;
             tc::fence_after();
             {
-                float t[32];
-                tc::ld32(d_addr, t);
-                uint32_t hi[16], lo[16];
-                const float2* dl = reinterpret_cast<const float2*>(info + 2 * T + 32 * wg);
+                float v[NC];
+                tc::ldn(d_addr, v);
 #pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    uint64_t shift = nd2;
-                    if (DKV) {
-                        const float2 d = dl[u];
-                        shift = tc::mul2(tc::pack2(d.x, d.y), nd2);
-                    }
-                    const uint64_t v = tc::mul2(tc::pack2(e[2 * u], e[2 * u + 1]), tc::fma2(tc::pack2(t[2 * u], t[2 * u + 1]), fg2, shift));
-                    float x, y;
-                    tc::unpack2(v, x, y);
-                    tc::split_pair(x, y, hi[u], lo[u]);
-                }
-                tc::st_pairs(d_addr, hi, lo);
+                for (int u = 0; u < NC; u += 2) tc::unpack2(dscore2(t, tc::pack2(e[u], e[u + 1]), v[u], v[u + 1], NC * wg + u), v[u], v[u + 1]);
+                tc::st_split(d_addr, v);
             }
             tc::st_wait();
             tc::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(ds_full(j));
             if (NB == 2 && j >= 1) add_tile(j - 1);
-            // now the factors of tile j
-            if (DKV) {
-                f1 = a.scale * y1_inv * ps_inv * tc::pow2_inverse(G);
-                f2 = y2_inv * ps_inv;
-            } else {
-                f1 = a.scale * il_row * y1_inv * tc::pow2_inverse(G);
-            }
+            factors(t, y1_inv, y2_inv);
+            if (!ok) break;
         }
         if (ok && n > 0) add_tile(n - 1);
 
-        // ---- through the stages to memory: 16-byte chunk q of row r at chunk q ^ (r & 7) ----
-        float* const buf = reinterpret_cast<float*>(smem);
-        const bool valid = i < x_rows;
-        auto write = [&](const float* acc, const TenmoHeadsView& out, int vec) {
-            __syncthreads();
+        // ---- to memory, through the stages ----
+        const bool valid = i < x_rows;  // rows that take no part: zeros
+        const int row0 = x_tile * ROWS + 32 * (warp & 3), here = (DKV ? a.Sk : a.Sq) - row0;
+        auto out_row = [&](const TenmoHeadsView& out) { return out.ptr + b * out.sb + h * out.sh + (int64_t)row0 * out.sr; };
+        float* const scratch = reinterpret_cast<float*>(smem) + warp * (32 * W);  // all products are done: the stages are free
 #pragma unroll
-            for (int d = 0; d < W; d += 4) {
-                const int q = (wg * W + d) >> 2;
-                *reinterpret_cast<float4*>(buf + row * DP + ((q ^ (row & 7)) << 2)) =
-                    valid ? make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            __syncthreads();
-            const int total = DKV ? a.Sk : a.Sq, here = min(ROWS, total - x_tile * ROWS);
-            float* base = out.ptr + b * out.sb + h * out.sh + (int64_t)x_tile * ROWS * out.sr;
-            for (int q = threadIdx.x; q < here * (DP / 4); q += 256) {
-                const int r = q / (DP / 4), ch = q % (DP / 4), d = 4 * ch;
-                if (d >= a.D) continue;
-                float4 x = *reinterpret_cast<const float4*>(buf + r * DP + ((ch ^ (r & 7)) << 2));
-                float* dst = base + r * out.sr + d;
-                if (vec) {
-                    if (p.beta != 0.f) {
-                        const float4 o = *reinterpret_cast<const float4*>(dst);
-                        x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
-                    }
-                    *reinterpret_cast<float4*>(dst) = x;
-                } else {
-                    const float v[4] = {x.x, x.y, x.z, x.w};
-                    for (int u = 0; u < 4 && d + u < a.D; ++u) dst[u] = p.beta != 0.f ? dst[u] + v[u] : v[u];
-                }
-            }
-        };
-        write(acc1, p.out1, p.out1_vec);
-        if (DKV) write(acc2, p.out2, p.out2_vec);
+        for (int d = 0; d < W; ++d) acc1[d] = valid ? acc1[d] : 0.f;
+        tenmo_attn_write_rows<W>(acc1, out_row(p.out1) + wg * W, p.out1.sr, here, a.D - wg * W, p.out1_vec, p.beta != 0.f, scratch);
+        if constexpr (DKV) {
+#pragma unroll
+            for (int d = 0; d < W; ++d) acc2[d] = valid ? acc2[d] : 0.f;
+            tenmo_attn_write_rows<W>(acc2, out_row(p.out2) + wg * W, p.out2.sr, here, a.D - wg * W, p.out2_vec, p.beta != 0.f, scratch);
+        }
     }
     tc::fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, TENMO_DEV_TIMEOUT);
-    if (warp == 8) {
+    if (warp == C::ISSUER) {
         tc::fence_after();
         tc::dealloc(tmem, C::TMEM);
     }
@@ -482,7 +480,7 @@ int launch(tenmo_ctx* ctx, const BwdParams& p) {
     const int smem = BwdCfg<DP, DKV>::SMEM;
     TENMO_CUDA_TRY(ctx, cudaFuncSetAttribute(attn_bwd_tc_kernel<DP, DKV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const unsigned grid = (unsigned)((int64_t)p.a.B * p.a.H * p.x_tiles);
-    attn_bwd_tc_kernel<DP, DKV><<<grid, THREADS, smem, ctx->stream>>>(p);
+    attn_bwd_tc_kernel<DP, DKV><<<grid, BwdCfg<DP, DKV>::THREADS, smem, ctx->stream>>>(p);
     TENMO_LAUNCH_CHECK(ctx, "attn_bwd_tc_kernel");
     return TENMO_OK;
 }

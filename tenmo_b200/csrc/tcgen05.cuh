@@ -102,6 +102,51 @@ __device__ __forceinline__ Desc desc_k(uint32_t panel) { return desc2(panel, 16u
 constexpr int STEP_MN = 128;
 __device__ __forceinline__ Desc desc_mn(uint32_t plane, int rows) { return desc2(plane, (uint32_t)(rows * 128), 1024u); }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// packed pairs: two round-to-nearest operations per instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// fp16 pairs (first value in the low half)
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+// hi / lo of two values.  hi is the value cut to 11 significant bits (a logical AND instead of a conversion back), which fp16
+// holds exactly down to 2^-14; below that hi is rounded to the fp16 grid and the pair is good to 2^-25 absolute, the same floor
+// that lo has.  The cut leaves lo at most 13 bits, of which fp16 keeps 11: 22 bits together.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+    hi = half_pair(ah, bh);
+    float al, bl;
+    unpack2(fma2(pack2(ah, bh), pack2(-1.f, -1.f), pack2(a, b)), al, bl);  // both differences, exact, in one instruction
+    lo = half_pair(al, bl);
+}
+
 // 64 / 32 / 16 consecutive columns of this warp's 32 lanes; the wait is part of the instruction, so nothing reads too early
 __device__ __forceinline__ void ld32(uint32_t addr, float (&f)[32]) {
     uint32_t r[32];
@@ -153,6 +198,39 @@ __device__ __forceinline__ void ld16(uint32_t addr, float (&f)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(r[i]);
 }
+// two places at once
+__device__ __forceinline__ void ld16x2(uint32_t addr_a, uint32_t addr_b, float (&f)[16], float (&g)[16]) {
+    uint32_t r[16], s[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(s[0]), "=r"(s[1]), "=r"(s[2]), "=r"(s[3]), "=r"(s[4]), "=r"(s[5]), "=r"(s[6]), "=r"(s[7]), "=r"(s[8]), "=r"(s[9]), "=r"(s[10]), "=r"(s[11]), "=r"(s[12]), "=r"(s[13]), "=r"(s[14]), "=r"(s[15])
+        : "r"(addr_a), "r"(addr_b)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        f[i] = __uint_as_float(r[i]);
+        g[i] = __uint_as_float(s[i]);
+    }
+}
+__device__ __forceinline__ void ld32x2(uint32_t addr_a, uint32_t addr_b, float (&f)[32], float (&g)[32]) {
+    uint32_t r[32], s[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(s[0]), "=r"(s[1]), "=r"(s[2]), "=r"(s[3]), "=r"(s[4]), "=r"(s[5]), "=r"(s[6]), "=r"(s[7]), "=r"(s[8]), "=r"(s[9]), "=r"(s[10]), "=r"(s[11]), "=r"(s[12]), "=r"(s[13]), "=r"(s[14]), "=r"(s[15]), "=r"(s[16]), "=r"(s[17]), "=r"(s[18]), "=r"(s[19]), "=r"(s[20]), "=r"(s[21]), "=r"(s[22]), "=r"(s[23]), "=r"(s[24]), "=r"(s[25]), "=r"(s[26]), "=r"(s[27]), "=r"(s[28]), "=r"(s[29]), "=r"(s[30]), "=r"(s[31])
+        : "r"(addr_a), "r"(addr_b)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        f[i] = __uint_as_float(r[i]);
+        g[i] = __uint_as_float(s[i]);
+    }
+}
 __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -166,18 +244,21 @@ __device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-// 32 values as fp16 pairs over the 32 columns that they came from: of every 16 columns eight of hi pairs, then eight of lo pairs
-__device__ __forceinline__ void st_pairs(uint32_t addr, const uint32_t (&hi)[16], const uint32_t (&lo)[16]) {
-    uint32_t a[16], b[16];
+// N values as fp16 pairs over the N columns that they came from: of every 16 columns eight of hi pairs, then eight of lo pairs
+template <int N>
+__device__ __forceinline__ void st_split(uint32_t addr, const float (&x)[N]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        a[i] = hi[i];
-        a[8 + i] = lo[i];
-        b[i] = hi[8 + i];
-        b[8 + i] = lo[8 + i];
+    for (int g = 0; g < N / 16; ++g) {
+        uint32_t r[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split_pair(x[16 * g + 2 * e], x[16 * g + 2 * e + 1], r[e], r[8 + e]);
+        st16(addr + 16 * g, r);
     }
-    st16(addr, a);
-    st16(addr + 16, b);
+}
+template <int N>
+__device__ __forceinline__ void ldn(uint32_t addr, float (&f)[N]) {
+    if constexpr (N == 16) ld16(addr, f);
+    else ld32(addr, f);
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -190,51 +271,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                  "r"(bytes), "r"(bar)
                  : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// packed pairs: two round-to-nearest operations per instruction
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-// fp16 pairs (first value in the low half)
-__device__ __forceinline__ uint32_t half_pair(float a, float b) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
-    return r;
-}
-// hi / lo of two values.  hi is the value cut to 11 significant bits (a logical AND instead of a conversion back), which fp16
-// holds exactly down to 2^-14; below that hi is rounded to the fp16 grid and the pair is good to 2^-25 absolute, the same floor
-// that lo has.  The cut leaves lo at most 13 bits, of which fp16 keeps 11: 22 bits together.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-    hi = half_pair(ah, bh);
-    float al, bl;
-    unpack2(fma2(pack2(ah, bh), pack2(-1.f, -1.f), pack2(a, b)), al, bl);  // both differences, exact, in one instruction
-    lo = half_pair(al, bl);
 }
 
 // 2^e that brings `largest` (finite, >= 0) into [2^14, 2^15), and its inverse.  0 and what is too small to be brought there
