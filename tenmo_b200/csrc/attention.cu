@@ -66,7 +66,7 @@ __device__ __forceinline__ bool warp_row(int64_t rows_per_head, int heads, int64
 // A lane holds four columns; LPK lanes are a row of k or v, so a warp's load covers 32 / LPK whole rows.  Scores: partial dot products of
 // eight loads, summed over the lanes by halving (a lane passes on the half it does not keep: V shuffles for V sums instead of
 // log2(LPK) V).  The exponentials of 32 keys are taken with a lane per key, and go through shared memory to be multiplied with v.
-// Four warps take 32 keys in turn and are joined at the end; with few rows and many keys the keys are cut into slices, one block
+// Four warps take 32 keys (16 above 32 columns) in turn and are joined at the end; with few rows and many keys the keys are cut into slices, one block
 // each, which attn_join_kernel adds in order.
 // Bound: HBM for one token (k and v are read once, 16 bytes a lane), launch latency for the smallest calls.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -87,7 +87,8 @@ __device__ __forceinline__ void few_row(const TenmoAttnParams& p, int kvh, int r
 
 template <int LPK, int R>
 __global__ void __launch_bounds__(FEW_WARPS * 32) attn_fwd_few_kernel(const FewParams f) {
-    constexpr int KPL = 32 / LPK, V = 8 * R;  // rows per load; partial sums of eight loads
+    constexpr int KPL = 32 / LPK, V = 8 * R;           // rows per load; partial sums of eight loads
+    constexpr int LOADS = LPK == 32 ? 16 : 8, KEYS = LOADS * KPL;  // of a warp at a time: 32 keys, 16 above 32 columns
     __shared__ __align__(16) float pk[FEW_WARPS][32 * R];
     __shared__ __align__(16) float so[FEW_WARPS][R][4 * LPK];
     __shared__ float sm[FEW_WARPS][R], sl[FEW_WARPS][R];
@@ -117,8 +118,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) attn_fwd_few_kernel(const FewP
             }
         }
     }
-    // this block's keys: whole groups of 128
-    const int per = ((most + f.slices - 1) / f.slices + 127) / 128 * 128;
+    // this block's keys: whole groups of what its warps take at a time
+    constexpr int ALL = KEYS * FEW_WARPS;
+    const int per = ((most + f.slices - 1) / f.slices + ALL - 1) / ALL * ALL;
     const int begin = min(most, slice * per), end = min(most, begin + per);
     const float* k = p.k.ptr + b * p.k.sb + kvh * p.k.sh;
     const float* v = p.v.ptr + b * p.v.sb + kvh * p.v.sh;
@@ -146,18 +148,20 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) attn_fwd_few_kernel(const FewP
         o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float* const mine = pk[warp];
-    for (int j0 = begin + 32 * warp; j0 < end; j0 += 32 * FEW_WARPS) {
+    for (int j0 = begin + KEYS * warp; j0 < end; j0 += KEYS * FEW_WARPS) {
+        float4 xk[LOADS], xv[LOADS];  // the rows of k and of v are all in flight before the first is used
 #pragma unroll
-        for (int t0 = 0; t0 < LPK; t0 += 8) {
-            float4 x[8];
+        for (int t = 0; t < LOADS; ++t) xk[t] = load(k, p.k.sr, j0 + t * KPL + sub, f.k_vec);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) x[t] = load(k, p.k.sr, j0 + (t0 + t) * KPL + sub, f.k_vec);
+        for (int t = 0; t < LOADS; ++t) xv[t] = load(v, p.v.sr, j0 + t * KPL + sub, f.v_vec);
+#pragma unroll
+        for (int t0 = 0; t0 < LOADS; t0 += 8) {
             float s[V];
 #pragma unroll
             for (int t = 0; t < 8; ++t)
 #pragma unroll
                 for (int r = 0; r < R; ++r)
-                    s[t * R + r] = fmaf(x[t].x, q[r].x, x[t].y * q[r].y) + fmaf(x[t].z, q[r].z, x[t].w * q[r].w);
+                    s[t * R + r] = fmaf(xk[t0 + t].x, q[r].x, xk[t0 + t].y * q[r].y) + fmaf(xk[t0 + t].z, q[r].z, xk[t0 + t].w * q[r].w);
             int n = V, at = 0;
 #pragma unroll
             for (int w = LPK / 2; w > 0; w >>= 1) {
@@ -185,31 +189,25 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) attn_fwd_few_kernel(const FewP
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float s = j0 + lane < min(end, seen[r]) ? mine[lane * R + r] * p.scale_log2 : -INFINITY;
+            const float s = lane < KEYS && j0 + lane < min(end, seen[r]) ? mine[(lane % KEYS) * R + r] * p.scale_log2 : -INFINITY;
             const float top = fmaxf(m[r], tenmo_warp_max(s));
             const float base = top == -INFINITY ? 0.f : top;  // every score so far is -inf
             const float e = exp2f(s - base), shrink = exp2f(m[r] - base);
             m[r] = top;
             l[r] = l[r] * shrink + e;
             o[r].x *= shrink; o[r].y *= shrink; o[r].z *= shrink; o[r].w *= shrink;
-            mine[lane * R + r] = e;
+            if (lane < KEYS) mine[lane * R + r] = e;
         }
         __syncwarp();
 #pragma unroll
-        for (int t0 = 0; t0 < LPK; t0 += 8) {
-            float4 x[8];
+        for (int t = 0; t < LOADS; ++t) {
+            const float* w = mine + (t * KPL + sub) * R;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) x[t] = load(v, p.v.sr, j0 + (t0 + t) * KPL + sub, f.v_vec);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float* w = mine + ((t0 + t) * KPL + sub) * R;
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    o[r].x = fmaf(w[r], x[t].x, o[r].x);
-                    o[r].y = fmaf(w[r], x[t].y, o[r].y);
-                    o[r].z = fmaf(w[r], x[t].z, o[r].z);
-                    o[r].w = fmaf(w[r], x[t].w, o[r].w);
-                }
+            for (int r = 0; r < R; ++r) {
+                o[r].x = fmaf(w[r], xv[t].x, o[r].x);
+                o[r].y = fmaf(w[r], xv[t].y, o[r].y);
+                o[r].z = fmaf(w[r], xv[t].z, o[r].z);
+                o[r].w = fmaf(w[r], xv[t].w, o[r].w);
             }
         }
         __syncwarp();
@@ -265,20 +263,30 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const FewParams f) {
     const int lane = threadIdx.x & 31;
     const int64_t row = ((int64_t)b * p.H + h) * p.Sq + i;
     const float* src = f.partial + row * f.slices * f.ldp;
-    float top = -INFINITY;
-    for (int s = lane; s < f.slices; s += 32) top = fmaxf(top, src[s * f.ldp + p.D]);
+    // a lane per slice (at most 64) for the weights, then a lane per column
+    float ms[2], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        ms[u] = lane + 32 * u < f.slices ? src[(lane + 32 * u) * f.ldp + p.D] : -INFINITY;
+        top = fmaxf(top, ms[u]);
+    }
     top = tenmo_warp_max(top);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[DSLOTS];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        ms[u] = exp2f(ms[u] - base);
+        if (lane + 32 * u < f.slices) sum = fmaf(src[(lane + 32 * u) * f.ldp + p.D + 1], ms[u], sum);
+    }
+    sum = tenmo_warp_sum(sum);
+    float x[DSLOTS];
 #pragma unroll
     for (int t = 0; t < DSLOTS; ++t) x[t] = 0.f;
+#pragma unroll 4
     for (int s = 0; s < f.slices; ++s) {
-        const float* part = src + s * f.ldp;
-        const float w = exp2f(part[p.D] - base);
-        sum = fmaf(part[p.D + 1], w, sum);
+        const float w = __shfl_sync(0xffffffffu, s < 32 ? ms[0] : ms[1], s & 31);
 #pragma unroll
         for (int t = 0; t < DSLOTS; ++t)
-            if (lane + 32 * t < p.D) x[t] = fmaf(part[lane + 32 * t], w, x[t]);
+            if (lane + 32 * t < p.D) x[t] = fmaf(src[s * f.ldp + lane + 32 * t], w, x[t]);
     }
     float* o = p.o.ptr + b * p.o.sb + h * p.o.sh + i * p.o.sr;
 #pragma unroll
@@ -427,8 +435,8 @@ int few_fwd(tenmo_ctx* ctx, const TenmoAttnParams& p) {
     const int64_t groups = (total + R - 1) / R, blocks = groups * p.Hkv * p.B;
     if (groups > INT32_MAX || blocks > INT32_MAX / 64) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "attention_fwd: too many rows in one call");
     f.groups = (int)groups;
-    // slices of at least 256 keys, as many as it takes to give every SM about four blocks
-    int64_t slices = (4 * (int64_t)ctx->sm_count + blocks - 1) / blocks;
+    // slices of at least 256 keys, as many as it takes to give every SM about eight blocks
+    int64_t slices = (8 * (int64_t)ctx->sm_count + blocks - 1) / blocks;
     if (slices > p.Sk / 256) slices = p.Sk / 256;
     if (slices > 64) slices = 64;
     if (slices < 1) slices = 1;

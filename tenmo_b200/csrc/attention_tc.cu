@@ -1,30 +1,32 @@
 // Tensor-core attention, forward: tile images and the fused kernel.
 //
 // Kernel.  A CTA owns 128 rows of one head.  Its q rows are split into fp16 pairs (scaled per row) and kept in tensor memory as
-// the left operand; k and v come as 64-row tile images through a ring of three stages.  Per tile j:
+// the left operand; k and v come as 128-row tile images through a ring of three slots (k_0, v_0, k_1, ...).  Per tile j:
 //   S_j = q k_j^T          left operand and accumulator in tensor memory
 //   P_j = exp2(S_j c - m)  by warpgroups, a row per thread, written over S_j as fp16 pairs: the next left operand
 //   O_j = P_j v_j          a fresh accumulator, added to the row's registers (and rescaled) with rounding
 // The running reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.
-// What bounds the kernel is not a pipe but the chain S -> maximum -> exponentials -> P -> O of a tile, a few thousand cycles of
-// latencies.  So the columns of a tile are shared by two warpgroups (dim up to 64; 32 columns of S and of O a thread) or four (up
-// to 128), which exchange their maxima through shared memory; the output of tile j - 1 is added after P_j; two or three S buffers
-// let S_{j+1} run meanwhile; and up to dim 64, where everything fits twice into an SM (96 KB, 256 columns), two CTAs fill each
-// other's gaps.  One warp issues the MMAs, one the copies.
+// What bounds the kernel is not a pipe but the instructions around the products and the chain S -> maximum -> exponentials -> P -> O
+// of a tile, thousands of cycles of latencies.  So tiles are wide (128 keys: the waits, fences and exchanges of a tile are paid half as
+// often as with 64), their columns are shared by two warpgroups (dim up to 64; 64 columns of S, 32 of O a thread) or four (up to
+// 128), which exchange their maxima through shared memory, and up to dim 64, where everything fits twice into an SM (96 KB,
+// 256 columns), two CTAs fill each other's gaps: one's products run while the other's exponentials are taken.  Up to dim 128 one
+// CTA has the SM and a second S buffer lets S_{j+1} run while P_j is made.  One warp issues the MMAs, one the copies.
 // Bound: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
 #include "attention_tc.cuh"
 
 namespace {
 
 constexpr int ROWS = 128;
-constexpr int T = ATTN_TILE;
-constexpr int STAGES = 3;
+constexpr int T = 128;     // keys of a tile
+constexpr int SLOTS = 3;   // of the ring
+constexpr int RT = ATTN_TILE;  // rows of a tile with row numbers
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Tile images.  A block makes one tile: 8 columns (a 16-byte chunk of each plane) per thread and step.
 // ---------------------------------------------------------------------------------------------------------------------
 // delta_i = sum_d go o and the saved statistics of a tile's rows (x: this thread's columns of go)
-template <int DP>
+template <int DP, int T>
 __device__ __forceinline__ void attn_row_numbers(const TenmoTileJobs& jobs, const TenmoTileJob& j, int64_t t, int b, int h, int tile, int rows,
                                                  const float (&x)[T * (DP / 8) / 256][8]) {
     constexpr int CHUNKS = DP / 8, STEPS = T * CHUNKS / 256;
@@ -75,7 +77,7 @@ __device__ __forceinline__ void attn_row_numbers(const TenmoTileJobs& jobs, cons
     __syncthreads();
 }
 
-template <int DP>
+template <int DP, int T>
 __global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs jobs) {
     constexpr int CHUNKS = DP / 8, STEPS = T * CHUNKS / 256;
     __shared__ float largest[8];
@@ -103,9 +105,18 @@ __global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs job
             for (int e = 0; e < 8; ++e) x[s][e] = r < rows && d + e < jobs.D ? __ldg(p + e) : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, tc::finite_abs(x[s][e]));
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));  // a NaN does not count
     }
-    if (j.o.ptr) attn_row_numbers<DP>(jobs, j, t, b, h, tile, rows, x);
+    if (!(mx <= 3.402823466e38f)) {  // an infinity does not either
+        mx = 0.f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, tc::finite_abs(x[s][e]));
+    }
+    if constexpr (T == RT) {
+        if (j.o.ptr) attn_row_numbers<DP, T>(jobs, j, t, b, h, tile, rows, x);
+    }
     mx = tenmo_warp_max(mx);
     if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = mx;
     __syncthreads();
@@ -146,14 +157,14 @@ struct FwdCfg {
     static constexpr int THREADS = 128 * WGS + 64;
     static constexpr int ISSUER = 4 * WGS, LOADER = ISSUER + 1;
     static constexpr int NC = T / WGS, W = DP / WGS;  // columns of S and of O of a thread
-    static constexpr int NB = DP == 64 ? 2 : 3;     // S / P buffers
+    static constexpr int NB = DP == 64 ? 1 : 2;     // S / P buffers
     static constexpr int PLANE = T * DP * 2;        // bytes of one plane of a tile
-    static constexpr int IMG = 2 * PLANE;           // a tile's hi and lo plane
-    static constexpr int STAGE = 2 * IMG;           // a slot for k, one for v
+    static constexpr int IMG = 2 * PLANE;           // a tile's hi and lo plane, a slot of the ring
     static constexpr int Q_COLS = DP;               // hi DP/2, lo DP/2
     static constexpr int S_COL = Q_COLS, O_COL = Q_COLS + NB * T;
     static constexpr int TMEM = DP == 64 ? 256 : 512;
-    static constexpr int SMEM = STAGES * STAGE + 2 * WGS * 128 * 4 + 512;
+    static constexpr int RING = SLOTS * IMG;
+    static constexpr int SMEM = RING + 2 * WGS * 128 * 4 + 512;
     static_assert(O_COL + DP <= TMEM, "tensor memory");
 };
 
@@ -161,15 +172,15 @@ template <int DP>
 __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams p) {
     using C = FwdCfg<DP>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    float* const shared_f = reinterpret_cast<float*>(smem + STAGES * C::STAGE);  // [2][WGS][128] row maxima
-    const uint32_t bars = smem_u32(smem + STAGES * C::STAGE + 2 * C::WGS * 128 * 4);
-    auto full = [&](int which, int slot) { return bars + 8u * (3 * which + slot); };         // which: 0 k, 1 v
-    auto empty = [&](int which, int slot) { return bars + 8u * (16 + 3 * which + slot); };
+    float* const shared_f = reinterpret_cast<float*>(smem + C::RING);  // [2][WGS][128] row maxima
+    const uint32_t bars = smem_u32(smem + C::RING + 2 * C::WGS * 128 * 4);
+    auto full = [&](int slot) { return bars + 8u * slot; };
+    auto empty = [&](int slot) { return bars + 8u * (3 + slot); };
     auto s_full = [&](int j) { return bars + 8u * (6 + (j & 1)); };
     auto p_full = [&](int j) { return bars + 8u * (8 + (j & 1)); };
     auto o_full = [&](int j) { return bars + 8u * (10 + (j & 1)); };
     const uint32_t o_free = bars + 8u * 12, drain = bars + 8u * 13;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * C::STAGE + 2 * C::WGS * 128 * 4 + 256);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::RING + 2 * C::WGS * 128 * 4 + 256);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const TenmoAttnParams& a = p.a;
@@ -187,7 +198,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     const int64_t tile0 = ((int64_t)b * a.Hkv + kvh) * p.tiles;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full(0, s), 1); mbar_init(full(1, s), 1); mbar_init(empty(0, s), 1); mbar_init(empty(1, s), 1); }
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4 * C::WGS); mbar_init(o_full(w), 1); }
         mbar_init(o_free, 4 * C::WGS);
         mbar_init(drain, 1);
@@ -200,20 +211,21 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     tc::fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // The ring of tiles: slot s holds k and v of a tile j = s mod STAGES, each refilled as soon as its product is done (one thread).
+    // The ring (one thread): tiles in the order in which the products use them, each as soon as its slot's last product is done.
+    // One S buffer: k_0, v_0, k_1, v_1, ...; two: k_0, k_1, v_0, k_2, v_1, ..., v_{n-1}.
     int fetched = 0, fetch_slot = 0, fetch_round = 0;
     auto fetch = [&](int until) {
         for (; fetched < until; ++fetched) {
-            for (int which = 0; which < 2; ++which) {
-                if (fetch_round && !mbar_wait(empty(which, fetch_slot), (uint32_t)(fetch_round - 1) & 1u, abort_flag)) return;
-                const uint32_t bar = full(which, fetch_slot);
-                mbar_expect_tx(bar, C::IMG);
-                tc::bulk_load(smem_u32(smem) + (fetch_slot * 2 + which) * C::IMG, (which ? p.v_img : p.k_img) + (tile0 + fetched) * C::IMG, C::IMG, bar);
-            }
-            if (++fetch_slot == STAGES) { fetch_slot = 0; ++fetch_round; }
+            if (fetch_round && !mbar_wait(empty(fetch_slot), (uint32_t)(fetch_round - 1) & 1u, abort_flag)) return;
+            const uint32_t bar = full(fetch_slot);
+            mbar_expect_tx(bar, C::IMG);
+            const bool v = C::NB == 1 ? (fetched & 1) != 0 : (fetched & 1) ? fetched == 2 * n_tiles - 1 : fetched != 0;
+            const int t = C::NB == 1 ? fetched >> 1 : v ? (fetched - 1) >> 1 : (fetched + 1) >> 1;
+            tc::bulk_load(smem_u32(smem) + fetch_slot * C::IMG, (v ? p.v_img : p.k_img) + (tile0 + t) * C::IMG, C::IMG, bar);
+            if (++fetch_slot == SLOTS) { fetch_slot = 0; ++fetch_round; }
         }
     };
-    if (threadIdx.x == 32 * C::LOADER) fetch(min(n_tiles, STAGES - 1));  // the last slot is scratch for now
+    if (threadIdx.x == 32 * C::LOADER) fetch(min(2 * n_tiles, SLOTS - 1));  // the last slot is scratch for now
 
     // ---- q into tensor memory ----
     const int wg = warp >> 2, row = threadIdx.x & 127;
@@ -223,7 +235,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     if (warp < C::ISSUER)  // the sign of the scale goes with q: the factor of the scores is then never negative
         q_inv = tenmo_attn_stationary<DP, false, C::WGS>(a.q.ptr + b * a.q.sb + h * a.q.sh + (int64_t)q_tile * ROWS * a.q.sr, a.q.sr,
                                                          q_rows - q_tile * ROWS, p.q_vec, a.D, a.scale < 0.f, lane_base, nullptr, shared_f,
-                                                         reinterpret_cast<float*>(smem + (STAGES - 1) * C::STAGE));
+                                                         reinterpret_cast<float*>(smem + (SLOTS - 1) * C::IMG));
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -231,22 +243,22 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     if (warp >= C::ISSUER) {
         if (warp == C::LOADER) {
             if (lane == 0) {
-                fetch(n_tiles);
-                // every copy has landed before shared memory is given back (bounded): by now they are the last STAGES tiles'
+                fetch(2 * n_tiles);
+                // every copy has landed before shared memory is given back (bounded): by now they are the last ones
                 int never = 0;
-                for (int t = max(0, fetched - STAGES); t < fetched; ++t)
-                    for (int which = 0; which < 2; ++which) mbar_wait(full(which, t % STAGES), (uint32_t)(t / STAGES) & 1u, &never);
+                for (int t = max(0, fetched - SLOTS); t < fetched; ++t) mbar_wait(full(t % SLOTS), (uint32_t)(t / SLOTS) & 1u, &never);
             }
         } else if (warp == C::ISSUER) {
             const uint32_t tm = tc::uniform(tmem), stages = tc::uniform(smem_u32(smem));
             const int n = tc::uniform(n_tiles);
             constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_O = tc::idesc_f16(DP, true);
             auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
-            int s_slot = 0, s_phase = 0, s_buf = 0;  // of the next S
+            int slot = 0, phase = 0;
+            auto next_slot = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
             auto scores = [&](int j) {
-                if (!wait(full(0, s_slot), s_phase)) return false;
+                if (!wait(full(slot), phase)) return false;
                 tc::fence_after();
-                const uint32_t hi = stages + s_slot * C::STAGE, d = tm + C::S_COL + (uint32_t)s_buf * T;
+                const uint32_t hi = stages + slot * C::IMG, d = tm + C::S_COL + (uint32_t)(j % C::NB) * T;
 #pragma unroll
                 for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + DP / 2 + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, c == 0);
 #pragma unroll
@@ -254,30 +266,32 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
 #pragma unroll
                 for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, false);
                 tc::commit(s_full(j));
-                tc::commit(empty(0, s_slot));
-                if (++s_slot == STAGES) { s_slot = 0; s_phase ^= 1; }
-                if (++s_buf == C::NB) s_buf = 0;
+                tc::commit(empty(slot));
+                next_slot();
                 return true;
             };
             bool ok = n == 0 || scores(0);
-            int v_slot = 0, v_phase = 0, p_buf = 0;
             for (int j = 0; ok && j < n; ++j) {
-                // Two buffers: S_{j+1} replaces P_{j-1}, whose product must be done.  Three: P_{j-2}, whose output has been read (o_free below).
-                if (C::NB == 2 && j >= 1) ok = wait(o_full(j - 1), (uint32_t)((j - 1) >> 1) & 1u);
-                if (ok && j + 1 < n) ok = scores(j + 1);
-                ok = ok && wait(full(1, v_slot), v_phase) && wait(p_full(j), (uint32_t)(j >> 1) & 1u) && (j == 0 || wait(o_free, (uint32_t)(j - 1) & 1u));
+                if (C::NB == 2 && j + 1 < n) {  // S_{j+1} replaces P_{j-1}, whose product must be done
+                    ok = (j == 0 || wait(o_full(j - 1), (uint32_t)((j - 1) >> 1) & 1u)) && scores(j + 1);
+                    if (!ok) break;
+                }
+                ok = wait(full(slot), phase) && wait(p_full(j), (uint32_t)(j >> 1) & 1u) && (j == 0 || wait(o_free, (uint32_t)(j - 1) & 1u));
                 if (!ok) break;
                 tc::fence_after();
-                const uint32_t hi = stages + v_slot * C::STAGE + C::IMG;
-                const uint32_t pr = tm + C::S_COL + (uint32_t)p_buf * T, d = tm + C::O_COL;
+                const uint32_t hi = stages + slot * C::IMG;
+                const uint32_t pr = tm + C::S_COL + (uint32_t)(j % C::NB) * T, d = tm + C::O_COL;
                 // keys 16 k ..: eight columns of hi pairs from 16 k on, then eight of lo pairs
-                tc::mma4_ts<16, tc::STEP_MN>(d, pr + 8, tc::desc_mn(hi, T), ID_O, true);
-                tc::mma4_ts<16, tc::STEP_MN>(d, pr, tc::desc_mn(hi + C::PLANE, T), ID_O, false);
-                tc::mma4_ts<16, tc::STEP_MN>(d, pr, tc::desc_mn(hi, T), ID_O, false);
+#pragma unroll
+                for (int g = 0; g < T / 64; ++g) tc::mma4_ts<16, tc::STEP_MN>(d, pr + 64 * g + 8, tc::desc_mn(hi + g * 8192, T), ID_O, g == 0);
+#pragma unroll
+                for (int g = 0; g < T / 64; ++g) tc::mma4_ts<16, tc::STEP_MN>(d, pr + 64 * g, tc::desc_mn(hi + C::PLANE + g * 8192, T), ID_O, false);
+#pragma unroll
+                for (int g = 0; g < T / 64; ++g) tc::mma4_ts<16, tc::STEP_MN>(d, pr + 64 * g, tc::desc_mn(hi + g * 8192, T), ID_O, false);
                 tc::commit(o_full(j));
-                tc::commit(empty(1, v_slot));
-                if (++v_slot == STAGES) { v_slot = 0; v_phase ^= 1; }
-                if (++p_buf == C::NB) p_buf = 0;
+                tc::commit(empty(slot));
+                next_slot();
+                if (C::NB == 1 && j + 1 < n) ok = wait(o_full(j), (uint32_t)(j >> 1) & 1u) && scores(j + 1);  // S_{j+1} replaces P_j
             }
             // Every MMA is done before tensor memory is given back: the readers of O have seen to it; after a wait that ran out, wait
             // again (bounded) here.
@@ -288,7 +302,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             }
         }
     } else {
-        constexpr int NC = C::NC, W = C::W;
+        constexpr int NC = C::NC, W = C::W, GW = 16;
         float m = -INFINITY, l = 0.f, o[W];  // l: of this thread's columns
 #pragma unroll
         for (int d = 0; d < W; ++d) o[d] = 0.f;
@@ -333,15 +347,18 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T + wg * NC;
             const int lim = n_row - j * T - wg * NC;  // visible columns of this thread
             const bool whole = __all_sync(0xffffffffu, lim >= NC);
-            float s[NC];
-            tc::ldn(s_addr, s);
             float mx = -INFINITY;
-            if (whole) {
 #pragma unroll
-                for (int e = 0; e < NC; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
-            } else {
+            for (int g = 0; g < NC / 32; ++g) {
+                float s[32];
+                tc::ld32(s_addr + 32 * g, s);
+                if (whole) {
 #pragma unroll
-                for (int e = 0; e < NC; ++e) mx = fmaxf(mx, e < lim ? s[e] : -INFINITY);
+                    for (int e = 0; e < 32; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, 32 * g + e < lim ? s[e] : -INFINITY);
+                }
             }
             float* const row_max = shared_f + (j & 1) * (C::WGS * 128) + row;
             row_max[wg * 128] = mx;
@@ -357,20 +374,25 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             const uint64_t c2 = tc::pack2(c, c), b2 = tc::pack2(base, base);
             uint64_t sum2 = 0;
 #pragma unroll
-            for (int e = 0; e < NC; e += 2) {
-                float x, y;
-                tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
-                x = tc::ex2(x);
-                y = tc::ex2(y);
-                if (!whole) {
-                    x = e < lim ? x : 0.f;
-                    y = e + 1 < lim ? y : 0.f;
+            for (int g = 0; g < NC / GW; ++g) {
+                float s[GW];  // loaded again: with the sums of O the registers do not hold all columns
+                tc::ldn(s_addr + GW * g, s);
+#pragma unroll
+                for (int e = 0; e < GW; e += 2) {
+                    float x, y;
+                    tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
+                    x = tc::ex2(x);
+                    y = tc::ex2(y);
+                    if (!whole) {
+                        x = GW * g + e < lim ? x : 0.f;
+                        y = GW * g + e + 1 < lim ? y : 0.f;
+                    }
+                    sum2 = tc::add2(sum2, tc::pack2(x, y));
+                    s[e] = x;
+                    s[e + 1] = y;
                 }
-                sum2 = tc::add2(sum2, tc::pack2(x, y));
-                s[e] = x;
-                s[e + 1] = y;
+                tc::st_split(s_addr + GW * g, s);  // over the scores that they come from
             }
-            tc::st_split(s_addr, s);  // over the scores that they come from
             tc::st_wait();
             tc::fence_before();
             __syncwarp();
@@ -421,15 +443,17 @@ bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D) {
     return D % 4 == 0 && v.sb % 4 == 0 && v.sh % 4 == 0 && v.sr % 4 == 0 && ((uintptr_t)v.ptr & 15u) == 0;
 }
 
-int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp) {
+int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp, int tile_rows) {
     int64_t most = 0;
     for (int c = 0; c < count; ++c) {
         const int64_t n = (int64_t)jobs.B * jobs.job[c].heads * jobs.job[c].tiles;
         if (n > most) most = n;
     }
     const dim3 grid((unsigned)most, (unsigned)count);
-    if (dp == 64) attn_tiles_kernel<64><<<grid, 256, 0, ctx->stream>>>(jobs);
-    else attn_tiles_kernel<128><<<grid, 256, 0, ctx->stream>>>(jobs);
+    if (dp == 64 && tile_rows == 64) attn_tiles_kernel<64, 64><<<grid, 256, 0, ctx->stream>>>(jobs);
+    else if (dp == 64) attn_tiles_kernel<64, 128><<<grid, 256, 0, ctx->stream>>>(jobs);
+    else if (tile_rows == 64) attn_tiles_kernel<128, 64><<<grid, 256, 0, ctx->stream>>>(jobs);
+    else attn_tiles_kernel<128, 128><<<grid, 256, 0, ctx->stream>>>(jobs);
     TENMO_LAUNCH_CHECK(ctx, "attn_tiles_kernel");
     return TENMO_OK;
 }
@@ -465,7 +489,7 @@ int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     jobs.D = a.D;
     jobs.job[0] = TenmoTileJob{a.k, a.k_lengths, w, (float*)p.k_inv, a.Hkv, a.Sk, p.tiles, tenmo_attn_row_vec(a.k, a.D)};
     jobs.job[1] = TenmoTileJob{a.v, a.k_lengths, w + img, (float*)p.v_inv, a.Hkv, a.Sk, p.tiles, tenmo_attn_row_vec(a.v, a.D)};
-    if ((st = tenmo_attn_make_tiles(ctx, jobs, 2, dp)) != TENMO_OK) return st;
+    if ((st = tenmo_attn_make_tiles(ctx, jobs, 2, dp, T)) != TENMO_OK) return st;
     const unsigned grid = (unsigned)((int64_t)a.B * a.H * p.q_tiles);
     if (dp == 64) {
         constexpr int THREADS = FwdCfg<64>::THREADS;

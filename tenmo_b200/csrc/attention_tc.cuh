@@ -9,11 +9,11 @@ int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& p);
 int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& p);
 
 // ---- tile images of (batch, heads, rows, dim) views (see tcgen05.cuh) ----
-constexpr int ATTN_TILE = 64;  // rows of an image
+constexpr int ATTN_TILE = 64;  // rows of an image in the backward pass
 struct TenmoTileJob {
     TenmoHeadsView src;
     const int32_t* lengths;  // rows from here on become zeros
-    uint8_t* img;            // tile t of head (b, h): ((b * heads + h) * tiles + t) * ATTN_TILE * DP * 4 bytes
+    uint8_t* img;            // tile t of head (b, h): ((b * heads + h) * tiles + t) * (rows of a tile) * DP * 4 bytes
     float* inverse;          // 2^-e of every tile
     int heads, rows, tiles, vec;
     // With o.ptr set (src is the gradient of o): the per-row numbers of the backward pass as well.  Per tile 256 floats:
@@ -29,7 +29,7 @@ struct TenmoTileJobs {
     TenmoTileJob job[4];
     int B, D;
 };
-int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp);
+int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp, int tile_rows);  // 64 or 128 (without row numbers)
 bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D);
 static inline int tenmo_attn_padded(int D) { return D <= 64 ? 64 : 128; }
 

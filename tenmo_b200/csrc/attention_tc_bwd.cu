@@ -519,7 +519,7 @@ int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     jobs.job[3].o_vec = tenmo_attn_row_vec(a.o, a.D);
     jobs.job[3].stats = a.stats;
     jobs.job[3].info = in;
-    if ((st = tenmo_attn_make_tiles(ctx, jobs, 4, dp)) != TENMO_OK) return st;
+    if ((st = tenmo_attn_make_tiles(ctx, jobs, 4, dp, T)) != TENMO_OK) return st;
 
     BwdParams p = {};
     p.a = a;

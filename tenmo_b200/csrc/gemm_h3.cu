@@ -34,15 +34,15 @@ static_assert(SMEM <= 232448, "shared memory of a CTA");
 // ---------------------------------------------------------------------------------------------------------------------
 // operand blocks
 // ---------------------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) h3_make_kernel(const float* src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, int vec,
+__global__ void __launch_bounds__(512) h3_make_kernel(const float* src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, int vec,
                                                       const void* labels, int is_i64, int64_t ignore, uint8_t* img, float* inverse,
                                                       int block_cols) {
     const int64_t block = blockIdx.x;
     const int64_t r0 = block / block_cols * H3_BLOCK, c0 = block % block_cols * H3_BLOCK + 8 * (threadIdx.x & 15);
-    float x[8][8];
+    float x[4][8];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        const int64_t r = r0 + (threadIdx.x >> 4) + 16 * s;
+    for (int s = 0; s < 4; ++s) {
+        const int64_t r = r0 + (threadIdx.x >> 4) + 32 * s;
         const bool in = r < rows && !(labels && tenmo_h3_label(labels, is_i64, r) == ignore);
         const float* p = src + r * rs + c0 * cs;
         if (in && vec && c0 + 8 <= cols) {
@@ -410,17 +410,19 @@ int encode(tenmo_ctx* ctx, CUtensorMap* map, const TenmoH3Operand& o, bool mn) {
     return TENMO_OK;
 }
 
-// Slices of the contraction: the number (at most 8, each at least 16 chunks) that fills the last round of tiles best.
+// Slices of the contraction: the number (at most 8, each at least 16 chunks) that finishes first by this count, in units of one 128-deep
+// chunk of a 256 x 256 tile, 2.3 us at the measured rate: the rounds of tiles that the pairs need, and the partial results, which
+// are written, read and folded at about 6 TB/s.
 int pick_slices(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K) {
     const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256), chunks = (K + 127) / 128;
     const int64_t pairs = (ctx->sm_count - ctx->reserve_sms) / 2 > 0 ? (ctx->sm_count - ctx->reserve_sms) / 2 : 1;
+    const double traffic = 4.0 * M * N / 6e6 / 2.3;  // one pass over the result
     int best = 1;
     double best_cost = 1e300;
     for (int s = 1; s <= 8 && (s == 1 || chunks >= 16 * s); ++s) {
         const int64_t rounds = (tiles * s + pairs - 1) / pairs;
-        // a round takes 1 / s of a tile's time, plus the partial results written and read (about one chunk's time each)
-        const double cost = (double)rounds * ((double)chunks / s + 1.0) + (s > 1 ? 2.0 * s : 0.0);
-        if (cost < best_cost * 0.97) { best = s; best_cost = cost; }
+        const double cost = (double)rounds * ((double)chunks / s + 1.0) + (s > 1 ? (2.0 * s + 1.0) * traffic + 2.0 : 0.0);
+        if (cost < best_cost * 0.99) { best = s; best_cost = cost; }
     }
     return best;
 }
@@ -430,7 +432,7 @@ int pick_slices(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K) {
 int tenmo_h3_make(tenmo_ctx* ctx, const float* src, int64_t rs, int64_t cs, const TenmoH3Operand& o, const void* labels, int is_i64, int64_t ignore) {
     if (o.blocks() > 0x7fffffffLL / 512) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "operand of %lld x %lld is too large", (long long)o.rows, (long long)o.cols);
     const int vec = cs == 1 && rs % 4 == 0 && ((uintptr_t)src & 15u) == 0;
-    h3_make_kernel<<<(unsigned)o.blocks(), 256, 0, ctx->stream>>>(src, rs, cs, o.rows, o.cols, vec, labels, is_i64, ignore, o.img, o.inverse, (int)o.block_cols());
+    h3_make_kernel<<<(unsigned)o.blocks(), 512, 0, ctx->stream>>>(src, rs, cs, o.rows, o.cols, vec, labels, is_i64, ignore, o.img, o.inverse, (int)o.block_cols());
     TENMO_LAUNCH_CHECK(ctx, "h3_make_kernel");
     return TENMO_OK;
 }

@@ -46,26 +46,33 @@ __device__ __forceinline__ int64_t tenmo_h3_label(const void* labels, int is_i64
     return is_i64 ? __ldg((const long long*)labels + n) : (int64_t)__ldg((const int*)labels + n);
 }
 
-// Splits the 128 x 128 values that the block's 256 threads hold (thread t: rows t / 16 + 16 s, columns 8 (t % 16) ..) into img.
-__device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[8][8], uint8_t* img, float* inverse) {
-    __shared__ float largest[8];
+// Splits the 128 x 128 values that the block's 512 threads hold (thread t: rows t / 16 + 32 s, columns 8 (t % 16) ..) into img.
+__device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[4][8], uint8_t* img, float* inverse) {
+    __shared__ float largest[16];
     float mx = 0.f;
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, tc::finite_abs(x[s][e]));
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));  // a NaN does not count
+    if (!(mx <= 3.402823466e38f)) {  // an infinity does not either
+        mx = 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, tc::finite_abs(x[s][e]));
+    }
     mx = tenmo_warp_max(mx);
     if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, largest[w]);
+    for (int w = 0; w < 16; ++w) mx = fmaxf(mx, largest[w]);
     float inv;
     const float scale = tc::block_scale(mx, &inv);
     if (threadIdx.x == 0) *inverse = inv;
     const int c = threadIdx.x & 15;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        const int r = (threadIdx.x >> 4) + 16 * s;
+    for (int s = 0; s < 4; ++s) {
+        const int r = (threadIdx.x >> 4) + 32 * s;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) tc::split_pair(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);
@@ -74,4 +81,3 @@ __device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[8][8], uin
         *reinterpret_cast<uint4*>(img + 2 * H3_PLANE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
-

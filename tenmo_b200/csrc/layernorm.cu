@@ -9,7 +9,7 @@
 // differences from the mean (two sums over the registers), not E[x^2] - mean^2, which cancels.
 // Split: a row belongs to as many threads as it has groups of eight columns (a warp for 256 columns, a block of up to 1024
 // threads for 8192), each holding two float4.  Few registers per thread keep several rows in flight per SM, which is what
-// hides the two block-wide sums.  Wider rows are walked in pieces and re-read from L2.
+// hides the two block-wide sums; the next row is fetched before this row's.  Wider rows are walked in pieces and re-read from L2.
 // The column sums of the backward pass: a block keeps them in registers for the rows it takes (rows are dealt round-robin to
 // a resident grid), writes one partial row, and a second kernel adds the partials in a fixed order, so that the gradients of
 // gamma and bias repeat bit for bit.
@@ -106,9 +106,13 @@ __global__ void __launch_bounds__(WARP ? 128 : LN_MAX_THREADS) ln_fwd_kernel(con
     float gam[LN_EPT], bia[LN_EPT];
     ln_load<VEC>(gam, p.gamma, p.C, t, threads);
     ln_load<VEC>(bia, p.bias, p.C, t, threads);
+    float next[LN_EPT];
+    if (first < p.M) ln_load<VEC>(next, p.x + first * p.ldx, p.C, t, threads);
     for (int64_t m = first; m < p.M; m += step) {
         float v[LN_EPT];
-        ln_load<VEC>(v, p.x + m * p.ldx, p.C, t, threads);
+#pragma unroll
+        for (int e = 0; e < LN_EPT; ++e) v[e] = next[e];
+        if (m + step < p.M) ln_load<VEC>(next, p.x + (m + step) * p.ldx, p.C, t, threads);  // in flight during the two sums
         float s = 0.f;
 #pragma unroll
         for (int e = 0; e < LN_EPT; ++e) s += v[e];
@@ -171,12 +175,24 @@ __global__ void __launch_bounds__(WARP ? 128 : LN_MAX_THREADS) ln_bwd_kernel(con
     ln_load<VEC>(gam, p.gamma, p.C, t, threads);
 #pragma unroll
     for (int e = 0; e < LN_EPT; ++e) dg[e] = db[e] = 0.f;
+    float next_x[LN_EPT], next_g[LN_EPT], next_mean = 0.f, next_rstd = 0.f;
+    auto fetch = [&](int64_t m) {
+        ln_load<VEC>(next_x, p.x + m * p.ldx, p.C, t, threads);
+        ln_load<VEC>(next_g, p.dy + m * p.C, p.C, t, threads);
+        next_mean = __ldg(p.mean + m);
+        next_rstd = __ldg(p.rstd + m);
+    };
+    if (first < p.M) fetch(first);
     int flip = 0;
     for (int64_t m = first; m < p.M; m += step) {
         float v[LN_EPT], g[LN_EPT];
-        ln_load<VEC>(v, p.x + m * p.ldx, p.C, t, threads);
-        ln_load<VEC>(g, p.dy + m * p.C, p.C, t, threads);
-        const float mean = __ldg(p.mean + m), rstd = __ldg(p.rstd + m);
+#pragma unroll
+        for (int e = 0; e < LN_EPT; ++e) {
+            v[e] = next_x[e];
+            g[e] = next_g[e];
+        }
+        const float mean = next_mean, rstd = next_rstd;
+        if (m + step < p.M) fetch(m + step);
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int e = 0; e < LN_EPT; ++e) {

@@ -128,23 +128,30 @@ struct LceStats {
     float ls;
     int is_i64, reduction;
 };
-// 32 rows per block; 8 warps take the column groups in turn, joined in order
-__global__ void __launch_bounds__(256) lce_stats_kernel(const LceStats p) {
-    __shared__ float sm[8][32], sl[8][32], sa[8][32];
+// 32 rows per block; the warps take the column groups in turn, four loads in flight, and are joined in order
+constexpr int LCE_STAT_WARPS = 32;
+__global__ void __launch_bounds__(32 * LCE_STAT_WARPS) lce_stats_kernel(const LceStats p) {
+    __shared__ float sm[LCE_STAT_WARPS][32], sl[LCE_STAT_WARPS][32], sa[LCE_STAT_WARPS][32];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t r = (int64_t)blockIdx.x * 32 + lane;
     float m = -INFINITY, l = 0.f, all = 0.f;
     if (r < p.rows) {
-        for (int64_t g = w; g < p.groups; g += 8) {
-            const float2 v = __ldg(p.stats + g * p.rows + r);
-            const float top = fmaxf(m, v.x);
-            if (top == -INFINITY) {  // nothing but -inf or NaN so far: 0, or the NaN of the sum
-                l += v.y;
-                continue;
+        for (int64_t g0 = w; g0 < p.groups; g0 += 4 * LCE_STAT_WARPS) {
+            float2 v[4];
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t g = g0 + k * LCE_STAT_WARPS;
+                v[k] = g < p.groups ? __ldg(p.stats + g * p.rows + r) : make_float2(-INFINITY, 0.f);
+                if (p.sums && g < p.groups) all += __ldg(p.sums + g * p.rows + r);
             }
-            l = l * expf(m - top) + v.y * expf(v.x - top);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, v[k].x);
+            const float base = top == -INFINITY ? 0.f : top;  // nothing but -inf or NaN so far: sums of 0 or NaN
+            l *= expf(m - base);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) l += v[k].x == -INFINITY ? v[k].y : v[k].y * expf(v[k].x - base);
             m = top;
-            if (p.sums) all += __ldg(p.sums + g * p.rows + r);
         }
     }
     sm[w][lane] = m;
@@ -152,12 +159,12 @@ __global__ void __launch_bounds__(256) lce_stats_kernel(const LceStats p) {
     sa[w][lane] = all;
     __syncthreads();
     if (w || r >= p.rows) return;
-    for (int k = 1; k < 8; ++k) m = fmaxf(m, sm[k][lane]);
+    for (int k = 1; k < LCE_STAT_WARPS; ++k) m = fmaxf(m, sm[k][lane]);
     const float base = m == -INFINITY ? 0.f : m;
     l = 0.f;
     all = 0.f;
-    for (int k = 0; k < 8; ++k) {
-        l += sl[k][lane] * expf(sm[k][lane] - base);
+    for (int k = 0; k < LCE_STAT_WARPS; ++k) {
+        l += sm[k][lane] == -INFINITY ? sl[k][lane] : sl[k][lane] * expf(sm[k][lane] - base);
         all += sa[k][lane];
     }
     const int64_t n = p.row0 + r, y = lce_label(p.labels, p.is_i64, n);
@@ -176,39 +183,50 @@ __global__ void __launch_bounds__(256) lce_stats_kernel(const LceStats p) {
 }
 
 // The logits of a 128 x 128 block become the gradient, as an operand image in their place, and its column sums per block row.
-__global__ void __launch_bounds__(256) lce_grad_kernel(uint8_t* z, float* inverse, const float4* numbers, const void* labels, int is_i64,
+__global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* inverse, const float4* numbers, const void* labels, int is_i64,
                                                        int64_t row0, int64_t rows, int64_t V, int block_cols, float ls, float* db_part) {
-    __shared__ float sums[16][H3_BLOCK];
+    __shared__ float sums[32][H3_BLOCK];
     const int64_t block = blockIdx.x;
     const int64_t r0 = block / block_cols * H3_BLOCK, c0 = block % block_cols * H3_BLOCK;
     const int c = 8 * (threadIdx.x & 15);
     const float* src = reinterpret_cast<const float*>(z + block * H3_BLOCK_BYTES);
     const float smooth = ls / (float)V;
-    float x[8][8], col[8];
+    const int cols = (int)min((int64_t)8, V - c0 - c);  // of this thread that exist
+    float x[4][8], col[8];
+    float4 num[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {  // all loads first; a row that takes no part has u = 0 and its logits are not looked at
+        const int lr = (threadIdx.x >> 4) + 32 * s;
+        num[s] = r0 + lr < rows ? __ldg(numbers + r0 + lr) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 a = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c), b = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c + 4);
+        x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
+        x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) col[e] = 0.f;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        const int lr = (threadIdx.x >> 4) + 16 * s;
-        const int64_t r = r0 + lr;
-        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-        int64_t y = -1;
-        if (r < rows) {
-            num = __ldg(numbers + r);
-            y = lce_label(labels, is_i64, row0 + r) - c0 - c;
+    for (int s = 0; s < 4; ++s) {
+        const int64_t r = r0 + (threadIdx.x >> 4) + 32 * s;
+        if (num[s].w == 0.f) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
+            continue;
         }
-        const bool in = num.w != 0.f;
-        if (in) {
-            const float4 a = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c), b = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c + 4);
-            x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
-            x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+        const int64_t y = lce_label(labels, is_i64, row0 + r) - c0 - c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = tc::ex2((x[s][e] - num[s].x) * 1.44269504088896341f) * num[s].y - smooth;
+        if (y >= 0 && y < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[s][e] -= e == (int)y ? 1.f - ls : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float p = tc::ex2((x[s][e] - num.x) * 1.44269504088896341f) * num.y;
-            x[s][e] = in && c0 + c + e < V ? (p - smooth - (e == y ? 1.f - ls : 0.f)) * num.z : 0.f;
-            col[e] += x[s][e];
+        for (int e = 0; e < 8; ++e) x[s][e] *= num[s].z;
+        if (cols < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[s][e] = e < cols ? x[s][e] : 0.f;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) col[e] += x[s][e];
     }
     if (db_part) {
 #pragma unroll
@@ -217,7 +235,7 @@ __global__ void __launch_bounds__(256) lce_grad_kernel(uint8_t* z, float* invers
         if (threadIdx.x < H3_BLOCK && c0 + threadIdx.x < V) {
             float t = 0.f;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) t += sums[k][threadIdx.x];
+            for (int k = 0; k < 32; ++k) t += sums[k][threadIdx.x];
             db_part[block / block_cols * V + c0 + threadIdx.x] = t;
         }
     }
@@ -347,10 +365,10 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
         if ((st = tenmo_h3_gemm(ctx, rows, c.V, c.D, X, false, W, !tied, e, nullptr)) != TENMO_OK) return st;
         const LceStats ps{e.stats, e.sums, e.at_label, groups, rows, r0, c.V, c.ignore, c.labels, c.upstream, (const float*)(at + factor),
                           (float*)(at + row_loss), c.grad ? (float4*)(at + numbers) : nullptr, ctx->dev_status, c.ls, c.is_i64, c.reduction};
-        lce_stats_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, ctx->stream>>>(ps);
+        lce_stats_kernel<<<(unsigned)((rows + 31) / 32), 32 * LCE_STAT_WARPS, 0, ctx->stream>>>(ps);
         TENMO_LAUNCH_CHECK(ctx, "lce_stats_kernel");
         if (!c.grad) continue;
-        lce_grad_kernel<<<(unsigned)Z.blocks(), 256, 0, ctx->stream>>>(Z.img, Z.inverse, ps.numbers, c.labels, c.is_i64, r0, rows, c.V, (int)vb, c.ls,
+        lce_grad_kernel<<<(unsigned)Z.blocks(), 512, 0, ctx->stream>>>(Z.img, Z.inverse, ps.numbers, c.labels, c.is_i64, r0, rows, c.V, (int)vb, c.ls,
                                                                        c.db ? (float*)(at + db_part) : nullptr);
         TENMO_LAUNCH_CHECK(ctx, "lce_grad_kernel");
         TenmoH3Epilogue ex = {};
