@@ -410,7 +410,7 @@ int encode(tenmo_ctx* ctx, CUtensorMap* map, const TenmoH3Operand& o, bool mn) {
     return TENMO_OK;
 }
 
-// Slices of the contraction: the number (at most 8, each at least 16 chunks) that finishes first by this count, in units of one 128-deep
+// Slices of the contraction: the number (at most 32, each at least 8 chunks) that finishes first by this count, in units of one 128-deep
 // chunk of a 256 x 256 tile, 2.3 us at the measured rate: the rounds of tiles that the pairs need, and the partial results, which
 // are written, read and folded at about 6 TB/s.
 int pick_slices(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K) {
@@ -419,7 +419,7 @@ int pick_slices(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K) {
     const double traffic = 4.0 * M * N / 6e6 / 2.3;  // one pass over the result
     int best = 1;
     double best_cost = 1e300;
-    for (int s = 1; s <= 8 && (s == 1 || chunks >= 16 * s); ++s) {
+    for (int s = 1; s <= 32 && (s == 1 || chunks >= 8 * s); ++s) {
         const int64_t rounds = (tiles * s + pairs - 1) / pairs;
         const double cost = (double)rounds * ((double)chunks / s + 1.0) + (s > 1 ? (2.0 * s + 1.0) * traffic + 2.0 : 0.0);
         if (cost < best_cost * 0.99) { best = s; best_cost = cost; }

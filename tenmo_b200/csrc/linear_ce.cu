@@ -11,6 +11,7 @@
 #include <cfloat>
 
 #include "gemm_h3.cuh"
+#include "linear_few.cuh"
 
 namespace {
 
@@ -74,7 +75,7 @@ struct LceRow {
 };
 
 // a block is a row
-__global__ void __launch_bounds__(LCE_THREADS) lce_row_kernel(const LceRow p) {
+__global__ void __launch_bounds__(1024) lce_row_kernel(const LceRow p) {
     __shared__ float slots[32];
     tenmo_grid_dependency_sync();
     const int64_t n = p.row0 + blockIdx.x;
@@ -85,14 +86,16 @@ __global__ void __launch_bounds__(LCE_THREADS) lce_row_kernel(const LceRow p) {
         if (counted && threadIdx.x == 0) atomicOr(p.status, TENMO_DEV_BAD_LABEL);
         if (threadIdx.x == 0) p.row_loss[n] = 0.f;
         if (p.grad)
-            for (int64_t v = threadIdx.x; v < p.V; v += LCE_THREADS) z[v] = 0.f;
+            for (int64_t v = threadIdx.x; v < p.V; v += blockDim.x) z[v] = 0.f;
         return;
     }
     float m = -INFINITY;
-    for (int64_t v = threadIdx.x; v < p.V; v += LCE_THREADS) m = fmaxf(m, z[v]);
+#pragma unroll 8
+    for (int64_t v = threadIdx.x; v < p.V; v += blockDim.x) m = fmaxf(m, z[v]);
     m = block_reduce<true>(m, slots);
     float l = 0.f, s = 0.f;
-    for (int64_t v = threadIdx.x; v < p.V; v += LCE_THREADS) {
+#pragma unroll 8
+    for (int64_t v = threadIdx.x; v < p.V; v += blockDim.x) {
         const float t = z[v] - m;
         l += expf(t);
         s += t;
@@ -110,7 +113,8 @@ __global__ void __launch_bounds__(LCE_THREADS) lce_row_kernel(const LceRow p) {
     float u = *p.factor;
     if (p.upstream) u *= p.upstream[p.reduction == 2 ? n : 0];
     const float inv = 1.f / l, smooth = p.ls / (float)p.V;
-    for (int64_t v = threadIdx.x; v < p.V; v += LCE_THREADS) {
+#pragma unroll 8
+    for (int64_t v = threadIdx.x; v < p.V; v += blockDim.x) {
         const float g = expf(z[v] - m) * inv - smooth - (v == y ? 1.f - p.ls : 0.f);
         z[v] = g * u;
     }
@@ -303,9 +307,10 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     return TENMO_OK;
 }
 
+constexpr double TC_FLOP = 2e8;  // of one product
 // Large problems: the products on tensor cores (gemm_h3.cu).  Without a gradient no logit is ever stored: the product's epilogue
 // reduces them to two numbers per row and 64 columns.
-bool tc_profitable(const LceCall& c) { return c.N >= 64 && c.D >= 32 && c.V >= 128 && 2.0 * c.N * c.D * c.V >= 2e9; }
+bool tc_profitable(const LceCall& c) { return c.N > TENMO_FEW_ROWS && 2.0 * c.N * c.D * c.V >= TC_FLOP; }
 
 int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     const int64_t vb = (c.V + H3_BLOCK - 1) / H3_BLOCK;
@@ -390,10 +395,50 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     return TENMO_OK;
 }
 
+// A handful of rows: the products of linear_few.cu, which read the weight once each and write its gradient once.
+int lce_run_few(tenmo_ctx* ctx, const LceCall& c) {
+    const bool tied = c.w->row_stride == 1 && c.w->col_stride != 1;
+    const int64_t ldw = tied ? c.w->col_stride : c.w->row_stride;
+    const float* w = c.w->ptr + c.w->offset;
+    size_t need = 0;
+    auto take = [&](size_t bytes) { const size_t at = need; need += (bytes + 255) & ~(size_t)255; return at; };
+    const size_t z_at = take((size_t)c.N * c.V * sizeof(float)), x_at = take((size_t)c.N * c.D * sizeof(float)), l_at = take(c.N * sizeof(float)), f_at = take(sizeof(float));
+    size_t part = tenmo_few_bytes(ctx, c.N, c.V, c.D);
+    if (c.grad && tenmo_few_bytes(ctx, c.N, c.D, c.V) > part) part = tenmo_few_bytes(ctx, c.N, c.D, c.V);
+    const size_t p_at = take(part);
+    void* ws = nullptr;
+    int st = tenmo_op_workspace(ctx, need, &ws);
+    if (st != TENMO_OK) return st;
+    float *z = (float*)((char*)ws + z_at), *x = (float*)((char*)ws + x_at), *row_loss = (float*)((char*)ws + l_at), *factor = (float*)((char*)ws + f_at);
+    float* partial = (float*)((char*)ws + p_at);
+    TENMO_CUDA_TRY(ctx, tenmo_launch(lce_count_kernel, 1, 1024, 0, ctx->stream, ctx->pdl, c.labels, c.is_i64, c.N, c.ignore, c.reduction, c.valid, factor));
+    TENMO_LAUNCH_CHECK(ctx, "lce_count_kernel");
+    lce_rows_kernel<<<tenmo_stream_grid(ctx, c.N * c.D, 256, 8), 256, 0, ctx->stream>>>(c.x->ptr + c.x->offset, c.x->row_stride, c.x->col_stride, c.labels,
+                                                                                       c.is_i64, c.ignore, 0, c.N, c.D, x);
+    TENMO_LAUNCH_CHECK(ctx, "lce_rows_kernel");
+    st = tied ? tenmo_few_dot(ctx, x, c.D, c.N, c.D, w, ldw, c.V, c.bias, z, c.V, partial) : tenmo_few_cols(ctx, x, c.D, c.N, c.D, w, ldw, c.V, c.bias, z, c.V, partial);
+    if (st != TENMO_OK) return st;
+    const LceRow p{z, c.labels, row_loss, c.upstream, factor, ctx->dev_status, 0, c.V, c.ignore, c.ls, c.is_i64, c.reduction, c.grad};
+    lce_row_kernel<<<(unsigned)c.N, c.V > 4096 ? 1024 : LCE_THREADS, 0, ctx->stream>>>(p);
+    TENMO_LAUNCH_CHECK(ctx, "lce_row_kernel");
+    if (c.grad) {
+        st = tied ? tenmo_few_cols(ctx, z, c.V, c.N, c.V, w, ldw, c.D, nullptr, c.dx, c.D, partial) : tenmo_few_dot(ctx, z, c.V, c.N, c.V, w, ldw, c.D, nullptr, c.dx, c.D, partial);
+        if (st != TENMO_OK) return st;
+        st = tied ? tenmo_few_outer(ctx, z, c.V, x, c.D, c.N, c.V, c.D, c.dw) : tenmo_few_outer(ctx, x, c.D, z, c.V, c.N, c.D, c.V, c.dw);
+        if (st != TENMO_OK) return st;
+        if (c.db && (st = tenmo_colsum_f32(ctx, z, c.N, c.V, c.V, c.db, 0.f)) != TENMO_OK) return st;
+    }
+    const int grid = c.reduction == 2 ? tenmo_stream_grid(ctx, c.N, 1024, 1) : 1;
+    TENMO_CUDA_TRY(ctx, tenmo_launch(lce_loss_kernel, grid, 1024, 0, ctx->stream, ctx->pdl, (const float*)row_loss, c.N, c.reduction, (const int32_t*)c.valid, c.loss));
+    TENMO_LAUNCH_CHECK(ctx, "lce_loss_kernel");
+    return TENMO_OK;
+}
+
 int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     int st = check(ctx, who, c);
     if (st != TENMO_OK) return st;
     TenmoDeviceGuard guard(ctx);
+    if (c.N > 0 && c.N <= 2 * TENMO_FEW_ROWS && !(c.N > TENMO_FEW_ROWS && tc_profitable(c))) return lce_run_few(ctx, c);
     if (tc_profitable(c)) return lce_run_tc(ctx, c);
     int64_t piece = (int64_t)(LCE_PIECE_BYTES / ((size_t)c.V * sizeof(float))) / 128 * 128;
     if (piece < 128) piece = 128;
@@ -421,7 +466,7 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
         st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, rows, c.V, c.D, &mx, c.w, z, 0.f, c.bias, TENMO_ACT_NONE, nullptr, nullptr);
         if (st != TENMO_OK) return st;
         const LceRow p{z, c.labels, row_loss, c.upstream, factor, ctx->dev_status, r0, c.V, c.ignore, c.ls, c.is_i64, c.reduction, c.grad};
-        lce_row_kernel<<<(unsigned)rows, LCE_THREADS, 0, ctx->stream>>>(p);
+        lce_row_kernel<<<(unsigned)rows, c.V > 4096 ? 1024 : LCE_THREADS, 0, ctx->stream>>>(p);
         TENMO_LAUNCH_CHECK(ctx, "lce_row_kernel");
         if (!c.grad) continue;
         const float beta = r0 ? 1.f : 0.f;
