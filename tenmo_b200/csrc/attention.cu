@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) attn_bwd_dq_row_kernel(const T
             ds = pr * (dot_row(sg[warp], v + j * p.v.sr, p.D, vv) - delta) * p.scale;
         }
         const int cnt = min(32, n - j0);
+#pragma unroll 8
         for (int jj = 0; jj < cnt; ++jj) {
             const float w = __shfl_sync(0xffffffffu, ds, jj);
             const float* row = k + (j0 + jj) * p.k.sr;
@@ -390,6 +391,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) attn_bwd_dkv_row_kernel(const 
                 }
             }
             const int cnt = min(32, rows - i0);
+#pragma unroll 8
             for (int ii = 0; ii < cnt; ++ii) {
                 const float wp = __shfl_sync(0xffffffffu, pr, ii), wd = __shfl_sync(0xffffffffu, ds, ii);
                 const float* rq = q + (i0 + ii) * p.q.sr;

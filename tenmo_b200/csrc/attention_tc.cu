@@ -458,11 +458,18 @@ int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, 
     return TENMO_OK;
 }
 
-// The tensor-core kernels work on tiles of 128 rows x 64 keys whatever the sizes; below a good part of a tile, and where the
-// whole call is a few launches' latency, the row kernels are faster.
+// Which kernels, from both sides measured over 4 .. 256 heads, dims 32 .. 128 and 16 .. 3000 rows and keys.
+// Forward: the few-row kernel takes about 10 us plus 3.7 ns for every row and 128 keys (dim 64), the tensor-core one 14 us plus the
+// split of k and v, so it pays from some 2500 rows x 128 keys on (32 heads of 96x96: 15 us against 27; of 64x64: 15 against 13) -- but not for a
+// few rows per head, which leave its 128-row tiles empty (256 heads of 4 rows and 3000 keys: 228 against 110).
+// Backward: the row kernels take a warp through all keys (rows) of its row (key), the tensor-core ones 24 us at least: level at 64
+// rows or keys with few heads (4 heads of 64x64: 24 us against 28) and at some 65,000 pairs with many (256 heads of 16x16: 40 against
+// 32, of 32x32: 44 against 105).
 bool tenmo_attn_tc_profitable(const TenmoAttnParams& p, bool backward) {
-    (void)backward;
-    return p.Sq >= 64 && p.Sk >= 64 && (int64_t)p.Sq * p.Sk >= 128 * 128;
+    const int64_t rows = (int64_t)p.B * p.H * p.Sq;
+    if (p.Sq == 0 || p.Sk == 0) return false;
+    if (!backward) return p.Sq >= 16 && rows * ((p.Sk + 127) / 128) >= 2560;
+    return p.Sq >= 64 || p.Sk >= 64 || rows * p.Sk > 65536;
 }
 
 int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
