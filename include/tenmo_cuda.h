@@ -306,6 +306,10 @@ int tenmo_ce_fwd_bwd_f32(tenmo_ctx* ctx, const float* logits, int64_t ld_logits,
                          const float* upstream_dev, float* dlogits);
 
 /* ---- transformer operators ----------------------------------------------------------------------
+ * They share a workspace of the context.  A call on another stream than the one before waits for that stream; graphs that were
+ * captured from one context use the same workspace and must not be replayed at the same time (capture from two contexts for that).
+ * The first call of its size allocates, which a stream that is being captured refuses: run it once before.
+ *
  * Layer normalisation over the last axis (layernorm.mojo of the reference; no GPU-side counterpart on this path):
  *   y = (x - mean) * rstd * gamma + bias,  rstd = 1 / sqrt(var + eps),  var the mean squared difference from the mean.
  * x has leading dimension ldx, y / dy / dx are contiguous (M, C); gamma and bias are C floats.  mean and rstd (M floats each)
@@ -323,17 +327,22 @@ int tenmo_layernorm_bwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const f
  *   heads     q, o, go, dq: (batch, heads, q_len, dim); k, v, dk, dv: (batch, kv_heads, k_len, dim); heads is a multiple of
  *             kv_heads and query head h reads key / value head h / (heads / kv_heads).  dim is 1 .. 128.
  *   views     element (b, h, row, d) at ptr[b*batch_stride + h*head_stride + row*row_stride + d]: the dim axis is contiguous,
- *             the others have any non-negative stride (0 broadcasts an input).  Outputs may not overlap: in themselves, with
- *             one another or with an input.
+ *             the others have any non-negative stride (0 broadcasts an input).  Outputs may not overlap: in themselves (refused
+ *             unless the strides of their axes, in some order, step over one another), with one another or with an input.
  *   mask      causal != 0: key j is visible to row i when j <= i + k_len - q_len (the last row sees every key).
  *             k_lengths / q_lengths (batch int32 on the device, or NULL): keys / rows from the length on do not take part,
  *             whatever they hold; a length outside [0, k_len] ([0, q_len]) counts as the nearest bound.
  *             A row without a visible key gives o = 0 and dq = 0 and adds nothing to dk and dv; a key that no row sees gives
- *             dk = dv = 0.
- *   stats     (batch, heads, q_len, 2) floats: per row the largest score in units of log 2 and the sum of exponentials; written
- *             by the forward pass (NULL when no backward pass follows) and read by the backward pass.
+ *             dk = dv = 0; both may hold anything.
+ *   stats     (batch, heads, q_len, 2) floats: per row a reference, the largest score in units of log 2 or the next whole number,
+ *             and the sum of exponentials relative to it; written by the forward pass (NULL when no backward pass follows) and
+ *             read by the backward pass.
  * Backward recomputes the probabilities; beta == 1 adds to what dq, dk, dv hold.  No atomics: results repeat bit for bit.
- * A row whose scores hold a NaN or +inf gives NaN. */
+ * Precision: sums in 32 bits.  Larger problems multiply on tensor cores with every operand held to 22 bits, down to 2^-18 of the
+ * largest entry of its row or of its tile of 64 or 128 rows, and to 2^-40 of that entry below.  A recomputed score differs from the
+ * forward pass's by some 2^-20 of sum |q k|, and the gradients by that factor: they mean little where scores pass 10^5.
+ * A NaN or infinity that takes part gives NaN: in q in its row of o and dq, in k or v (as in the product P . V of the composed
+ * operators) in any row of the heads that read it, in q or go also in dk and dv of its head's keys. */
 typedef struct {
     int64_t batch, heads, kv_heads, q_len, k_len, dim;
 } tenmo_attn_shape;
@@ -354,11 +363,15 @@ int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
  *   x       (N, D), any non-negative strides.  w: (D, V) as Linear keeps it, or the transposed view of a (V, D) embedding; one
  *           of its axes has unit stride.  bias: V floats or NULL.
  *   labels, ignore_index, label_smoothing, reduction, loss, valid_count: as tenmo_ce_fwd_f32 (with the mean over no rows 0).
- *           Rows whose label is ignore_index take no part, whatever their x holds.
+ *           Rows whose label is ignore_index take no part, whatever their x holds; their dx is 0 where W is finite.
  *   fwd_bwd loss and gradients in one call: dx (N, D) contiguous; dw contiguous in the order of w's storage, (D, V) or
  *           (V, D); db V floats or NULL.  They are written, not added to.  upstream: 1 float (mean / sum) or N floats (none) on
  *           the device, NULL for 1.
- * The logits of a piece of the rows at a time live in the workspace. */
+ *           Outputs may not overlap an input or one another.
+ * The logits of a piece of the rows at a time (at most 512 MB, or 256 rows) live in the workspace.  A class may be masked with a bias
+ * of -inf or the lowest number (without label smoothing).  Results repeat bit for bit.
+ * Precision: sums in 32 bits (the loss over the rows in 64).  Larger problems multiply on tensor cores with every operand held to 22
+ * bits, down to 2^-18 of the largest entry of its 128 x 128 block and to 2^-40 of that entry below. */
 int tenmo_linear_ce_fwd_f32(tenmo_ctx* ctx, const tenmo_mat* x, const tenmo_mat* w, const float* bias, const void* labels,
                             int label_is_i64, int64_t N, int64_t D, int64_t V, int64_t ignore_index, float label_smoothing,
                             int reduction, float* loss, int32_t* valid_count);

@@ -295,8 +295,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const FewParams f) {
     if (p.stats && lane == 0) { p.stats[2 * row] = top; p.stats[2 * row + 1] = sum; }
 }
 
-// probability from the recomputed score and the saved (maximum, sum)
-__device__ __forceinline__ float prob(float s_log2, float m, float inv_l) { return exp2f(s_log2 - m) * inv_l; }
+// probability from the recomputed score and the saved (maximum, sum); scores whose rounding exceeds 1 stay at the maximum's probability
+__device__ __forceinline__ float prob(float s_log2, float m, float inv_l) {
+    const float e = exp2f(s_log2 - m);
+    return (e > 1.f ? 1.f : e) * inv_l;
+}
 
 __global__ void __launch_bounds__(ROW_WARPS * 32) attn_bwd_dq_row_kernel(const TenmoAttnParams p) {
     __shared__ __align__(16) float sq[ROW_WARPS][TENMO_ATTN_MAX_DIM], sg[ROW_WARPS][TENMO_ATTN_MAX_DIM];
@@ -479,7 +482,7 @@ int check_shape(tenmo_ctx* ctx, const char* who, const tenmo_attn_shape* s, floa
     const int64_t longest = s->q_len > s->k_len ? s->q_len : s->k_len;
     if (s->batch * s->heads * longest >= ((int64_t)1 << 32))
         return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "%s: more than 2^32 rows in one call", who);
-    if (!(fabsf(scale) <= FLT_MAX)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: scale is not finite", who);
+    if (!(fabsf(scale) <= FLT_MAX / 2)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: scale is not finite, or too large", who);
     p->B = (int)s->batch; p->H = (int)s->heads; p->Hkv = (int)s->kv_heads;
     p->Sq = (int)s->q_len; p->Sk = (int)s->k_len; p->D = (int)s->dim;
     p->scale = scale;
@@ -487,15 +490,33 @@ int check_shape(tenmo_ctx* ctx, const char* who, const tenmo_attn_shape* s, floa
     return TENMO_OK;
 }
 
-int take_view(tenmo_ctx* ctx, const char* who, const char* name, const tenmo_heads* t, bool needed, bool output, int64_t rows, int64_t dim,
-              TenmoHeadsView* v) {
+int take_view(tenmo_ctx* ctx, const char* who, const char* name, const tenmo_heads* t, bool needed, bool output, int64_t batch, int64_t heads,
+              int64_t rows, int64_t dim, TenmoHeadsView* v) {
     if (!t || (!t->ptr && needed)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: %s is NULL", who, name);
     if (t->batch_stride < 0 || t->head_stride < 0 || t->row_stride < 0)
         return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: %s has a negative stride", who, name);
-    // rows of an output that overlap would be written by several warps at once
-    if (output && rows > 1 && t->row_stride < dim)
-        return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: rows of %s overlap (row stride %lld, dim %lld)", who, name,
-                               (long long)t->row_stride, (long long)dim);
+    // an output's rows must not overlap: several blocks would write (or, with beta, add to) the same places.  From the smallest
+    // stride up, each axis has to step over all that the axes before it cover.
+    if (output && needed) {
+        struct { int64_t n, stride; } axis[3] = {{batch, t->batch_stride}, {heads, t->head_stride}, {rows, t->row_stride}};
+        for (int pass = 0; pass < 2; ++pass)
+            for (int e = 0; e < 2; ++e)
+                if (axis[e].stride > axis[e + 1].stride) {
+                    const auto swap = axis[e];
+                    axis[e] = axis[e + 1];
+                    axis[e + 1] = swap;
+                }
+        int64_t covered = dim;
+        for (int e = 0; e < 3; ++e) {
+            if (axis[e].n <= 1) continue;
+            if (axis[e].stride < covered)
+                return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: rows of %s overlap (strides %lld, %lld, %lld)", who, name,
+                                       (long long)t->batch_stride, (long long)t->head_stride, (long long)t->row_stride);
+            if (axis[e].stride > (INT64_MAX - covered) / (axis[e].n - 1))
+                return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: strides of %s are too large", who, name);
+            covered += axis[e].stride * (axis[e].n - 1);
+        }
+    }
     *v = TenmoHeadsView{t->ptr, t->batch_stride, t->head_stride, t->row_stride};
     return TENMO_OK;
 }
@@ -513,11 +534,13 @@ int tenmo_attention_fwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
     int st = check_shape(ctx, who, shape, scale, &p);
     if (st != TENMO_OK) return st;
     const bool any_q = p.B && p.Sq, any_k = p.B && p.Sk && p.Sq;
-    if ((st = take_view(ctx, who, "q", q, any_k, false, p.Sq, p.D, &p.q)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "k", k, any_k, false, p.Sk, p.D, &p.k)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "v", v, any_k, false, p.Sk, p.D, &p.v)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "o", o, any_q, true, p.Sq, p.D, &p.o)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "q", q, any_k, false, p.B, p.H, p.Sq, p.D, &p.q)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "k", k, any_k, false, p.B, p.Hkv, p.Sk, p.D, &p.k)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "v", v, any_k, false, p.B, p.Hkv, p.Sk, p.D, &p.v)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "o", o, any_q, true, p.B, p.H, p.Sq, p.D, &p.o)) != TENMO_OK) return st;
     if (!any_q) return TENMO_OK;
+    if (any_k && (o->ptr == q->ptr || o->ptr == k->ptr || o->ptr == v->ptr))
+        return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: o is one of the inputs", who);
     p.stats = stats;
     p.causal = causal != 0;
     p.q_lengths = q_lengths;
@@ -538,15 +561,22 @@ int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
     if (st != TENMO_OK) return st;
     if (beta != 0.f && beta != 1.f) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "attention_bwd: beta must be 0 or 1");
     const bool any_q = p.B && p.Sq, any_k = p.B && p.Sk;
-    if ((st = take_view(ctx, who, "q", q, any_q, false, p.Sq, p.D, &p.q)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "k", k, any_k, false, p.Sk, p.D, &p.k)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "v", v, any_k, false, p.Sk, p.D, &p.v)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "o", o, any_q, false, p.Sq, p.D, &p.o)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "go", go, any_q, false, p.Sq, p.D, &p.go)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "dq", dq, any_q, true, p.Sq, p.D, &p.dq)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "dk", dk, any_k, true, p.Sk, p.D, &p.dk)) != TENMO_OK) return st;
-    if ((st = take_view(ctx, who, "dv", dv, any_k, true, p.Sk, p.D, &p.dv)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "q", q, any_q, false, p.B, p.H, p.Sq, p.D, &p.q)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "k", k, any_k, false, p.B, p.Hkv, p.Sk, p.D, &p.k)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "v", v, any_k, false, p.B, p.Hkv, p.Sk, p.D, &p.v)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "o", o, any_q, false, p.B, p.H, p.Sq, p.D, &p.o)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "go", go, any_q, false, p.B, p.H, p.Sq, p.D, &p.go)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "dq", dq, any_q, true, p.B, p.H, p.Sq, p.D, &p.dq)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "dk", dk, any_k, true, p.B, p.Hkv, p.Sk, p.D, &p.dk)) != TENMO_OK) return st;
+    if ((st = take_view(ctx, who, "dv", dv, any_k, true, p.B, p.Hkv, p.Sk, p.D, &p.dv)) != TENMO_OK) return st;
     if (any_q && !stats) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "attention_bwd: stats is NULL");
+    const float* in[5] = {p.q.ptr, p.k.ptr, p.v.ptr, p.o.ptr, p.go.ptr};
+    const float* out[3] = {p.dq.ptr, p.dk.ptr, p.dv.ptr};
+    for (int e = 0; e < 3 && any_q && any_k; ++e) {
+        for (int u = 0; u < 5; ++u)
+            if (out[e] == in[u]) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: a gradient is one of the inputs", who);
+        if (out[e] == out[(e + 1) % 3]) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: two gradients are the same", who);
+    }
     p.stats = const_cast<float*>(stats);
     p.causal = causal != 0;
     p.q_lengths = q_lengths;

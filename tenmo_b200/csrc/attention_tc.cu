@@ -5,7 +5,8 @@
 //   S_j = q k_j^T          left operand and accumulator in tensor memory
 //   P_j = exp2(S_j c - m)  by warpgroups, a row per thread, written over S_j as fp16 pairs: the next left operand
 //   O_j = P_j v_j          a fresh accumulator, added to the row's registers (and rescaled) with rounding
-// The running reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.
+// The running reference m is kept a whole number (the ceiling of the maximum), which makes every rescaling an exact power of two.  What is
+// kept is 15 - m, rounded downwards: scores beyond 2^24, where not every whole number exists, then still keep P below 2^15.
 // What bounds the kernel is not a pipe but the instructions around the products and the chain S -> maximum -> exponentials -> P -> O
 // of a tile, thousands of cycles of latencies.  So tiles are wide (128 keys: the waits, fences and exchanges of a tile are paid half as
 // often as with 64), their columns are shared by two warpgroups (dim up to 64; 64 columns of S, 32 of O a thread) or four (up to
@@ -87,22 +88,25 @@ __global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs job
     const int tile = (int)(t % j.tiles);
     const int64_t bh = t / j.tiles;
     const int h = (int)(bh % j.heads), b = (int)(bh / j.heads);
-    const int rows = tenmo_attn_rows(j.lengths, b, j.rows) - tile * T;
+    int rows = tenmo_attn_rows(j.lengths, b, j.rows);
+    if (j.seen_by) rows = min(rows, max(0, tenmo_attn_rows(j.q_lengths, b, j.seen_by) + j.offset));
+    rows -= tile * T;
     if (rows <= 0) return;  // no kernel reads a tile behind the length
     const float* src = j.src.ptr + b * j.src.sb + h * j.src.sh + (int64_t)tile * T * j.src.sr;
+    const int skip = j.first - tile * T;
     float x[STEPS][8];
     float mx = 0.f;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int q = threadIdx.x + s * 256, r = q / CHUNKS, d = (q % CHUNKS) * 8;
         const float* p = src + r * j.src.sr + d;
-        if (r < rows && j.vec && d + 8 <= jobs.D) {
+        if (r < rows && r >= skip && j.vec && d + 8 <= jobs.D) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(p)), c = __ldg(reinterpret_cast<const float4*>(p) + 1);
             x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
             x[s][4] = c.x; x[s][5] = c.y; x[s][6] = c.z; x[s][7] = c.w;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[s][e] = r < rows && d + e < jobs.D ? __ldg(p + e) : 0.f;
+            for (int e = 0; e < 8; ++e) x[s][e] = r < rows && r >= skip && d + e < jobs.D ? __ldg(p + e) : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));  // a NaN does not count
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(256) attn_tiles_kernel(const TenmoTileJobs job
         const int q = threadIdx.x + s * 256, r = q / CHUNKS, c = q % CHUNKS;
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tc::split_pair(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);
+        for (int e = 0; e < 4; ++e) tc::split_rounded(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);
         const int at = (c >> 3) * (T * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(img + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(img + T * DP * 2 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
         }
     } else {
         constexpr int NC = C::NC, W = C::W, GW = 16;
-        float m = -INFINITY, l = 0.f, o[W];  // l: of this thread's columns
+        float ref = INFINITY, l = 0.f, o[W];  // ref: 15 - m, infinite until a key was seen; l: of this thread's columns
 #pragma unroll
         for (int d = 0; d < W; ++d) o[d] = 0.f;
         const float c_row = fabsf(a.scale_log2) * q_inv;
@@ -366,12 +370,14 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
 #pragma unroll
             for (int w = 0; w < C::WGS; ++w) mx = fmaxf(mx, row_max[w * 128]);
             if (!ok) continue;
-            const float m_new = mx == -INFINITY ? m : fmaxf(m, ceilf(mx * c));
-            const float shrink_next = m == -INFINITY ? 0.f : tc::ex2(m - m_new);
-            m = m_new;
+            const float ref_new = mx == -INFINITY ? ref : fminf(ref, __fsub_rd(15.f, ceilf(mx * c)));
+            const float shrink_next = ref == INFINITY ? 0.f : tc::ex2(ref_new - ref);
+            ref = ref_new;
             // p = 2^15 exp2(s c - m): the factor 2^15 brings p into fp16's range and divides out with l
-            const float base = m == -INFINITY ? 0.f : 15.f - m;
+            const float base = ref == INFINITY ? 0.f : ref;
             const uint64_t c2 = tc::pack2(c, c), b2 = tc::pack2(base, base);
+            // From 2^22 on the rounding of m, which an exact s c would leave in P, matters: there s c is rounded like m was.
+            const bool plain = __all_sync(0xffffffffu, whole && fabsf(base) < 4194304.f);
             uint64_t sum2 = 0;
 #pragma unroll
             for (int g = 0; g < NC / GW; ++g) {
@@ -380,10 +386,15 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
 #pragma unroll
                 for (int e = 0; e < GW; e += 2) {
                     float x, y;
-                    tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
+                    if (plain) {
+                        tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
+                    } else {
+                        x = __fadd_rn(__fmul_rn(s[e], c), base);
+                        y = __fadd_rn(__fmul_rn(s[e + 1], c), base);
+                    }
                     x = tc::ex2(x);
                     y = tc::ex2(y);
-                    if (!whole) {
+                    if (!plain) {
                         x = GW * g + e < lim ? x : 0.f;
                         y = GW * g + e + 1 < lim ? y : 0.f;
                     }
@@ -413,14 +424,15 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
         l = 0.f;
 #pragma unroll
         for (int w = 0; w < C::WGS; ++w) l += shared_f[w * 128 + row];
-        // rows without keys: sum 0, output 0 (0 * 0); a NaN in the sum reaches the output
+        // rows without keys: sum 0, output 0; a NaN in the sum reaches the output
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int d = 0; d < W; ++d) o[d] *= inv;
+        for (int d = 0; d < W; ++d) o[d] = l == 0.f ? 0.f : o[d] * inv;  // (0 times a NaN that other rows of the tile see)
         if (wg == 0 && a.stats && i < a.Sq) {
             float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + i) * 2;
+            const float m = 15.f - ref;
             st[0] = m;
-            st[1] = l * 3.0517578125e-5f;  // 2^-15
+            st[1] = l == 0.f ? 0.f : l * exp2f(-(m + ref));  // 2^-15, but for the rounding of m
         }
         const int row0 = q_tile * ROWS + 32 * (warp & 3);
         tenmo_attn_write_rows<W>(o, a.o.ptr + b * a.o.sb + h * a.o.sh + (int64_t)row0 * a.o.sr + wg * W, a.o.sr, a.Sq - row0, a.D - wg * W, p.o_vec,
@@ -441,6 +453,13 @@ size_t align_up(size_t n) { return (n + 1023) & ~(size_t)1023; }
 
 bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D) {
     return D % 4 == 0 && v.sb % 4 == 0 && v.sh % 4 == 0 && v.sr % 4 == 0 && ((uintptr_t)v.ptr & 15u) == 0;
+}
+
+void tenmo_attn_causal_keys(const TenmoAttnParams& a, TenmoTileJob* j) {
+    if (!a.causal) return;
+    j->q_lengths = a.q_lengths;
+    j->seen_by = a.Sq;
+    j->offset = a.Sk - a.Sq;
 }
 
 int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp, int tile_rows) {
@@ -496,6 +515,7 @@ int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     jobs.D = a.D;
     jobs.job[0] = TenmoTileJob{a.k, a.k_lengths, w, (float*)p.k_inv, a.Hkv, a.Sk, p.tiles, tenmo_attn_row_vec(a.k, a.D)};
     jobs.job[1] = TenmoTileJob{a.v, a.k_lengths, w + img, (float*)p.v_inv, a.Hkv, a.Sk, p.tiles, tenmo_attn_row_vec(a.v, a.D)};
+    for (int e = 0; e < 2; ++e) tenmo_attn_causal_keys(a, &jobs.job[e]);
     if ((st = tenmo_attn_make_tiles(ctx, jobs, 2, dp, T)) != TENMO_OK) return st;
     const unsigned grid = (unsigned)((int64_t)a.B * a.H * p.q_tiles);
     if (dp == 64) {

@@ -16,6 +16,10 @@ struct TenmoTileJob {
     uint8_t* img;            // tile t of head (b, h): ((b * heads + h) * tiles + t) * (rows of a tile) * DP * 4 bytes
     float* inverse;          // 2^-e of every tile
     int heads, rows, tiles, vec;
+    int first;               // rows before this one become zeros too: they see no key
+    // causal keys (seen_by > 0): what the last row that takes part does not see becomes zeros
+    const int32_t* q_lengths;
+    int seen_by, offset;     // rows of q, k_len - q_len
     // With o.ptr set (src is the gradient of o): the per-row numbers of the backward pass as well.  Per tile 256 floats:
     // for rows 2 r, 2 r + 1 the four at 4 r: their -m (-inf for rows that take no part) and their 1 / l times the tile's power of two
     // PS that brings the largest to at most 2^15 (0 for those rows); [128, 192) delta; 192: PS, 193: the largest |delta|, 194: 1 / PS.
@@ -30,6 +34,7 @@ struct TenmoTileJobs {
     int B, D;
 };
 int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp, int tile_rows);  // 64 or 128 (without row numbers)
+void tenmo_attn_causal_keys(const TenmoAttnParams& a, TenmoTileJob* j);  // fills seen_by and so on of a job of k or v
 bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D);
 static inline int tenmo_attn_padded(int D) { return D <= 64 ? 64 : 128; }
 
@@ -126,7 +131,7 @@ __device__ __forceinline__ float tenmo_attn_stationary(const float* src, int64_t
     for (int g = 0; g < W / 16; ++g) {
         uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tc::split_pair(x[16 * g + 2 * e] * scale, x[16 * g + 2 * e + 1] * scale, hi[e], lo[e]);
+        for (int e = 0; e < 8; ++e) tc::split_rounded(x[16 * g + 2 * e] * scale, x[16 * g + 2 * e + 1] * scale, hi[e], lo[e]);
         if (SMEM) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {

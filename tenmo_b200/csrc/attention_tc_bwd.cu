@@ -320,8 +320,10 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
             float G, ps_inv;
             const float* info;
             int lim;                // first visible column (dkv) or their number (dq), of this thread's columns
-            bool whole;
+            bool whole;             // no column is masked, and the scores' rounding cannot lift P far above 1
         };
+        // |S| <= DP 2^30 and a recomputed S c differs from the forward pass's by 2^-19 of that times c at most: below 1?
+        auto rounding = [](float c) { return c * (DP * 2048.f) < 1.f; };
         auto set_up = [&](int j, float y1_inv, float y2_inv) {
             Tile t;
             const float c = c_row * y1_inv, f = x2_inv * y2_inv;  // dP = f * accumulator
@@ -333,14 +335,14 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
                 t.G = tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, t.info[3 * T + 1]));
                 t.ng2 = tc::pack2(-t.G, -t.G);
                 t.lim = a.causal ? (int)max((int64_t)-1, min((int64_t)T, i - off - (int64_t)(first + j) * T)) - col0 : 0;
-                t.whole = __all_sync(0xffffffffu, t.lim <= 0);
+                t.whole = __all_sync(0xffffffffu, t.lim <= 0 && rounding(c));
             } else {
                 t.info = nullptr;
                 t.ps_inv = 1.f;
                 t.G = 32768.f * tc::pow2_below_inverse(fmaf((float)DP * 1073741824.f, f, fabsf(delta_row)));
                 t.ng2 = tc::pack2(-delta_row * t.G, -delta_row * t.G);
                 t.lim = n_row - j * T - col0;
-                t.whole = __all_sync(0xffffffffu, t.lim >= NC);
+                t.whole = __all_sync(0xffffffffu, t.lim >= NC && rounding(c));
             }
             t.fg2 = tc::pack2(f * t.G, f * t.G);
             return t;
@@ -361,8 +363,9 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
             }
             if (!t.whole) {
                 tc::unpack2(v, x, y);
-                x = (DKV ? u >= t.lim : u < t.lim) ? x : 0.f;
-                y = (DKV ? u + 1 >= t.lim : u + 1 < t.lim) ? y : 0.f;
+                const float most = DKV ? 32768.f : 1.f;  // (a NaN stays)
+                x = (DKV ? u >= t.lim : u < t.lim) ? (x > most ? most : x) : 0.f;
+                y = (DKV ? u + 1 >= t.lim : u + 1 < t.lim) ? (y > most ? most : y) : 0.f;
                 v = tc::pack2(x, y);
             }
             return v;
@@ -434,7 +437,8 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
         if (ok && n > 0) add_tile(n - 1);
 
         // ---- to memory, through the stages ----
-        const bool valid = i < x_rows;  // rows that take no part: zeros
+        // rows that see no key, keys that no row sees: zeros, whatever their neighbours in the tile hold
+        const bool valid = i < x_rows && (DKV ? !a.causal || i <= (int64_t)q_rows - 1 + off : n_row > 0);
         const int row0 = x_tile * ROWS + 32 * (warp & 3), here = (DKV ? a.Sk : a.Sq) - row0;
         auto out_row = [&](const TenmoHeadsView& out) { return out.ptr + b * out.sb + h * out.sh + (int64_t)row0 * out.sr; };
         float* const scratch = reinterpret_cast<float*>(smem) + warp * (32 * W);  // all products are done: the stages are free
@@ -513,8 +517,10 @@ int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     jobs.D = a.D;
     jobs.job[0] = TenmoTileJob{a.k, a.k_lengths, ik, vk, a.Hkv, a.Sk, k_tiles, tenmo_attn_row_vec(a.k, a.D)};
     jobs.job[1] = TenmoTileJob{a.v, a.k_lengths, iv, vv, a.Hkv, a.Sk, k_tiles, tenmo_attn_row_vec(a.v, a.D)};
-    jobs.job[2] = TenmoTileJob{a.q, a.q_lengths, iq, vq, a.H, a.Sq, q_tiles, tenmo_attn_row_vec(a.q, a.D)};
-    jobs.job[3] = TenmoTileJob{a.go, a.q_lengths, ig, vg, a.H, a.Sq, q_tiles, tenmo_attn_row_vec(a.go, a.D)};
+    for (int e = 0; e < 2; ++e) tenmo_attn_causal_keys(a, &jobs.job[e]);
+    const int first = a.causal && a.Sq > a.Sk ? a.Sq - a.Sk : 0;  // the first row that sees a key
+    jobs.job[2] = TenmoTileJob{a.q, a.q_lengths, iq, vq, a.H, a.Sq, q_tiles, tenmo_attn_row_vec(a.q, a.D), first};
+    jobs.job[3] = TenmoTileJob{a.go, a.q_lengths, ig, vg, a.H, a.Sq, q_tiles, tenmo_attn_row_vec(a.go, a.D), first};
     jobs.job[3].o = a.o;
     jobs.job[3].o_vec = tenmo_attn_row_vec(a.o, a.D);
     jobs.job[3].stats = a.stats;

@@ -48,6 +48,10 @@ struct tenmo_ctx {
     bool op_ws_captured = false;
     void* op_retired[16] = {nullptr};
     int n_op_retired = 0;
+    // The stream of the last call that used it, and an event on that stream: a call on another stream waits for it.
+    cudaStream_t op_stream = nullptr;
+    cudaEvent_t op_event = nullptr;
+    bool op_used = false, op_recorded = false;
     // small fixed device scratch: [0] status word, [8..15] cross-entropy tickets/accumulators
     uint32_t* dev_status = nullptr;
     // ticket counters of the split column-sum kernel: zero between calls (the last CTA resets its own)

@@ -51,6 +51,13 @@ int tenmo_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
     return TENMO_OK;
 }
 
+static cudaError_t record_op_event(tenmo_ctx* ctx) {
+    cudaError_t e = ctx->op_event ? cudaSuccess : cudaEventCreateWithFlags(&ctx->op_event, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventRecord(ctx->op_event, ctx->op_stream);
+    ctx->op_recorded = e == cudaSuccess;
+    return e;
+}
+
 int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     const bool capturing = cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
@@ -80,7 +87,24 @@ int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
         }
         ctx->op_ws_bytes = want;
     }
-    if (capturing) ctx->op_ws_captured = true;
+    if (capturing) {
+        ctx->op_ws_captured = true;
+    } else {
+        // the call before may still be running on another stream
+        if (ctx->op_used && ctx->op_stream != ctx->stream) {
+            cudaError_t e = cudaSuccess;
+            if (!ctx->op_recorded) {
+                if (cudaStreamIsCapturing(ctx->op_stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone)
+                    return tenmo_set_error(ctx, TENMO_ERR_STATE, "the stream of the last call that used the workspace is being captured");
+                e = record_op_event(ctx);
+            }
+            if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->stream, ctx->op_event, 0);
+            if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace order: %s", cudaGetErrorString(e));
+        }
+        ctx->op_stream = ctx->stream;
+        ctx->op_used = true;
+        ctx->op_recorded = false;
+    }
     *out = ctx->op_ws;
     return TENMO_OK;
 }
@@ -181,6 +205,7 @@ void tenmo_cuda_destroy(tenmo_ctx* ctx) {
     if (ctx->p2p_buf) tenmo_dp_p2p_close(ctx);
     if (ctx->stream) cudaStreamSynchronize(ctx->stream);
     if (ctx->ws) cudaFree(ctx->ws);
+    if (ctx->op_event) cudaEventDestroy(ctx->op_event);
     if (ctx->op_ws) cudaFree(ctx->op_ws);
     for (int i = 0; i < ctx->n_op_retired; ++i) cudaFree(ctx->op_retired[i]);
     if (ctx->dev_status) cudaFree(ctx->dev_status);
@@ -199,7 +224,18 @@ const char* tenmo_cuda_last_error(tenmo_ctx* ctx) { return ctx ? ctx->err : g_in
 
 int tenmo_cuda_set_stream(tenmo_ctx* ctx, void* cuda_stream) {
     TENMO_CHECK_CTX(ctx);
-    ctx->stream = cuda_stream == TENMO_STREAM_OWN ? ctx->own_stream : (cudaStream_t)cuda_stream;
+    cudaStream_t next = cuda_stream == TENMO_STREAM_OWN ? ctx->own_stream : (cudaStream_t)cuda_stream;
+    // The operators' workspace goes with the context: note how far the stream that used it last has come, while the caller still has
+    // that stream.  A stream that is being captured is left alone (a graph's order is its owner's).
+    if (ctx->op_used && ctx->op_stream == ctx->stream && next != ctx->stream) {
+        TenmoDeviceGuard guard(ctx);
+        cudaStreamCaptureStatus a = cudaStreamCaptureStatusNone, b = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(ctx->stream, &a) == cudaSuccess && cudaStreamIsCapturing(next, &b) == cudaSuccess &&
+            a == cudaStreamCaptureStatusNone && b == cudaStreamCaptureStatusNone)
+            record_op_event(ctx);
+        cudaGetLastError();  // what failed here is tried again by the next call that needs it
+    }
+    ctx->stream = next;
     // remember the streams the context has run on (most recent first): a workspace growth and the status check wait for them
     int at = -1;
     for (int i = 0; i < ctx->n_bound; ++i)

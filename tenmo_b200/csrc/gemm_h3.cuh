@@ -75,7 +75,7 @@ __device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[4][8], uin
         const int r = (threadIdx.x >> 4) + 32 * s;
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tc::split_pair(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);
+        for (int e = 0; e < 4; ++e) tc::split_rounded(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);
         const int at = (c >> 3) * H3_PLANE + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(img + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(img + 2 * H3_PLANE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);

@@ -300,6 +300,7 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     if (c.grad && c.db && !c.bias) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: db without a bias", who);
     if (c.x->batch_rank || c.w->batch_rank) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: x and w are plain matrices", who);
     if (c.x->row_stride < 0 || c.x->col_stride < 0) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: x has a negative stride", who);
+    if (c.w->row_stride < 0 || c.w->col_stride < 0) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: w has a negative stride", who);
     if (c.w->row_stride != 1 && c.w->col_stride != 1)
         return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "%s: w needs a unit stride on one axis", who);
     if (c.reduction < 0 || c.reduction > 2) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "%s: reduction %d", who, c.reduction);

@@ -3,8 +3,8 @@
 // Arithmetic.  A block of an fp32 operand is scaled by a power of two 2^e (its largest finite entry comes to lie in
 // [2^14, 2^15)) and written as hi + lo, two fp16 numbers: hi = fp16(x 2^e), lo = fp16(x 2^e - hi).  That keeps 22 bits of an
 // entry down to 2^-18 of the block's largest one and an absolute 2^-40 of it below.  A product of two such operands is
-// lo.hi + hi.lo + hi.hi, three tcgen05.mma of kind::f16 into one fp32 accumulator (the dropped lo.lo is below 2^-22 of the
-// term); the powers of two come off in fp32, exactly.  fp16 runs at twice the rate of TF32 and its planes are half as
+// lo.hi + hi.lo + hi.hi, three tcgen05.mma of kind::f16 into one fp32 accumulator; the dropped lo.lo is at most 2^-22 of the
+// term, or 2^-21 where an operand made inside a loop is cut instead of rounded.  The powers of two come off in fp32, exactly.  fp16 runs at twice the rate of TF32 and its planes are half as
 // large, which is why these kernels do not use the three TF32 products of the dense GEMM.
 // The tensor core adds into its accumulator with truncation, so a chain is kept short (one tile) and tiles are added in
 // registers with rounding; within a chain the two small products go first, while the accumulator is small.
@@ -136,12 +136,25 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
     asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
     return r;
 }
-// hi / lo of two values.  hi is the value cut to 11 significant bits (a logical AND instead of a conversion back), which fp16
-// holds exactly down to 2^-14; below that hi is rounded to the fp16 grid and the pair is good to 2^-25 absolute, the same floor
-// that lo has.  The cut leaves lo at most 13 bits, of which fp16 keeps 11: 22 bits together.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+// the same, what lies beyond fp16's range as its largest number (infinities too; a NaN stays one)
+__device__ __forceinline__ uint32_t half_pair_finite(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+// hi / lo of two scaled entries of an operand: hi rounded to fp16, lo the difference, rounded.  |lo| <= 2^-11 |x|; together they miss
+// x by at most 2^-23 of it, or 2^-25 where fp16 ends.
+__device__ __forceinline__ void split_rounded(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = half_pair(a, b);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    lo = half_pair(a - h.x, b - h.y);
+}
+// The same inside the loops (P, dS), where instructions count: hi is the value cut to 11 significant bits, a logical AND instead of a
+// conversion back; fp16 holds it exactly down to 2^-14, and below that the pair is good to 2^-25 absolute, like lo.  |lo| < 2^-10 |x|, of whose at
+// most 13 bits fp16 keeps 11: together they miss x by at most 2^-22 of it.
+__device__ __forceinline__ void split_cut(float a, float b, uint32_t& hi, uint32_t& lo) {
     const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-    hi = half_pair(ah, bh);
+    hi = half_pair_finite(ah, bh);
     float al, bl;
     unpack2(fma2(pack2(ah, bh), pack2(-1.f, -1.f), pack2(a, b)), al, bl);  // both differences, exact, in one instruction
     lo = half_pair(al, bl);
@@ -251,7 +264,7 @@ __device__ __forceinline__ void st_split(uint32_t addr, const float (&x)[N]) {
     for (int g = 0; g < N / 16; ++g) {
         uint32_t r[16];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) split_pair(x[16 * g + 2 * e], x[16 * g + 2 * e + 1], r[e], r[8 + e]);
+        for (int e = 0; e < 8; ++e) split_cut(x[16 * g + 2 * e], x[16 * g + 2 * e + 1], r[e], r[8 + e]);
         st16(addr + 16 * g, r);
     }
 }

@@ -158,6 +158,124 @@ def test_nan_and_infinity_stay_in_their_rows(size):
         ar.check("o", got[:, h, rows], (want[0][:, h, rows], want[1][:, h, rows]))
 
 
+@pytest.mark.parametrize("Sq,Sk,H,D", [(50, 20, 2, 24), (60, 30, 2, 64), (300, 100, 16, 64), (300, 100, 16, 100), (320, 192, 16, 32)])
+def test_rows_that_see_nothing_may_hold_anything(Sq, Sk, H, D):
+    """Causal with more rows than keys: what the first Sq - Sk rows hold reaches nothing, and their own results are zeros."""
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    q, go = (_make(gen, 2, H, Sq, D) for _ in range(2))
+    k, v = (_make(gen, 2, H, Sk, D) for _ in range(2))
+    q[:, :, :Sq - Sk] = NAN
+    go[:, :, :Sq - Sk, ::2] = math.inf
+    got = compare(q, k, v, go, causal=True)
+    assert float(got["o"][:, :, :Sq - Sk].abs().max()) == 0 and float(got["dq"][:, :, :Sq - Sk].abs().max()) == 0
+
+
+@pytest.mark.parametrize("size,H", [(50, 2), (200, 16)])
+def test_keys_that_no_row_sees_may_hold_anything(size, H):
+    """Causal with rows cut off by q_lengths: the keys behind the last row's are zeros in dk and dv and reach nothing."""
+    gen = torch.Generator(device="cuda").manual_seed(20)
+    q, k, v, go = (_make(gen, 2, H, size, 64) for _ in range(4))
+    rows = [size - 21, 7]
+    for b, n in enumerate(rows):
+        k[b, :, n:] = NAN
+        v[b, :, n:] = math.inf
+        q[b, :, n:] = math.inf
+        go[b, :, n:] = NAN
+    got = compare(q, k, v, go, causal=True, q_lengths=ints(rows))
+    for b, n in enumerate(rows):
+        assert float(got["dk"][b, :, n:].abs().max()) == 0 and float(got["dv"][b, :, n:].abs().max()) == 0
+
+
+@pytest.mark.parametrize("size", [40, 300])
+@pytest.mark.parametrize("big", [300.0, 1e3, 2e3, 4e3, 1e4, 1e5])
+def test_scores_beyond_the_whole_numbers(size, big):
+    """Scores up to 1e11, whose 32-bit values are further apart than 1: a row whose best key leads by more than the scores' error takes that
+    key's v, and everything stays finite."""
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    q, k, v, go = (_make(gen, 1, 2 if size < 100 else 4, size, 64) for _ in range(4))
+    q, k = big * q, big * k
+    got = run(q, k, v, go)
+    for t in got.values():
+        assert bool(t.isfinite().all())
+    s = q.double() @ k.double().transpose(-1, -2) / 8
+    top = s.topk(2, dim=-1)
+    # 2^-17 of the sum of |q k|: (dim + 64) u with room; exp(-60) of the others is below half a step of v's largest entry
+    lead = top.values[..., 0] - top.values[..., 1] > 60 + 2.0 ** -16 * (q.abs().double() @ k.abs().double().transpose(-1, -2)).amax(-1) / 8
+    assert int(lead.sum()) > size
+    want = torch.take_along_dim(v, top.indices[..., :1], 2).double()
+    # One term P v / P.  P = hi + lo misses 2^-22, v 2^-23 (or 2^-38 of its tile's largest), the dropped lo lo is at most 2^-10 2^-11; three partial
+    # products are added with truncation, 2^-23 each, and the division and its product round, 2 * 2^-24:
+    # 2^-22 + 2^-23 + 2^-21 + 3 * 2^-23 + 2^-23 = 1.375 * 2^-20 < 2^-19.
+    off = (got["o"].double() - want).abs()
+    assert bool((off <= 2.0 ** -19 * want.abs() + 2.0 ** -36 * v.abs().max())[lead].all())
+
+
+def test_calls_on_two_streams_do_not_share_the_workspace_at_once():
+    """A call on another stream right behind a long one: the workspace that both use is waited for."""
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    a = [_make(gen, 8, 8, 1024, 64) for _ in range(4)]
+    b = [_make(gen, 4, 8, 300, 40) for _ in range(4)]
+    c = [_make(gen, 2, 4, 1, 40)] + [_make(gen, 2, 4, 3000, 40) for _ in range(2)]
+    want = run(*a), run(*b), run(*c)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    from tenmo_b200 import make_heads
+    from tests import gpu_util as g
+
+    view = lambda t: make_heads(t.data_ptr(), t.stride())
+    for _ in range(3):
+        got = []
+        for stream, (q, k, v, *go) in zip(streams, (a, b, c)):
+            out = dict(o=torch.full_like(q, NAN))
+            stats = g.empty(*q.shape[:3], 2)
+            shape = (q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
+            if go:
+                out.update(dq=torch.full_like(q, NAN), dk=torch.full_like(k, NAN), dv=torch.full_like(v, NAN))
+            got.append((stream, shape, q, k, v, go, out, stats))
+        torch.cuda.synchronize()
+        for stream, shape, q, k, v, go, out, stats in got:
+            with torch.cuda.stream(stream):
+                h = g.handle()
+                scale = 1 / math.sqrt(q.shape[3])
+                h.attention_fwd(shape, view(q), view(k), view(v), view(out["o"]), stats.data_ptr(), scale)
+                if go:
+                    h.attention_bwd(shape, view(q), view(k), view(v), view(out["o"]), stats.data_ptr(), view(go[0]), view(out["dq"]),
+                                    view(out["dk"]), view(out["dv"]), scale)
+        torch.cuda.synchronize()
+        for (_, _, _, _, _, _, out, _), ref in zip(got, want):
+            for name in out:
+                assert torch.equal(out[name], ref[name]), name
+    g.handle().check_device_status()
+
+
+@pytest.mark.parametrize("q_len", [1, 20, 130])
+def test_offsets_beyond_32_bits(q_len):
+    """A cache whose rows lie 65536 numbers apart: offsets pass 2^31 (and, in bytes, 2^32)."""
+    from tenmo_b200 import make_heads
+    from tests import gpu_util as g
+
+    gen = torch.Generator(device="cuda").manual_seed(23)
+    n, stride, D = 36000, 65536, 40
+    buf = torch.empty(n * stride, device="cuda")
+    at = lambda c: torch.as_strided(buf, (1, 2, n, D), (0, D, stride, 1), c * 2 * D)
+    k, v, dk, dv = (at(c) for c in range(4))
+    for t in (k, v):
+        t.copy_(torch.randn(t.shape, device="cuda", generator=gen))
+    for t in (dk, dv):
+        t.fill_(NAN)
+    q, go = (_make(gen, 1, 4, q_len, D) for _ in range(2))
+    o, dq, stats = torch.full_like(q, NAN), torch.full_like(q, NAN), g.empty(1, 4, q_len, 2)
+    h = g.handle()
+    view = lambda t: make_heads(t.data_ptr(), (n * stride, *t.stride()[1:]))
+    shape = (1, 4, 2, q_len, n, D)
+    h.attention_fwd(shape, view(q), view(k), view(v), view(o), stats.data_ptr(), 0.3)
+    h.attention_bwd(shape, view(q), view(k), view(v), view(o), stats.data_ptr(), view(go), view(dq), view(dk), view(dv), 0.3)
+    h.check_device_status()
+    want = ar.reference(q, k.contiguous(), v.contiguous(), go, scale=0.3)
+    for name, t in dict(o=o, dq=dq, dk=dk, dv=dv).items():
+        ar.check(name, t, want[name])
+
+
 @pytest.mark.parametrize("size", [30, 260])
 def test_broadcast_inputs_and_wide_strides(size):
     """k and v shared by the whole batch (stride 0), q inside a wider row, o inside a wider row."""
@@ -237,6 +355,23 @@ def test_refusals():
     refused(-1, scale=NAN)
     refused(-1, q=make_heads(t.data_ptr(), (1024, 256, -16)))
     refused(-1, o=make_heads(t.data_ptr(), (1024, 256, 8)))
+    other = g.empty(65536)
+    out = lambda *strides: make_heads(other.data_ptr(), strides)
+    many = (2, 4, 2, 8, 8, 16)
+    h.attention_fwd(many, v, v, v, out(512, 128, 16), 0, 1.0)
+    h.attention_fwd(many, v, v, v, out(512, 16, 64), 0, 1.0)  # heads inside the row
+    h.attention_fwd(many, v, v, v, out(16, 32, 128), 0, 1.0)
+    for strides in ((512, 127, 16), (0, 128, 16), (511, 128, 16), (512, 0, 16), (512, 16, 63), (16, 16, 128), (512, 128, 2 ** 62)):
+        refused(-1, many, o=out(*strides))
+    refused(-1, many, o=v)  # o is an input
+    refused(-1, scale=3e38)
+    ok_out = [make_heads(other.data_ptr() + 4 * 4096 * e, (512, 128, 16)) for e in range(5)]
+    stats = g.empty(1024)
+    h.attention_bwd(many, v, v, v, ok_out[0], stats.data_ptr(), ok_out[1], *ok_out[2:], 1.0)
+    for bad in ((v, ok_out[3], ok_out[4]), (ok_out[2], ok_out[0], ok_out[4]), (ok_out[2], ok_out[3], ok_out[1]), (ok_out[2], ok_out[2], ok_out[4]),
+                (ok_out[2], ok_out[3], make_heads(other.data_ptr() + 16 * 4096 * 4, (512, 0, 16)))):
+        with pytest.raises(TenmoError):
+            h.attention_bwd(many, v, v, v, ok_out[0], stats.data_ptr(), ok_out[1], *bad, 1.0)
     with pytest.raises(TenmoError):
         h.attention_bwd(ok, v, v, v, v, None, v, v, v, v, 1.0)
     with pytest.raises(TenmoError):

@@ -98,6 +98,18 @@ def test_unaligned_pointers():
         _check(name, got[name], ref[name])
 
 
+@pytest.mark.parametrize("C", [40, 300, 9000])
+def test_rows_far_apart(C):
+    """Rows of x so far apart that their offsets pass 2^31."""
+    x, gamma, bias, dy = _inputs(300, C, 9)
+    stride = (1 << 31) // 299 + 77
+    far = torch.as_strided(torch.empty(300 * stride, device="cuda"), (300, C), (stride, 1))
+    far.copy_(x)
+    a, b = _run(far, gamma, bias, dy), _reference(far, gamma, bias, dy)
+    for name in a:
+        _check(name, a[name], b[name])
+
+
 def test_large_mean_does_not_cancel():
     """mean 1e4, deviation 2: E[x^2] - mean^2 would lose everything in 32 bits."""
     x, gamma, bias, dy = _inputs(64, 1000, 7, shift=1e4)

@@ -7,6 +7,8 @@ c = 128 + V / 256 (the length of a thread's sum).  Then
   dz     |u_n| (r p + 4 u (p + 1[y] + ls / V)), and 2^-36 of the largest |dz| of the call where tiles are scaled
   dx     sum_v e_dz |w| + (64 + V / 32) u sum_v |dz w|;  dw, db alike over the rows
 """
+import math
+
 import numpy as np
 import pytest
 
@@ -201,6 +203,97 @@ def test_several_pieces_give_what_one_gives():
         assert torch.equal(got[n], again[n])
 
 
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -math.inf], ids=["lowest", "-inf"])
+@pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
+@pytest.mark.parametrize("size", [(30, 20, 500), (100, 20, 500), (200, 256, 2000)], ids=str)
+def test_classes_masked_through_the_bias(size, tied, low):
+    """Classes whose bias is the type's lowest value or -inf: the same loss and gradients as without them, and none of their own."""
+    N, D, V = size
+    x, w, b, y = make(N, D, V, 21, tied=tied, bias=True)
+    keep = torch.rand(V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(22)) < 0.5
+    keep[64:192] = False  # whole groups of columns too
+    keep[:5] = True
+    at = keep.nonzero()[:, 0]
+    y = torch.where(y == IGN, y, at[y.clamp(min=0) % len(at)])
+    got = run(x, w, torch.where(keep, b, low), y)
+    place = torch.full((V,), -1, device="cuda", dtype=torch.int64)
+    place[at] = torch.arange(len(at), device="cuda")
+    y_kept = torch.where(y == IGN, y, place[y.clamp(min=0)])
+    want = reference(x, w[:, at], b[at], y_kept)
+    check("loss", got["loss"], want["loss"])
+    check("dx", got["dx"], want["dx"])
+    check("dw", got["dw"][:, at], want["dw"])
+    check("db", got["db"][at], want["db"])
+    assert float(got["dw"][:, ~keep].abs().max()) == 0 and float(got["db"][~keep].abs().max()) == 0
+
+
+@pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
+@pytest.mark.parametrize("size", [(7, 36, 200), (100, 36, 200), (257, 256, 2000)], ids=str)
+def test_pointers_that_are_not_aligned(size, tied):
+    """Every buffer begins 4 bytes behind a 16-byte boundary, and nothing is written outside."""
+    from tenmo_b200 import make_mat
+    from tests import gpu_util as g
+
+    N, D, V = size
+    x, w, b, y = make(N, D, V, 23, tied=tied, bias=True)
+    ref = run(x, w, b, y)
+
+    def odd(t):
+        buf = torch.full((t.numel() + 8,), float("nan"), device="cuda")
+        return buf, torch.as_strided(buf, t.shape, t.stride(), 1)
+    put = lambda t: odd(t)[1].copy_(t)
+    xo, wo, bo = put(x), put(w), put(b)
+    bufs = {n: odd(ref[n]) for n in ("dx", "dw", "db")}
+    loss, valid = torch.empty(1, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+    h = g.handle()
+    h.linear_ce_fwd_bwd(make_mat(xo.data_ptr(), (N, D), xo.stride()), make_mat(wo.data_ptr(), (D, V), wo.stride()), bo.data_ptr(), y.data_ptr(), True,
+                        N, D, V, IGN, 0.0, 0, loss.data_ptr(), valid.data_ptr(), 0, *(bufs[n][1].data_ptr() for n in ("dx", "dw", "db")))
+    h.check_device_status()
+    want = reference(x, w, b, y)
+    check("loss", loss[0], want["loss"])
+    for n, (buf, t) in bufs.items():
+        check(n, t, want[n])
+        assert bool(buf[0].isnan()) and bool(buf[1 + t.numel():].isnan().all()), n
+
+
+@pytest.mark.parametrize("size", [(20, 32, 100), (300, 32, 100), (300, 256, 2000)], ids=str)
+def test_rows_far_apart(size):
+    """Rows of x so far apart that their offsets pass 2^31."""
+    N, D, V = size
+    x, w, b, y = make(N, D, V, 24)
+    stride = (1 << 31) // (N - 1) + 77
+    far = torch.as_strided(torch.empty(N * stride, device="cuda"), (N, D), (stride, 1))
+    far.copy_(x)
+    compare(far, w, b, y)
+
+
+@pytest.mark.parametrize("N", [8, 40])
+def test_more_than_2_31_weights(N):
+    """A tied weight whose entries are counted beyond 2^31, on both sides of the choice of kernels."""
+    D, V = 2048, 1049000
+    gen = torch.Generator(device="cuda").manual_seed(25)
+    x = torch.randn(N, D, device="cuda", generator=gen)
+    w = torch.randn(V, D, device="cuda", generator=gen) / D ** 0.5
+    y = torch.randint(V - 50, V, (N,), device="cuda", generator=gen)
+    y[0] = 3
+    got = run(x, w.t(), None, y)
+    z = torch.cat([x.double() @ w[v0:v0 + (1 << 16)].double().t() for v0 in range(0, V, 1 << 16)], 1)
+    lse = z.logsumexp(1)
+    loss = (lse - z[torch.arange(N, device="cuda"), y]).mean()
+    # a logit is off by at most (D + 64) u sum |x w|, some 2^-15; the rest follows as in reference()
+    assert abs(float(got["loss"]) - float(loss)) <= 2.0 ** -15
+    dz = (z - lse[:, None]).exp()
+    dz[torch.arange(N, device="cuda"), y] -= 1
+    dz /= N
+    near = torch.cat([torch.arange(100, device="cuda"), torch.arange(V - 100, V, device="cuda")])
+    dw = dz[:, near].t() @ x.double()
+    off = (got["dw"].t()[near].double() - dw).abs()
+    assert bool((off <= 2.0 ** -14 * (dz[:, near].abs().t() @ x.abs().double()) + 2.0 ** -36).all())
+    dx = sum(dz[:, v0:v0 + (1 << 16)] @ w[v0:v0 + (1 << 16)].double() for v0 in range(0, V, 1 << 16))
+    size = sum(dz[:, v0:v0 + (1 << 16)].abs() @ w[v0:v0 + (1 << 16)].abs().double() for v0 in range(0, V, 1 << 16))
+    assert bool(((got["dx"].double() - dx).abs() <= 2.0 ** -14 * size).all())
+
+
 def test_no_rows():
     x, w, b, y = make(0, 8, 20, 11, bias=True)
     got = run(x, w, b, y)
@@ -233,6 +326,8 @@ def test_refusals():
     refused(-1, x=make_mat(p, (4, 8), (-8, 1)))
     refused(-1, x=make_mat(p, (2, 4, 8), (32, 8, 1)))
     refused(-3, w=make_mat(p, (8, 16), (32, 2)))
+    refused(-1, w=make_mat(p, (8, 16), (-16, 1)))
+    refused(-1, w=make_mat(p, (8, 16), (1, -8)))
     with pytest.raises(TenmoError):
         h.linear_ce_fwd_bwd(x, w, 0, y, True, 4, 8, 16, IGN, 0.0, 0, p, p, 0, p, None)
     with pytest.raises(TenmoError):  # a bias gradient without a bias
