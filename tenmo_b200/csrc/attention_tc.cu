@@ -13,7 +13,14 @@
 // 128), which exchange their maxima through shared memory, and up to dim 64, where everything fits twice into an SM (96 KB,
 // 256 columns), two CTAs fill each other's gaps: one's products run while the other's exponentials are taken.  Up to dim 128 one
 // CTA has the SM and a second S buffer lets S_{j+1} run while P_j is made.  One warp issues the MMAs, one the copies.
-// Bound: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
+// S and P are handed over in halves of 64 keys, so the maximum of the first half is taken while the second is computed and O_j
+// starts while the second half's exponentials are taken; O_{j-1} is added while S_j is computed.
+// Floor: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
+// Measured at 384 heads of 512 rows and keys, dim 64: 128 us behind 26 us of images (25.8 GF, 47 us of tensor time).  A tile of 128 x 128
+// takes 3900 cycles with one CTA on the SM, 3350 with two, where the products and the exponentials (measured apart) need 1540 each and do
+// not slow each other; a CTA costs 14,000 cycles besides (q's way into tensor memory, the first tile's way to the exponentials, the
+// output).  Tensor pipe 32 % busy, exponential unit 24 %: the chain of a tile decides.  Two sides per CTA under one issuer were slower
+// (202 us for 167 in all), and so was one S buffer per 64 keys.
 #include "attention_tc.cuh"
 
 namespace {
@@ -160,7 +167,7 @@ struct FwdCfg {
     static constexpr int WGS = DP / 32;             // warpgroups that share a tile
     static constexpr int THREADS = 128 * WGS + 64;
     static constexpr int ISSUER = 4 * WGS, LOADER = ISSUER + 1;
-    static constexpr int NC = T / WGS, W = DP / WGS;  // columns of S and of O of a thread
+    static constexpr int HC = T / 2 / WGS, W = DP / WGS;  // columns of a half of S and of O of a thread
     static constexpr int NB = DP == 64 ? 1 : 2;     // S / P buffers
     static constexpr int PLANE = T * DP * 2;        // bytes of one plane of a tile
     static constexpr int IMG = 2 * PLANE;           // a tile's hi and lo plane, a slot of the ring
@@ -180,10 +187,10 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     const uint32_t bars = smem_u32(smem + C::RING + 2 * C::WGS * 128 * 4);
     auto full = [&](int slot) { return bars + 8u * slot; };
     auto empty = [&](int slot) { return bars + 8u * (3 + slot); };
-    auto s_full = [&](int j) { return bars + 8u * (6 + (j & 1)); };
-    auto p_full = [&](int j) { return bars + 8u * (8 + (j & 1)); };
-    auto o_full = [&](int j) { return bars + 8u * (10 + (j & 1)); };
-    const uint32_t o_free = bars + 8u * 12, drain = bars + 8u * 13;
+    auto s_full = [&](int j, int half) { return bars + 8u * (6 + 2 * (j & 1) + half); };
+    auto p_full = [&](int j, int half) { return bars + 8u * (10 + 2 * (j & 1) + half); };
+    auto o_full = [&](int j) { return bars + 8u * (14 + (j & 1)); };
+    const uint32_t o_free = bars + 8u * 16, drain = bars + 8u * 17;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + C::RING + 2 * C::WGS * 128 * 4 + 256);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -203,7 +210,10 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4 * C::WGS); mbar_init(o_full(w), 1); }
+        for (int w = 0; w < 2; ++w) {
+            for (int half = 0; half < 2; ++half) { mbar_init(s_full(w, half), 1); mbar_init(p_full(w, half), 4 * C::WGS); }
+            mbar_init(o_full(w), 1);
+        }
         mbar_init(o_free, 4 * C::WGS);
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -255,47 +265,57 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
         } else if (warp == C::ISSUER) {
             const uint32_t tm = tc::uniform(tmem), stages = tc::uniform(smem_u32(smem));
             const int n = tc::uniform(n_tiles);
-            constexpr uint32_t ID_S = tc::idesc_f16(T, false), ID_O = tc::idesc_f16(DP, true);
+            constexpr uint32_t ID_S = tc::idesc_f16(T / 2, false), ID_O = tc::idesc_f16(DP, true);
             auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
             int slot = 0, phase = 0;
             auto next_slot = [&]() { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
+            // S_j, each half (64 keys: an accumulator of its own) handed over as soon as it is there
             auto scores = [&](int j) {
-                if (!wait(full(slot), phase)) return false;
                 tc::fence_after();
-                const uint32_t hi = stages + slot * C::IMG, d = tm + C::S_COL + (uint32_t)(j % C::NB) * T;
 #pragma unroll
-                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + DP / 2 + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, c == 0);
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t hi = stages + slot * C::IMG + half * 8192, d = tm + C::S_COL + (uint32_t)(j % C::NB) * T + 64 * half;
 #pragma unroll
-                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + C::PLANE + c * T * 128), ID_S, false);
+                    for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + DP / 2 + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, c == 0);
 #pragma unroll
-                for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, false);
-                tc::commit(s_full(j));
+                    for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + C::PLANE + c * T * 128), ID_S, false);
+#pragma unroll
+                    for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, tm + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, false);
+                    tc::commit(s_full(j, half));
+                }
                 tc::commit(empty(slot));
                 next_slot();
-                return true;
             };
-            bool ok = n == 0 || scores(0);
+            // In each place the wait that ends last comes last: one that is over costs its latency all the same.
+            bool ok = n == 0 || wait(full(slot), phase);
+            if (ok && n) scores(0);
             for (int j = 0; ok && j < n; ++j) {
                 if (C::NB == 2 && j + 1 < n) {  // S_{j+1} replaces P_{j-1}, whose product must be done
-                    ok = (j == 0 || wait(o_full(j - 1), (uint32_t)((j - 1) >> 1) & 1u)) && scores(j + 1);
+                    ok = wait(full(slot), phase) && (j == 0 || wait(o_full(j - 1), (uint32_t)((j - 1) >> 1) & 1u));
                     if (!ok) break;
+                    scores(j + 1);
                 }
-                ok = wait(full(slot), phase) && wait(p_full(j), (uint32_t)(j >> 1) & 1u) && (j == 0 || wait(o_free, (uint32_t)(j - 1) & 1u));
+                ok = wait(full(slot), phase) && (j == 0 || wait(o_free, (uint32_t)(j - 1) & 1u));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && wait(p_full(j, half), (uint32_t)(j >> 1) & 1u);
+                    if (!ok) break;
+                    tc::fence_after();
+                    // keys 16 k ..: eight columns of hi pairs from 16 k on, then eight of lo pairs
+                    const uint32_t hi = stages + slot * C::IMG + half * 8192;
+                    const uint32_t pr = tm + C::S_COL + (uint32_t)(j % C::NB) * T + 64 * half, d = tm + C::O_COL;
+                    tc::mma4_ts<16, tc::STEP_MN>(d, pr + 8, tc::desc_mn(hi, T), ID_O, half == 0);
+                    tc::mma4_ts<16, tc::STEP_MN>(d, pr, tc::desc_mn(hi + C::PLANE, T), ID_O, false);
+                    tc::mma4_ts<16, tc::STEP_MN>(d, pr, tc::desc_mn(hi, T), ID_O, false);
+                }
                 if (!ok) break;
-                tc::fence_after();
-                const uint32_t hi = stages + slot * C::IMG;
-                const uint32_t pr = tm + C::S_COL + (uint32_t)(j % C::NB) * T, d = tm + C::O_COL;
-                // keys 16 k ..: eight columns of hi pairs from 16 k on, then eight of lo pairs
-#pragma unroll
-                for (int g = 0; g < T / 64; ++g) tc::mma4_ts<16, tc::STEP_MN>(d, pr + 64 * g + 8, tc::desc_mn(hi + g * 8192, T), ID_O, g == 0);
-#pragma unroll
-                for (int g = 0; g < T / 64; ++g) tc::mma4_ts<16, tc::STEP_MN>(d, pr + 64 * g, tc::desc_mn(hi + C::PLANE + g * 8192, T), ID_O, false);
-#pragma unroll
-                for (int g = 0; g < T / 64; ++g) tc::mma4_ts<16, tc::STEP_MN>(d, pr + 64 * g, tc::desc_mn(hi + g * 8192, T), ID_O, false);
                 tc::commit(o_full(j));
                 tc::commit(empty(slot));
                 next_slot();
-                if (C::NB == 1 && j + 1 < n) ok = wait(o_full(j), (uint32_t)(j >> 1) & 1u) && scores(j + 1);  // S_{j+1} replaces P_j
+                if (C::NB == 1 && j + 1 < n) {  // S_{j+1} replaces P_j
+                    ok = wait(full(slot), phase) && wait(o_full(j), (uint32_t)(j >> 1) & 1u);
+                    if (ok) scores(j + 1);
+                }
             }
             // Every MMA is done before tensor memory is given back: the readers of O have seen to it; after a wait that ran out, wait
             // again (bounded) here.
@@ -306,7 +326,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             }
         }
     } else {
-        constexpr int NC = C::NC, W = C::W, GW = 16;
+        constexpr int HC = C::HC, W = C::W, GW = 16;
         float ref = INFINITY, l = 0.f, o[W];  // ref: 15 - m, infinite until a key was seen; l: of this thread's columns
 #pragma unroll
         for (int d = 0; d < W; ++d) o[d] = 0.f;
@@ -346,22 +366,23 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
                 k_ahead = __ldg(p.k_inv + tile0 + j + 1);
                 v_ahead = __ldg(p.v_inv + tile0 + j + 1);
             }
-            await(s_full(j), j >> 1);
-            tc::fence_after();
-            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T + wg * NC;
-            const int lim = n_row - j * T - wg * NC;  // visible columns of this thread
-            const bool whole = __all_sync(0xffffffffu, lim >= NC);
+            if (C::NB == 1 && j > 0) add_output(j - 1);  // its product is done before S_j begins: taken while S_j is computed
+            const uint32_t s_addr = lane_base + C::S_COL + (uint32_t)(j % C::NB) * T + wg * HC;  // and 64 columns further for the second half
+            const int lim = n_row - j * T - wg * HC;  // visible columns from there on
+            const bool whole = __all_sync(0xffffffffu, lim >= 64 + HC);
             float mx = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < NC / 32; ++g) {
-                float s[32];
-                tc::ld32(s_addr + 32 * g, s);
+            for (int half = 0; half < 2; ++half) {
+                await(s_full(j, half), j >> 1);
+                tc::fence_after();
+                float s[HC];
+                tc::ldn(s_addr + 64 * half, s);
                 if (whole) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
+                    for (int e = 0; e < HC; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, 32 * g + e < lim ? s[e] : -INFINITY);
+                    for (int e = 0; e < HC; ++e) mx = fmaxf(mx, 64 * half + e < lim ? s[e] : -INFINITY);
                 }
             }
             float* const row_max = shared_f + (j & 1) * (C::WGS * 128) + row;
@@ -379,39 +400,55 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             // From 2^22 on the rounding of m, which an exact s c would leave in P, matters: there s c is rounded like m was.
             const bool plain = __all_sync(0xffffffffu, whole && fabsf(base) < 4194304.f);
             uint64_t sum2 = 0;
+            auto hand_over = [&](int half) {
+                tc::st_wait();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(j, half));
+            };
+            if (plain) {  // two loops: a choice inside would cost every element its instructions
 #pragma unroll
-            for (int g = 0; g < NC / GW; ++g) {
-                float s[GW];  // loaded again: with the sums of O the registers do not hold all columns
-                tc::ldn(s_addr + GW * g, s);
+                for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                for (int e = 0; e < GW; e += 2) {
-                    float x, y;
-                    if (plain) {
-                        tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
-                    } else {
-                        x = __fadd_rn(__fmul_rn(s[e], c), base);
-                        y = __fadd_rn(__fmul_rn(s[e + 1], c), base);
+                    for (int g = 0; g < HC / GW; ++g) {
+                        float s[GW];  // loaded again: with the sums of O the registers do not hold all columns
+                        tc::ldn(s_addr + 64 * half + GW * g, s);
+#pragma unroll
+                        for (int e = 0; e < GW; e += 2) {
+                            float x, y;
+                            tc::unpack2(tc::fma2(tc::pack2(s[e], s[e + 1]), c2, b2), x, y);
+                            s[e] = tc::ex2(x);
+                            s[e + 1] = tc::ex2(y);
+                            sum2 = tc::add2(sum2, tc::pack2(s[e], s[e + 1]));
+                        }
+                        tc::st_split(s_addr + 64 * half + GW * g, s);  // over the scores that they come from
                     }
-                    x = tc::ex2(x);
-                    y = tc::ex2(y);
-                    if (!plain) {
-                        x = GW * g + e < lim ? x : 0.f;
-                        y = GW * g + e + 1 < lim ? y : 0.f;
-                    }
-                    sum2 = tc::add2(sum2, tc::pack2(x, y));
-                    s[e] = x;
-                    s[e + 1] = y;
+                    hand_over(half);
                 }
-                tc::st_split(s_addr + GW * g, s);  // over the scores that they come from
+            } else {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll 1
+                    for (int g = 0; g < HC / GW; ++g) {
+                        const int col = 64 * half + GW * g;
+                        float s[GW];
+                        tc::ldn(s_addr + col, s);
+#pragma unroll
+                        for (int e = 0; e < GW; ++e) {
+                            const float x = tc::ex2(__fadd_rn(__fmul_rn(s[e], c), base));
+                            s[e] = col + e < lim ? x : 0.f;
+                        }
+#pragma unroll
+                        for (int e = 0; e < GW; e += 2) sum2 = tc::add2(sum2, tc::pack2(s[e], s[e + 1]));
+                        tc::st_split(s_addr + col, s);
+                    }
+                    hand_over(half);
+                }
             }
-            tc::st_wait();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(j));
             float x, y;
             tc::unpack2(sum2, x, y);
             l = fmaf(l, shrink_next, x + y);
-            if (j > 0) add_output(j - 1);  // the tile before: its product ran meanwhile
+            if (C::NB == 2 && j > 0) add_output(j - 1);  // the tile before: its product ran meanwhile
             shrink = shrink_next;
             v_inv = v_next;
         }
