@@ -185,12 +185,11 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
                 for (int c = 0; c < DP / 64; ++c) tc::mma4_ts<8, tc::STEP_K>(d, x + 32 * c, tc::desc_k(hi + c * T * 128), ID_S, false);
             };
             int s_slot = 0, s_phase = 0;  // of the next S
+            auto arrived = [&]() { return wait(full(s_slot), s_phase); };  // asked before the wait that ends last: one that is over costs its latency too
             auto scores = [&](int j) {
-                if (!wait(full(s_slot), s_phase)) return false;
                 tc::fence_after();
                 over_columns(tm + C::S_COL + (uint32_t)(j % NB) * T, tm, stages + s_slot * C::STAGE);
                 tc::commit(s_full(j));
-                return true;
             };
             auto grads = [&](int j) {  // dP_j; its tile has arrived: S_j was issued before
                 const uint32_t hi = stages + s_slot * C::STAGE + 2 * C::PLANE, d = tm + C::P_COL + (uint32_t)(j % NB) * T;
@@ -221,8 +220,8 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
             // something that is done while another product runs: S for P_j v (dkv) or for S_j's readers (dq), dP for the products of dS_j.
             bool ok = true;
             for (int j = 0; ok && j < min(tiles, NB); ++j) {
-                ok = scores(j);
-                if (ok) grads(j);
+                ok = arrived();
+                if (ok) { scores(j); grads(j); }
             }
             int slot = 0;  // of tile j
             for (int j = 0; ok && j < tiles; ++j) {
@@ -230,8 +229,9 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
                 const bool more = j + NB < tiles;
                 auto sums_taken = [&]() { return j == 0 || wait(acc_free(j - 1), (j - 1) >> 1); };
                 if (NB == 1 && !DKV && more) {  // one buffer: S_{j+1} runs while the warpgroups make dS_j
-                    ok = wait(s_read(j), j >> 1) && scores(j + 1);
+                    ok = arrived() && wait(s_read(j), j >> 1);
                     if (!ok) break;
+                    scores(j + 1);
                 }
                 if (DKV) {
                     ok = wait(p_full(j), j >> 1) && sums_taken();
@@ -248,9 +248,12 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
                 tc::commit(empty(slot));  // the tile is over
                 if (++slot == C::STAGES) slot = 0;
                 if (more) {
-                    if (DKV) ok = wait(pv_done, j) && scores(j + NB);  // P_j has been read
-                    else if (NB == 2) ok = scores(j + NB);             // S_j has, before dS_j was there
-                    ok = ok && wait(acc_full(j), j >> 1);              // dS_j has been read
+                    if (DKV || NB == 2) {  // P_j has been read (dkv), or S_j has, before dS_j was there
+                        ok = arrived() && (!DKV || wait(pv_done, j));
+                        if (!ok) break;
+                        scores(j + NB);
+                    }
+                    ok = wait(acc_full(j), j >> 1);  // dS_j has been read
                     if (!ok) break;
                     tc::fence_after();
                     grads(j + NB);
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
         };
         const uint64_t negm2 = tc::pack2(negm_row, negm_row);
         // columns u, u + 1 (of this thread's; info0: their rows' place in the tile): P, and its masking
-        auto prob2 = [&](const Tile& t, float x, float y, int u, int info0) {
+        auto prob2 = [&](const Tile& t, float x, float y, int u, int info0, bool whole) {
             uint64_t v;
             if (DKV) {
                 const float4 mi = *reinterpret_cast<const float4*>(t.info + 2 * info0);
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
                 tc::unpack2(v, x, y);
                 v = tc::pack2(tc::ex2(x), tc::ex2(y));
             }
-            if (!t.whole) {
+            if (!whole) {
                 tc::unpack2(v, x, y);
                 const float most = DKV ? 32768.f : 1.f;  // (a NaN stays)
                 x = (DKV ? u >= t.lim : u < t.lim) ? (x > most ? most : x) : 0.f;
@@ -405,8 +408,13 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_read(j));
             }
+            if (t.whole) {  // two loops: a choice inside would cost every element its instructions
 #pragma unroll
-            for (int u = 0; u < NC; u += 2) tc::unpack2(prob2(t, e[u], e[u + 1], u, NC * wg + u), e[u], e[u + 1]);
+                for (int u = 0; u < NC; u += 2) tc::unpack2(prob2(t, e[u], e[u + 1], u, NC * wg + u, true), e[u], e[u + 1]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < NC; u += 2) tc::unpack2(prob2(t, e[u], e[u + 1], u, NC * wg + u, false), e[u], e[u + 1]);
+            }
             if (DKV) {
                 tc::st_split(s_addr, e);
                 tc::st_wait();
@@ -460,20 +468,40 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
     }
 }
 
-// dk, dv (+)= the sums of the partial gradients of a group's heads, in order
+// dk, dv (+)= the sums of the partial gradients of a group's heads, in order.  A warp is a key; VEC: 16 bytes a lane.
+// Bound: HBM.  16 heads on 4, 4001 keys, dim 128: 65 MB read.
+template <bool VEC>
 __global__ void __launch_bounds__(256) attn_fold_kernel(const float* dk_part, const float* dv_part, const TenmoAttnParams a) {
-    const int group = a.H / a.Hkv;
-    const int64_t total = (int64_t)a.B * a.Hkv * a.Sk * a.D, per_head = (int64_t)a.Sk * a.D;
-    const float* part = blockIdx.y ? dv_part : dk_part;
+    const int group = a.H / a.Hkv, lane = threadIdx.x & 31;
+    const int64_t per_head = (int64_t)a.Sk * a.D;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= (int64_t)a.B * a.Hkv * a.Sk) return;
+    const int64_t bh = row / a.Sk, j = row - bh * a.Sk;
+    const int b = (int)(bh / a.Hkv), kvh = (int)(bh % a.Hkv);
+    const float* src = (blockIdx.y ? dv_part : dk_part) + ((int64_t)b * a.H + (int64_t)kvh * group) * per_head + j * a.D;
     const TenmoHeadsView& out = blockIdx.y ? a.dv : a.dk;
-    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t bh = e / per_head, at = e % per_head;
-        const int b = (int)(bh / a.Hkv), kvh = (int)(bh % a.Hkv);
-        const float* src = part + ((int64_t)b * a.H + (int64_t)kvh * group) * per_head + at;
-        float s = 0.f;
-        for (int g = 0; g < group; ++g) s += __ldg(src + g * per_head);
-        float* dst = out.ptr + b * out.sb + kvh * out.sh + (at / a.D) * out.sr + at % a.D;
-        *dst = a.beta != 0.f ? *dst + s : s;
+    float* dst = out.ptr + b * out.sb + kvh * out.sh + j * out.sr;
+    if (VEC) {
+        const int d = 4 * lane;  // D <= 128: one step
+        if (d >= a.D) return;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int g = 0; g < group; ++g) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(src + g * per_head + d));
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        if (a.beta != 0.f) {
+            const float4 o = *reinterpret_cast<const float4*>(dst + d);
+            s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+        }
+        *reinterpret_cast<float4*>(dst + d) = s;
+    } else {
+        for (int d = lane; d < a.D; d += 32) {
+            float s = 0.f;
+#pragma unroll 4
+            for (int g = 0; g < group; ++g) s += __ldg(src + g * per_head + d);
+            dst[d] = a.beta != 0.f ? dst[d] + s : s;
+        }
     }
 }
 
@@ -560,8 +588,9 @@ int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     p.out2_vec = tenmo_attn_row_vec(p.out2, a.D);
     if ((st = dp == 64 ? launch<64, true>(ctx, p) : launch<128, true>(ctx, p)) != TENMO_OK) return st;
     if (grouped) {
-        const dim3 grid((unsigned)tenmo_stream_grid(ctx, (int64_t)a.B * a.Hkv * a.Sk * a.D, 1024, 8), 2);
-        attn_fold_kernel<<<grid, 256, 0, ctx->stream>>>(pk, pv, a);
+        const dim3 grid((unsigned)(((int64_t)a.B * a.Hkv * a.Sk + 7) / 8), 2);
+        if (tenmo_attn_row_vec(a.dk, a.D) && tenmo_attn_row_vec(a.dv, a.D)) attn_fold_kernel<true><<<grid, 256, 0, ctx->stream>>>(pk, pv, a);
+        else attn_fold_kernel<false><<<grid, 256, 0, ctx->stream>>>(pk, pv, a);
         TENMO_LAUNCH_CHECK(ctx, "attn_fold_kernel");
     }
     return TENMO_OK;
