@@ -124,10 +124,10 @@ __device__ __forceinline__ void tenmo_grid_dependency_sync() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel in the stream may start launching
 }
 template <typename... KArgs, typename... Args>
-static inline cudaError_t tenmo_launch(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+static inline cudaError_t tenmo_launch(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s,
                                        bool pdl, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

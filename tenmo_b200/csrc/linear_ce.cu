@@ -414,13 +414,14 @@ int lce_run_few(tenmo_ctx* ctx, const LceCall& c) {
     float* partial = (float*)((char*)ws + p_at);
     TENMO_CUDA_TRY(ctx, tenmo_launch(lce_count_kernel, 1, 1024, 0, ctx->stream, ctx->pdl, c.labels, c.is_i64, c.N, c.ignore, c.reduction, c.valid, factor));
     TENMO_LAUNCH_CHECK(ctx, "lce_count_kernel");
-    lce_rows_kernel<<<tenmo_stream_grid(ctx, c.N * c.D, 256, 8), 256, 0, ctx->stream>>>(c.x->ptr + c.x->offset, c.x->row_stride, c.x->col_stride, c.labels,
-                                                                                       c.is_i64, c.ignore, 0, c.N, c.D, x);
+    const int rows_grid = tenmo_stream_grid(ctx, c.N * c.D, 256, 8);
+    TENMO_CUDA_TRY(ctx, tenmo_launch(lce_rows_kernel, rows_grid, 256, 0, ctx->stream, tenmo_pdl_ok(ctx, rows_grid), c.x->ptr + c.x->offset, c.x->row_stride,
+                                     c.x->col_stride, c.labels, c.is_i64, c.ignore, (int64_t)0, c.N, c.D, x));
     TENMO_LAUNCH_CHECK(ctx, "lce_rows_kernel");
     st = tied ? tenmo_few_dot(ctx, x, c.D, c.N, c.D, w, ldw, c.V, c.bias, z, c.V, partial) : tenmo_few_cols(ctx, x, c.D, c.N, c.D, w, ldw, c.V, c.bias, z, c.V, partial);
     if (st != TENMO_OK) return st;
     const LceRow p{z, c.labels, row_loss, c.upstream, factor, ctx->dev_status, 0, c.V, c.ignore, c.ls, c.is_i64, c.reduction, c.grad};
-    lce_row_kernel<<<(unsigned)c.N, c.V > 4096 ? 1024 : LCE_THREADS, 0, ctx->stream>>>(p);
+    TENMO_CUDA_TRY(ctx, tenmo_launch(lce_row_kernel, (unsigned)c.N, c.V > 4096 ? 1024 : LCE_THREADS, 0, ctx->stream, tenmo_pdl_ok(ctx, c.N), p));
     TENMO_LAUNCH_CHECK(ctx, "lce_row_kernel");
     if (c.grad) {
         st = tied ? tenmo_few_cols(ctx, z, c.V, c.N, c.V, w, ldw, c.D, nullptr, c.dx, c.D, partial) : tenmo_few_dot(ctx, z, c.V, c.N, c.V, w, ldw, c.D, nullptr, c.dx, c.D, partial);

@@ -297,7 +297,7 @@ int fold(tenmo_ctx* ctx, const FewArgs& p) {
 
 template <typename K>
 int launch(tenmo_ctx* ctx, K kernel, dim3 grid, const FewArgs& p, const char* name) {
-    kernel<<<grid, 32 * WARPS, 0, ctx->stream>>>(p);
+    TENMO_CUDA_TRY(ctx, tenmo_launch(kernel, grid, 32 * WARPS, 0, ctx->stream, tenmo_pdl_ok(ctx, (int64_t)grid.x * grid.y * grid.z), p));
     TENMO_LAUNCH_CHECK(ctx, name);
     return fold(ctx, p);
 }
@@ -341,7 +341,7 @@ int tenmo_few_outer(tenmo_ctx* ctx, const float* a, int64_t lda, const float* b,
         return TENMO_OK;
     }
     const int vec = C % 4 == 0 && ((uintptr_t)out & 15u) == 0;
-    few_outer_kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, ctx->stream>>>(a, lda, b, ldb, N, R, C, out, vec);
+    TENMO_CUDA_TRY(ctx, tenmo_launch(few_outer_kernel, dim3((unsigned)gx, (unsigned)gy), 256, 0, ctx->stream, tenmo_pdl_ok(ctx, gx * gy), a, lda, b, ldb, N, R, C, out, vec));
     TENMO_LAUNCH_CHECK(ctx, "few_outer_kernel");
     return TENMO_OK;
 }
