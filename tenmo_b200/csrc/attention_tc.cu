@@ -158,6 +158,7 @@ struct FwdParams {
     const float* k_inv; const float* v_inv;
     int tiles;    // tiles of a head of k
     int q_tiles;  // 128-row tiles of a head of q
+    TenmoAttnOrder order;
     int q_vec, o_vec;
     uint32_t* status;
 };
@@ -197,8 +198,9 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     const TenmoAttnParams& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the longest rows of a causal head first: the last tiles have the most keys
-    const int q_tile = p.q_tiles - 1 - (int)(blockIdx.x / ((unsigned)a.B * a.H));
-    const int bh = (int)(blockIdx.x % ((unsigned)a.B * a.H));
+    int q_tile, bh;
+    tenmo_attn_block(p.order, blockIdx.x, &q_tile, &bh);
+    q_tile = p.q_tiles - 1 - q_tile;
     const int h = bh % a.H, b = bh / a.H, kvh = h / (a.H / a.Hkv);
     const int q_rows = tenmo_attn_rows(a.q_lengths, b, a.Sq), keys = tenmo_attn_rows(a.k_lengths, b, a.Sk);
     // keys that the last row of the tile that takes part sees
@@ -207,6 +209,16 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     if (a.causal) seen = min(seen, max(0, last + a.Sk - a.Sq + 1));
     const int n_tiles = (seen + T - 1) / T;
     const int64_t tile0 = ((int64_t)b * a.Hkv + kvh) * p.tiles;
+    if (n_tiles == 0) {  // rows behind the length, or none with a visible key
+        const int row0 = q_tile * ROWS;
+        tenmo_attn_zero_rows<DP>(a.o.ptr + b * a.o.sb + h * a.o.sh, a.o.sr, row0, a.Sq, a.D, p.o_vec);
+        if (a.stats && threadIdx.x < ROWS && row0 + (int)threadIdx.x < a.Sq) {
+            float* st = a.stats + (((int64_t)b * a.H + h) * a.Sq + row0 + threadIdx.x) * 2;
+            st[0] = -INFINITY;
+            st[1] = 0.f;
+        }
+        return;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -539,6 +551,7 @@ int tenmo_attn_tc_fwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     p.status = ctx->dev_status;
     const int64_t n = (int64_t)a.B * a.Hkv * p.tiles;
     const size_t img = align_up((size_t)n * T * dp * 4), inv = align_up((size_t)n * sizeof(float));
+    p.order = tenmo_attn_order(a, p.q_tiles, 2 * img);
     void* ws = nullptr;
     int st = tenmo_op_workspace(ctx, 2 * (img + inv), &ws);
     if (st != TENMO_OK) return st;

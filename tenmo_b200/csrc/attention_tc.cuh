@@ -36,6 +36,23 @@ struct TenmoTileJobs {
 int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, int dp, int tile_rows);  // 64 or 128 (without row numbers)
 void tenmo_attn_causal_keys(const TenmoAttnParams& a, TenmoTileJob* j);  // fills seen_by and so on of a job of k or v
 bool tenmo_attn_row_vec(const TenmoHeadsView& v, int D);
+
+// Order of the blocks: heads in groups whose images fit into half of L2, so that a head's tiles are read again while L2 holds them (one
+// group over 384 heads of 512x64, 100 MB, read 437 MB from HBM, two read 192 MB and took 125 us for 131); within a group tile by tile, so
+// that the long ones of a causal head start first.  Smaller groups than that end unevenly: 16 heads of 4001x128 causal, 64 MB, took 191 us
+// in one group and 204 in two.
+struct TenmoAttnOrder { unsigned heads, group; int tiles; };
+constexpr int64_t TENMO_ATTN_GROUP_BYTES = (int64_t)64 << 20;
+static inline TenmoAttnOrder tenmo_attn_order(const TenmoAttnParams& a, int tiles, size_t image_bytes) {
+    const int64_t heads = (int64_t)a.B * a.H, most = ((int64_t)image_bytes + TENMO_ATTN_GROUP_BYTES - 1) / TENMO_ATTN_GROUP_BYTES;
+    const int64_t groups = most < 1 ? 1 : most < heads ? most : heads;
+    return TenmoAttnOrder{(unsigned)heads, (unsigned)((heads + groups - 1) / groups), tiles};
+}
+__device__ __forceinline__ void tenmo_attn_block(const TenmoAttnOrder& o, unsigned block, int* tile, int* head) {
+    const unsigned first = block / (o.group * o.tiles) * o.group, in = block - first * o.tiles, heads = min(o.group, o.heads - first);
+    *tile = (int)(in / heads);
+    *head = (int)(first + in % heads);
+}
 static inline int tenmo_attn_padded(int D) { return D <= 64 ? 64 : 128; }
 
 // A warp's 32 rows x W columns between memory and one row per thread, through `scratch` (32 * W floats of the warp's own): the 16-byte
@@ -102,6 +119,26 @@ __device__ __forceinline__ void tenmo_attn_write_rows(const float (&x)[W], float
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (4 * q + u < cols) p[u] = add ? p[u] + f[u] : f[u];
+        }
+    }
+}
+
+// A block whose rows take no part: zeros in rows [row0, row0 + 128) of `rows`, by the whole block.
+template <int DP>
+__device__ __forceinline__ void tenmo_attn_zero_rows(float* head, int64_t stride, int row0, int rows, int D, bool vec) {
+    constexpr int Q = DP / 4;
+    const int n = min(128, rows - row0) * Q;
+    float* const first = head + row0 * stride;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < n; e += blockDim.x) {
+        const int d = 4 * (e % Q);
+        float* p = first + (e / Q) * stride + d;
+        if (vec) {
+            if (d < D) *reinterpret_cast<float4*>(p) = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (d + u < D) p[u] = 0.f;
         }
     }
 }

@@ -33,6 +33,7 @@ struct BwdParams {
     int tiles;           // tiles of a head of Y
     int q_info_tiles;    // 64-row tiles of a head of q
     int x_tiles;         // 128-row tiles of a head of X
+    TenmoAttnOrder order;
     TenmoHeadsView x1, x2, out1, out2;  // out1: dq or dk, out2: dv
     int x1_vec, x2_vec, out1_vec, out2_vec;
     float beta;
@@ -84,10 +85,10 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
 
     const TenmoAttnParams& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2, row = threadIdx.x & 127;
-    const unsigned heads = (unsigned)a.B * a.H;
     // causal: the last rows of q see the most keys, the first keys are seen by the most rows; those blocks start first
-    const int x_tile = DKV ? (int)(blockIdx.x / heads) : p.x_tiles - 1 - (int)(blockIdx.x / heads);
-    const int bh = (int)(blockIdx.x % heads);
+    int x_tile, bh;
+    tenmo_attn_block(p.order, blockIdx.x, &x_tile, &bh);
+    if (!DKV) x_tile = p.x_tiles - 1 - x_tile;
     const int h = bh % a.H, b = bh / a.H, kvh = h / (a.H / a.Hkv);
     const int q_rows = tenmo_attn_rows(a.q_lengths, b, a.Sq), keys = tenmo_attn_rows(a.k_lengths, b, a.Sk);
     const int off = a.Sk - a.Sq;  // causal: key j is visible to row i when j <= i + off
@@ -108,6 +109,13 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
     }
     const int yh = DKV ? h : kvh, y_heads = DKV ? a.H : a.Hkv;
     const int64_t tile0 = ((int64_t)b * y_heads + yh) * p.tiles + first;
+    if (n == 0) {  // nothing to add: rows (keys) behind the length, or none that sees (is seen by) another
+        if (p.beta == 0.f) {
+            tenmo_attn_zero_rows<DP>(p.out1.ptr + b * p.out1.sb + h * p.out1.sh, p.out1.sr, x_tile * ROWS, DKV ? a.Sk : a.Sq, a.D, p.out1_vec);
+            if (DKV) tenmo_attn_zero_rows<DP>(p.out2.ptr + b * p.out2.sb + h * p.out2.sh, p.out2.sr, x_tile * ROWS, a.Sk, a.D, p.out2_vec);
+        }
+        return;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -564,6 +572,7 @@ int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     p.y1_img = ik; p.y2_img = iv; p.y1_inv = vk; p.y2_inv = vv;
     p.tiles = k_tiles;
     p.x_tiles = (a.Sq + ROWS - 1) / ROWS;
+    p.order = tenmo_attn_order(a, p.x_tiles, 2 * k_img);
     p.x1 = a.q; p.x2 = a.go; p.out1 = a.dq; p.out2 = a.dq;
     p.x1_vec = tenmo_attn_row_vec(a.q, a.D); p.x2_vec = tenmo_attn_row_vec(a.go, a.D);
     p.out1_vec = p.out2_vec = tenmo_attn_row_vec(a.dq, a.D);
@@ -573,6 +582,7 @@ int tenmo_attn_tc_bwd(tenmo_ctx* ctx, const TenmoAttnParams& a) {
     p.y1_img = iq; p.y2_img = ig; p.y1_inv = vq; p.y2_inv = vg;
     p.tiles = q_tiles;
     p.x_tiles = (a.Sk + ROWS - 1) / ROWS;
+    p.order = tenmo_attn_order(a, p.x_tiles, 2 * q_img);
     p.x1 = a.k; p.x2 = a.v;
     p.x1_vec = tenmo_attn_row_vec(a.k, a.D); p.x2_vec = tenmo_attn_row_vec(a.v, a.D);
     if (grouped) {
