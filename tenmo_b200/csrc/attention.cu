@@ -69,6 +69,9 @@ __device__ __forceinline__ bool warp_row(int64_t rows_per_head, int heads, int64
 // Four warps take 32 keys (16 above 32 columns) in turn and are joined at the end; with few rows and many keys the keys are cut into slices, one block
 // each, which attn_join_kernel adds in order.
 // Bound: HBM for one token (k and v are read once, 16 bytes a lane), launch latency for the smallest calls.
+// Measured: 16 requests of one token, 16 heads on 4, dim 64, up to 4099 keys (97 MB): 34 us and 8 us to join, 2.8 TB/s: the chain of a step (dot
+// products, sums over the lanes, maximum, exponentials, weighted sum, some 2000 cycles) with 12 warps on an SM.  Loading a step ahead did
+// not help.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int FEW_WARPS = 4;
 struct FewParams {

