@@ -15,7 +15,8 @@
 // slices whose partial results a second kernel adds in order.
 // Bound: tensor pipe, 3 * 2 M N K flop.
 // Measured: 2048 x 65536 over 2048 (logits) 1.17 ms = 470 TFLOP/s of the product, 1410 of the pipe; over 65536 (gradient of x) 1.21 ms.  With a
-// contraction of 768 the epilogue's statistics and 256 KB of results per tile of six chunks leave the pipe 55 % busy (360 TFLOP/s).
+// contraction of 768 the epilogue's statistics and 256 KB of results per tile of six chunks show: 2048 x 32011 logits 243 us (415 TFLOP/s; 206 us
+// without storing them; 291 us when they went through shared memory and every element was asked for its column).
 #include <cuda.h>
 
 #include "gemm_h3.cuh"
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(512) h3_make_kernel(const float* src, int64_t 
             for (int e = 0; e < 8; ++e) x[s][e] = in && c0 + e < cols ? __ldg(p + e * cs) : 0.f;
         }
     }
-    tenmo_h3_write_block(x, img + block * H3_BLOCK_BYTES, inverse + block);
+    tenmo_h3_write_block(x, threadIdx.x >> 4, threadIdx.x & 15, img + block * H3_BLOCK_BYTES, inverse + block);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -123,7 +124,9 @@ __device__ __forceinline__ void h3_tile(int t, int tiles_m, int tiles_n, int* tm
     *tn = in / rows;
 }
 
-template <bool A_MN, bool B_MN>
+// STATS: the product goes with the softmax statistics (and blocked results); in a kernel of its own, since their registers cost the other
+// products 5 %.
+template <bool A_MN, bool B_MN, bool STATS>
 __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                              const __grid_constant__ H3Params p) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -217,13 +220,13 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
                 return mn ? tc::desc(plane + (uint32_t)k * 2048u, PLANE / 2, 1024u) : tc::desc(plane + (uint32_t)k * 32u, 16u, 1024u);
             };
             int stage = 0, acc = 0;
-            uint32_t phase = 0, acc_phase[2] = {0, 0};
+            uint32_t phase = 0, acc_phases = 0;  // a bit per accumulator (an array would live in local memory)
             bool ok = true;
             for (int64_t u = pair; ok && u < units; u += pairs) {
                 int tm, tn, c0, c1;
                 range(u, &tm, &tn, &c0, &c1);
                 for (int c = c0; ok && c < c1; ++c) {
-                    if (!mbar_wait(tempty(acc), acc_phase[acc] ^ 1u, abort_flag)) { ok = false; break; }
+                    if (!mbar_wait(tempty(acc), ((acc_phases >> acc) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                     tc::fence_after();
                     const uint32_t d = tmem + (uint32_t)acc * 256u;
                     for (int h = 0; h < 2; ++h) {
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
                     }
                     if (!ok) break;
                     commit_pair(tfull(acc));
-                    acc_phase[acc] ^= 1u;
+                    acc_phases ^= 1u << acc;
                     acc ^= 1;
                 }
             }
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
         float* const stage_buf = staging + ew * (32 * ST_LD);
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * 64);
         int acc = 0;
-        uint32_t acc_phase[2] = {0, 0};
+        uint32_t acc_phases = 0;  // a bit per accumulator
         bool ok = true;
         for (int64_t u = pair; ok && u < units; u += pairs) {
             int tm, tn, c0, c1;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
 #pragma unroll
             for (int e = 0; e < 64; ++e) s[e] = 0.f;
             for (int c = c0; c < c1; ++c) {
-                ok = __all_sync(0xffffffffu, mbar_wait(tfull(acc), acc_phase[acc], abort_flag));
+                ok = __all_sync(0xffffffffu, mbar_wait(tfull(acc), (acc_phases >> acc) & 1u, abort_flag));
                 if (!ok) break;
                 tc::fence_after();
                 const float f = __ldg(p.a_inv + (A_MN ? (int64_t)c * p.a_cb + mb : (int64_t)mb * p.a_cb + c)) *
@@ -284,42 +287,58 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_cluster(in_leader(tempty(acc)));
-                acc_phase[acc] ^= 1u;
+                acc_phases ^= 1u << acc;
                 acc ^= 1;
             }
             if (!ok) break;
             const int64_t m0 = (int64_t)tm * 256 + rank * 128 + quarter * 32, n0 = (int64_t)tn * 256 + group * 64;
             if (m0 >= p.M || n0 >= p.N) continue;  // uniform over the warp
             // element (row, column) of this warp's part at C[row * ldc + column]
-            float* C = p.e.C ? p.e.C + m0 * p.e.ldc + n0 : nullptr;
+            float* C = p.e.C + m0 * p.e.ldc + n0;
             int64_t ldc = p.e.ldc;
             bool add = p.e.add != 0, vec = p.vec != 0;
-            if (p.slices > 1) {
+            if (!STATS && p.slices > 1) {
                 C = p.partial + ((u % p.slices) * p.M + m0) * p.ldp + n0;
                 ldc = p.ldp;
                 add = false;
                 vec = true;
-            } else {
-                if (p.e.blocked && C) {
-                    C = p.e.C + ((int64_t)(2 * tm + rank) * p.b_nb + 2 * tn + (group >> 1)) * (H3_BLOCK * H3_BLOCK) + quarter * 32 * H3_BLOCK + (group & 1) * 64;
-                    ldc = H3_BLOCK;
-                    vec = true;
-                }
+            }
+            if (STATS) {
                 if (p.e.bias) {
 #pragma unroll
                     for (int e = 0; e < 64; ++e) s[e] += n0 + e < p.N ? __ldg(p.e.bias + n0 + e) : 0.f;
                 }
-                if (p.e.stats) {
+                {
                     const int64_t m = m0 + lane;
                     const int cols = (int)min((int64_t)64, p.N - n0);
                     float mx = -INFINITY, sum = 0.f, all = 0.f;
+                    if (cols == 64) {  // apart from the ragged edge, where every element is asked for
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) mx = fmaxf(mx, e < cols ? s[e] : -INFINITY);
+                        for (int e = 0; e < 64; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[e], s[e + 1]), fmaxf(s[e + 2], s[e + 3])));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, e < cols ? s[e] : -INFINITY);
+                    }
                     const float base = mx == -INFINITY ? 0.f : mx;
+                    if (cols == 64) {
+                        const uint64_t nb2 = tc::pack2(-base, -base), l2 = tc::pack2(1.44269504088896341f, 1.44269504088896341f);
+                        uint64_t sum2 = 0;
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
-                        sum += e < cols ? tc::ex2((s[e] - base) * 1.44269504088896341f) : 0.f;
-                        all += e < cols ? s[e] : 0.f;
+                        for (int e = 0; e < 64; e += 2) {  // the difference first: it is exact where it matters
+                            float x, y;
+                            tc::unpack2(tc::mul2(tc::add2(tc::pack2(s[e], s[e + 1]), nb2), l2), x, y);
+                            sum2 = tc::add2(sum2, tc::pack2(tc::ex2(x), tc::ex2(y)));
+                        }
+                        float x, y;
+                        tc::unpack2(sum2, x, y);
+                        sum = x + y;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) sum += e < cols ? tc::ex2((s[e] - base) * 1.44269504088896341f) : 0.f;
+                    }
+                    if (p.e.sums) {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) all += e < cols ? s[e] : 0.f;
                     }
                     if (m < p.M) {
                         const int64_t at = (n0 >> 6) * p.M + m;
@@ -335,7 +354,16 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
                     }
                 }
             }
-            if (!C) continue;
+            if (STATS) {  // blocks, or nothing
+                if (p.e.C) {
+                    float* out = p.e.C + ((int64_t)(2 * tm + rank) * p.b_nb + 2 * tn + (group >> 1)) * (H3_BLOCK * H3_BLOCK);
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        *reinterpret_cast<float4*>(out + tenmo_h3_patch(quarter * 32 + lane, (group & 1) * 16 + q)) =
+                            make_float4(s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]);
+                }
+                continue;
+            }
             // out through the warp's staging block, 16 columns at a time: 16-byte chunk q of row r at chunk q ^ ((r >> 1) & 3); a warp-wide
             // store then covers eight rows of 64 contiguous bytes
             const int q = lane & 3, sub = lane >> 2;
@@ -456,7 +484,9 @@ int tenmo_h3_gemm(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, const TenmoH3
     p.vec = e.ldc % 4 == 0 && ((uintptr_t)e.C & 15u) == 0;
     p.chunks = (int)((K + 127) / 128);
     p.tiles_m = (int)((M + 255) / 256); p.tiles_n = (int)((N + 255) / 256);
-    const bool plain = !e.stats && !e.bias;
+    const bool plain = !e.stats;
+    if (plain && (e.bias || e.blocked || !e.C)) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "h3_gemm: a bias and blocks go with the statistics");
+    if (!plain && (!e.at_label || !e.labels || (e.C && !e.blocked) || a_rows_are_k)) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "h3_gemm: this epilogue is not built");
     p.slices = plain && partial ? pick_slices(ctx, M, N, K) : 1;
     p.partial = (float*)partial;
     p.ldp = (N + 3) / 4 * 4;
@@ -487,7 +517,8 @@ int tenmo_h3_gemm(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, const TenmoH3
         return TENMO_OK;
     };
     if (a_rows_are_k && !b_rows_are_k) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "h3_gemm: this pair of layouts is not built");
-    st = a_rows_are_k ? go(h3_gemm_kernel<true, true>) : b_rows_are_k ? go(h3_gemm_kernel<false, true>) : go(h3_gemm_kernel<false, false>);
+    if (plain) st = a_rows_are_k ? go(h3_gemm_kernel<true, true, false>) : b_rows_are_k ? go(h3_gemm_kernel<false, true, false>) : go(h3_gemm_kernel<false, false, false>);
+    else st = b_rows_are_k ? go(h3_gemm_kernel<false, true, true>) : go(h3_gemm_kernel<false, false, true>);
     if (st != TENMO_OK) return st;
     if (p.slices > 1) {
         h3_fold_kernel<<<tenmo_stream_grid(ctx, M * (p.ldp / 4), 256 * 2, 8), 256, 0, ctx->stream>>>(p.partial, p.slices, M, N, p.ldp, e.C, e.ldc, e.add);

@@ -25,7 +25,9 @@ int tenmo_h3_make(tenmo_ctx* ctx, const float* src, int64_t rs, int64_t cs, cons
 struct TenmoH3Epilogue {
     float* C;            // result, leading dimension ldc, or NULL (statistics only)
     int64_t ldc;
-    int blocked;         // C is stored as 128 x 128 blocks, row-major over the blocks (ldc unused): an operand image can replace it
+    // C is stored as 128 x 128 blocks (ldc unused), row-major over the blocks, each as tenmo_h3_patch says: an operand image can replace it.
+    // Blocks are written whole; what lies past M or N in them is unspecified.
+    int blocked;
     int add;             // C += product
     const float* bias;   // N floats added to every row, or NULL
     // softmax statistics of the rows (stats != NULL): for every row and 64-column group g, at [g * M + row]: the maximum and the
@@ -42,12 +44,16 @@ size_t tenmo_h3_partial_bytes(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_
 int tenmo_h3_gemm(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, const TenmoH3Operand& A, bool a_rows_are_k, const TenmoH3Operand& B,
                   bool b_rows_are_k, const TenmoH3Epilogue& e, void* partial);
 
+// Place (in floats) of columns [4 q, 4 q + 4) of row r in a block of logits: 32 rows x 64 columns are contiguous, and of those the 32 rows of four
+// columns, which is how a warp of the epilogue (a row per lane) holds them: its stores need no staging.
+__device__ __forceinline__ int tenmo_h3_patch(int r, int q) { return ((((r >> 5) * 2 + (q >> 4)) * 16 + (q & 15)) * 32 + (r & 31)) * 4; }
+
 __device__ __forceinline__ int64_t tenmo_h3_label(const void* labels, int is_i64, int64_t n) {
     return is_i64 ? __ldg((const long long*)labels + n) : (int64_t)__ldg((const int*)labels + n);
 }
 
-// Splits the 128 x 128 values that the block's 512 threads hold (thread t: rows t / 16 + 32 s, columns 8 (t % 16) ..) into img.
-__device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[4][8], uint8_t* img, float* inverse) {
+// Splits the 128 x 128 values that the block's 512 threads hold (a thread: rows row + 32 s, columns 8 c ..) into img.
+__device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[4][8], int row, int c, uint8_t* img, float* inverse) {
     __shared__ float largest[16];
     float mx = 0.f;
 #pragma unroll
@@ -69,10 +75,9 @@ __device__ __forceinline__ void tenmo_h3_write_block(const float (&x)[4][8], uin
     float inv;
     const float scale = tc::block_scale(mx, &inv);
     if (threadIdx.x == 0) *inverse = inv;
-    const int c = threadIdx.x & 15;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        const int r = (threadIdx.x >> 4) + 32 * s;
+        const int r = row + 32 * s;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) tc::split_rounded(x[s][2 * e] * scale, x[s][2 * e + 1] * scale, hi[e], lo[e]);

@@ -191,10 +191,11 @@ __global__ void __launch_bounds__(32 * LCE_STAT_WARPS) lce_stats_kernel(const Lc
 // The logits of a 128 x 128 block become the gradient, as an operand image in their place, and its column sums per block row.
 __global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* inverse, const float4* numbers, const void* labels, int is_i64,
                                                        int64_t row0, int64_t rows, int64_t V, int block_cols, float ls, float* db_part) {
-    __shared__ float sums[32][H3_BLOCK];
+    __shared__ float sums[32][H3_BLOCK + 1];  // + 1: the eight rows of a warp in different banks
     const int64_t block = blockIdx.x;
     const int64_t r0 = block / block_cols * H3_BLOCK, c0 = block % block_cols * H3_BLOCK;
-    const int c = 8 * (threadIdx.x & 15);
+    // a warp takes 8 rows x 32 columns: 128 contiguous bytes of each four columns (tenmo_h3_patch)
+    const int row = (threadIdx.x & 7) + 8 * (threadIdx.x >> 7), c = 8 * ((threadIdx.x >> 3) & 15);
     const float* src = reinterpret_cast<const float*>(z + block * H3_BLOCK_BYTES);
     const float smooth = ls / (float)V;
     const int cols = (int)min((int64_t)8, V - c0 - c);  // of this thread that exist
@@ -202,9 +203,9 @@ __global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* invers
     float4 num[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {  // all loads first; a row that takes no part has u = 0 and its logits are not looked at
-        const int lr = (threadIdx.x >> 4) + 32 * s;
+        const int lr = row + 32 * s;
         num[s] = r0 + lr < rows ? __ldg(numbers + r0 + lr) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c), b = *reinterpret_cast<const float4*>(src + lr * H3_BLOCK + c + 4);
+        const float4 a = *reinterpret_cast<const float4*>(src + tenmo_h3_patch(lr, c >> 2)), b = *reinterpret_cast<const float4*>(src + tenmo_h3_patch(lr, (c >> 2) + 1));
         x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
         x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
     }
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* invers
     for (int e = 0; e < 8; ++e) col[e] = 0.f;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        const int64_t r = r0 + (threadIdx.x >> 4) + 32 * s;
+        const int64_t r = r0 + row + 32 * s;
         if (num[s].w == 0.f) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* invers
     }
     if (db_part) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 4][c + e] = col[e];
+        for (int e = 0; e < 8; ++e) sums[row][c + e] = col[e];
         __syncthreads();
         if (threadIdx.x < H3_BLOCK && c0 + threadIdx.x < V) {
             float t = 0.f;
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* invers
         }
     }
     // every thread's logits are in registers (the barrier inside) before the image is written over them
-    tenmo_h3_write_block(x, z + block * H3_BLOCK_BYTES, inverse + block);
+    tenmo_h3_write_block(x, row, c >> 3, z + block * H3_BLOCK_BYTES, inverse + block);
 }
 
 // loss from the row losses, added in a fixed order (double: the mean of many rows keeps the bits of each)
