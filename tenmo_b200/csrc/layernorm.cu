@@ -165,8 +165,11 @@ struct LnBwd {
     int64_t ldx, M; int C; float inv_c; int add;
 };
 
-template <bool VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : LN_MAX_THREADS) ln_bwd_kernel(const LnBwd p) {
+// MOST: threads of a block.  Scalar loads need more registers than 1024 threads leave (their addresses), so rows of up to 4096 have a
+// kernel for 512 threads.
+template <bool VEC, int MOST>
+__global__ void __launch_bounds__(MOST, 1) ln_bwd_kernel(const LnBwd p) {
+    constexpr bool WARP = MOST == 128;
     __shared__ float2 slots[2][32];
     extern __shared__ float fold[];  // WARP: one row pair of partials per block
     tenmo_grid_dependency_sync();
@@ -184,17 +187,19 @@ __global__ void __launch_bounds__(WARP ? 128 : LN_MAX_THREADS) ln_bwd_kernel(con
         next_mean = __ldg(p.mean + m);
         next_rstd = __ldg(p.rstd + m);
     };
-    if (first < p.M) fetch(first);
+    constexpr bool AHEAD = VEC || MOST < LN_MAX_THREADS;  // a row ahead, where the registers allow it
+    if (AHEAD && first < p.M) fetch(first);
     int flip = 0;
     for (int64_t m = first; m < p.M; m += step) {
         float v[LN_EPT], g[LN_EPT];
+        if (!AHEAD) fetch(m);
 #pragma unroll
         for (int e = 0; e < LN_EPT; ++e) {
             v[e] = next_x[e];
             g[e] = next_g[e];
         }
         const float mean = next_mean, rstd = next_rstd;
-        if (m + step < p.M) fetch(m + step);
+        if (AHEAD && m + step < p.M) fetch(m + step);
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int e = 0; e < LN_EPT; ++e) {
@@ -359,8 +364,8 @@ int tenmo_layernorm_bwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const f
     if (wide) {
         ln_bwd_wide_kernel<<<grid, block, 0, ctx->stream>>>(p);
     } else {
-        auto kernel = vec ? (warp ? ln_bwd_kernel<true, true> : ln_bwd_kernel<true, false>)
-                          : (warp ? ln_bwd_kernel<false, true> : ln_bwd_kernel<false, false>);
+        auto kernel = vec ? (warp ? ln_bwd_kernel<true, 128> : ln_bwd_kernel<true, LN_MAX_THREADS>)
+                          : (warp ? ln_bwd_kernel<false, 128> : block <= 512 ? ln_bwd_kernel<false, 512> : ln_bwd_kernel<false, LN_MAX_THREADS>);
         const size_t smem = warp ? 2 * (size_t)C * sizeof(float) : 0;
         TENMO_CUDA_TRY(ctx, tenmo_launch(kernel, grid, block, smem, ctx->stream, tenmo_pdl_ok(ctx, grid), p));
     }

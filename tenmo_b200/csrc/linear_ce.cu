@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(32 * LCE_STAT_WARPS) lce_stats_kernel(const Lc
 }
 
 // The logits of a 128 x 128 block become the gradient, as an operand image in their place, and its column sums per block row.
-__global__ void __launch_bounds__(512) lce_grad_kernel(uint8_t* z, float* inverse, const float4* numbers, const void* labels, int is_i64,
+// Two blocks on an SM (64 registers): one's loads run beside the other's stores.
+__global__ void __launch_bounds__(512, 2) lce_grad_kernel(uint8_t* z, float* inverse, const float4* numbers, const void* labels, int is_i64,
                                                        int64_t row0, int64_t rows, int64_t V, int block_cols, float ls, float* db_part) {
     __shared__ float sums[32][H3_BLOCK + 1];  // + 1: the eight rows of a warp in different banks
     const int64_t block = blockIdx.x;
