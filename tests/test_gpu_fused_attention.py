@@ -311,6 +311,28 @@ def test_accumulates_and_repeats(size):
         assert torch.equal(added[name], 2 * first[name])
 
 
+@pytest.mark.parametrize("D,H,Hkv", [(64, 4, 1), (66, 6, 2), (128, 4, 4), (33, 4, 2)])
+def test_accumulates_on_a_padded_batch(D, H, Hkv):
+    """beta = 1 where whole tiles take no part (what is there stays), one head or several per key/value head, aligned rows and others."""
+    gen = torch.Generator(device="cuda").manual_seed(26)
+    q, go = (_make(gen, 4, H, 300, D) for _ in range(2))
+    k, v = (_make(gen, 4, Hkv, 280, D) for _ in range(2))
+    mask = dict(q_lengths=ints([300, 100, 0, 257]), k_lengths=ints([280, 3, 140, 0]))
+    first = run(q, k, v, go, **mask)
+    start = [_make(gen, *t.shape) for t in (q, k, v)]
+    added = run(q, k, v, go, beta=1.0, into=[t.clone() for t in start], **mask)
+    for name, t in zip(("dq", "dk", "dv"), start):
+        assert torch.equal(added[name], t + first[name])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_heads_in_groups(causal):
+    """So many heads that their tile images (105 MB) are worked on in two groups, of 161 and 160."""
+    gen = torch.Generator(device="cuda").manual_seed(27)
+    q, k, v, go = (_make(gen, 107, 3, 520, 40) for _ in range(4))
+    compare(q, k, v, go, causal=causal)
+
+
 @pytest.mark.parametrize("size", [24, 200])
 def test_gradients_against_differences(size):
     """Central differences of sum(go * o) in 64 bits of the formula, along random directions, against the kernel's gradients."""
