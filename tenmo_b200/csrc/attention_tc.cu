@@ -220,23 +220,6 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
         return;
     }
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int w = 0; w < 2; ++w) {
-            for (int half = 0; half < 2; ++half) { mbar_init(s_full(w, half), 1); mbar_init(p_full(w, half), 4 * C::WGS); }
-            mbar_init(o_full(w), 1);
-        }
-        mbar_init(o_free, 4 * C::WGS);
-        mbar_init(drain, 1);
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == C::ISSUER) tc::alloc(tmem_slot, C::TMEM);
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    const uint32_t tmem = *tmem_slot;
-
     // The ring (one thread): tiles in the order in which the products use them, each as soon as its slot's last product is done.
     // One S buffer: k_0, v_0, k_1, v_1, ...; two: k_0, k_1, v_0, k_2, v_1, ..., v_{n-1}.
     int fetched = 0, fetch_slot = 0, fetch_round = 0;
@@ -251,7 +234,30 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
             if (++fetch_slot == SLOTS) { fetch_slot = 0; ++fetch_round; }
         }
     };
-    if (threadIdx.x == 32 * C::LOADER) fetch(min(2 * n_tiles, SLOTS - 1));  // the last slot is scratch for now
+    if (threadIdx.x == 32 * C::LOADER) {  // the thread that copies: the first tiles are on their way before the block meets
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int w = 0; w < 2; ++w) {
+            for (int half = 0; half < 2; ++half) { mbar_init(s_full(w, half), 1); mbar_init(p_full(w, half), 4 * C::WGS); }
+            mbar_init(o_full(w), 1);
+        }
+        mbar_init(o_free, 4 * C::WGS);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::fence_proxy_async();
+        fetch(min(2 * n_tiles, SLOTS - 1));  // the last slot is scratch for now
+    }
+
+    float x[C::W];  // q
+    if (warp < C::ISSUER)
+        tenmo_attn_fetch<DP, C::WGS>(x, a.q.ptr + b * a.q.sb + h * a.q.sh + (int64_t)q_tile * ROWS * a.q.sr, a.q.sr, q_rows - q_tile * ROWS, p.q_vec, a.D,
+                                     reinterpret_cast<float*>(smem + (SLOTS - 1) * C::IMG));
+
+    if (warp == C::ISSUER) tc::alloc(tmem_slot, C::TMEM);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_slot;
 
     // ---- q into tensor memory ----
     const int wg = warp >> 2, row = threadIdx.x & 127;
@@ -259,9 +265,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float q_inv = 1.f;
     if (warp < C::ISSUER)  // the sign of the scale goes with q: the factor of the scores is then never negative
-        q_inv = tenmo_attn_stationary<DP, false, C::WGS>(a.q.ptr + b * a.q.sb + h * a.q.sh + (int64_t)q_tile * ROWS * a.q.sr, a.q.sr,
-                                                         q_rows - q_tile * ROWS, p.q_vec, a.D, a.scale < 0.f, lane_base, nullptr, shared_f,
-                                                         reinterpret_cast<float*>(smem + (SLOTS - 1) * C::IMG));
+        q_inv = tenmo_attn_stationary<DP, false, C::WGS>(x, a.scale < 0.f, lane_base, nullptr, shared_f);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();

@@ -143,16 +143,21 @@ __device__ __forceinline__ void tenmo_attn_zero_rows(float* head, int64_t stride
     }
 }
 
-// The rows of an operand (128 of them), split into fp16 pairs scaled by a power of two per row, into tensor memory (hi from `addr` on,
-// lo DP / 2 columns further) or, with SMEM, into a 128-row tile image in shared memory.  Called by the threads of WGS warpgroups, which
-// share the columns of a row; `exchange` holds WGS * 128 floats, `scratch` 128 * DP.  Returns the row's inverse scale.
-template <int DP, bool SMEM, int WGS>
-__device__ __forceinline__ float tenmo_attn_stationary(const float* src, int64_t stride, int rows, bool vec, int D, bool negate, uint32_t addr,
-                                                       uint8_t* plane, float* exchange, float* scratch) {
+// This thread's columns of its row of an operand; `scratch` holds 128 * DP floats.  Asked for before anything else of a block: the way to memory
+// takes as long as the barriers and the tensor memory.
+template <int DP, int WGS>
+__device__ __forceinline__ void tenmo_attn_fetch(float (&x)[DP / WGS], const float* src, int64_t stride, int rows, bool vec, int D, float* scratch) {
     constexpr int W = DP / WGS;
-    const int warp = threadIdx.x >> 5, wg = warp >> 2, row = threadIdx.x & 127, row0 = 32 * (warp & 3);
-    float x[W];
+    const int warp = threadIdx.x >> 5, wg = warp >> 2, row0 = 32 * (warp & 3);
     tenmo_attn_read_rows<W>(x, src + row0 * stride + wg * W, stride, rows - row0, D - wg * W, vec, scratch + warp * (32 * W));
+}
+// The rows of an operand (128 of them; x: this thread's columns of its row), split into fp16 pairs scaled by a power of two per row, into
+// tensor memory (hi from `addr` on, lo DP / 2 columns further) or, with SMEM, into a 128-row tile image in shared memory.  Called by the
+// threads of WGS warpgroups, which share the columns of a row; `exchange` holds WGS * 128 floats.  Returns the row's inverse scale.
+template <int DP, bool SMEM, int WGS>
+__device__ __forceinline__ float tenmo_attn_stationary(const float (&x)[DP / WGS], bool negate, uint32_t addr, uint8_t* plane, float* exchange) {
+    constexpr int W = DP / WGS;
+    const int wg = threadIdx.x >> 7, row = threadIdx.x & 127;
     float mx = 0.f;
 #pragma unroll
     for (int e = 0; e < W; ++e) mx = fmaxf(mx, tc::finite_abs(x[e]));
@@ -183,7 +188,7 @@ __device__ __forceinline__ float tenmo_attn_stationary(const float* src, int64_t
             tc::st8(addr + DP / 2 + col, lo);
         }
     }
-    tc::fence_proxy_async();  // the scratch is a stage that a copy fills next (and with SMEM the tensor core reads the image)
+    tc::fence_proxy_async();  // the rows came through a stage that a copy fills next (and with SMEM the tensor core reads the image)
     if (!SMEM) tc::st_wait();
     return inverse;
 }

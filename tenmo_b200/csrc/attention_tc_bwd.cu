@@ -119,7 +119,20 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
         return;
     }
 
-    if (threadIdx.x == 0) {
+    // the ring of tiles (one thread): a slot is refilled when all products of its tile are done
+    int fetched = 0, fetch_slot = 0, fetch_round = 0;
+    auto fetch = [&](int until) {
+        for (; fetched < until; ++fetched) {
+            if (fetch_round && !mbar_wait(empty(fetch_slot), (uint32_t)(fetch_round - 1) & 1u, abort_flag)) return;
+            const uint32_t dst = smem_u32(smem) + fetch_slot * C::STAGE, bar = full(fetch_slot);
+            mbar_expect_tx(bar, 4 * C::PLANE + (DKV ? 1024u : 0u));
+            tc::bulk_load(dst, p.y1_img + (tile0 + fetched) * (2 * C::PLANE), 2 * C::PLANE, bar);
+            tc::bulk_load(dst + 2 * C::PLANE, p.y2_img + (tile0 + fetched) * (2 * C::PLANE), 2 * C::PLANE, bar);
+            if (DKV) tc::bulk_load(dst + 4 * C::PLANE, p.info + (tile0 + fetched) * ATTN_INFO, 1024, bar);
+            if (++fetch_slot == C::STAGES) { fetch_slot = 0; ++fetch_round; }
+        }
+    };
+    if (threadIdx.x == 32 * C::LOADER) {  // the thread that copies: the first tiles are on their way before the block meets
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int w = 0; w < 2; ++w) {
             mbar_init(s_full(w), 1);
@@ -134,7 +147,22 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
         mbar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::fence_proxy_async();
+        fetch(min(n, C::STAGES - 1));  // the last slot is scratch for now
     }
+
+    auto fetch_x = [&](const TenmoHeadsView& v, bool vec, float (&x)[W]) {
+        const int64_t x0 = (int64_t)x_tile * ROWS;
+        tenmo_attn_fetch<DP, C::WGS>(x, v.ptr + b * v.sb + (DKV ? kvh : h) * v.sh + x0 * v.sr, v.sr, x_rows - x_tile * ROWS, vec, a.D,
+                                     reinterpret_cast<float*>(smem + (C::STAGES - 1) * C::STAGE));
+    };
+    constexpr bool BOTH = W <= 32;  // as the registers allow
+    float x1[W], x2[W];
+    if (warp < C::ISSUER) {
+        fetch_x(p.x1, p.x1_vec, x1);
+        if (BOTH) fetch_x(p.x2, p.x2_vec, x2);
+    }
+
     if (warp == C::ISSUER) tc::alloc(tmem_slot, C::TMEM);
     tc::fence_before();
     __syncthreads();
@@ -142,30 +170,12 @@ __global__ void __launch_bounds__(BwdCfg<DP, DKV>::THREADS, 1) attn_bwd_tc_kerne
     const uint32_t tmem = *tmem_slot;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 
-    // the ring of tiles (one thread): a slot is refilled when all products of its tile are done
-    int fetched = 0, fetch_slot = 0, fetch_round = 0;
-    auto fetch = [&](int until) {
-        for (; fetched < until; ++fetched) {
-            if (fetch_round && !mbar_wait(empty(fetch_slot), (uint32_t)(fetch_round - 1) & 1u, abort_flag)) return;
-            const uint32_t dst = smem_u32(smem) + fetch_slot * C::STAGE, bar = full(fetch_slot);
-            mbar_expect_tx(bar, 4 * C::PLANE + (DKV ? 1024u : 0u));
-            tc::bulk_load(dst, p.y1_img + (tile0 + fetched) * (2 * C::PLANE), 2 * C::PLANE, bar);
-            tc::bulk_load(dst + 2 * C::PLANE, p.y2_img + (tile0 + fetched) * (2 * C::PLANE), 2 * C::PLANE, bar);
-            if (DKV) tc::bulk_load(dst + 4 * C::PLANE, p.info + (tile0 + fetched) * ATTN_INFO, 1024, bar);
-            if (++fetch_slot == C::STAGES) { fetch_slot = 0; ++fetch_round; }
-        }
-    };
-    if (threadIdx.x == 32 * C::LOADER) fetch(min(n, C::STAGES - 1));  // the last slot is scratch for now
 
     float x1_inv = 1.f, x2_inv = 1.f;
     if (warp < C::ISSUER) {
-        const int xh = DKV ? kvh : h, rows = x_rows - x_tile * ROWS;
-        const int64_t x0 = (int64_t)x_tile * ROWS;
-        float* const scratch = reinterpret_cast<float*>(smem + (C::STAGES - 1) * C::STAGE);
-        x1_inv = tenmo_attn_stationary<DP, false, C::WGS>(p.x1.ptr + b * p.x1.sb + xh * p.x1.sh + x0 * p.x1.sr, p.x1.sr, rows, p.x1_vec, a.D, a.scale < 0.f,
-                                                     lane_base, nullptr, exchange, scratch);
-        x2_inv = tenmo_attn_stationary<DP, C::X2S, C::WGS>(p.x2.ptr + b * p.x2.sb + xh * p.x2.sh + x0 * p.x2.sr, p.x2.sr, rows, p.x2_vec, a.D, false,
-                                                      lane_base + C::X2_COL, x2_plane, exchange, scratch);
+        x1_inv = tenmo_attn_stationary<DP, false, C::WGS>(x1, a.scale < 0.f, lane_base, nullptr, exchange);
+        if (!BOTH) fetch_x(p.x2, p.x2_vec, x2);
+        x2_inv = tenmo_attn_stationary<DP, C::X2S, C::WGS>(x2, false, lane_base + C::X2_COL, x2_plane, exchange);
     }
     tc::fence_before();
     __syncthreads();
