@@ -312,7 +312,7 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     return TENMO_OK;
 }
 
-constexpr double TC_FLOP = 2e8;  // of one product
+constexpr double TC_FLOP = 2e8;  // of one product: 33 rows and more; level with the other kernels at 512x512x300 (1.6e8)
 // Large problems: the products on tensor cores (gemm_h3.cu).  Without a gradient no logit is ever stored: the product's epilogue
 // reduces them to two numbers per row and 64 columns.
 bool tc_profitable(const LceCall& c) { return c.N > TENMO_FEW_ROWS && 2.0 * c.N * c.D * c.V >= TC_FLOP; }
@@ -444,8 +444,11 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     int st = check(ctx, who, c);
     if (st != TENMO_OK) return st;
     TenmoDeviceGuard guard(ctx);
-    if (c.N > 0 && c.N <= 2 * TENMO_FEW_ROWS && !(c.N > TENMO_FEW_ROWS && tc_profitable(c))) return lce_run_few(ctx, c);
     if (tc_profitable(c)) return lce_run_tc(ctx, c);
+    // Up to 256 rows the kernels for a handful of rows, taken in groups of 32, keep more of the GPU busy than the strict-fp32 GEMM's tiles:
+    // 204x1884x28 forward 34 us for 81, 180x855x112 training 54 for 87, 100x768x1000 training 83 for 116; level at 300x128x1000,
+    // behind at 512x512x300 (155 for 89).
+    if (c.N > 0 && c.N <= 8 * TENMO_FEW_ROWS) return lce_run_few(ctx, c);
     int64_t piece = (int64_t)(LCE_PIECE_BYTES / ((size_t)c.V * sizeof(float))) / 128 * 128;
     if (piece < 128) piece = 128;
     if (piece > c.N) piece = c.N;

@@ -114,8 +114,9 @@ def compare(x, w, b, y, **kw):
     return got
 
 
-# up to 32 rows (64 in small products): the few-row kernels; from 2e8 flop a product on: tensor cores; else the strict-fp32 GEMM
-SHAPES = [(1, 1, 1), (1, 16, 10), (3, 5, 2), (7, 33, 1003), (13, 260, 4100), (32, 64, 130), (33, 128, 640), (64, 128, 1000), (64, 512, 4000), (130, 70, 129), (257, 64, 515), (300, 200, 4099), (515, 768, 2001)]
+# up to 32 rows (256 in small products): the few-row kernels; from 2e8 flop a product on: tensor cores; else the strict-fp32 GEMM
+SHAPES = [(1, 1, 1), (1, 16, 10), (3, 5, 2), (7, 33, 1003), (13, 260, 4100), (32, 64, 130), (33, 128, 640), (64, 128, 1000), (64, 512, 4000), (130, 70, 129), (257, 64, 515), (300, 200, 4099), (515, 768, 2001),
+          (256, 33, 700), (300, 40, 129), (700, 100, 31)]
 
 
 @pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
@@ -128,7 +129,7 @@ def test_against_64_bits(shape, tied):
     check("loss", loss, reference(x, w, b, y)["loss"])
 
 
-@pytest.mark.parametrize("size", [(30, 40, 201), (60, 40, 200), (100, 40, 200), (300, 256, 3000)], ids=str)
+@pytest.mark.parametrize("size", [(30, 40, 201), (60, 40, 200), (100, 40, 200), (300, 40, 200), (300, 256, 3000)], ids=str)
 @pytest.mark.parametrize("reduction", [0, 1, 2])
 def test_reductions_smoothing_upstream_and_label_types(size, reduction):
     N, D, V = size
@@ -138,7 +139,7 @@ def test_reductions_smoothing_upstream_and_label_types(size, reduction):
         compare(x, w, b, y, ls=ls, reduction=reduction, upstream=up)
 
 
-@pytest.mark.parametrize("size", [(30, 40, 201), (60, 40, 200), (100, 40, 200), (300, 256, 3000)], ids=str)
+@pytest.mark.parametrize("size", [(30, 40, 201), (60, 40, 200), (100, 40, 200), (300, 40, 200), (300, 256, 3000)], ids=str)
 def test_ignored_rows_may_hold_anything(size):
     x, w, b, y = make(*size, 4, bias=True, ignored=0.4)
     x[y == IGN] = float("nan")
@@ -147,7 +148,7 @@ def test_ignored_rows_may_hold_anything(size):
     assert float(got["dx"][y == IGN].abs().max()) == 0
 
 
-@pytest.mark.parametrize("size", [(30, 20, 50), (100, 20, 50), (200, 256, 2000)], ids=str)
+@pytest.mark.parametrize("size", [(30, 20, 50), (100, 20, 50), (300, 20, 50), (200, 256, 2000)], ids=str)
 def test_every_row_ignored(size):
     x, w, b, y = make(*size, 5, bias=True, ignored=2.0)
     got = run(x, w, b, y)
@@ -156,13 +157,13 @@ def test_every_row_ignored(size):
         assert float(got[n].abs().max()) == 0
 
 
-@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (256, 256, 2048)], ids=str)
+@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (300, 32, 100), (256, 256, 2048)], ids=str)
 def test_large_logits(size):
     x, w, b, y = make(*size, 6, scale=40.0)
     compare(x, w, b, y)
 
 
-@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (256, 256, 2048)], ids=str)
+@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (300, 32, 100), (256, 256, 2048)], ids=str)
 def test_rows_and_classes_of_very_different_size(size):
     N, D, V = size
     x, w, b, y = make(N, D, V, 7, tied=True)
@@ -180,7 +181,7 @@ def test_strided_x():
     compare(x.t().contiguous().t(), w, b, y)
 
 
-@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (256, 256, 2048)], ids=str)
+@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (300, 32, 100), (256, 256, 2048)], ids=str)
 def test_bad_label_sets_the_status_and_contributes_nothing(size):
     from tenmo_b200 import TenmoError
     from tests import gpu_util as g
@@ -205,7 +206,7 @@ def test_several_pieces_give_what_one_gives():
 
 @pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -math.inf], ids=["lowest", "-inf"])
 @pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
-@pytest.mark.parametrize("size", [(30, 20, 500), (100, 20, 500), (200, 256, 2000)], ids=str)
+@pytest.mark.parametrize("size", [(30, 20, 500), (100, 20, 500), (300, 20, 500), (200, 256, 2000)], ids=str)
 def test_classes_masked_through_the_bias(size, tied, low):
     """Classes whose bias is the type's lowest value or -inf: the same loss and gradients as without them, and none of their own."""
     N, D, V = size
@@ -228,7 +229,7 @@ def test_classes_masked_through_the_bias(size, tied, low):
 
 
 @pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
-@pytest.mark.parametrize("size", [(7, 36, 200), (100, 36, 200), (257, 256, 2000)], ids=str)
+@pytest.mark.parametrize("size", [(7, 36, 200), (100, 36, 200), (300, 36, 200), (257, 256, 2000)], ids=str)
 def test_pointers_that_are_not_aligned(size, tied):
     """Every buffer begins 4 bytes behind a 16-byte boundary, and nothing is written outside."""
     from tenmo_b200 import make_mat
@@ -334,7 +335,7 @@ def test_refusals():
         h.linear_ce_fwd_bwd(x, w, 0, y, True, 4, 8, 16, IGN, 0.0, 0, p, p, 0, p, p, p)
 
 
-@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (300, 256, 2100)], ids=str)
+@pytest.mark.parametrize("size", [(40, 32, 100), (100, 32, 100), (300, 32, 100), (300, 256, 2100)], ids=str)
 def test_captured_graph_replays_with_new_inputs(size):
     x, w, b, y = make(*size, 12, tied=True)
     run(x, w, b, y)
