@@ -375,25 +375,28 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
                     *reinterpret_cast<float4*>(stage_buf + lane * ST_LD + (((e >> 2) ^ ((lane >> 1) & 3)) << 2)) =
                         make_float4(s[16 * g + e], s[16 * g + e + 1], s[16 * g + e + 2], s[16 * g + e + 3]);
                 __syncwarp();
-                const int at = 16 * g + 4 * q;
-                const int64_t n = n0 + at;
+                if (vec && n0 + 16 * g + 16 <= p.N) {
+                    const int at = 16 * g + 4 * q;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 8 * i + sub;
-                    float4 x = *reinterpret_cast<const float4*>(stage_buf + r * ST_LD + ((q ^ ((r >> 1) & 3)) << 2));
-                    if (m0 + r >= p.M || n >= p.N) continue;
-                    float* dst = C + r * ldc + at;
-                    if (n + 3 < p.N && vec) {
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * i + sub;
+                        float4 x = *reinterpret_cast<const float4*>(stage_buf + r * ST_LD + ((q ^ ((r >> 1) & 3)) << 2));
+                        if (m0 + r >= p.M) continue;
+                        float* dst = C + r * ldc + at;
                         if (add) {
                             const float4 o = *reinterpret_cast<const float4*>(dst);
                             x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
                         }
                         *reinterpret_cast<float4*>(dst) = x;
-                    } else {
-                        const float v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (n + e < p.N) dst[e] = add ? dst[e] + v[e] : v[e];
+                    }
+                } else {  // unaligned rows, and the ragged edge: a store covers two rows of 64 contiguous bytes
+                    const int c = lane & 15, at = 16 * g + c;
+#pragma unroll 4
+                    for (int r = lane >> 4; r < 32; r += 2) {
+                        const float x = stage_buf[r * ST_LD + (((c >> 2) ^ ((r >> 1) & 3)) << 2) + (c & 3)];
+                        if (m0 + r >= p.M || n0 + at >= p.N) continue;
+                        float* dst = C + r * ldc + at;
+                        *dst = add ? *dst + x : x;
                     }
                 }
             }

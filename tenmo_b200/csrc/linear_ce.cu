@@ -312,10 +312,13 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     return TENMO_OK;
 }
 
-constexpr double TC_FLOP = 2e8;  // of one product: 33 rows and more; level with the other kernels at 512x512x300 (1.6e8)
+constexpr double TC_FLOP = 2e8;  // of one product; level with the other kernels at 512x512x300 (1.6e8)
+// Rows: with 17 to 32 the weight's split into blocks costs less than the few-row kernels' arithmetic on large weights (24x1318x44771 476 us
+// for 607, its loss alone 206 for 263; 24x1024x8000 128 for 122); with up to 16 those read the weight as fast (16x1318x44771 451 us for 475).
+constexpr int TC_ROWS = 16;
 // Large problems: the products on tensor cores (gemm_h3.cu).  Without a gradient no logit is ever stored: the product's epilogue
 // reduces them to two numbers per row and 64 columns.
-bool tc_profitable(const LceCall& c) { return c.N > TENMO_FEW_ROWS && 2.0 * c.N * c.D * c.V >= TC_FLOP; }
+bool tc_profitable(const LceCall& c) { return c.N > TC_ROWS && 2.0 * c.N * c.D * c.V >= TC_FLOP; }
 
 int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     const int64_t vb = (c.V + H3_BLOCK - 1) / H3_BLOCK;

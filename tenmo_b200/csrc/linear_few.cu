@@ -9,8 +9,8 @@
 //         exchanged by halving at the end (a lane passes on the half it does not keep)
 // Where the output axis gives too few blocks, the contraction is cut into slices that a second kernel adds in order.
 // Bound: HBM, 4 bytes per element of the matrix.
-// Measured (kernels of a call, cold): 64 rows of 128 x 1000, 12 us for the logits, 8 + 4 for dx, 8 for dW; 6 rows of 481 x 44931, training, 162 us in
-// all for 260 MB.
+// Measured (kernels of a call, cold): 64 rows of 128 x 1000, 12 us for the logits, 8 + 4 for dx, 8 for dW; 16 rows of 1318 x 44771 (236 MB), 132 us for
+// the logits, 164 for dx, 100 for dW; 7 rows of 1039 x 33938 (141 MB) 47, 62 and 44.
 #include "linear_few.cuh"
 
 namespace {
@@ -34,8 +34,9 @@ __device__ __forceinline__ void few_store(const FewArgs& p, int slice, int64_t n
     else p.out[n * p.ldo + c] = p.bias ? v + __ldg(p.bias + c) : v;
 }
 
+// Two blocks on an SM up to 16 rows: the loads in flight are what reads the matrix fast.
 template <int NR>
-__global__ void __launch_bounds__(32 * WARPS) few_cols_kernel(const FewArgs p) {
+__global__ void __launch_bounds__(32 * WARPS, NR <= 16 ? 2 : 1) few_cols_kernel(const FewArgs p) {
     __shared__ __align__(16) float as[KC][NR + 4];  // + 4: rows stay aligned and the staging stores spread over the banks
     __shared__ __align__(16) float sum[NR][128];
     tenmo_grid_dependency_sync();
@@ -124,8 +125,9 @@ __global__ void __launch_bounds__(32 * WARPS) few_cols_kernel(const FewArgs p) {
     }
 }
 
+// Two blocks on an SM up to 16 rows: the loads in flight are what reads the matrix fast.
 template <int NR>
-__global__ void __launch_bounds__(32 * WARPS) few_dot_kernel(const FewArgs p) {
+__global__ void __launch_bounds__(32 * WARPS, NR <= 16 ? 2 : 1) few_dot_kernel(const FewArgs p) {
     __shared__ __align__(16) float as[NR][CC];
     tenmo_grid_dependency_sync();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = blockIdx.y;
@@ -219,57 +221,79 @@ __global__ void __launch_bounds__(256) few_fold_kernel(const FewArgs p) {
     }
 }
 
-// 32 rows x 128 columns of the result per block, 4 x 4 per thread
-__global__ void __launch_bounds__(256) few_outer_kernel(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t N, int64_t R, int64_t C,
-                                                        float* out, int vec) {
+// 128 columns of the result per block, 32 of its rows at a time (`tiles` times), 4 x 4 per thread.  Up to 32 of the contraction stay for all the block's row
+// tiles (b's part in shared memory; a's next part is fetched while this one is multiplied); more are taken in turn per row tile.
+// Columns of a thread: 4 in a row where the result's rows are aligned, else 32 apart, so that scalar stores cover whole sectors too.
+template <bool VEC>
+__global__ void __launch_bounds__(256) few_outer_kernel(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t N, int64_t R, int64_t C, float* out, int tiles) {
     __shared__ __align__(16) float sa[TENMO_FEW_ROWS][32], sb[TENMO_FEW_ROWS][128];
     tenmo_grid_dependency_sync();
-    const int64_t r0 = (int64_t)blockIdx.y * 32, c0 = (int64_t)blockIdx.x * 128;
-    const int tr = (threadIdx.x >> 5) * 4, tc = (threadIdx.x & 31) * 4;
-    float acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-    for (int64_t n0 = 0; n0 < N; n0 += TENMO_FEW_ROWS) {
-        const int rows = (int)min((int64_t)TENMO_FEW_ROWS, N - n0);
-        __syncthreads();
-        float av[4], bv[16];  // all loads first
+    const int64_t first = (int64_t)blockIdx.y * (32 * tiles), c0 = (int64_t)blockIdx.x * 128;
+    const int tr = (threadIdx.x >> 5) * 4, lane = threadIdx.x & 31;
+    const int64_t parts = (N + TENMO_FEW_ROWS - 1) / TENMO_FEW_ROWS;
+    const int64_t end = min(R, first + 32 * tiles);
+    float av[4];
+    auto fetch_a = [&](int64_t r0, int64_t n0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int n = (threadIdx.x >> 5) + 8 * i, r = threadIdx.x & 31;
-            av[i] = n < rows && r0 + r < R ? __ldg(a + (n0 + n) * lda + r0 + r) : 0.f;
+            const int64_t n = n0 + (threadIdx.x >> 5) + 8 * i, r = r0 + lane;
+            av[i] = n < N && r < R ? __ldg(a + n * lda + r) : 0.f;
+        }
+    };
+    fetch_a(first, 0);
+    for (int64_t r0 = first; r0 < end; r0 += 32) {
+        float acc[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        for (int64_t part = 0; part < parts; ++part) {
+            const int64_t n0 = part * TENMO_FEW_ROWS;
+            const int rows = (int)min((int64_t)TENMO_FEW_ROWS, N - n0);
+            const bool load_b = parts > 1 || r0 == first;
+            float bv[16];
+            if (load_b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {  // all loads first
+                    const int n = (threadIdx.x >> 7) + 2 * i, c = threadIdx.x & 127;
+                    bv[i] = n < rows && c0 + c < C ? __ldg(b + (n0 + n) * ldb + c0 + c) : 0.f;
+                }
+            }
+            __syncthreads();  // the part before has been read
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sa[(threadIdx.x >> 5) + 8 * i][lane] = av[i];
+            if (load_b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sb[(threadIdx.x >> 7) + 2 * i][threadIdx.x & 127] = bv[i];
+            }
+            if (part + 1 < parts) fetch_a(r0, n0 + TENMO_FEW_ROWS);
+            else if (r0 + 32 < end) fetch_a(r0 + 32, 0);
+            __syncthreads();
+#pragma unroll 4
+            for (int n = 0; n < rows; ++n) {
+                const float4 x = *reinterpret_cast<const float4*>(&sa[n][tr]);
+                float4 y;
+                if (VEC) y = *reinterpret_cast<const float4*>(&sb[n][4 * lane]);
+                else y = make_float4(sb[n][lane], sb[n][lane + 32], sb[n][lane + 64], sb[n][lane + 96]);
+                const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int n = (threadIdx.x >> 7) + 2 * i, c = threadIdx.x & 127;
-            bv[i] = n < rows && c0 + c < C ? __ldg(b + (n0 + n) * ldb + c0 + c) : 0.f;
-        }
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = r0 + tr + i;
+            if (r >= R) continue;
+            float* dst = out + r * C + c0;
+            if (VEC) {
+                if (c0 + 4 * lane < C) *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sa[(threadIdx.x >> 5) + 8 * i][threadIdx.x & 31] = av[i];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sb[(threadIdx.x >> 7) + 2 * i][threadIdx.x & 127] = bv[i];
-        __syncthreads();
-        for (int n = 0; n < rows; ++n) {
-            const float4 x = *reinterpret_cast<const float4*>(&sa[n][tr]), y = *reinterpret_cast<const float4*>(&sb[n][tc]);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t r = r0 + tr + i, c = c0 + tc;
-        if (r >= R || c >= C) continue;
-        float* dst = out + r * C + c;
-        if (vec) {
-            *reinterpret_cast<float4*>(dst) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c + j < C) dst[j] = acc[i][j];
+                for (int j = 0; j < 4; ++j)
+                    if (c0 + lane + 32 * j < C) dst[lane + 32 * j] = acc[i][j];
+            }
         }
     }
 }
@@ -334,16 +358,20 @@ int tenmo_few_dot(tenmo_ctx* ctx, const float* a, int64_t lda, int64_t N, int64_
 }
 
 int tenmo_few_outer(tenmo_ctx* ctx, const float* a, int64_t lda, const float* b, int64_t ldb, int64_t N, int64_t R, int64_t C, float* out) {
-    const int64_t gx = (C + 127) / 128, gy = (R + 31) / 32;
+    // as many row tiles per block, up to eight, as leave every SM four blocks: 44771 x 1318 of 16 rows 100 us with eight
+    const int64_t gx = (C + 127) / 128, fit = gx * ((R + 31) / 32) / (4 * (int64_t)ctx->sm_count);
+    const int tiles = fit > 8 ? 8 : fit < 1 ? 1 : (int)fit;
+    const int64_t TILE = 32 * tiles, gy = (R + TILE - 1) / TILE;
     if (gy > 65535) {  // the grid's second axis: in parts
-        for (int64_t r = 0; r < R; r += 65535 * 32) {
-            const int st = tenmo_few_outer(ctx, a + r, lda, b, ldb, N, R - r < 65535 * 32 ? R - r : 65535 * 32, C, out + r * C);
+        for (int64_t r = 0; r < R; r += 65535 * TILE) {
+            const int st = tenmo_few_outer(ctx, a + r, lda, b, ldb, N, R - r < 65535 * TILE ? R - r : 65535 * TILE, C, out + r * C);
             if (st != TENMO_OK) return st;
         }
         return TENMO_OK;
     }
-    const int vec = C % 4 == 0 && ((uintptr_t)out & 15u) == 0;
-    TENMO_CUDA_TRY(ctx, tenmo_launch(few_outer_kernel, dim3((unsigned)gx, (unsigned)gy), 256, 0, ctx->stream, tenmo_pdl_ok(ctx, gx * gy), a, lda, b, ldb, N, R, C, out, vec));
+    const bool vec = C % 4 == 0 && ((uintptr_t)out & 15u) == 0;
+    TENMO_CUDA_TRY(ctx, tenmo_launch(vec ? few_outer_kernel<true> : few_outer_kernel<false>, dim3((unsigned)gx, (unsigned)gy), 256, 0, ctx->stream,
+                                     tenmo_pdl_ok(ctx, gx * gy), a, lda, b, ldb, N, R, C, out, tiles));
     TENMO_LAUNCH_CHECK(ctx, "few_outer_kernel");
     return TENMO_OK;
 }
