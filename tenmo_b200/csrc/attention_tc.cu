@@ -16,11 +16,11 @@
 // S and P are handed over in halves of 64 keys, so the maximum of the first half is taken while the second is computed and O_j
 // starts while the second half's exponentials are taken; O_{j-1} is added while S_j is computed.
 // Floor: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
-// Measured at 384 heads of 512 rows and keys, dim 64: 128 us behind 26 us of images (25.8 GF, 47 us of tensor time).  A tile of 128 x 128
+// Measured at 384 heads of 512 rows and keys, dim 64: 122 us behind 26 us of images (25.8 GF, 47 us of tensor time).  A tile of 128 x 128
 // takes 3900 cycles with one CTA on the SM, 3350 with two, where the products and the exponentials (measured apart) need 1540 each and do
 // not slow each other; a CTA costs 14,000 cycles besides (q's way into tensor memory, the first tile's way to the exponentials, the
 // output).  Tensor pipe 32 % busy, exponential unit 24 %: the chain of a tile decides.  Two sides per CTA under one issuer were slower
-// (202 us for 167 in all), and so was one S buffer per 64 keys.
+// (202 us for 167 in all at the time), and so was one S buffer per 64 keys.
 #include "attention_tc.cuh"
 
 namespace {

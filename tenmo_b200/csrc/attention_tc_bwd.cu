@@ -18,7 +18,7 @@
 // Shared key / value heads: the dkv pass works per query head into the workspace and a last kernel adds the heads of a group
 // in order (per group it would leave most SMs idle behind the longest).
 // Bound: tensor pipe, 3 * 14 * rows * keys * dim flop.
-// Measured: 384 heads of 512x64, dq pass 198 us, dkv pass 253 us, pipe 31 % busy (a tile's chain and what a block costs besides); 16 heads of
+// Measured: 384 heads of 512x64, dq pass 193 us, dkv pass 245 us, pipe 31 to 33 % busy (a tile's chain and what a block costs besides); 16 heads of
 // 4001x128 causal, 288 and 394 us, pipe 58 and 55 %.
 #include "attention_tc.cuh"
 

@@ -14,7 +14,7 @@
 // Tiles go round-robin to the pairs; with few tiles and a long contraction (the gradient of x) the contraction is cut into equal
 // slices whose partial results a second kernel adds in order.
 // Bound: tensor pipe, 3 * 2 M N K flop.
-// Measured: 2048 x 65536 over 2048 (logits) 1.17 ms = 470 TFLOP/s of the product, 1410 of the pipe; over 65536 (gradient of x) 1.21 ms.  With a
+// Measured: 2048 x 65536 over 2048 (logits) 1.11 ms = 495 TFLOP/s of the product, 1490 of the pipe; over 65536 (gradient of x) 1.24 ms.  With a
 // contraction of 768 the epilogue's statistics and 256 KB of results per tile of six chunks show: 2048 x 32011 logits 243 us (415 TFLOP/s; 206 us
 // without storing them; 291 us when they went through shared memory and every element was asked for its column).
 #include <cuda.h>

@@ -9,7 +9,7 @@
 // loss that forgets the logits between forward and backward needs a fourth to recompute them.
 // Ignored rows: their x is replaced by zeros, so that whatever padding holds (NaN included) reaches no gradient.
 // Bound: the three products (gemm_h3.cu); turning a piece's logits into the gradient is a pass over HBM, 8 bytes an element: 2048 x 65536 in
-// 0.25 ms (4.3 TB/s) beside 3.6 ms of products.
+// 0.24 ms (4.5 TB/s) beside 3.6 ms of products.
 #include <cfloat>
 
 #include "gemm_h3.cuh"
