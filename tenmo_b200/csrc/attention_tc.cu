@@ -539,7 +539,7 @@ int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, 
 // 32, of 32x32: 44 against 105).
 bool tenmo_attn_tc_profitable(const TenmoAttnParams& p, bool backward) {
     const int64_t rows = (int64_t)p.B * p.H * p.Sq;
-    if (p.Sq == 0 || p.Sk == 0) return false;
+    if (rows == 0 || p.Sk == 0) return false;
     if (!backward) return p.Sq >= 16 && rows * ((p.Sk + 127) / 128) >= 2560;
     return p.Sq >= 64 || p.Sk >= 64 || rows * p.Sk > 65536;
 }

@@ -123,6 +123,13 @@ def test_no_keys_or_no_rows(q_len, k_len):
         assert float(t.abs().sum()) == 0  # also: written, not left as NaN
 
 
+@pytest.mark.parametrize("length", [7, 300])
+def test_an_empty_batch(length):
+    gen = torch.Generator(device="cuda").manual_seed(28)
+    got = run(*(_make(gen, 0, 2, length, 16) for _ in range(4)))
+    assert got["dk"].shape == (0, 2, length, 16)
+
+
 @pytest.mark.parametrize("size", [40, 300])
 def test_large_and_small_scores(size):
     """Scores of several hundred (a softmax that picks one key) and of almost zero (uniform), and the scale's sign."""
