@@ -12,11 +12,12 @@
 // often as with 64), their columns are shared by two warpgroups (dim up to 64; 64 columns of S, 32 of O a thread) or four (up to
 // 128), which exchange their maxima through shared memory, and up to dim 64, where everything fits twice into an SM (96 KB,
 // 256 columns), two CTAs fill each other's gaps: one's products run while the other's exponentials are taken.  Up to dim 128 one
-// CTA has the SM and a second S buffer lets S_{j+1} run while P_j is made.  One warp issues the MMAs, one the copies.
+// CTA has the SM and a second S buffer lets S_{j+1} run while P_j is made.  One warp issues the MMAs and (or
+// another warp, with one CTA on the SM) the copies.
 // S and P are handed over in halves of 64 keys, so the maximum of the first half is taken while the second is computed and O_j
 // starts while the second half's exponentials are taken; O_{j-1} is added while S_j is computed.
 // Floor: tensor pipe, 3 * 4 * rows * keys * dim flop; the images cost one read and one write of k and v in front.
-// Measured at 384 heads of 512 rows and keys, dim 64: 122 us behind 26 us of images (25.8 GF, 47 us of tensor time).  A tile of 128 x 128
+// Measured at 384 heads of 512 rows and keys, dim 64: 119 us behind 26 us of images (25.8 GF, 47 us of tensor time).  A tile of 128 x 128
 // takes 3900 cycles with one CTA on the SM, 3350 with two, where the products and the exponentials (measured apart) need 1540 each and do
 // not slow each other; a CTA costs 14,000 cycles besides (q's way into tensor memory, the first tile's way to the exponentials, the
 // output).  Tensor pipe 32 % busy, exponential unit 24 %: the chain of a tile decides.  Two sides per CTA under one issuer were slower
@@ -166,8 +167,9 @@ struct FwdParams {
 template <int DP>
 struct FwdCfg {
     static constexpr int WGS = DP / 32;             // warpgroups that share a tile
-    static constexpr int THREADS = 128 * WGS + 64;
-    static constexpr int ISSUER = 4 * WGS, LOADER = ISSUER + 1;
+    static constexpr bool OWN_LOADER = DP != 64;    // up to dim 64 the issuing warp copies too (119 us for 122 below)
+    static constexpr int ISSUER = 4 * WGS, LOADER = OWN_LOADER ? ISSUER + 1 : ISSUER;
+    static constexpr int THREADS = 32 * (LOADER + 1);
     static constexpr int HC = T / 2 / WGS, W = DP / WGS;  // columns of a half of S and of O of a thread
     static constexpr int NB = DP == 64 ? 1 : 2;     // S / P buffers
     static constexpr int PLANE = T * DP * 2;        // bytes of one plane of a tile
@@ -271,14 +273,23 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
     tc::fence_after();
 
     if (warp >= C::ISSUER) {
-        if (warp == C::LOADER) {
+        // every copy has landed before shared memory is given back (bounded): by now they are the last ones
+        auto landed = [&]() {
+            int never = 0;
+            for (int t = max(0, fetched - SLOTS); t < fetched; ++t) mbar_wait(full(t % SLOTS), (uint32_t)(t / SLOTS) & 1u, &never);
+        };
+        if (C::OWN_LOADER && warp == C::LOADER) {
             if (lane == 0) {
                 fetch(2 * n_tiles);
-                // every copy has landed before shared memory is given back (bounded): by now they are the last ones
-                int never = 0;
-                for (int t = max(0, fetched - SLOTS); t < fetched; ++t) mbar_wait(full(t % SLOTS), (uint32_t)(t / SLOTS) & 1u, &never);
+                landed();
             }
         } else if (warp == C::ISSUER) {
+            auto refill = [&](int until) {  // without a loader
+                if (lane == 0) fetch(min(2 * n_tiles, until));
+                __syncwarp();
+            };
+            if (!C::OWN_LOADER) refill(SLOTS);
+
             const uint32_t tm = tc::uniform(tmem), stages = tc::uniform(smem_u32(smem));
             const int n = tc::uniform(n_tiles);
             constexpr uint32_t ID_S = tc::idesc_f16(T / 2, false), ID_O = tc::idesc_f16(DP, true);
@@ -331,6 +342,7 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
                 if (C::NB == 1 && j + 1 < n) {  // S_{j+1} replaces P_j
                     ok = wait(full(slot), phase) && wait(o_full(j), (uint32_t)(j >> 1) & 1u);
                     if (ok) scores(j + 1);
+                    if (ok && !C::OWN_LOADER) refill(2 * j + 2 + SLOTS);  // S_j and O_j are done: their two slots
                 }
             }
             // Every MMA is done before tensor memory is given back: the readers of O have seen to it; after a wait that ran out, wait
@@ -339,6 +351,10 @@ __global__ void __launch_bounds__(FwdCfg<DP>::THREADS, DP == 64 ? 2 : 1) attn_fw
                 int never = 0;
                 tc::commit(drain);
                 mbar_wait(drain, 0, &never);
+            }
+            if (!C::OWN_LOADER) {
+                if (lane == 0) landed();
+                __syncwarp();
             }
         }
     } else {
