@@ -21,7 +21,7 @@
 // takes 3900 cycles with one CTA on the SM, 3350 with two, where the products and the exponentials (measured apart) need 1540 each and do
 // not slow each other; a CTA costs 14,000 cycles besides (q's way into tensor memory, the first tile's way to the exponentials, the
 // output).  Tensor pipe 32 % busy, exponential unit 24 %: the chain of a tile decides.  Two sides per CTA under one issuer were slower
-// (202 us for 167 in all at the time), and so was one S buffer per 64 keys.
+// (202 us for 167 in all at the time); tiles of 64 keys with two S buffers took 131 us.
 #include "attention_tc.cuh"
 
 namespace {
