@@ -312,13 +312,17 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     return TENMO_OK;
 }
 
-constexpr double TC_FLOP = 2e8;  // of one product; level with the other kernels at 512x512x300 (1.6e8)
+// Of one product: against the few-row kernels, which up to 256 rows otherwise run (200x300x1200, 1.4e8: 100 us for 97; 100x768x1000, 1.5e8:
+// 97 us for 83), and against the strict-fp32 GEMM (594x40x2465, 1.2e8: 109 us for 201; 980x207x450, 1.8e8: 104 for 114; 512x512x300,
+// 1.6e8: 94 for 86; 790x39x1249, 0.8e8: 107 for 123, 1442x72x249, 0.5e8: 100 for 82).
+constexpr double TC_FLOP_FEW = 2e8, TC_FLOP = 1e8;
 // Rows: with 17 to 32 the weight's split into blocks costs less than the few-row kernels' arithmetic on large weights (24x1318x44771 476 us
 // for 607, its loss alone 206 for 263; 24x1024x8000 128 for 122); with up to 16 those read the weight as fast (16x1318x44771 451 us for 475).
 constexpr int TC_ROWS = 16;
+constexpr int LCE_FEW_MOST = 8 * TENMO_FEW_ROWS;  // rows of the few-row kernels
 // Large problems: the products on tensor cores (gemm_h3.cu).  Without a gradient no logit is ever stored: the product's epilogue
 // reduces them to two numbers per row and 64 columns.
-bool tc_profitable(const LceCall& c) { return c.N > TC_ROWS && 2.0 * c.N * c.D * c.V >= TC_FLOP; }
+bool tc_profitable(const LceCall& c) { return c.N > TC_ROWS && 2.0 * c.N * c.D * c.V >= (c.N <= LCE_FEW_MOST ? TC_FLOP_FEW : TC_FLOP); }
 
 int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     const int64_t vb = (c.V + H3_BLOCK - 1) / H3_BLOCK;
@@ -451,7 +455,7 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     // Up to 256 rows the kernels for a handful of rows, taken in groups of 32, keep more of the GPU busy than the strict-fp32 GEMM's tiles:
     // 204x1884x28 forward 34 us for 81, 180x855x112 training 54 for 87, 100x768x1000 training 83 for 116; level at 300x128x1000,
     // behind at 512x512x300 (155 for 89).
-    if (c.N > 0 && c.N <= 8 * TENMO_FEW_ROWS) return lce_run_few(ctx, c);
+    if (c.N > 0 && c.N <= LCE_FEW_MOST) return lce_run_few(ctx, c);
     int64_t piece = (int64_t)(LCE_PIECE_BYTES / ((size_t)c.V * sizeof(float))) / 128 * 128;
     if (piece < 128) piece = 128;
     if (piece > c.N) piece = c.N;

@@ -114,9 +114,9 @@ def compare(x, w, b, y, **kw):
     return got
 
 
-# up to 16 rows (256 in small products): the few-row kernels; from 2e8 flop a product on: tensor cores; else the strict-fp32 GEMM
+# up to 16 rows (256 in small products): the few-row kernels; from 1e8 flop a product on (2e8 up to 256 rows): tensor cores; else the strict-fp32 GEMM
 SHAPES = [(1, 1, 1), (1, 16, 10), (3, 5, 2), (7, 33, 1003), (13, 260, 4100), (32, 64, 130), (33, 128, 640), (64, 128, 1000), (64, 512, 4000), (130, 70, 129), (257, 64, 515), (300, 200, 4099), (515, 768, 2001),
-          (16, 700, 20001), (17, 702, 20001), (16, 90, 90001), (256, 33, 700), (300, 40, 129), (700, 100, 31)]
+          (16, 700, 20001), (17, 702, 20001), (16, 90, 90001), (256, 33, 700), (594, 40, 2465), (300, 40, 129), (700, 100, 31)]
 
 
 @pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
