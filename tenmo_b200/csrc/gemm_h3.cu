@@ -445,14 +445,16 @@ int encode(tenmo_ctx* ctx, CUtensorMap* map, const TenmoH3Operand& o, bool mn) {
 
 // Slices of the contraction: the number (at most 32, each at least 8 chunks) that finishes first by this count, in units of one 128-deep
 // chunk of a 256 x 256 tile, 2.3 us at the measured rate: the rounds of tiles that the pairs need, and the partial results, which
-// are written, read and folded at about 6 TB/s.
-int pick_slices(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K) {
+// are written, read and folded at about 6 TB/s.  A shorter contraction can come out with more slices than a longer one (the rounds go by whole
+// tiles), so scratch is asked for by every size that is used, and a count whose results do not fit `room` bytes is not taken.
+size_t slice_bytes(int slices, int64_t M, int64_t N) { return (size_t)slices * (size_t)M * (size_t)((N + 3) / 4 * 4) * sizeof(float); }
+int pick_slices(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, size_t room) {
     const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256), chunks = (K + 127) / 128;
     const int64_t pairs = (ctx->sm_count - ctx->reserve_sms) / 2 > 0 ? (ctx->sm_count - ctx->reserve_sms) / 2 : 1;
     const double traffic = 4.0 * M * N / 6e6 / 2.3;  // one pass over the result
     int best = 1;
     double best_cost = 1e300;
-    for (int s = 1; s <= 32 && (s == 1 || chunks >= 8 * s); ++s) {
+    for (int s = 1; s <= 32 && (s == 1 || (chunks >= 8 * s && slice_bytes(s, M, N) <= room)); ++s) {
         const int64_t rounds = (tiles * s + pairs - 1) / pairs;
         const double cost = (double)rounds * ((double)chunks / s + 1.0) + (s > 1 ? (2.0 * s + 1.0) * traffic + 2.0 : 0.0);
         if (cost < best_cost * 0.99) { best = s; best_cost = cost; }
@@ -470,13 +472,13 @@ int tenmo_h3_make(tenmo_ctx* ctx, const float* src, int64_t rs, int64_t cs, cons
     return TENMO_OK;
 }
 
-size_t tenmo_h3_partial_bytes(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, bool plain) {
-    const int s = plain ? pick_slices(ctx, M, N, K) : 1;
-    return s > 1 ? (size_t)s * (size_t)M * (size_t)((N + 3) / 4 * 4) * sizeof(float) : 0;
+size_t tenmo_h3_partial_bytes(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K) {
+    const int s = pick_slices(ctx, M, N, K, SIZE_MAX);
+    return s > 1 ? slice_bytes(s, M, N) : 0;
 }
 
 int tenmo_h3_gemm(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, const TenmoH3Operand& A, bool a_rows_are_k, const TenmoH3Operand& B,
-                  bool b_rows_are_k, const TenmoH3Epilogue& e, void* partial) {
+                  bool b_rows_are_k, const TenmoH3Epilogue& e, void* partial, size_t partial_bytes) {
     int st = tenmo_tma_init(ctx);
     if (st != TENMO_OK) return st;
     CUtensorMap ma, mb;
@@ -490,7 +492,7 @@ int tenmo_h3_gemm(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, const TenmoH3
     const bool plain = !e.stats;
     if (plain && (e.bias || e.blocked || !e.C)) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "h3_gemm: a bias and blocks go with the statistics");
     if (!plain && (!e.at_label || !e.labels || (e.C && !e.blocked) || a_rows_are_k)) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "h3_gemm: this epilogue is not built");
-    p.slices = plain && partial ? pick_slices(ctx, M, N, K) : 1;
+    p.slices = plain && partial ? pick_slices(ctx, M, N, K, partial_bytes) : 1;
     p.partial = (float*)partial;
     p.ldp = (N + 3) / 4 * 4;
     p.a_inv = A.inverse; p.b_inv = B.inverse;

@@ -39,10 +39,11 @@ struct TenmoH3Epilogue {
     int label_is_i64;
 };
 // product = A . B over K.  a_rows_are_k: A is stored (K, M), else (M, K); b_rows_are_k: B is stored (K, N), else (N, K).
-// (A stored (K, M) with B stored (N, K) is not built.)  `partial`: scratch of tenmo_h3_partial_bytes.
-size_t tenmo_h3_partial_bytes(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, bool plain);
+// (A stored (K, M) with B stored (N, K) is not built.)  `partial`: scratch for the slices of a contraction; tenmo_h3_partial_bytes says how
+// much lets the product choose freely, and with less it takes fewer slices.
+size_t tenmo_h3_partial_bytes(const tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K);
 int tenmo_h3_gemm(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, const TenmoH3Operand& A, bool a_rows_are_k, const TenmoH3Operand& B,
-                  bool b_rows_are_k, const TenmoH3Epilogue& e, void* partial);
+                  bool b_rows_are_k, const TenmoH3Epilogue& e, void* partial, size_t partial_bytes);
 
 // Place (in floats) of columns [4 q, 4 q + 4) of row r in a block of logits: 32 rows x 64 columns are contiguous, and of those the 32 rows of four
 // columns, which is how a warp of the epilogue (a row per lane) holds them: its stores need no staging.

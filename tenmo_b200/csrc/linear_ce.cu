@@ -342,12 +342,12 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     const size_t at_label = take(piece * sizeof(float)), numbers = c.grad ? take(piece * sizeof(float4)) : 0;
     const size_t row_loss = take(c.N * sizeof(float)), factor = take(sizeof(float));
     const size_t db_part = c.db ? take((size_t)((piece + H3_BLOCK - 1) / H3_BLOCK) * c.V * sizeof(float)) : 0;
-    size_t part = 0;
-    if (c.grad) {
-        part = tenmo_h3_partial_bytes(ctx, piece, c.D, c.V, true);
-        const size_t last = c.N % piece ? tenmo_h3_partial_bytes(ctx, c.N % piece, c.D, c.V, true) : 0;
-        const size_t dw = tied ? tenmo_h3_partial_bytes(ctx, c.V, c.D, piece, true) : tenmo_h3_partial_bytes(ctx, c.D, c.V, piece, true);
-        if (last > part) part = last;
+    size_t part = 0;  // for dx and dw of a whole piece and of the last one
+    for (int64_t rows : {piece, c.N % piece}) {
+        if (!c.grad || !rows) continue;
+        const size_t dx = tenmo_h3_partial_bytes(ctx, rows, c.D, c.V);
+        const size_t dw = tied ? tenmo_h3_partial_bytes(ctx, c.V, c.D, rows) : tenmo_h3_partial_bytes(ctx, c.D, c.V, rows);
+        if (dx > part) part = dx;
         if (dw > part) part = dw;
     }
     const size_t partial = take(part);
@@ -379,7 +379,7 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
         e.at_label = (float*)(at + at_label);
         e.labels = labels;
         e.label_is_i64 = c.is_i64;
-        if ((st = tenmo_h3_gemm(ctx, rows, c.V, c.D, X, false, W, !tied, e, nullptr)) != TENMO_OK) return st;
+        if ((st = tenmo_h3_gemm(ctx, rows, c.V, c.D, X, false, W, !tied, e, nullptr, 0)) != TENMO_OK) return st;
         const LceStats ps{e.stats, e.sums, e.at_label, groups, rows, r0, c.V, c.ignore, c.labels, c.upstream, (const float*)(at + factor),
                           (float*)(at + row_loss), c.grad ? (float4*)(at + numbers) : nullptr, ctx->dev_status, c.ls, c.is_i64, c.reduction};
         lce_stats_kernel<<<(unsigned)((rows + 31) / 32), 32 * LCE_STAT_WARPS, 0, ctx->stream>>>(ps);
@@ -391,12 +391,12 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
         TenmoH3Epilogue ex = {};
         ex.C = c.dx + r0 * c.D;
         ex.ldc = c.D;
-        if ((st = tenmo_h3_gemm(ctx, rows, c.D, c.V, Z, false, W, tied, ex, at + partial)) != TENMO_OK) return st;
+        if ((st = tenmo_h3_gemm(ctx, rows, c.D, c.V, Z, false, W, tied, ex, at + partial, part)) != TENMO_OK) return st;
         TenmoH3Epilogue ew = {};
         ew.C = c.dw;
         ew.ldc = tied ? c.D : c.V;
         ew.add = r0 > 0;
-        st = tied ? tenmo_h3_gemm(ctx, c.V, c.D, rows, Z, true, X, true, ew, at + partial) : tenmo_h3_gemm(ctx, c.D, c.V, rows, X, true, Z, true, ew, at + partial);
+        st = tied ? tenmo_h3_gemm(ctx, c.V, c.D, rows, Z, true, X, true, ew, at + partial, part) : tenmo_h3_gemm(ctx, c.D, c.V, rows, X, true, Z, true, ew, at + partial, part);
         if (st != TENMO_OK) return st;
         if (c.db && (st = tenmo_colsum_f32(ctx, (const float*)(at + db_part), Z.block_rows(), c.V, c.V, c.db, r0 ? 1.f : 0.f)) != TENMO_OK) return st;
     }

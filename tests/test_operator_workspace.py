@@ -1,0 +1,80 @@
+"""What the host code of the transformer operators does with its workspace: sizes, lifetimes and order, without a GPU."""
+import random
+import shutil
+
+import pytest
+
+from tests import fake_cuda
+
+MB = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def library(tmp_path_factory):
+    return fake_cuda.build(tmp_path_factory.mktemp("fake"))
+
+
+@pytest.fixture()
+def fake(library, tmp_path):
+    f = fake_cuda.Fake(shutil.copy(library, tmp_path))  # a copy: its state begins anew
+    yield f
+    f.handle.close()
+    assert f.misuse() == []
+
+
+def linear_ce(fake, N, D, V, tied=False, bias=False, forward_only=False, handle=None):
+    """The operands' addresses are never read here."""
+    from tenmo_b200 import make_mat
+
+    x = make_mat(1 << 40, (N, D), (D, 1))
+    w = make_mat(1 << 41, (D, V), (1, D) if tied else (V, 1))
+    args = (x, w, (1 << 42) if bias else 0, 1 << 43, True, N, D, V, -100, 0.0, 0, 1 << 44, (1 << 44) + 64)
+    h = handle or fake.handle
+    if forward_only:
+        h.linear_ce_fwd(*args)
+    else:
+        h.linear_ce_fwd_bwd(*args, 0, 1 << 45, 1 << 46, (1 << 47) if bias else 0)
+
+
+# rows, dim and classes whose last piece of the rows splits its product for dw into more slices than a whole piece
+MORE_SLICES_IN_THE_LAST_PIECE = [(38912, 576, 6300), (46080, 832, 5000), (151040, 1856, 1200), (50972, 1024, 4888)]
+
+
+def check_slices(fake):
+    """Every product cut into slices writes them inside the workspace: the fold reads (slices, M, ldp) floats from `partial`."""
+    seen = 0
+    for _, name, args in fake.launches():
+        if "h3_fold_kernel" in name:
+            partial, slices, M, N, ldp = args[:5]
+            assert fake.lib.fake_room_behind(partial) >= slices * M * ldp * 4, (slices, M, N)
+            seen += 1
+    fake.lib.fake_forget_launches()
+    return seen
+
+
+@pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
+@pytest.mark.parametrize("shape", MORE_SLICES_IN_THE_LAST_PIECE, ids=str)
+def test_slices_of_every_piece_fit_the_workspace(fake, shape, tied):
+    fake.watch("h3_fold_kernel", "PiqqqPqi")
+    linear_ce(fake, *shape, tied=tied)
+    assert check_slices(fake) > 0
+
+
+def test_slices_fit_over_the_range(fake):
+    """Sizes at random, most of them in several pieces, each from an empty workspace."""
+    from tenmo_b200 import TenmoCuda, TenmoError
+
+    rng = random.Random(1)
+    fake.watch("h3_fold_kernel", "PiqqqPqi")
+    seen = 0
+    for _ in range(3000):
+        D, V = 8 * int(2 ** rng.uniform(4, 8)), int(2 ** rng.uniform(9, 14))
+        N = int((128 << 20) / V * 2 ** rng.uniform(-3, 2))
+        handle = TenmoCuda(0, path=fake.path).require()
+        try:
+            linear_ce(fake, N, D, V, tied=rng.random() < 0.5, bias=rng.random() < 0.5, handle=handle)
+        except TenmoError as e:
+            assert e.status == -4  # more than the card holds
+        seen += check_slices(fake)
+        handle.close()
+    assert seen > 1000
