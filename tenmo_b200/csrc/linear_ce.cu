@@ -14,6 +14,7 @@
 
 #include "gemm_h3.cuh"
 #include "linear_few.cuh"
+#include "reduce.cuh"
 
 namespace {
 
@@ -342,15 +343,16 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     const size_t at_label = take(piece * sizeof(float)), numbers = c.grad ? take(piece * sizeof(float4)) : 0;
     const size_t row_loss = take(c.N * sizeof(float)), factor = take(sizeof(float));
     const size_t db_part = c.db ? take((size_t)((piece + H3_BLOCK - 1) / H3_BLOCK) * c.V * sizeof(float)) : 0;
-    size_t part = 0;  // for dx and dw of a whole piece and of the last one
+    size_t part = 0, db_sums = 0;  // for dx, dw and db of a whole piece and of the last one
     for (int64_t rows : {piece, c.N % piece}) {
         if (!c.grad || !rows) continue;
+        if (c.db) db_sums = max(db_sums, tenmo_colsum_own_bytes(ctx, (rows + H3_BLOCK - 1) / H3_BLOCK, c.V));
         const size_t dx = tenmo_h3_partial_bytes(ctx, rows, c.D, c.V);
         const size_t dw = tied ? tenmo_h3_partial_bytes(ctx, c.V, c.D, rows) : tenmo_h3_partial_bytes(ctx, c.D, c.V, rows);
         if (dx > part) part = dx;
         if (dw > part) part = dw;
     }
-    const size_t partial = take(part);
+    const size_t partial = take(part), db_scratch = take(db_sums);
     void* ws = nullptr;
     int st = tenmo_op_workspace(ctx, need, &ws);
     if (st != TENMO_OK) return st;
@@ -398,7 +400,7 @@ int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
         ew.add = r0 > 0;
         st = tied ? tenmo_h3_gemm(ctx, c.V, c.D, rows, Z, true, X, true, ew, at + partial, part) : tenmo_h3_gemm(ctx, c.D, c.V, rows, X, true, Z, true, ew, at + partial, part);
         if (st != TENMO_OK) return st;
-        if (c.db && (st = tenmo_colsum_f32(ctx, (const float*)(at + db_part), Z.block_rows(), c.V, c.V, c.db, r0 ? 1.f : 0.f)) != TENMO_OK) return st;
+        if (c.db && (st = tenmo_colsum_own(ctx, (const float*)(at + db_part), Z.block_rows(), c.V, c.V, c.db, r0 ? 1.f : 0.f, at + db_scratch)) != TENMO_OK) return st;
     }
     const int grid = c.reduction == 2 ? tenmo_stream_grid(ctx, c.N, 1024, 1) : 1;
     TENMO_CUDA_TRY(ctx, tenmo_launch(lce_loss_kernel, grid, 1024, 0, ctx->stream, ctx->pdl, (const float*)(at + row_loss), c.N, c.reduction,
@@ -439,7 +441,7 @@ int lce_run_few(tenmo_ctx* ctx, const LceCall& c) {
         if (st != TENMO_OK) return st;
         st = tied ? tenmo_few_outer(ctx, z, c.V, x, c.D, c.N, c.V, c.D, c.dw) : tenmo_few_outer(ctx, x, c.D, z, c.V, c.N, c.D, c.V, c.dw);
         if (st != TENMO_OK) return st;
-        if (c.db && (st = tenmo_colsum_f32(ctx, z, c.N, c.V, c.V, c.db, 0.f)) != TENMO_OK) return st;
+        if (c.db && (st = tenmo_colsum_own(ctx, z, c.N, c.V, c.V, c.db, 0.f, nullptr)) != TENMO_OK) return st;
     }
     const int grid = c.reduction == 2 ? tenmo_stream_grid(ctx, c.N, 1024, 1) : 1;
     TENMO_CUDA_TRY(ctx, tenmo_launch(lce_loss_kernel, grid, 1024, 0, ctx->stream, ctx->pdl, (const float*)row_loss, c.N, c.reduction, (const int32_t*)c.valid, c.loss));
@@ -461,9 +463,10 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     if (piece > c.N) piece = c.N;
     const size_t z_bytes = ((size_t)piece * c.V * sizeof(float) + 255) & ~(size_t)255;
     const size_t x_bytes = ((size_t)piece * c.D * sizeof(float) + 255) & ~(size_t)255;
-    const size_t l_bytes = ((size_t)c.N * sizeof(float) + 255) & ~(size_t)255;
+    const size_t l_bytes = ((size_t)c.N * sizeof(float) + 255) & ~(size_t)255, db_at = z_bytes + x_bytes + l_bytes + 256;
+    const size_t db_sums = c.db && piece ? max(tenmo_colsum_own_bytes(ctx, piece, c.V), tenmo_colsum_own_bytes(ctx, c.N % piece, c.V)) : 0;
     void* ws = nullptr;
-    if ((st = tenmo_op_workspace(ctx, z_bytes + x_bytes + l_bytes + 256, &ws)) != TENMO_OK) return st;
+    if ((st = tenmo_op_workspace(ctx, db_at + db_sums, &ws)) != TENMO_OK) return st;
     float* z = (float*)ws;
     float* xr = (float*)((char*)ws + z_bytes);
     float* row_loss = (float*)((char*)ws + z_bytes + x_bytes);
@@ -494,7 +497,7 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
         else
             st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, c.D, c.V, rows, &xt, &mz, c.dw, beta, nullptr, TENMO_ACT_NONE, nullptr, nullptr);
         if (st != TENMO_OK) return st;
-        if (c.db && (st = tenmo_colsum_f32(ctx, z, rows, c.V, c.V, c.db, beta)) != TENMO_OK) return st;
+        if (c.db && (st = tenmo_colsum_own(ctx, z, rows, c.V, c.V, c.db, beta, (char*)ws + db_at)) != TENMO_OK) return st;
     }
     if (c.N == 0 && c.grad) {
         TENMO_CUDA_TRY(ctx, cudaMemsetAsync(c.dw, 0, (size_t)c.D * c.V * sizeof(float), ctx->stream));

@@ -181,15 +181,12 @@ int tenmo_colsum_scratch(tenmo_ctx* ctx, int slabs, int64_t N, int strips, float
     return TENMO_OK;
 }
 
-extern "C" int tenmo_colsum_f32(tenmo_ctx* ctx, const float* x, int64_t M, int64_t N, int64_t ldx, float* out,
-                                float beta) {
-    TENMO_CHECK_CTX(ctx);
-    if (M < 0 || N < 0) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: negative shape");
-    if (beta != 0.f && beta != 1.f) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: beta must be 0 or 1");
-    if (N == 0) return TENMO_OK;
-    if (!out || (M > 0 && !x)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: NULL pointer");
-    if (M > 0 && ldx < N) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: ldx (%lld) < N (%lld)", (long long)ldx, (long long)N);
-    TENMO_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
+namespace {
+
+size_t own_tickets(int64_t N) { return ((size_t)((N + 31) / 32) * sizeof(unsigned int) + 255) & ~(size_t)255; }
+
+// `scratch` NULL: the context's workspace and tickets
+int colsum(tenmo_ctx* ctx, const float* x, int64_t M, int64_t N, int64_t ldx, float* out, float beta, void* scratch) {
     if (M <= TENMO_COLSUM_SEQ_ROWS) {
         const int grid = (int)((N + CS_THREADS - 1) / CS_THREADS);
         colsum_seq_kernel<<<grid, CS_THREADS, 0, ctx->stream>>>(x, M, N, ldx, out, beta);
@@ -201,9 +198,45 @@ extern "C" int tenmo_colsum_f32(tenmo_ctx* ctx, const float* x, int64_t M, int64
     tenmo_colsum_plan(ctx->sm_count, M, N, vec, &strips, &slabs, &rps);
     float* partials = nullptr;
     unsigned int* tickets = nullptr;
-    int st = tenmo_colsum_scratch(ctx, slabs, N, strips, &partials, &tickets);
-    if (st != TENMO_OK) return st;
+    if (scratch) {  // the tickets, which other uses of the scratch overwrite, then the partial sums
+        tickets = static_cast<unsigned int*>(scratch);
+        partials = reinterpret_cast<float*>(static_cast<char*>(scratch) + own_tickets(N));
+        TENMO_CUDA_TRY(ctx, cudaMemsetAsync(tickets, 0, (size_t)strips * sizeof(unsigned int), ctx->stream));
+    } else {
+        const int st = tenmo_colsum_scratch(ctx, slabs, N, strips, &partials, &tickets);
+        if (st != TENMO_OK) return st;
+    }
     return tenmo_colsum_launch(ctx, x, M, N, ldx, out, beta, partials, tickets, strips, slabs, rps, vec);
+}
+
+}  // namespace
+
+size_t tenmo_colsum_own_bytes(const tenmo_ctx* ctx, int64_t M, int64_t N) {
+    if (M <= TENMO_COLSUM_SEQ_ROWS) return 0;
+    int most = 0;
+    for (bool vec : {false, true}) {
+        int strips, slabs, rps;
+        tenmo_colsum_plan(ctx->sm_count, M, N, vec, &strips, &slabs, &rps);
+        if (slabs > most) most = slabs;
+    }
+    return own_tickets(N) + (size_t)most * (size_t)N * sizeof(float);
+}
+
+int tenmo_colsum_own(tenmo_ctx* ctx, const float* x, int64_t M, int64_t N, int64_t ldx, float* out, float beta, void* scratch) {
+    if (M > TENMO_COLSUM_SEQ_ROWS && !scratch) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: scratch is NULL");
+    return colsum(ctx, x, M, N, ldx, out, beta, scratch);
+}
+
+extern "C" int tenmo_colsum_f32(tenmo_ctx* ctx, const float* x, int64_t M, int64_t N, int64_t ldx, float* out,
+                                float beta) {
+    TENMO_CHECK_CTX(ctx);
+    if (M < 0 || N < 0) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: negative shape");
+    if (beta != 0.f && beta != 1.f) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: beta must be 0 or 1");
+    if (N == 0) return TENMO_OK;
+    if (!out || (M > 0 && !x)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: NULL pointer");
+    if (M > 0 && ldx < N) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "colsum: ldx (%lld) < N (%lld)", (long long)ldx, (long long)N);
+    TENMO_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
+    return colsum(ctx, x, M, N, ldx, out, beta, nullptr);
 }
 
 // ---------------------------------------------------------------------------------------------------

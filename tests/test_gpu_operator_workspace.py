@@ -22,3 +22,31 @@ def test_last_piece_takes_more_slices_than_a_whole_one():
         g._handle.close()
     finally:
         g._handle = shared
+
+
+@pytest.mark.parametrize("size", [(700, 100, 31), (70000, 256, 100)], ids=str)
+def test_captured_bias_gradient_survives_growth(size):
+    """A bias gradient summed over more than 512 rows (blocks of rows), captured; column sums of other calls grow what the library
+    shares before the replay."""
+    from tests import gpu_util as g
+
+    x, w, b, y = lce.make(*size, 33, bias=True)
+    lce.run(x, w, b, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        got = lce.run(x, w, b, y)
+    x2, w2, b2, y2 = lce.make(*size, 34, bias=True)
+    for t, new in ((x, x2), (w, w2), (b, b2), (y, y2)):
+        t.copy_(new)
+    for rows, cols in ((20000, 1 << 15), (600, 1 << 20)):
+        wide = torch.ones(rows, cols, device="cuda")
+        out = g.empty(cols)
+        g.handle().colsum(wide.data_ptr(), rows, cols, cols, out.data_ptr())
+        assert bool((out == rows).all())
+    graph.replay()
+    torch.cuda.synchronize()
+    want = lce.reference(x, w, b, y)
+    for n in ("loss", "dx", "dw", "db"):
+        lce.check(n, got[n], want[n])
+    g.handle().check_device_status()

@@ -78,3 +78,54 @@ def test_slices_fit_over_the_range(fake):
         seen += check_slices(fake)
         handle.close()
     assert seen > 1000
+
+
+# row sums of db above 512 rows, in the strict-fp32 form (rows) and in the tensor-core form (blocks of 128 rows)
+@pytest.mark.parametrize("shape", [(700, 100, 31), (100000, 256, 100)], ids=str)
+def test_a_captured_bias_gradient_keeps_its_scratch(fake, shape):
+    """Larger column sums after the capture grow the library's ordinary workspace and its tickets; what the graph uses stays allocated."""
+    fake.watch("colsum_split_kernel", "PqqqPfPPi")
+    linear_ce(fake, *shape, bias=True)
+    stream = fake.lib.fake_stream_create(0)
+    fake.handle.set_stream(stream)
+    fake.lib.fake_capture(stream, 1)
+    linear_ce(fake, *shape, bias=True)
+    fake.lib.fake_capture(stream, 0)
+    fake.handle.colsum(1 << 40, 100000, 1 << 19, 1 << 19, 1 << 41)
+    fake.handle.colsum(1 << 40, 1000, 1 << 22, 1 << 22, 1 << 41)
+    used = [args for i, name, args in fake.launches() if fake.captured(i) and "colsum_split_kernel" in name]
+    assert len(used) == 1
+    strips = -(-shape[2] // 32)
+    rows = shape[0] if shape[0] == 700 else -(-shape[0] // 128)
+    for x, M, N, _, _, _, partials, tickets, per_slab in used:
+        assert (M, N) == (rows, shape[2])
+        assert fake.lib.fake_room_behind(partials) >= -(-M // per_slab) * N * 4
+        assert fake.lib.fake_room_behind(tickets) >= strips * 4
+        assert fake.lib.fake_room_behind(x) >= M * N * 4
+
+
+def test_column_sums_fit_over_the_range(fake):
+    """Sizes at random whose bias gradient is summed over more than 512 rows, or over more than 512 blocks of rows."""
+    from tenmo_b200 import TenmoCuda
+
+    rng = random.Random(2)
+    fake.watch("colsum_split_kernel", "PqqqPfPPi")
+    seen = 0
+    for e in range(600):
+        if e % 2:
+            N = int(2 ** rng.uniform(9.1, 14))
+            V = int(2 ** rng.uniform(0, 20))
+            D = max(1, int(4e7 / N / V))
+        else:
+            N, V, D = int(2 ** rng.uniform(16, 22)), int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(6, 9))
+        handle = TenmoCuda(0, path=fake.path).require()
+        linear_ce(fake, N, D, V, tied=rng.random() < 0.5, bias=True, handle=handle)
+        for _, name, args in fake.launches():
+            if "colsum_split_kernel" in name:
+                x, M, n, _, _, _, partials, tickets, per_slab = args
+                assert fake.lib.fake_room_behind(partials) >= -(-M // per_slab) * n * 4, (N, D, V)
+                assert partials - tickets >= -(-n // 32) * 4 and partials >= x + M * n * 4
+                seen += 1
+        fake.lib.fake_forget_launches()
+        handle.close()
+    assert seen > 300
