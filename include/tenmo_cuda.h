@@ -368,8 +368,9 @@ int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
  *           (V, D); db V floats or NULL.  They are written, not added to.  upstream: 1 float (mean / sum) or N floats (none) on
  *           the device, NULL for 1.
  *           Outputs may not overlap an input or one another.
- * The logits of a piece of the rows at a time (at most 512 MB, or 256 rows) live in the workspace.  A class may be masked with a bias
- * of -inf or the lowest number (without label smoothing).  Results repeat bit for bit.
+ * The workspace holds a piece of the rows at a time, its logits and its rows of x (at most 512 MB each, or 256 rows), 4 bytes for every entry
+ * of w (rounded up to 128 x 128) where the products run on tensor cores, and the partial results of products with few tiles.  A class may
+ * be masked with a bias of -inf or the lowest number (without label smoothing).  Results repeat bit for bit.
  * Precision: sums in 32 bits (the loss over the rows in 64).  Larger problems multiply on tensor cores with every operand held to 22
  * bits, down to 2^-18 of the largest entry of its 128 x 128 block and to 2^-40 of that entry below. */
 int tenmo_linear_ce_fwd_f32(tenmo_ctx* ctx, const tenmo_mat* x, const tenmo_mat* w, const float* bias, const void* labels,

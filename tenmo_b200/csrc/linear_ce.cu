@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr size_t LCE_PIECE_BYTES = (size_t)512 << 20;  // logits of one piece
+constexpr size_t LCE_PIECE_BYTES = (size_t)512 << 20;  // logits (or statistics) of one piece, and as much for its rows of x
 constexpr int LCE_THREADS = 256;
 
 __device__ __forceinline__ int64_t lce_label(const void* labels, int is_i64, int64_t n) {
@@ -325,14 +325,18 @@ constexpr int LCE_FEW_MOST = 8 * TENMO_FEW_ROWS;  // rows of the few-row kernels
 // reduces them to two numbers per row and 64 columns.
 bool tc_profitable(const LceCall& c) { return c.N > TC_ROWS && 2.0 * c.N * c.D * c.V >= (c.N <= LCE_FEW_MOST ? TC_FLOP_FEW : TC_FLOP); }
 
+// rows of a piece, a multiple of `whole`: what takes z_row bytes a row and what takes x_row bytes each within the budget
+int64_t piece_rows(const LceCall& c, size_t z_row, size_t x_row, int64_t whole) {
+    const int64_t rows = (int64_t)(LCE_PIECE_BYTES / max(z_row, x_row)) / whole * whole;
+    return min(max(rows, whole), c.N);
+}
+
 int lce_run_tc(tenmo_ctx* ctx, const LceCall& c) {
     const int64_t vb = (c.V + H3_BLOCK - 1) / H3_BLOCK;
     const bool tied = c.w->row_stride == 1 && c.w->col_stride != 1;  // storage is (V, D)
-    // a piece's rows: logits (with a gradient) or statistics within the budget, whole tiles of 256 rows
-    const size_t per_row = c.grad ? (size_t)vb * H3_BLOCK * sizeof(float) : (size_t)vb * 2 * sizeof(float2);
-    int64_t piece = (int64_t)(LCE_PIECE_BYTES / per_row) / 256 * 256;
-    if (piece < 256) piece = 256;
-    if (piece > c.N) piece = c.N;
+    // whole tiles of 256 rows
+    const size_t x_row = (size_t)((c.D + H3_BLOCK - 1) / H3_BLOCK) * H3_BLOCK * sizeof(float);
+    const int64_t piece = piece_rows(c, c.grad ? (size_t)vb * H3_BLOCK * sizeof(float) : (size_t)vb * 2 * sizeof(float2), x_row, 256);
     TenmoH3Operand W = {nullptr, nullptr, tied ? c.V : c.D, tied ? c.D : c.V}, X = {nullptr, nullptr, piece, c.D}, Z = {nullptr, nullptr, piece, c.V};
     const int64_t groups = (c.V + 63) / 64;
     size_t need = 0;
@@ -458,9 +462,7 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     // 204x1884x28 forward 34 us for 81, 180x855x112 training 54 for 87, 100x768x1000 training 83 for 116; level at 300x128x1000,
     // behind at 512x512x300 (155 for 89).
     if (c.N > 0 && c.N <= LCE_FEW_MOST) return lce_run_few(ctx, c);
-    int64_t piece = (int64_t)(LCE_PIECE_BYTES / ((size_t)c.V * sizeof(float))) / 128 * 128;
-    if (piece < 128) piece = 128;
-    if (piece > c.N) piece = c.N;
+    const int64_t piece = piece_rows(c, (size_t)c.V * sizeof(float), (size_t)c.D * sizeof(float), 128);
     const size_t z_bytes = ((size_t)piece * c.V * sizeof(float) + 255) & ~(size_t)255;
     const size_t x_bytes = ((size_t)piece * c.D * sizeof(float) + 255) & ~(size_t)255;
     const size_t l_bytes = ((size_t)c.N * sizeof(float) + 255) & ~(size_t)255, db_at = z_bytes + x_bytes + l_bytes + 256;

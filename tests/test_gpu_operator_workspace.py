@@ -50,3 +50,12 @@ def test_captured_bias_gradient_survives_growth(size):
     for n in ("loss", "dx", "dw", "db"):
         lce.check(n, got[n], want[n])
     g.handle().check_device_status()
+
+
+@pytest.mark.parametrize("ls", [0.0, 0.1])
+def test_several_pieces_for_the_rows_of_x(ls):
+    """Few classes, so that the rows of x and not the logits end a piece (131,072 rows, then 8,928)."""
+    x, w, b, y = lce.make(140000, 1000, 60, 35, bias=True)
+    lce.compare(x, w, b, y, ls=ls)
+    loss = lce.run(x, w, b, y, ls=ls, forward_only=True)["loss"]
+    lce.check("loss", loss, lce.reference(x, w, b, y, ls=ls)["loss"])

@@ -129,3 +129,19 @@ def test_column_sums_fit_over_the_range(fake):
         fake.lib.fake_forget_launches()
         handle.close()
     assert seen > 300
+
+
+def largest_operands(N, D, V):
+    """Bytes beside a piece of the rows: the image of the weight, the row losses."""
+    up = lambda n: -(-n // 128) * 128
+    return 4 * up(D) * up(V) + 4 * N
+
+
+@pytest.mark.parametrize("shape,forward_only", [((1000000, 4096, 1000), True), ((1000000, 2048, 1000), True), ((1000000, 4096, 100), False),
+                                                ((3000000, 300, 10), False), ((1000000, 47, 1), False)], ids=str)
+def test_a_piece_counts_the_rows_of_x(fake, shape, forward_only):
+    """Few classes: many rows of logits fit the budget of a piece, but its copy of x has to fit one too.  (The slices of dx's and
+    dw's products, at most 32 of a piece's or the weight's size, come on top.)"""
+    N, D, V = shape
+    linear_ce(fake, *shape, bias=True, forward_only=forward_only)
+    assert fake.lib.fake_bytes_alive() < 3 * (512 * MB) + largest_operands(N, D, V)
