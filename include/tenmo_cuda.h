@@ -306,8 +306,10 @@ int tenmo_ce_fwd_bwd_f32(tenmo_ctx* ctx, const float* logits, int64_t ld_logits,
                          const float* upstream_dev, float* dlogits);
 
 /* ---- transformer operators ----------------------------------------------------------------------
- * They share a workspace of the context.  A call on another stream than the one before waits for that stream; graphs that were
- * captured from one context use the same workspace and must not be replayed at the same time (capture from two contexts for that).
+ * They share a workspace of the context.  A call on another stream than the one before waits for that stream.
+ * Graphs have a workspace apart from it, so a replay and calls outside of graphs may overlap.  But all graphs that were captured from one
+ * context share theirs: they must not be replayed at the same time (capture from two contexts for that).  The first replay has to come
+ * after the calls that were issued before the capture, whose block the graph may have taken over.
  * The first call of its size allocates, which a stream that is being captured refuses: run it once before.
  *
  * Layer normalisation over the last axis (layernorm.mojo of the reference; no GPU-side counterpart on this path):

@@ -41,12 +41,13 @@ struct tenmo_ctx {
     // workspace (grown on demand, never shrunk): lo planes for the 3xTF32 kernel, reduction partials
     void* ws = nullptr;
     size_t ws_bytes = 0;
-    // workspace of the transformer operators (tenmo_op_workspace).  A block that a captured CUDA graph uses is never freed
-    // before the context: growing puts it on the retired list.
+    // workspace of the transformer operators (tenmo_op_workspace): one block for calls that run, one for calls that are recorded into CUDA
+    // graphs.  A block that graphs hold is never freed before the context: a larger one for later graphs puts it on the retired list.
     void* op_ws = nullptr;
     size_t op_ws_bytes = 0;
-    bool op_ws_captured = false;
-    void* op_retired[16] = {nullptr};
+    void* op_graph_ws = nullptr;
+    size_t op_graph_bytes = 0;
+    void** op_retired = nullptr;
     int n_op_retired = 0;
     // The stream of the last call that used it, and an event on that stream: a call on another stream waits for it.
     cudaStream_t op_stream = nullptr;

@@ -1,4 +1,6 @@
 // Context lifetime, error strings, stream binding, workspace.
+#include <cstdlib>
+
 #include "common.cuh"
 #include "op_util.cuh"
 
@@ -58,28 +60,45 @@ static cudaError_t record_op_event(tenmo_ctx* ctx) {
     return e;
 }
 
-int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    const bool capturing = cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
-    if (bytes > ctx->op_ws_bytes) {
-        if (capturing)
+// A call that is being captured: it keeps its block as long as the context lives, apart from what calls outside graphs use.
+static int op_graph_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
+    if (bytes > ctx->op_graph_bytes) {  // the capture forbids an allocation: the graphs take over the block of the calls before
+        if (bytes > ctx->op_ws_bytes)
             return tenmo_set_error(ctx, TENMO_ERR_STATE,
                                    "the workspace must grow to %zu bytes but the stream is capturing: run the call once outside the capture first",
                                    bytes);
+        if (ctx->op_graph_ws) {
+            void** list = (void**)realloc(ctx->op_retired, (ctx->n_op_retired + 1) * sizeof(void*));
+            if (!list) return tenmo_set_error(ctx, TENMO_ERR_NOMEM, "no host memory for the list of workspaces");
+            ctx->op_retired = list;
+            ctx->op_retired[ctx->n_op_retired++] = ctx->op_graph_ws;
+        }
+        ctx->op_graph_ws = ctx->op_ws;
+        ctx->op_graph_bytes = ctx->op_ws_bytes;
+        ctx->op_ws = nullptr;
+        ctx->op_ws_bytes = 0;
+    }
+    *out = ctx->op_graph_ws;
+    return TENMO_OK;
+}
+
+int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) return op_graph_workspace(ctx, bytes, out);
+    if (bytes > ctx->op_ws_bytes) {
         if (ctx->op_ws) {
-            const int slots = (int)(sizeof(ctx->op_retired) / sizeof(ctx->op_retired[0]));
-            if (ctx->op_ws_captured && ctx->n_op_retired == slots)
-                return tenmo_set_error(ctx, TENMO_ERR_STATE, "the workspace has grown %d times between graph captures: make the largest call first", slots);
             cudaError_t e = sync_bound_streams(ctx);  // the old block may be in use on any stream the context was bound to
             if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace sync: %s", cudaGetErrorString(e));
-            if (ctx->op_ws_captured) ctx->op_retired[ctx->n_op_retired++] = ctx->op_ws;
-            else cudaFree(ctx->op_ws);
+            cudaFree(ctx->op_ws);
             ctx->op_ws = nullptr;
             ctx->op_ws_bytes = 0;
-            ctx->op_ws_captured = false;
         }
         const size_t want = (bytes + ((size_t)1 << 20) - 1) & ~(((size_t)1 << 20) - 1);
+        // another stream may be in the middle of a capture that has just taken the block before: an allocation does not concern it
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool exchanged = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
         cudaError_t e = cudaMalloc(&ctx->op_ws, want);
+        if (exchanged) cudaThreadExchangeStreamCaptureMode(&mode);
         if (e != cudaSuccess) {
             cudaGetLastError();
             ctx->op_ws = nullptr;
@@ -87,24 +106,20 @@ int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
         }
         ctx->op_ws_bytes = want;
     }
-    if (capturing) {
-        ctx->op_ws_captured = true;
-    } else {
-        // the call before may still be running on another stream
-        if (ctx->op_used && ctx->op_stream != ctx->stream) {
-            cudaError_t e = cudaSuccess;
-            if (!ctx->op_recorded) {
-                if (cudaStreamIsCapturing(ctx->op_stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone)
-                    return tenmo_set_error(ctx, TENMO_ERR_STATE, "the stream of the last call that used the workspace is being captured");
-                e = record_op_event(ctx);
-            }
-            if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->stream, ctx->op_event, 0);
-            if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace order: %s", cudaGetErrorString(e));
+    // the call before may still be running on another stream
+    if (ctx->op_used && ctx->op_stream != ctx->stream) {
+        cudaError_t e = cudaSuccess;
+        if (!ctx->op_recorded) {
+            if (cudaStreamIsCapturing(ctx->op_stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone)
+                return tenmo_set_error(ctx, TENMO_ERR_STATE, "the stream of the last call that used the workspace is being captured");
+            e = record_op_event(ctx);
         }
-        ctx->op_stream = ctx->stream;
-        ctx->op_used = true;
-        ctx->op_recorded = false;
+        if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->stream, ctx->op_event, 0);
+        if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace order: %s", cudaGetErrorString(e));
     }
+    ctx->op_stream = ctx->stream;
+    ctx->op_used = true;
+    ctx->op_recorded = false;
     *out = ctx->op_ws;
     return TENMO_OK;
 }
@@ -207,7 +222,9 @@ void tenmo_cuda_destroy(tenmo_ctx* ctx) {
     if (ctx->ws) cudaFree(ctx->ws);
     if (ctx->op_event) cudaEventDestroy(ctx->op_event);
     if (ctx->op_ws) cudaFree(ctx->op_ws);
+    if (ctx->op_graph_ws) cudaFree(ctx->op_graph_ws);
     for (int i = 0; i < ctx->n_op_retired; ++i) cudaFree(ctx->op_retired[i]);
+    free(ctx->op_retired);
     if (ctx->dev_status) cudaFree(ctx->dev_status);
     if (ctx->tickets) cudaFree(ctx->tickets);
     if (ctx->sgd_desc_dev) cudaFree(ctx->sgd_desc_dev);

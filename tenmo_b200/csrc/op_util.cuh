@@ -17,5 +17,6 @@ struct TenmoDeviceGuard {
 };
 
 // A second workspace block, apart from the one of tenmo_workspace: these operators call the library's GEMMs while they
-// hold intermediate results.  Same rules: grown on demand, refused while the stream is being captured.
+// hold intermediate results.  Grown on demand; a call that is being captured takes a block that has been used at its size before (else it is
+// refused) and keeps it for its graph, so that a replay never meets a call outside of graphs.
 int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out);

@@ -42,6 +42,7 @@ uintptr_t next_address = 0x100000000000ull;
 unsigned long long next_id = 2;
 uintptr_t next_handle = 0x5000;
 size_t bytes_alive = 0;
+cudaStreamCaptureMode mode = cudaStreamCaptureModeGlobal;  // of the calling thread
 constexpr size_t MEMORY = (size_t)180 << 30;
 
 void merge(Clock& to, const Clock& from) {
@@ -126,7 +127,7 @@ void fake_capture(uintptr_t handle, int on) { find((cudaStream_t)handle, "captur
 
 // ---- memory ----
 cudaError_t cudaMalloc(void** p, size_t n) {
-    if (capturing()) return while_capturing("cudaMalloc");
+    if (capturing() && mode != cudaStreamCaptureModeRelaxed) return while_capturing("cudaMalloc");
     if (bytes_alive + n > MEMORY) return cudaErrorMemoryAllocation;
     *p = (void*)next_address;
     alive[next_address] = n;
@@ -189,6 +190,12 @@ const char* cudaGetErrorString(cudaError_t) { return "error of the runtime witho
 cudaError_t cudaFuncSetAttribute(const void*, cudaFuncAttribute, int) { return cudaSuccess; }
 
 // ---- streams and events ----
+cudaError_t cudaThreadExchangeStreamCaptureMode(cudaStreamCaptureMode* m) {
+    const cudaStreamCaptureMode before = mode;
+    mode = *m;
+    *m = before;
+    return cudaSuccess;
+}
 cudaError_t cudaStreamCreateWithFlags(cudaStream_t* s, unsigned) { *s = (cudaStream_t)fake_stream_create(0); return cudaSuccess; }
 cudaError_t cudaStreamDestroy(cudaStream_t s) {
     if (!find(s, "cudaStreamDestroy")) return cudaErrorContextIsDestroyed;

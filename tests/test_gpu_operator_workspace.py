@@ -59,3 +59,56 @@ def test_several_pieces_for_the_rows_of_x(ls):
     lce.compare(x, w, b, y, ls=ls)
     loss = lce.run(x, w, b, y, ls=ls, forward_only=True)["loss"]
     lce.check("loss", loss, lce.reference(x, w, b, y, ls=ls)["loss"])
+
+
+def test_replays_beside_eager_calls():
+    """A training step of attention and the head, captured, replayed on one stream while the same operators run eagerly on another, with
+    nothing that orders the two: both give what they give alone."""
+    from tests import gpu_util as g
+    from tests import test_gpu_fused_attention as att
+
+    gen = torch.Generator(device="cuda").manual_seed(36)
+    a = [att._make(gen, 8, 8, 512, 64) for _ in range(4)]
+    b = [att._make(gen, 8, 8, 500, 64) for _ in range(4)]
+    head_a, head_b = lce.make(2000, 256, 4000, 37, bias=True), lce.make(2100, 256, 3900, 38, bias=True)
+    step = lambda qkv, head: (att.run(*qkv), lce.run(*head))
+    want = step(a, head_a), step(b, head_b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def forward_and_backward(qkv, out, stats):
+        from tenmo_b200 import make_heads
+
+        q, k, v, go = qkv
+        view = lambda t: make_heads(t.data_ptr(), t.stride())
+        shape = (*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
+        h = g.handle()
+        h.attention_fwd(shape, view(q), view(k), view(v), view(out["o"]), stats.data_ptr(), 0.125)
+        h.attention_bwd(shape, view(q), view(k), view(v), view(out["o"]), stats.data_ptr(), view(go), view(out["dq"]), view(out["dk"]),
+                        view(out["dv"]), 0.125)
+    fresh = lambda qkv: (dict(zip(("o", "dq", "dk", "dv"), (torch.full_like(t, float("nan")) for t in qkv))), g.empty(*qkv[0].shape[:3], 2))
+    out_a, stats_a = fresh(a)
+    with torch.cuda.graph(graph, stream=stream):
+        forward_and_backward(a, out_a, stats_a)
+        head_out = lce.run(*head_a)
+    outs = [fresh(b) for _ in range(12)]
+    torch.cuda.synchronize()
+    eager_heads = []
+    for out, stats in outs:
+        with torch.cuda.stream(stream):
+            graph.replay()
+        with torch.cuda.stream(other):
+            forward_and_backward(b, out, stats)
+            eager_heads.append(lce.run(*head_b))
+    torch.cuda.synchronize()
+    for name, t in out_a.items():
+        assert torch.equal(t, want[0][0][name]), name
+    for name, t in head_out.items():
+        assert torch.equal(t, want[0][1][name]), name
+    for (out, _), head in zip(outs, eager_heads):
+        for name, t in out.items():
+            assert torch.equal(t, want[1][0][name]), name
+        for name, t in head.items():
+            assert torch.equal(t, want[1][1][name]), name
+    g.handle().check_device_status()

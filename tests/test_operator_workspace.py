@@ -145,3 +145,80 @@ def test_a_piece_counts_the_rows_of_x(fake, shape, forward_only):
     N, D, V = shape
     linear_ce(fake, *shape, bias=True, forward_only=forward_only)
     assert fake.lib.fake_bytes_alive() < 3 * (512 * MB) + largest_operands(N, D, V)
+
+
+# ---- graphs beside eager calls ----
+def layer_norm_bwd(fake, C=512, M=4096):
+    """A call that uses the workspace; returns where (its partial sums begin there)."""
+    fake.handle.layernorm_bwd(1 << 40, C, 1 << 41, 1 << 42, 1 << 43, 1 << 43, 1 << 44, 1 << 45, 1 << 46, M, C)
+    i, _, args = [l for l in fake.launches() if "ln_fold_kernel" in l[1]][-1]
+    return args[0], args[1] * 2 * C * 4, i
+
+
+def captured(fake, call, stream=None):
+    stream = stream or fake.lib.fake_stream_create(0)
+    fake.handle.set_stream(stream)
+    fake.lib.fake_capture(stream, 1)
+    try:
+        return call()
+    finally:
+        fake.lib.fake_capture(stream, 0)
+        fake.handle.set_stream(None)
+
+
+def overlap(a, b):
+    return a[0] < b[0] + b[1] and b[0] < a[0] + a[1]
+
+
+def test_eager_calls_stay_off_a_captured_block(fake):
+    """A replay and an eager call on another stream are not ordered by anything: they must not share a block."""
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    layer_norm_bwd(fake)
+    graph = captured(fake, lambda: layer_norm_bwd(fake))
+    for C in (512, 64, 4096, 512):
+        assert not overlap(graph, layer_norm_bwd(fake, C))
+    assert fake.lib.fake_room_behind(graph[0]) >= graph[1]
+
+
+def test_captures_and_eager_calls_in_turn(fake):
+    """Two blocks serve them however often they alternate; a larger capture takes a larger block, and every graph keeps its own."""
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    layer_norm_bwd(fake)
+    captured(fake, lambda: layer_norm_bwd(fake))
+    layer_norm_bwd(fake)
+    before = fake.lib.fake_bytes_alive()
+    for _ in range(40):
+        captured(fake, lambda: layer_norm_bwd(fake))
+        layer_norm_bwd(fake)
+    assert fake.lib.fake_bytes_alive() == before
+    graphs = []
+    for n in range(40):
+        eager = layer_norm_bwd(fake, 512 + 256 * n)
+        graphs.append(captured(fake, lambda: layer_norm_bwd(fake, 512 + 256 * n)))
+        assert fake.lib.fake_room_behind(eager[0]) >= eager[1]
+        for g in graphs:
+            assert fake.lib.fake_room_behind(g[0]) >= g[1] and not overlap(g, layer_norm_bwd(fake, 64))
+
+
+def test_a_capture_larger_than_every_call_before_is_refused(fake):
+    from tenmo_b200 import TenmoError
+
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    layer_norm_bwd(fake, 64)
+    with pytest.raises(TenmoError) as e:
+        captured(fake, lambda: layer_norm_bwd(fake, 4096))
+    assert e.value.status == -7
+    layer_norm_bwd(fake, 4096)
+    captured(fake, lambda: layer_norm_bwd(fake, 4096))
+
+
+def test_an_eager_call_beside_a_capture_in_progress(fake):
+    """The block went to the graph a moment ago; the eager call gets another although a stream is being captured."""
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    layer_norm_bwd(fake)
+
+    def call():
+        graph = layer_norm_bwd(fake)
+        fake.handle.set_stream(None)
+        assert not overlap(graph, layer_norm_bwd(fake))
+    captured(fake, call)
