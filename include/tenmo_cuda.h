@@ -19,8 +19,8 @@
  *     and one set of stream-K fix-up flags, so calls that use them (the GEMMs, the column sums, cross-entropy) must
  *     not be in flight on two streams of the same context at once.  Rebinding the context to another stream between
  *     calls is fine when the streams are ordered by events (a side stream that only runs the gradient exchange and
- *     the optimiser, as the trainers do); the library waits for the eight most recently bound streams before it
- *     frees and regrows the workspace and before it reads the status word.  A call that must grow the workspace while
+ *     the optimiser, as the trainers do); the library waits for the eight most recently bound streams, which must still exist,
+ *     before it frees and regrows the workspace and before it reads the status word.  A call that must grow the workspace while
  *     its stream is being captured into a CUDA graph returns TENMO_ERR_STATE: run it once outside the capture first.
  */
 #ifndef TENMO_CUDA_H
@@ -306,7 +306,8 @@ int tenmo_ce_fwd_bwd_f32(tenmo_ctx* ctx, const float* logits, int64_t ld_logits,
                          const float* upstream_dev, float* dlogits);
 
 /* ---- transformer operators ----------------------------------------------------------------------
- * They share a workspace of the context.  A call on another stream than the one before waits for that stream.
+ * They share a workspace of the context.  A call on another stream than the one before waits for that call (the host waits for the device
+ * once, the first time that this happens); a stream may be destroyed when its calls have returned.
  * Graphs have a workspace apart from it, so a replay and calls outside of graphs may overlap.  But all graphs that were captured from one
  * context share theirs: they must not be replayed at the same time (capture from two contexts for that).  The first replay has to come
  * after the calls that were issued before the capture, whose block the graph may have taken over.

@@ -49,10 +49,11 @@ struct tenmo_ctx {
     size_t op_graph_bytes = 0;
     void** op_retired = nullptr;
     int n_op_retired = 0;
-    // The stream of the last call that used it, and an event on that stream: a call on another stream waits for it.
-    cudaStream_t op_stream = nullptr;
+    // Order of the calls that use op_ws.  The caller may destroy a stream as soon as a call has returned, so no handle is kept: what is kept is
+    // the stream's id, and an event that each call records at its end from the second stream on (op_many).
+    unsigned long long op_stream_id = 0;
     cudaEvent_t op_event = nullptr;
-    bool op_used = false, op_recorded = false;
+    bool op_used = false, op_many = false, op_recorded = false, op_open = false;
     // small fixed device scratch: [0] status word, [8..15] cross-entropy tickets/accumulators
     uint32_t* dev_status = nullptr;
     // ticket counters of the split column-sum kernel: zero between calls (the last CTA resets its own)

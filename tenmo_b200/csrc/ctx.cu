@@ -53,13 +53,6 @@ int tenmo_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
     return TENMO_OK;
 }
 
-static cudaError_t record_op_event(tenmo_ctx* ctx) {
-    cudaError_t e = ctx->op_event ? cudaSuccess : cudaEventCreateWithFlags(&ctx->op_event, cudaEventDisableTiming);
-    if (e == cudaSuccess) e = cudaEventRecord(ctx->op_event, ctx->op_stream);
-    ctx->op_recorded = e == cudaSuccess;
-    return e;
-}
-
 // A call that is being captured: it keeps its block as long as the context lives, apart from what calls outside graphs use.
 static int op_graph_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
     if (bytes > ctx->op_graph_bytes) {  // the capture forbids an allocation: the graphs take over the block of the calls before
@@ -87,7 +80,7 @@ int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
     if (cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) return op_graph_workspace(ctx, bytes, out);
     if (bytes > ctx->op_ws_bytes) {
         if (ctx->op_ws) {
-            cudaError_t e = sync_bound_streams(ctx);  // the old block may be in use on any stream the context was bound to
+            cudaError_t e = cudaDeviceSynchronize();  // the old block may be in use on a stream that the context has left
             if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace sync: %s", cudaGetErrorString(e));
             cudaFree(ctx->op_ws);
             ctx->op_ws = nullptr;
@@ -106,22 +99,32 @@ int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out) {
         }
         ctx->op_ws_bytes = want;
     }
-    // the call before may still be running on another stream
-    if (ctx->op_used && ctx->op_stream != ctx->stream) {
-        cudaError_t e = cudaSuccess;
-        if (!ctx->op_recorded) {
-            if (cudaStreamIsCapturing(ctx->op_stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone)
-                return tenmo_set_error(ctx, TENMO_ERR_STATE, "the stream of the last call that used the workspace is being captured");
-            e = record_op_event(ctx);
-        }
-        if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->stream, ctx->op_event, 0);
-        if (e != cudaSuccess) return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace order: %s", cudaGetErrorString(e));
+    // The call before may still be running on another stream: its event is waited for.  The first time that the stream changes there is none.
+    unsigned long long id = 0;
+    cudaError_t e = cudaStreamGetId(ctx->stream, &id);
+    if (e == cudaSuccess && ctx->op_used && id != ctx->op_stream_id) {
+        e = ctx->op_recorded ? cudaStreamWaitEvent(ctx->stream, ctx->op_event, 0) : cudaDeviceSynchronize();
+        ctx->op_many = true;
     }
-    ctx->op_stream = ctx->stream;
-    ctx->op_used = true;
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return tenmo_set_error(ctx, TENMO_ERR_CUDA, "workspace order: %s", cudaGetErrorString(e));
+    }
+    ctx->op_stream_id = id;
+    ctx->op_used = ctx->op_open = true;
     ctx->op_recorded = false;
     *out = ctx->op_ws;
     return TENMO_OK;
+}
+
+void tenmo_op_done(tenmo_ctx* ctx) {
+    if (!ctx->op_open) return;
+    ctx->op_open = false;
+    if (!ctx->op_many) return;
+    cudaError_t e = ctx->op_event ? cudaSuccess : cudaEventCreateWithFlags(&ctx->op_event, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventRecord(ctx->op_event, ctx->stream);
+    ctx->op_recorded = e == cudaSuccess;  // else a change of the stream waits for the device
+    if (e != cudaSuccess) cudaGetLastError();
 }
 
 void tenmo_prof_before(tenmo_ctx* ctx) {
@@ -241,18 +244,7 @@ const char* tenmo_cuda_last_error(tenmo_ctx* ctx) { return ctx ? ctx->err : g_in
 
 int tenmo_cuda_set_stream(tenmo_ctx* ctx, void* cuda_stream) {
     TENMO_CHECK_CTX(ctx);
-    cudaStream_t next = cuda_stream == TENMO_STREAM_OWN ? ctx->own_stream : (cudaStream_t)cuda_stream;
-    // The operators' workspace goes with the context: note how far the stream that used it last has come, while the caller still has
-    // that stream.  A stream that is being captured is left alone (a graph's order is its owner's).
-    if (ctx->op_used && ctx->op_stream == ctx->stream && next != ctx->stream) {
-        TenmoDeviceGuard guard(ctx);
-        cudaStreamCaptureStatus a = cudaStreamCaptureStatusNone, b = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(ctx->stream, &a) == cudaSuccess && cudaStreamIsCapturing(next, &b) == cudaSuccess &&
-            a == cudaStreamCaptureStatusNone && b == cudaStreamCaptureStatusNone)
-            record_op_event(ctx);
-        cudaGetLastError();  // what failed here is tried again by the next call that needs it
-    }
-    ctx->stream = next;
+    ctx->stream = cuda_stream == TENMO_STREAM_OWN ? ctx->own_stream : (cudaStream_t)cuda_stream;
     // remember the streams the context has run on (most recent first): a workspace growth and the status check wait for them
     int at = -1;
     for (int i = 0; i < ctx->n_bound; ++i)

@@ -318,7 +318,7 @@ int tenmo_layernorm_fwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const f
     if (!(eps >= 0.f)) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "layernorm_fwd: eps must be >= 0");
     if (M == 0) return TENMO_OK;
     if (!x || !gamma || !bias || !y) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "layernorm_fwd: null pointer");
-    TenmoDeviceGuard guard(ctx);
+    TenmoOpCall call(ctx);
     const LnFwd p{x, gamma, bias, y, mean, rstd, ldx, M, (int)C, eps, 1.f / (float)C};
     const bool vec = C % 4 == 0 && ldx % 4 == 0 && aligned16(x) && aligned16(gamma) && aligned16(bias) && aligned16(y);
     const int threads = row_threads(C);
@@ -344,7 +344,7 @@ int tenmo_layernorm_bwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const f
     if (M < 0 || C < 1 || C > INT32_MAX / 2 || ldx < C)
         return tenmo_set_error(ctx, TENMO_ERR_INVALID, "layernorm_bwd: M=%lld C=%lld ldx=%lld", (long long)M, (long long)C, (long long)ldx);
     if (beta != 0.f && beta != 1.f) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "layernorm_bwd: beta must be 0 or 1");
-    TenmoDeviceGuard guard(ctx);
+    TenmoOpCall call(ctx);
     if (M == 0) {  // sums over no rows
         if (beta == 0.f && dgamma) TENMO_CUDA_TRY(ctx, cudaMemsetAsync(dgamma, 0, C * sizeof(float), ctx->stream));
         if (beta == 0.f && dbias) TENMO_CUDA_TRY(ctx, cudaMemsetAsync(dbias, 0, C * sizeof(float), ctx->stream));

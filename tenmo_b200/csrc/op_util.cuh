@@ -20,3 +20,12 @@ struct TenmoDeviceGuard {
 // hold intermediate results.  Grown on demand; a call that is being captured takes a block that has been used at its size before (else it is
 // refused) and keeps it for its graph, so that a replay never meets a call outside of graphs.
 int tenmo_op_workspace(tenmo_ctx* ctx, size_t bytes, void** out);
+void tenmo_op_done(tenmo_ctx* ctx);
+
+// Held by an entry point for its length: the context's device is current, and at the end it is noted how far the workspace is used.
+struct TenmoOpCall {
+    tenmo_ctx* const ctx;
+    TenmoDeviceGuard device;
+    explicit TenmoOpCall(tenmo_ctx* c) : ctx(c), device(c) {}
+    ~TenmoOpCall() { tenmo_op_done(ctx); }
+};

@@ -37,7 +37,7 @@ std::vector<Launch> launches;
 std::vector<Watch> watches;
 std::vector<Config> configs;
 std::vector<std::string> misuse;
-Clock host;
+Clock host, gone;  // gone: what destroyed streams had been given
 uintptr_t next_address = 0x100000000000ull;
 unsigned long long next_id = 2;
 uintptr_t next_handle = 0x5000;
@@ -119,6 +119,7 @@ int fake_misuse() { return (int)misuse.size(); }
 const char* fake_misuse_text(int i) { return misuse[i].c_str(); }
 uintptr_t fake_stream_create(uintptr_t handle) {  // 0: a new handle
     if (!handle) handle = next_handle += 16;
+    else if (streams.count((cudaStream_t)handle)) merge(gone, streams[(cudaStream_t)handle].clock);
     streams[(cudaStream_t)handle] = Stream{next_id++, true, false, {}};
     return handle;
 }
@@ -178,6 +179,7 @@ cudaError_t cudaDeviceGetAttribute(int* v, cudaDeviceAttr, int) { *v = 1965000; 
 cudaError_t cudaDeviceSynchronize() {
     if (capturing()) return while_capturing("cudaDeviceSynchronize");
     for (auto& s : streams) merge(host, s.second.clock);  // a destroyed stream's work too
+    merge(host, gone);
     return cudaSuccess;
 }
 cudaError_t cudaGetDriverEntryPoint(const char*, void** fn, unsigned long long, cudaDriverEntryPointQueryResult* q) {

@@ -112,3 +112,51 @@ def test_replays_beside_eager_calls():
         for name, t in head.items():
             assert torch.equal(t, want[1][1][name]), name
     g.handle().check_device_status()
+
+
+def test_a_stream_destroyed_behind_its_calls():
+    """The context is bound to a stream of the caller's, which is destroyed while a long call may still be running on it; the next call, on
+    another stream, uses the workspace after it."""
+    import ctypes
+
+    from tenmo_b200 import TenmoCuda
+    from tests import gpu_util as g
+    from tests import test_gpu_layernorm as ln
+
+    runtime = ctypes.CDLL("libcudart.so.12")
+    shared, h = g._handle, TenmoCuda(0).require()
+    try:
+        long, short = ln._inputs(200000, 1024, 39), ln._inputs(100, 1024, 40)
+
+        def call(x, gamma, bias, dy, out):
+            M, C = x.shape
+            h.layernorm_fwd(x.data_ptr(), C, gamma.data_ptr(), bias.data_ptr(), 1e-5, out["y"].data_ptr(), out["mean"].data_ptr(), out["rstd"].data_ptr(), M, C)
+            h.layernorm_bwd(x.data_ptr(), C, dy.data_ptr(), gamma.data_ptr(), out["mean"].data_ptr(), out["rstd"].data_ptr(), out["dx"].data_ptr(),
+                            out["dgamma"].data_ptr(), out["dbias"].data_ptr(), M, C)
+
+        def room(x, *_):
+            M, C = x.shape
+            return dict(y=g.empty(M, C), dx=g.empty(M, C), dgamma=g.empty(C), dbias=g.empty(C), mean=g.empty(M), rstd=g.empty(M))
+        want = []
+        for inputs in (long, short):
+            want.append(room(*inputs))
+            h.set_stream(torch.cuda.current_stream().cuda_stream)
+            call(*inputs, want[-1])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            got = [room(*inputs) for inputs in (long, short)]
+            torch.cuda.synchronize()
+            stream = ctypes.c_void_p()
+            assert runtime.cudaStreamCreateWithFlags(ctypes.byref(stream), 1) == 0
+            h.set_stream(stream.value)
+            call(*long, got[0])
+            assert runtime.cudaStreamDestroy(stream) == 0
+            h.set_stream(None)
+            call(*short, got[1])
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                for name in a:
+                    assert torch.equal(a[name], b[name]), name
+        h.close()
+    finally:
+        g._handle = shared

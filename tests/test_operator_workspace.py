@@ -222,3 +222,84 @@ def test_an_eager_call_beside_a_capture_in_progress(fake):
         fake.handle.set_stream(None)
         assert not overlap(graph, layer_norm_bwd(fake))
     captured(fake, call)
+
+
+# ---- streams ----
+def first_and_last(fake, call):
+    """The launches of a call: its first and its last one."""
+    n = fake.lib.fake_launches()
+    call()
+    assert fake.lib.fake_launches() > n
+    return n, fake.lib.fake_launches() - 1
+
+
+def test_calls_on_several_streams_wait_for_one_another(fake):
+    streams = [0] + [fake.lib.fake_stream_create(0) for _ in range(3)]
+    before = None
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    for n in (0, 1, 1, 2, 0, 0, 3, 2, 1):
+        fake.handle.set_stream(streams[n])
+        at = first_and_last(fake, lambda: layer_norm_bwd(fake, 64 + 8 * n))
+        assert before is None or fake.comes_before(before, at[0])
+        before = at[1]
+
+
+@pytest.mark.parametrize("used_before", [False, True], ids=["one stream so far", "several streams so far"])
+def test_a_destroyed_stream_is_not_touched(fake, used_before):
+    """A caller may destroy a stream as soon as its calls have returned: nothing may use the handle again, and what still runs there comes
+    before the next call."""
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    if used_before:
+        layer_norm_bwd(fake, 64)
+    stream = fake.lib.fake_stream_create(0)
+    fake.handle.set_stream(stream)
+    a = first_and_last(fake, lambda: layer_norm_bwd(fake, 512))
+    fake.lib.fake_stream_destroy(stream)
+    fake.handle.set_stream(None)
+    b = first_and_last(fake, lambda: layer_norm_bwd(fake, 512))
+    assert fake.comes_before(a[1], b[0])
+    c = first_and_last(fake, lambda: layer_norm_bwd(fake, 8000))  # the workspace grows
+    assert fake.comes_before(b[1], c[0])
+    assert fake.misuse() == []
+
+
+def test_a_handle_that_is_used_again_is_another_stream(fake):
+    """A new stream can get the address of one that was destroyed while its work was still running."""
+    fake.watch("ln_fold_kernel", "PiiPPi")
+    stream = fake.lib.fake_stream_create(0)
+    fake.handle.set_stream(stream)
+    a = first_and_last(fake, lambda: layer_norm_bwd(fake))
+    fake.lib.fake_stream_destroy(stream)
+    assert fake.lib.fake_stream_create(stream) == stream
+    fake.handle.set_stream(stream)
+    b = first_and_last(fake, lambda: layer_norm_bwd(fake))
+    assert fake.comes_before(a[1], b[0])
+
+
+def test_every_operator_orders_its_workspace(fake):
+    """Each entry point that uses the workspace, on one stream and then another."""
+    from tenmo_b200 import make_heads
+
+    streams = [fake.lib.fake_stream_create(0) for _ in range(2)]
+    fake.watch("ln_fold_kernel", "PiiPPi")
+
+    def attention(q_len, k_len, H, backward):
+        B, D, Hkv = 2, 64, H // 2
+        view = lambda at, heads, n: make_heads(at << 40, (heads * n * D, n * D, D))
+        q, k, v, o = view(1, H, q_len), view(2, Hkv, k_len), view(3, Hkv, k_len), view(4, H, q_len)
+        shape = (B, H, Hkv, q_len, k_len, D)
+        if backward:
+            fake.handle.attention_bwd(shape, q, k, v, o, 5 << 40, view(6, H, q_len), view(7, H, q_len), view(8, Hkv, k_len), view(9, Hkv, k_len), 0.125)
+        else:
+            fake.handle.attention_fwd(shape, q, k, v, o, 5 << 40, 0.125)
+    calls = [lambda: attention(1, 4000, 4, False), lambda: attention(600, 600, 8, False), lambda: attention(20, 20, 4, True),
+             lambda: attention(600, 600, 8, True), lambda: layer_norm_bwd(fake), lambda: linear_ce(fake, 20, 30, 40),
+             lambda: linear_ce(fake, 300, 30, 400, bias=True), lambda: linear_ce(fake, 3000, 300, 4000, bias=True),
+             lambda: linear_ce(fake, 3000, 300, 4000, forward_only=True)]
+    before = None
+    for call in calls + calls[::-1] + calls:
+        fake.handle.set_stream(streams[0])
+        streams.reverse()
+        at = first_and_last(fake, call)
+        assert before is None or fake.comes_before(before, at[0])
+        before = at[1]
