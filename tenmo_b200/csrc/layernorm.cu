@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(MOST, 1) ln_bwd_kernel(const LnBwd p) {
 __global__ void __launch_bounds__(LN_MAX_THREADS) ln_bwd_wide_kernel(const LnBwd p) {
     __shared__ float2 slots[2][32];
     float* out = p.partial + (int64_t)blockIdx.x * 2 * p.C;
-    for (int c = threadIdx.x; c < 2 * p.C; c += blockDim.x) out[c] = 0.f;
+    for (int64_t c = threadIdx.x; c < 2 * (int64_t)p.C; c += blockDim.x) out[c] = 0.f;  // (2 C + 1023 can pass 2^31)
     __syncthreads();
     int flip = 0;
     for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x) {
