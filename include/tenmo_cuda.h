@@ -313,6 +313,11 @@ int tenmo_ce_fwd_bwd_f32(tenmo_ctx* ctx, const float* logits, int64_t ld_logits,
  * after the calls that were issued before the capture, whose block the graph may have taken over.
  * The first call of its size allocates, which a stream that is being captured refuses: run it once before.
  *
+ * tenmo_operators_set_algo: TENMO_ALGO_SIMT_FP32 keeps the products of attention and of linear cross-entropy in fp32 (24 bits, no tensor cores) at
+ * every size, TENMO_ALGO_AUTO (the start) lets larger ones run on tensor cores with the bits stated at each operator. */
+int tenmo_operators_set_algo(tenmo_ctx* ctx, int algo);
+
+/*
  * Layer normalisation over the last axis (layernorm.mojo of the reference; no GPU-side counterpart on this path):
  *   y = (x - mean) * rstd * gamma + bias,  rstd = 1 / sqrt(var + eps),  var the mean squared difference from the mean.
  * x has leading dimension ldx, y / dy / dx are contiguous (M, C); gamma and bias are C floats.  mean and rstd (M floats each)

@@ -550,7 +550,7 @@ int tenmo_attention_fwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
     p.q_lengths = q_lengths;
     p.k_lengths = k_lengths;
     TenmoOpCall call(ctx);
-    if (tenmo_attn_tc_profitable(p, false)) return tenmo_attn_tc_fwd(ctx, p);
+    if (!ctx->op_fp32 && tenmo_attn_tc_profitable(p, false)) return tenmo_attn_tc_fwd(ctx, p);
     return few_fwd(ctx, p);
 }
 
@@ -587,7 +587,7 @@ int tenmo_attention_bwd_f32(tenmo_ctx* ctx, const tenmo_attn_shape* shape, const
     p.k_lengths = k_lengths;
     p.beta = beta;
     TenmoOpCall call(ctx);
-    if (tenmo_attn_tc_profitable(p, true)) return tenmo_attn_tc_bwd(ctx, p);
+    if (!ctx->op_fp32 && tenmo_attn_tc_profitable(p, true)) return tenmo_attn_tc_bwd(ctx, p);
     void* ws = nullptr;
     if ((st = tenmo_op_workspace(ctx, (size_t)p.B * p.H * p.Sq * sizeof(float) + 16, &ws)) != TENMO_OK) return st;
     p.delta = (float*)ws;

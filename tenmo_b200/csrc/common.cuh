@@ -49,6 +49,7 @@ struct tenmo_ctx {
     size_t op_graph_bytes = 0;
     void** op_retired = nullptr;
     int n_op_retired = 0;
+    bool op_fp32 = false;  // attention and linear cross-entropy without tensor cores (tenmo_operators_set_algo)
     // Order of the calls that use op_ws.  The caller may destroy a stream as soon as a call has returned, so no handle is kept: what is kept is
     // the stream's id, and an event that each call records at its end from the second stream on (op_many).
     unsigned long long op_stream_id = 0;

@@ -258,6 +258,13 @@ int tenmo_cuda_set_stream(tenmo_ctx* ctx, void* cuda_stream) {
     return TENMO_OK;
 }
 
+int tenmo_operators_set_algo(tenmo_ctx* ctx, int algo) {
+    TENMO_CHECK_CTX(ctx);
+    if (algo != TENMO_ALGO_AUTO && algo != TENMO_ALGO_SIMT_FP32) return tenmo_set_error(ctx, TENMO_ERR_INVALID, "operators_set_algo: unknown algo %d", algo);
+    ctx->op_fp32 = algo == TENMO_ALGO_SIMT_FP32;
+    return TENMO_OK;
+}
+
 int tenmo_cuda_reserve_sms(tenmo_ctx* ctx, int n) {
     TENMO_CHECK_CTX(ctx);
     if (n < 0 || n >= ctx->sm_count)

@@ -457,7 +457,7 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     int st = check(ctx, who, c);
     if (st != TENMO_OK) return st;
     TenmoOpCall call(ctx);
-    if (tc_profitable(c)) return lce_run_tc(ctx, c);
+    if (!ctx->op_fp32 && tc_profitable(c)) return lce_run_tc(ctx, c);
     // Up to 256 rows the kernels for a handful of rows, taken in groups of 32, keep more of the GPU busy than the strict-fp32 GEMM's tiles:
     // 204x1884x28 forward 34 us for 81, 180x855x112 training 54 for 87, 100x768x1000 training 83 for 116; level at 300x128x1000,
     // behind at 512x512x300 (155 for 89).

@@ -30,7 +30,7 @@ EXPORTS = [
     "tenmo_conv_out_size", "tenmo_conv2d_fwd_f32", "tenmo_conv2d_bwd_input_f32", "tenmo_conv2d_bwd_weight_f32", "tenmo_im2col_f32", "tenmo_col2im_f32", "tenmo_channel_sum_f32", "tenmo_maxpool2d_fwd_f32",
     "tenmo_maxpool2d_bwd_f32",
     "tenmo_colsum_f32_static", "tenmo_softmax_fwd_f32", "tenmo_softmax_bwd_f32", "tenmo_ce_fwd_f32", "tenmo_ce_bwd_f32", "tenmo_ce_fwd_bwd_f32", "tenmo_sgd_step_f32", "tenmo_sgd_step_lo_f32", "tenmo_accuracy_f32", "tenmo_dp_get_unique_id",
-    "tenmo_layernorm_fwd_f32", "tenmo_layernorm_bwd_f32", "tenmo_attention_fwd_f32", "tenmo_attention_bwd_f32",
+    "tenmo_operators_set_algo", "tenmo_layernorm_fwd_f32", "tenmo_layernorm_bwd_f32", "tenmo_attention_fwd_f32", "tenmo_attention_bwd_f32",
     "tenmo_linear_ce_fwd_f32", "tenmo_linear_ce_fwd_bwd_f32",
     "tenmo_dp_init", "tenmo_dp_allreduce_sum_f32", "tenmo_dp_finalize",
     "tenmo_dp_p2p_alloc", "tenmo_dp_p2p_connect", "tenmo_dp_p2p_allreduce_sum_f32", "tenmo_dp_p2p_sgd_step_f32", "tenmo_dp_p2p_set_coresident", "tenmo_dp_p2p_close",
@@ -159,6 +159,7 @@ def _bind(lib):
         "tenmo_ce_fwd_f32": (I, [P, P, I64, P, I, I64, I64, I64, F, I, P, P, P]),
         "tenmo_ce_bwd_f32": (I, [P, P, P, I, I64, I64, I64, F, I, P, P, P, F]),
         "tenmo_ce_fwd_bwd_f32": (I, [P, P, I64, P, I, I64, I64, I64, F, I, P, P, P, P, P]),
+        "tenmo_operators_set_algo": (I, [P, I]),
         "tenmo_layernorm_fwd_f32": (I, [P, P, I64, P, P, F, P, P, P, I64, I64]),
         "tenmo_layernorm_bwd_f32": (I, [P, P, I64, P, P, P, P, P, P, P, F, I64, I64]),
         "tenmo_attention_fwd_f32": (I, [P, C.POINTER(AttnShape)] + [C.POINTER(Heads)] * 4 + [P, F, I, P, P]),
@@ -193,6 +194,7 @@ class TenmoCuda:
         self._lib = None
         self._ctx = C.c_void_p()
         self._error = ""
+        self._operators_algo = ALGO_AUTO
         self.path = path or LIB_PATH
         try:
             self._lib = C.CDLL(self.path)
@@ -390,6 +392,12 @@ class TenmoCuda:
                valid_count, dlogits, beta=0.0):
         self._call("tenmo_ce_bwd_f32", softmax, labels, 1 if label_is_i64 else 0, M, Cn, ignore_index,
                    label_smoothing, reduction, upstream or None, valid_count or None, dlogits, beta)
+
+    def operators_set_algo(self, algo: int):
+        """ALGO_SIMT_FP32: attention and linear cross-entropy multiply in fp32 at every size; ALGO_AUTO: larger ones on tensor cores."""
+        if algo != self._operators_algo:
+            self._call("tenmo_operators_set_algo", algo)
+            self._operators_algo = algo
 
     def layernorm_fwd(self, x, ldx, gamma, bias, eps, y, mean, rstd, M, Cn):
         """Layer norm over the last axis; mean / rstd (0: not wanted) are what the backward pass needs."""

@@ -50,11 +50,13 @@ def handle(device: int | None = None) -> TenmoCuda:
         h = TenmoCuda(dev).require()
         _handles[dev] = h
     h.set_stream(torch.cuda.current_stream(dev).cuda_stream)
+    h.operators_set_algo(_lib.ALGO_SIMT_FP32 if _gemm_algo == _lib.ALGO_SIMT_FP32 else _lib.ALGO_AUTO)
     return h
 
 
 def set_gemm_algo(name: str):
-    """'auto' | 'simt' (strict fp32) | '3xtf32' (tcgen05): the run-time switch TENMO_CUDA_GEMM."""
+    """'auto' | 'simt' (strict fp32) | '3xtf32' (tcgen05): the run-time switch TENMO_CUDA_GEMM.  'simt' holds for the products of
+    Attention and LinearCrossEntropyLoss too."""
     global _gemm_algo
     _gemm_algo = {"auto": _lib.ALGO_AUTO, "simt": _lib.ALGO_SIMT_FP32, "3xtf32": _lib.ALGO_TC_3XTF32}[name]
 

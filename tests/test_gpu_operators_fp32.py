@@ -1,0 +1,70 @@
+"""The strict-fp32 switch on attention and linear cross-entropy, at sizes that otherwise run on tensor cores."""
+import numpy as np
+import pytest
+
+from tests import attention_reference as ar
+from tests import test_gpu_fused_attention as att
+from tests import test_gpu_linear_ce as lce
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture()
+def strict():
+    from tenmo_b200 import ALGO_AUTO, ALGO_SIMT_FP32
+    from tests import gpu_util as g
+
+    g.handle().operators_set_algo(ALGO_SIMT_FP32)
+    yield
+    g.handle().operators_set_algo(ALGO_AUTO)
+
+
+@pytest.mark.parametrize("D", [40, 64, 128])
+def test_attention(strict, D):
+    """A key and a value of 2^30 in their tile, which the row does not see: 24 bits of the others are kept, where a scale per tile of 64 or 128
+    would leave none."""
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    q, go = (att._make(gen, 2, 4, 300, D) for _ in range(2))
+    k, v = (att._make(gen, 2, 2, 310, D) for _ in range(2))
+    att.compare(q, k, v, go, causal=True, k_lengths=att.ints([310, 129]))
+    want = ar.reference(q, k, v, scale=D ** -0.5, causal=True)["o"]
+    for t in (k, v):
+        t[:, :, -1] = 2.0 ** 30
+    got = att.run(q, k, v, causal=True)["o"]
+    ar.check("o", got[:, :, :-1], (want[0][:, :, :-1], want[1][:, :, :-1]))
+
+
+@pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
+def test_linear_cross_entropy(strict, tied):
+    x, w, b, y = lce.make(700, 300, 2000, 42, tied=tied, bias=True)
+    lce.compare(x, w, b, y, ls=0.1)
+
+
+def test_the_switch_of_the_host_mirror():
+    """set_gemm_algo('simt') holds for Attention and LinearCrossEntropyLoss."""
+    import tenmo_b200.tensor as T
+    from tenmo_b200.attention import Attention
+    from tenmo_b200.crossentropy import LinearCrossEntropyLoss
+    from tenmo_b200 import ALGO_AUTO, ALGO_SIMT_FP32
+
+    rng = np.random.default_rng(43)
+    q, k, v = (T.Tensor.from_numpy(rng.standard_normal((2, 4, 300, 64)).astype(np.float32)) for _ in range(3))
+    x, w, b, y = lce.make(700, 300, 2000, 44)
+    X, W, Y = T.Tensor.from_numpy(x.cpu().numpy()), T.Tensor.from_numpy(w.cpu().numpy()), T.Tensor.labels(y.cpu().numpy())
+    both = lambda: (Attention()(q, k, v).numpy(), LinearCrossEntropyLoss()(X, W, Y).numpy())
+    h = T.handle()
+    fast = both()
+    try:
+        T.set_gemm_algo("simt")
+        strict = both()
+        assert T.handle()._operators_algo == ALGO_SIMT_FP32
+    finally:
+        T.set_gemm_algo("auto")
+    again = both()
+    assert T.handle() is h and h._operators_algo == ALGO_AUTO
+    assert all(np.array_equal(a, b) for a, b in zip(fast, again))
+    assert not np.array_equal(fast[0], strict[0])
+    dev = lambda t: torch.from_numpy(np.ascontiguousarray(t.numpy())).cuda()
+    ar.check("o", torch.from_numpy(strict[0]).cuda(), ar.reference(dev(q), dev(k), dev(v), scale=0.125)["o"])
+    lce.check("loss", torch.from_numpy(strict[1]).cuda().reshape(()), lce.reference(x, w, None, y)["loss"])

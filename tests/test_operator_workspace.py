@@ -303,3 +303,33 @@ def test_every_operator_orders_its_workspace(fake):
         at = first_and_last(fake, call)
         assert before is None or fake.comes_before(before, at[0])
         before = at[1]
+
+
+# ---- strict fp32 ----
+def test_strict_fp32_reaches_no_tensor_core_kernel(fake):
+    """Sizes that otherwise run on tensor cores, attention and linear cross-entropy."""
+    from tenmo_b200 import ALGO_AUTO, ALGO_SIMT_FP32, ALGO_TC_3XTF32, TenmoError, make_heads
+
+    view = lambda at, heads, n: make_heads(at << 40, (heads * n * 64, n * 64, 64))
+
+    def kernels():
+        B, H, n = 4, 8, 600
+        shape, t = (B, H, H, n, n, 64), [view(at, H, n) for at in range(1, 10)]
+        fake.lib.fake_forget_launches()
+        fake.handle.attention_fwd(shape, *t[:4], 5 << 50, 0.125)
+        fake.handle.attention_bwd(shape, *t[:4], 5 << 50, *t[4:8], 0.125)
+        linear_ce(fake, 3000, 300, 4000, bias=True)
+        linear_ce(fake, 100, 3000, 4000, bias=True, tied=True)
+        linear_ce(fake, 3000, 300, 4000, forward_only=True)
+        return [name for _, name, _ in fake.launches()]
+    on_tensor_cores = ("attn_fwd_tc", "attn_bwd_tc", "attn_tiles", "h3_")
+    some = kernels()
+    for part in on_tensor_cores:
+        assert any(part in name for name in some)
+    fake.handle.operators_set_algo(ALGO_SIMT_FP32)
+    assert not any(part in name for name in kernels() for part in on_tensor_cores)
+    fake.handle.operators_set_algo(ALGO_AUTO)
+    assert kernels() == some
+    for bad in (ALGO_TC_3XTF32, 7, -2):
+        with pytest.raises(TenmoError):
+            fake.handle.operators_set_algo(bad)
