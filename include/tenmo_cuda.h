@@ -346,8 +346,10 @@ int tenmo_layernorm_bwd_f32(tenmo_ctx* ctx, const float* x, int64_t ldx, const f
  *             and the sum of exponentials relative to it; written by the forward pass (NULL when no backward pass follows) and
  *             read by the backward pass.
  * Backward recomputes the probabilities; beta == 1 adds to what dq, dk, dv hold.  No atomics: results repeat bit for bit.
- * Precision: sums in 32 bits.  Larger problems multiply on tensor cores with every operand held to 22 bits, down to 2^-18 of the
- * largest entry of its row or of its tile of 64 or 128 rows, and to 2^-40 of that entry below.  A recomputed score differs from the
+ * Precision: sums in 32 bits.  Larger problems multiply on tensor cores with q, k, v, go and the probabilities held to 22 bits, down to 2^-18
+ * of the largest entry of their row or of their tile of 64 or 128 rows, and to 2^-40 of that entry below.  The scores' gradient is held against
+ * a bound of its size, 4 * dim (64 or 128) * the largest |go| * the largest |v| of the row and tile, + |go . o|: 22 bits down to 2^-18 of the
+ * bound, which for normal data is 2^-11 of the largest gradient, and 2^-39 of the bound below.  A recomputed score differs from the
  * forward pass's by some 2^-20 of sum |q k|, and the gradients by that factor: they mean little where scores pass 10^5.
  * A NaN or infinity that takes part gives NaN: in q in its row of o and dq, in k or v (as in the product P . V of the composed
  * operators) in any row of the heads that read it, in q or go also in dk and dv of its head's keys. */

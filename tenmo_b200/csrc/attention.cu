@@ -444,7 +444,7 @@ int few_fwd(tenmo_ctx* ctx, const TenmoAttnParams& p) {
     if (groups > INT32_MAX || blocks > INT32_MAX / 64) return tenmo_set_error(ctx, TENMO_ERR_UNSUPPORTED, "attention_fwd: too many rows in one call");
     f.groups = (int)groups;
     // slices of at least 256 keys, as many as it takes to fill every SM once (by registers: two blocks of eight rows, three of four,
-    // four of fewer).  16 requests of one token against 4099 keys, 16 heads on 4: 45 us for 49 with eight blocks per SM.
+    // four of fewer), rounded up: the last few blocks may start in a second round (four of 448 in the following case).  16 requests of one token against 4099 keys, 16 heads on 4: 45 us for 49 with eight blocks per SM.
     int64_t slices = ((R == 8 ? 2 : R == 4 ? 3 : 4) * (int64_t)ctx->sm_count + blocks - 1) / blocks;
     if (slices > p.Sk / 256) slices = p.Sk / 256;
     if (slices > 64) slices = 64;

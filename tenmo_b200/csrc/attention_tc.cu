@@ -546,7 +546,8 @@ int tenmo_attn_make_tiles(tenmo_ctx* ctx, const TenmoTileJobs& jobs, int count, 
     return TENMO_OK;
 }
 
-// Which kernels, from both sides measured over 4 .. 256 heads, dims 32 .. 128 and 16 .. 3000 rows and keys.
+// Which kernels, from both sides measured over 4 .. 256 heads, dims 32 .. 128 and 16 .. 3000 rows and keys (one to three heads take the same rule
+// without a measurement of their own; the tensor-core kernels never cut the keys, so few heads of few rows leave SMs idle).
 // Forward: the few-row kernel takes about 10 us plus 3.7 ns for every row and 128 keys (dim 64), the tensor-core one 14 us plus the
 // split of k and v, so it pays from some 2500 rows x 128 keys on (32 heads of 96x96: 15 us against 27; of 64x64: 15 against 13) -- but not for a
 // few rows per head, which leave its 128-row tiles empty (256 heads of 4 rows and 3000 keys: 228 against 110).

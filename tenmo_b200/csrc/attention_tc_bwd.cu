@@ -9,7 +9,9 @@
 // images serve both as the right operand over the columns (S, dP) and over the rows (gradients).  The gradients of a tile are
 // fresh accumulators that the warpgroups add to their registers with rounding.
 // fp16 range of dS: |dP - delta| is bounded by the operands' scales (dim * 2^30 times the two inverse scales) and by the largest
-// |delta|; a power of two from that bound brings dS to at most 2^15, exactly taken back when the tile is added.
+// |delta|; a power of two from that bound brings dS to at most 2^15, exactly taken back when the tile is added.  The bound lies some 2^6 to
+// 2^8 above the largest dS of normal data (dim times two maxima for a sum of random signs), so the pair's 22 bits end at 2^-11 of that dS
+// and its error at 2^-31 of it; a bound from the rows' norms would be closer but would need them per row and key.
 // One warp issues the MMAs, one the copies.  As in the forward pass the chain of a tile (S -> P -> dP -> dS -> sums) decides, so its
 // columns are shared by four warpgroups (16 of the 64 columns of S a thread, a quarter of the gradient's; the dkv pass of dim 128, whose
 // sums take 256 registers a row, has two).  Up to dim 64 S and dP have two buffers: the scores of tiles j + 1 and j + 2 are computed

@@ -275,7 +275,8 @@ __global__ void __launch_bounds__(THREADS, 1) h3_gemm_kernel(const __grid_consta
                 const float f = __ldg(p.a_inv + (A_MN ? (int64_t)c * p.a_cb + mb : (int64_t)mb * p.a_cb + c)) *
                                 __ldg(p.b_inv + (B_MN ? (int64_t)c * p.b_cb + nb : (int64_t)nb * p.b_cb + c));
                 const uint64_t f2 = tc::pack2(f, f);
-                // 16 columns at a time: 64 sums, 16 loaded values and the addresses stay within a thread's 96 registers
+                // 16 columns at a time: 64 sums, 16 loaded values and the addresses, of which a thread's 112 registers leave out 32 to 80 bytes
+                // (spilled, by form)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     float t[16];
