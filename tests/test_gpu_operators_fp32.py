@@ -53,16 +53,16 @@ def test_the_switch_of_the_host_mirror():
     x, w, b, y = lce.make(700, 300, 2000, 44)
     X, W, Y = T.Tensor.from_numpy(x.cpu().numpy()), T.Tensor.from_numpy(w.cpu().numpy()), T.Tensor.labels(y.cpu().numpy())
     both = lambda: (Attention()(q, k, v).numpy(), LinearCrossEntropyLoss()(X, W, Y).numpy())
-    h = T.handle()
-    fast = both()
+    before, h = T._gemm_algo, T.handle()
     try:
-        T.set_gemm_algo("simt")
-        strict = both()
-        assert T.handle()._operators_algo == ALGO_SIMT_FP32
+        results = []
+        for name, operators in (("auto", ALGO_AUTO), ("simt", ALGO_SIMT_FP32), ("3xtf32", ALGO_AUTO)):
+            T.set_gemm_algo(name)
+            results.append(both())
+            assert T.handle() is h and h._operators_algo == operators
     finally:
-        T.set_gemm_algo("auto")
-    again = both()
-    assert T.handle() is h and h._operators_algo == ALGO_AUTO
+        T._gemm_algo = before
+    fast, strict, again = results
     assert all(np.array_equal(a, b) for a, b in zip(fast, again))
     assert not np.array_equal(fast[0], strict[0])
     dev = lambda t: torch.from_numpy(np.ascontiguousarray(t.numpy())).cuda()
