@@ -314,7 +314,7 @@ int check(tenmo_ctx* ctx, const char* who, const LceCall& c) {
 }
 
 // Of one product: against the few-row kernels, which up to 256 rows otherwise run (200x300x1200, 1.4e8: 100 us for 97; 100x768x1000, 1.5e8:
-// 97 us for 83), and against the strict-fp32 GEMM (594x40x2465, 1.2e8: 109 us for 201; 980x207x450, 1.8e8: 104 for 114; 512x512x300,
+// 97 us for 83), and against the strict-fp32 GEMM (594x40x2465, 1.2e8: 112 us for 120; 980x207x450, 1.8e8: 104 for 114; 512x512x300,
 // 1.6e8: 94 for 86; 790x39x1249, 0.8e8: 107 for 123, 1442x72x249, 0.5e8: 100 for 82).
 constexpr double TC_FLOP_FEW = 2e8, TC_FLOP = 1e8;
 // Rows: with 17 to 32 the weight's split into blocks costs less than the few-row kernels' arithmetic on large weights (24x1318x44771 476 us
@@ -453,6 +453,40 @@ int lce_run_few(tenmo_ctx* ctx, const LceCall& c) {
     return TENMO_OK;
 }
 
+// The strict-fp32 GEMM adds up the whole contraction in one chain, whose rounding grows with its length: 385,494 rows of dim 1 cost the weight's
+// gradient 1.5e-4 of its norm, 160,000 classes dx 1.2e-4 (as below: 2.6e-7 and 3.6e-7).  Above 2048 the contraction is therefore cut into slices of
+// 512 (longer ones where 512 slices, or the budget, do not suffice), all but the last in one batched product, and the partial results are
+// added in order.  From 1024 on it would take 83 us for 79 at 1030x200x200 and 81 for 87 at 1442x72x249; 20000x50x49 takes 138 for 540.
+struct LceSlices { int64_t length, count; };
+LceSlices lce_slices(int64_t results, int64_t K) {
+    const int64_t most = min((int64_t)TENMO_COLSUM_SEQ_ROWS, (int64_t)(LCE_PIECE_BYTES / sizeof(float)) / results);
+    if (K <= 2048 || most < 2) return LceSlices{K, 1};
+    const int64_t length = max((int64_t)512, (K + most - 1) / most);
+    return LceSlices{length, (K + length - 1) / length};
+}
+size_t lce_slice_bytes(int64_t results, int64_t K) {
+    const LceSlices s = lce_slices(results, K);
+    return s.count > 1 ? (size_t)s.count * (size_t)results * sizeof(float) : 0;
+}
+// C (M, N) (+)= A . B + bias; partial: lce_slice_bytes(M * N, K)
+int lce_product(tenmo_ctx* ctx, int64_t M, int64_t N, int64_t K, tenmo_mat A, tenmo_mat B, float* C, float beta, const float* bias, float* partial) {
+    const LceSlices s = lce_slices(M * N, K);
+    if (s.count == 1) return tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, M, N, K, &A, &B, C, beta, bias, TENMO_ACT_NONE, nullptr, nullptr);
+    const int64_t before = s.count - 1;
+    A.batch_rank = B.batch_rank = 1;
+    A.batch_shape[0] = B.batch_shape[0] = before;
+    A.batch_stride[0] = s.length * A.col_stride;
+    B.batch_stride[0] = s.length * B.row_stride;
+    int st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, M, N, s.length, &A, &B, partial, 0.f, nullptr, TENMO_ACT_NONE, nullptr, nullptr);
+    if (st != TENMO_OK) return st;
+    A.batch_rank = B.batch_rank = 0;
+    A.offset += before * A.batch_stride[0];
+    B.offset += before * B.batch_stride[0];
+    st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, M, N, K - before * s.length, &A, &B, partial + before * M * N, 0.f, bias, TENMO_ACT_NONE, nullptr, nullptr);
+    if (st != TENMO_OK) return st;
+    return tenmo_colsum_own(ctx, partial, s.count, M * N, M * N, C, beta, nullptr);
+}
+
 int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     int st = check(ctx, who, c);
     if (st != TENMO_OK) return st;
@@ -467,8 +501,16 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
     const size_t x_bytes = ((size_t)piece * c.D * sizeof(float) + 255) & ~(size_t)255;
     const size_t l_bytes = ((size_t)c.N * sizeof(float) + 255) & ~(size_t)255, db_at = z_bytes + x_bytes + l_bytes + 256;
     const size_t db_sums = c.db && piece ? max(tenmo_colsum_own_bytes(ctx, piece, c.V), tenmo_colsum_own_bytes(ctx, c.N % piece, c.V)) : 0;
+    const size_t part_at = db_at + ((db_sums + 255) & ~(size_t)255);
+    size_t part = 0;
+    for (int64_t rows : {piece, piece ? c.N % piece : 0}) {
+        if (!rows) continue;
+        part = max(part, lce_slice_bytes(rows * c.V, c.D));
+        if (c.grad) part = max(part, max(lce_slice_bytes(rows * c.D, c.V), lce_slice_bytes(c.D * c.V, rows)));
+    }
     void* ws = nullptr;
-    if ((st = tenmo_op_workspace(ctx, db_at + db_sums, &ws)) != TENMO_OK) return st;
+    if ((st = tenmo_op_workspace(ctx, part_at + part, &ws)) != TENMO_OK) return st;
+    float* partial = (float*)((char*)ws + part_at);
     float* z = (float*)ws;
     float* xr = (float*)((char*)ws + z_bytes);
     float* row_loss = (float*)((char*)ws + z_bytes + x_bytes);
@@ -484,20 +526,17 @@ int lce_run(tenmo_ctx* ctx, const char* who, const LceCall& c) {
             c.x->ptr + c.x->offset, c.x->row_stride, c.x->col_stride, c.labels, c.is_i64, c.ignore, r0, rows, c.D, xr);
         TENMO_LAUNCH_CHECK(ctx, "lce_rows_kernel");
         const tenmo_mat mx = plain(xr, c.D, 1), mz = plain(z, c.V, 1);
-        st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, rows, c.V, c.D, &mx, c.w, z, 0.f, c.bias, TENMO_ACT_NONE, nullptr, nullptr);
+        st = lce_product(ctx, rows, c.V, c.D, mx, *c.w, z, 0.f, c.bias, partial);
         if (st != TENMO_OK) return st;
         const LceRow p{z, c.labels, row_loss, c.upstream, factor, ctx->dev_status, r0, c.V, c.ignore, c.ls, c.is_i64, c.reduction, c.grad};
         lce_row_kernel<<<(unsigned)rows, c.V > 4096 ? 1024 : LCE_THREADS, 0, ctx->stream>>>(p);
         TENMO_LAUNCH_CHECK(ctx, "lce_row_kernel");
         if (!c.grad) continue;
         const float beta = r0 ? 1.f : 0.f;
-        st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, rows, c.D, c.V, &mz, &wt, c.dx + r0 * c.D, 0.f, nullptr, TENMO_ACT_NONE, nullptr, nullptr);
+        st = lce_product(ctx, rows, c.D, c.V, mz, wt, c.dx + r0 * c.D, 0.f, nullptr, partial);
         if (st != TENMO_OK) return st;
         const tenmo_mat zt = transposed(mz), xt = transposed(mx);
-        if (tied)
-            st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, c.V, c.D, rows, &zt, &mx, c.dw, beta, nullptr, TENMO_ACT_NONE, nullptr, nullptr);
-        else
-            st = tenmo_gemm_f32(ctx, TENMO_ALGO_SIMT_FP32, c.D, c.V, rows, &xt, &mz, c.dw, beta, nullptr, TENMO_ACT_NONE, nullptr, nullptr);
+        st = tied ? lce_product(ctx, c.V, c.D, rows, zt, mx, c.dw, beta, nullptr, partial) : lce_product(ctx, c.D, c.V, rows, xt, mz, c.dw, beta, nullptr, partial);
         if (st != TENMO_OK) return st;
         if (c.db && (st = tenmo_colsum_own(ctx, z, rows, c.V, c.V, c.db, beta, (char*)ws + db_at)) != TENMO_OK) return st;
     }

@@ -68,3 +68,26 @@ def test_the_switch_of_the_host_mirror():
     dev = lambda t: torch.from_numpy(np.ascontiguousarray(t.numpy())).cuda()
     ar.check("o", torch.from_numpy(strict[0]).cuda(), ar.reference(dev(q), dev(k), dev(v), scale=0.125)["o"])
     lce.check("loss", torch.from_numpy(strict[1]).cuda().reshape(()), lce.reference(x, w, None, y)["loss"])
+
+
+@pytest.mark.parametrize("shape", [(385494, 1, 88), (400000, 10, 10), (100000, 16, 30), (3001, 40, 300), (300, 1, 160000), (400, 2, 60000), (300, 50000, 3),
+                                   (300, 3, 2049), (300, 2049, 66), (2049, 100, 99), (300, 2048, 70)], ids=str)
+@pytest.mark.parametrize("tied", [False, True], ids=["linear", "tied"])
+def test_long_contractions_are_not_one_chain(shape, tied):
+    """Products below the tensor cores' sizes with a long contraction.  A slice is a chain of at most L = max(512, K / 511) (or K up to 2048) terms, and
+    at most 512 of them are added: (L + 512) u of the sum of the terms' sizes, in place of the (64 + K / 32) u that reference() allows."""
+    N, D, V = shape
+    x, w, b, y = lce.make(*shape, 45, tied=tied, bias=True)
+    x = x + 3
+    got = lce.run(x, w, b, y)
+    want = lce.reference(x, w, b, y)
+    chain = lambda K: K if K <= 2048 else max(512, K // 511 + 1) + 512
+    xs = torch.where((y != lce.IGN)[:, None], x.double(), 0.0)
+    z = xs @ w.double() + b.double()
+    dz = torch.softmax(z, 1)
+    dz = (dz - torch.zeros_like(z).scatter_(1, y.clamp(min=0)[:, None], 1.0)).abs() * (y != lce.IGN)[:, None] / int((y != lce.IGN).sum())
+    for name, K, size, allowed in (("dx", V, dz @ w.double().abs().t(), 64 + V / 32), ("dw", N, xs.abs().t() @ dz, 64 + N / 32)):
+        value, bound = want[name]
+        lce.check(name, got[name], (value, bound + (chain(K) - allowed) * lce.U * size))
+    for name in ("loss", "db"):
+        lce.check(name, got[name], want[name])

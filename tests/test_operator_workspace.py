@@ -333,3 +333,32 @@ def test_strict_fp32_reaches_no_tensor_core_kernel(fake):
     for bad in (ALGO_TC_3XTF32, 7, -2):
         with pytest.raises(TenmoError):
             fake.handle.operators_set_algo(bad)
+
+
+def test_slices_of_long_contractions_fit_over_the_range(fake):
+    """Strict fp32, sizes at random with long rows, classes and dims: the partial results that the sequential column sum adds lie in the
+    workspace."""
+    from tenmo_b200 import ALGO_SIMT_FP32, TenmoCuda, TenmoError
+
+    rng = random.Random(3)
+    fake.watch("colsum_seq_kernel", "PqqqPf")
+    seen = 0
+    for _ in range(600):
+        size = [2 ** rng.uniform(0, 9), 2 ** rng.uniform(0, 12), 2 ** rng.uniform(8.1, 20)]
+        rng.shuffle(size)
+        N, D, V = max(257, int(size[0])), int(size[1]), int(size[2])
+        handle = TenmoCuda(0, path=fake.path).require()
+        handle.operators_set_algo(ALGO_SIMT_FP32)
+        try:
+            linear_ce(fake, N, D, V, tied=rng.random() < 0.5, bias=rng.random() < 0.5, handle=handle)
+        except TenmoError as e:
+            assert e.status == -4  # more than the card holds
+        for _, name, args in fake.launches():
+            if "colsum_seq_kernel" in name:
+                x, M, n, ld, out, _ = args
+                assert ld == n and M <= 512
+                assert fake.lib.fake_room_behind(x) >= M * n * 4, (N, D, V)
+                seen += fake.lib.fake_room_behind(out) == 0  # not the bias gradient's part of the workspace
+        fake.lib.fake_forget_launches()
+        handle.close()
+    assert seen > 300
