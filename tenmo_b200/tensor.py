@@ -50,7 +50,9 @@ def handle(device: int | None = None) -> TenmoCuda:
         h = TenmoCuda(dev).require()
         _handles[dev] = h
     h.set_stream(torch.cuda.current_stream(dev).cuda_stream)
-    h.operators_set_algo(_lib.ALGO_SIMT_FP32 if _gemm_algo == _lib.ALGO_SIMT_FP32 else _lib.ALGO_AUTO)
+    operators = -1 if _gemm_algo else 0  # ALGO_AUTO, ALGO_SIMT_FP32
+    if h._operators_algo != operators:
+        h.operators_set_algo(operators)
     return h
 
 
